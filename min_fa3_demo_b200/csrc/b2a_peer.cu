@@ -146,7 +146,7 @@ int b2a_peer_copy(void* dst, const void* src, size_t bytes, int32_t num_blocks, 
     int rc = current_device_info(&dev);
     if (rc != B2A_OK) return rc;
     const int smem = kCopySlots * kCopySlotBytes;
-    rc = once_per_device(dev.device, 3, [] {
+    rc = once_per_device(dev.device, 5, [] {
         B2A_CUDA_OK(cudaFuncSetAttribute(peer_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kCopySlots * kCopySlotBytes));
         return static_cast<int>(B2A_OK);
