@@ -344,6 +344,95 @@ size_t b2a_ring_bwd_workspace_bytes(int32_t batch, int32_t world_size, int32_t r
 int b2a_ring_bwd(const b2a_ring_bwd_args* args, void* cuda_stream);
 
 /* ------------------------------------------------------------------------- */
+/* Rotary positions and the key/value cache                                   */
+/* No counterparts in the reference, which has neither positions nor a cache. */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Which angle each pair of a head's dimensions turns by: pair i by positions[axis[i]] times its frequency.  The
+ * frequency is given as the fraction of a turn a position makes, round(f / (2 pi) * 2^64) mod 2^64: the low 64 bits of
+ * position * turn are then the fraction of a turn that is left, exact however far the position is.
+ * pairs is a multiple of 8, at most 64; the dimensions behind the first 2 * pairs stay as they are.
+ */
+typedef struct b2a_rotary_axes {
+    uint64_t turn[64];
+    uint8_t axis[64];
+    int32_t pairs;
+    int32_t axes;               /* rows of positions */
+    int32_t adjacent;           /* pair i: dimensions (2 i, 2 i + 1); otherwise (i, i + pairs) */
+} b2a_rotary_axes;
+
+typedef struct b2a_rotary_args {
+    const b2a_rotary_axes* axes;
+    const void* q;              /* bf16 [batch, seqlen, heads_q, 128]; 16-byte aligned, strides multiples of 8 */
+    const void* k;              /* bf16 [batch, seqlen, heads_k, 128]; NULL with heads_k == 0 */
+    void* q_out;                /* contiguous */
+    void* k_out;
+    const void* positions;      /* int32 or int64 [axes, batch, seqlen] */
+    int64_t q_stride[3];        /* elements from sequence to sequence, token to token, head to head */
+    int64_t k_stride[3];
+    int64_t positions_stride[3]; /* axis, sequence, token */
+    int32_t positions_64;       /* 1: positions are int64 */
+    int32_t batch;
+    int32_t seqlen;
+    int32_t heads_q;
+    int32_t heads_k;
+    int32_t inverse;            /* 1: by the negative angles, which is the gradient's rotation */
+} b2a_rotary_args;
+
+/* q and k turned by their positions: y1 = x1 cos a - x2 sin a, y2 = x2 cos a + x1 sin a for each pair (x1, x2). */
+int b2a_rotary(const b2a_rotary_args* args, void* cuda_stream);
+
+/*
+ * A key/value cache.  Slot s of sequence b is row s % page_size of page block_table[b][s / page_size]; without a block
+ * table page b holds sequence b.  A sequence has page_size * table_width slots (page_size without a table).
+ * Base addresses are 16-byte aligned and strides multiples of 8 elements; the 128 values of a head are adjacent.
+ */
+typedef struct b2a_cache {
+    void* k;                    /* bf16 [pages, page_size, heads_k, 128] */
+    void* v;
+    const int32_t* block_table; /* device int32 [batch, table_width] or NULL */
+    int64_t table_stride;       /* elements from row to row of the block table */
+    int64_t k_stride[3];        /* elements from page to page, row to row, head to head */
+    int64_t v_stride[3];
+    int32_t pages;
+    int32_t page_size;          /* with a block table a multiple of 8 */
+    int32_t heads_k;
+    int32_t table_width;
+} b2a_cache;
+
+typedef struct b2a_append_args {
+    b2a_cache cache;
+    const int32_t* cache_lens;  /* device int32 [batch]: slots in use */
+    const int32_t* cu_seqlens;  /* device int32 [batch + 1]: packed tokens; NULL: seqlen tokens a sequence */
+    const void* k;              /* bf16 [total, heads_k, 128] */
+    const void* v;
+    const void* q;              /* bf16 [total, heads_q, 128] to be turned by positions, or NULL */
+    void* q_out;                /* contiguous */
+    const b2a_rotary_axes* axes; /* NULL: k goes into the cache as it is */
+    const void* positions;      /* int32 or int64 [axes, total] */
+    int64_t q_stride[3];        /* sequence (not looked at for packed tokens), token, head */
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t positions_stride[3];
+    int32_t positions_64;
+    int32_t batch;
+    int32_t seqlen;
+    int32_t total;
+    int32_t heads_q;
+    void* workspace;            /* device scratch, 16-byte aligned, at least 16 bytes: the status word */
+    size_t workspace_bytes;
+} b2a_append_args;
+
+/*
+ * Writes k and v of sequence b's new tokens to slots cache_lens[b], cache_lens[b] + 1, ... of the cache and, with axes,
+ * turns k (and q, if given) by their positions on the way.  cache_lens is not changed.  A token whose slot or page does not
+ * exist is left out and the status word says so (b2a_check_status); packed tokens behind cu_seqlens[batch] are left out, and
+ * their rows of q_out left as they were.
+ */
+int b2a_cache_append(const b2a_append_args* args, void* cuda_stream);
+
+/* ------------------------------------------------------------------------- */
 /* Device status                                                              */
 /* ------------------------------------------------------------------------- */
 

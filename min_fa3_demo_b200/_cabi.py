@@ -8,7 +8,7 @@ fails loudly instead of silently computing somewhere else.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libb200attn.so"
@@ -159,6 +159,84 @@ class RingBwdArgs(Structure):
     ]
 
 
+class RotaryAxes(Structure):
+    """Mirror of ``b2a_rotary_axes``."""
+
+    _fields_ = [
+        ("turn", ctypes.c_uint64 * 64),
+        ("axis", ctypes.c_uint8 * 64),
+        ("pairs", c_int32),
+        ("axes", c_int32),
+        ("adjacent", c_int32),
+    ]
+
+
+class RotaryArgs(Structure):
+    """Mirror of ``b2a_rotary_args``."""
+
+    _fields_ = [
+        ("axes", c_void_p),
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("q_out", c_void_p),
+        ("k_out", c_void_p),
+        ("positions", c_void_p),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("positions_stride", c_int64 * 3),
+        ("positions_64", c_int32),
+        ("batch", c_int32),
+        ("seqlen", c_int32),
+        ("heads_q", c_int32),
+        ("heads_k", c_int32),
+        ("inverse", c_int32),
+    ]
+
+
+class Cache(Structure):
+    """Mirror of ``b2a_cache``."""
+
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("block_table", c_void_p),
+        ("table_stride", c_int64),
+        ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3),
+        ("pages", c_int32),
+        ("page_size", c_int32),
+        ("heads_k", c_int32),
+        ("table_width", c_int32),
+    ]
+
+
+class AppendArgs(Structure):
+    """Mirror of ``b2a_append_args``."""
+
+    _fields_ = [
+        ("cache", Cache),
+        ("cache_lens", c_void_p),
+        ("cu_seqlens", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("q", c_void_p),
+        ("q_out", c_void_p),
+        ("axes", c_void_p),
+        ("positions", c_void_p),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3),
+        ("positions_stride", c_int64 * 3),
+        ("positions_64", c_int32),
+        ("batch", c_int32),
+        ("seqlen", c_int32),
+        ("total", c_int32),
+        ("heads_q", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 # symbol -> (restype, argtypes); must list every function include/b200attn.h declares.
 SIGNATURES = {
     "b2a_abi_version": (c_int32, []),
@@ -182,6 +260,8 @@ SIGNATURES = {
     "b2a_ring_fwd": (c_int32, [POINTER(RingFwdArgs), c_void_p]),
     "b2a_ring_bwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "b2a_ring_bwd": (c_int32, [POINTER(RingBwdArgs), c_void_p]),
+    "b2a_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
+    "b2a_cache_append": (c_int32, [POINTER(AppendArgs), c_void_p]),
     "b2a_check_status": (c_int32, [c_void_p, c_void_p]),
     "b2a_set_wait_timeout_ns": (c_int32, [ctypes.c_uint64]),
     "b2a_profile_enable": (c_int32, [c_int32]),

@@ -10,6 +10,7 @@ module does the pairing once:
 
 ``attention(q, k, v, is_causal)``                 BSHD, differentiable
 ``attention_varlen(q, k, v, cu_seqlens, ...)``    packed varlen, differentiable
+``rotary(q, k, positions, axes)``                  rotary positions, differentiable
 ``RingAttention``                                  context parallel over a process group: owns the
                                                    K/V arenas, the fp32 dK/dV accumulators and the
                                                    completion counter, copies local K/V into the
@@ -18,7 +19,7 @@ module does the pairing once:
 The dense operators are registered with ``torch.library.custom_op`` (namespace ``b200attn``)
 with fake (meta) implementations, so they trace under ``torch.compile`` / fake tensors; there
 is no CPU implementation — calling them with CPU tensors raises.  Gradients are first order: those of
-``attention`` refuse to be differentiated again, those of the other two carry no graph.
+``attention`` refuse to be differentiated again, those of the other two carry no graph; ``rotary``'s can be differentiated again.
 """
 
 from __future__ import annotations
@@ -163,6 +164,45 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         cu_seqlens_k_host = cu_seqlens_k.cpu()
     return _AttentionVarlen.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, cu_seqlens_q_host, cu_seqlens_k_host,
                                   int(max_seqlen_q), int(max_seqlen_k), bool(is_causal), bool(deterministic))
+
+
+# ------------------------------------------------------------------------------------------
+# Rotary positions
+# ------------------------------------------------------------------------------------------
+def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
+    # Gradients come in any layout (expanded, transposed) and may be lazily negated.
+    t = t.resolve_neg()
+    rows = [s for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+    return t if t.stride(-1) == 1 and not any(s % 8 for s in rows) and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, axes, inverse: bool):
+        _require_cuda(q, "q")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.axes, ctx.inverse = axes, inverse
+        return _op.rotary(_rows_in_order(q), None if k is None else _rows_in_order(k), positions, axes, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        # A rotation's gradient is the rotation back, whatever q and k were; through the same function, so that it can be
+        # differentiated again.
+        positions, = ctx.saved_tensors
+        back = not ctx.inverse
+        if dq is None:
+            if dk is not None:
+                dk, _ = _Rotary.apply(dk, None, positions, ctx.axes, back)
+        else:
+            dq, dk = _Rotary.apply(dq, dk, positions, ctx.axes, back)
+        return dq, dk, None, None, None
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, axes: "_op.RotaryAxes"
+           ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Differentiable :func:`min_fa3_op.rotary`: q and k (or None) turned by positions of one or several axes."""
+    return _Rotary.apply(q, k, positions, axes, False)
 
 
 # ------------------------------------------------------------------------------------------

@@ -1,0 +1,144 @@
+"""Attention over a key/value cache: writing it, trees of drafted tokens, what its slots received, and eviction.
+
+The cache is two tensors ``[pages, page_size, KVH, 128]`` and a block table ``[B, width]`` (int32, on the device) that says
+which pages hold a sequence, or, without a block table, ``[B, slots, KVH, 128]``.  Any strides will do as long as the 128
+values of a head are adjacent: pages with k and v side by side, heads before slots, one layer of many.  ``cache_lens``
+``[B]`` (int32, on the device) is the number of slots that are in use; no call changes it, so that the host never waits.
+
+A decoding step: :func:`append_cache` writes the drafted tokens behind ``cache_lens``, :func:`forward_tree` lets them attend,
+and once some are accepted the caller writes those again (their positions are the same) and adds them to ``cache_lens``.
+:func:`cache_weights` adds up the attention that slots receive, :func:`evict_cache` drops those that received least.
+
+No counterpart in the reference, which has no cache (``bindings.cpp:240-363`` take k and v whole).  Lengths and block
+tables live on the device, so the kernels check them: what does not exist is left out, and ``check_last_status`` raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _cabi
+from .min_fa3_op import (_INT32_MAX, _SM100, _check, _check_device_capability, _on_device, _remember_workspace, _stream_ptr,
+                         _workspace)
+from .rotary import RotaryAxes, _check_heads, _check_positions, _position_strides, _rows
+
+__all__ = ["append_cache"]
+
+_NONE3 = (0, 0, 0)
+
+
+def _check_cache(cache: torch.Tensor, name: str) -> None:
+    _check(cache.is_cuda, f"{name} must be a CUDA tensor")
+    _check(cache.dtype == torch.bfloat16, f"{name} must have dtype torch.bfloat16")
+    _check(cache.dim() == 4, f"{name} must have shape [pages, page_size, KVH, D]")
+    _check(cache.size(3) == 128, f"{name} must have head_dim D=128")
+    _check(cache.size(0) > 0 and cache.size(1) > 0 and cache.size(2) > 0, f"{name} must not be empty")
+    _check(cache.stride(3) == 1 and not any(s % 8 for s in _rows(cache, 4)) and cache.data_ptr() % 16 == 0,
+           f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
+    _check(all(n == 1 or s > 0 for n, s in zip(cache.shape, cache.stride())), f"{name} must not be expanded")
+
+
+def _check_int32(t: torch.Tensor, name: str, shape, device) -> None:
+    _check(t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.device == device, f"{name} must be on the same CUDA device as the cache")
+    _check(t.dtype == torch.int32, f"{name} must have dtype torch.int32")
+    _check(tuple(t.shape) == tuple(shape), f"{name} must have shape {list(shape)}. Got {list(t.shape)}")
+    _check(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def _check_table(block_table: Optional[torch.Tensor], k_cache: torch.Tensor, batch: int) -> None:
+    if block_table is None:
+        _check(k_cache.size(0) >= batch, f"a cache without block_table needs a row for each sequence. Got {k_cache.size(0)} for {batch}")
+        return
+    _check(block_table.is_cuda, "block_table must be a CUDA tensor")
+    _check(block_table.device == k_cache.device, "block_table must be on the same CUDA device as the cache")
+    _check(block_table.dtype == torch.int32, "block_table must have dtype torch.int32")
+    _check(block_table.dim() == 2 and block_table.size(0) == batch and block_table.size(1) > 0,
+           f"block_table must have shape [{batch}, width]. Got {list(block_table.shape)}")
+    _check(block_table.size(1) == 1 or block_table.stride(1) == 1, "the rows of block_table must be contiguous")
+    _check(k_cache.size(1) % 8 == 0, f"page_size must be a multiple of 8. Got {k_cache.size(1)}")
+
+
+def _check_pair(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    _check_cache(k_cache, "k_cache")
+    _check_cache(v_cache, "v_cache")
+    _check(k_cache.device == v_cache.device, "k_cache and v_cache must be on the same CUDA device")
+    _check(k_cache.shape == v_cache.shape, "k_cache and v_cache must have the same shape")
+
+
+def _tokens(t: torch.Tensor, name: str, batch: int, cu_seqlens: Optional[torch.Tensor], device) -> int:
+    """Checks new tokens ``[B, n, H, 128]``, or ``[total, H, 128]`` with cu_seqlens; returns their number of dimensions."""
+    dim = 4 if cu_seqlens is None else 3
+    _check_heads(t, name, dim)
+    _check(t.device == device, f"{name} must be on the same CUDA device as the cache")
+    if dim == 4:
+        _check(t.size(0) == batch, f"{name} must have the batch size of cache_lens. Got {t.size(0)} vs {batch}")
+    return dim
+
+
+def _check_lens(cache_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], name: str, device) -> int:
+    _check(cache_lens.dim() == 1 and cache_lens.numel() > 0, "cache_lens must have shape [B]")
+    batch = cache_lens.numel()
+    _check_int32(cache_lens, "cache_lens", (batch,), device)
+    if cu_seqlens is not None:
+        _check_int32(cu_seqlens, name, (batch + 1,), device)
+    return batch
+
+
+def _cache_fields(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: Optional[torch.Tensor]):
+    """``b2a_cache`` as a tuple."""
+    table = (0, 0) if block_table is None else (block_table.data_ptr(), block_table.stride(0))
+    v = (0, _NONE3) if v_cache is None else (v_cache.data_ptr(), _rows(v_cache, 4))
+    return (k_cache.data_ptr(), v[0], *table, _rows(k_cache, 4), v[1], k_cache.size(0), k_cache.size(1), k_cache.size(2),
+            1 if block_table is None else block_table.size(1))
+
+
+def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
+                 block_table: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                 q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                 axes: Optional[RotaryAxes] = None) -> Optional[torch.Tensor]:
+    """Writes new tokens behind those that the cache holds, in place, and turns k (and q) by their positions on the way.
+
+    k, v ``[B, n, KVH, 128]``, or ``[total, KVH, 128]`` with ``cu_seqlens`` ``[B + 1]`` (int32, on the device): token ``i`` of
+    sequence ``b`` goes to slot ``cache_lens[b] + i``.  With ``axes`` and ``positions`` ``[axes, B, n]`` (``[axes, total]``)
+    k is turned as :func:`rotary` turns it; q, if given, likewise, and is returned.  Packed tokens behind
+    ``cu_seqlens[B]`` go nowhere, and their rows of the returned q are not written.  A token without a slot is left out
+    and reported by ``check_last_status("append_cache")``.
+    """
+    _check_pair(k_cache, v_cache)
+    device = k_cache.device
+    batch = _check_lens(cache_lens, cu_seqlens, "cu_seqlens", device)
+    _check_table(block_table, k_cache, batch)
+    dim = _tokens(k, "k", batch, cu_seqlens, device)
+    _tokens(v, "v", batch, cu_seqlens, device)
+    _check(k.shape == v.shape, "k and v must have the same shape")
+    _check(k.size(-2) == k_cache.size(2), f"k and the cache must have the same KV head count. Got {k.size(-2)} vs {k_cache.size(2)}")
+    _check((positions is None) == (axes is None), "positions and axes go together")
+    _check(q is None or axes is not None, "q is turned by positions, so it needs positions and axes")
+    if axes is not None:
+        _check_positions(positions, axes, k.shape[:-2], device)
+    if q is not None:
+        _tokens(q, "q", batch, cu_seqlens, device)
+        _check(q.shape[:-2] == k.shape[:-2], "q and k must have the same tokens")
+    if device.index not in _SM100:
+        _check_device_capability(device, "min_fa3_demo_b200 append_cache")
+    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
+    if k.numel() == 0:
+        return q_out
+    lib = _cabi.load()
+    ws = _workspace(16, device)
+    total = k.size(0) * k.size(1) if dim == 4 else k.size(0)
+    args = _cabi.AppendArgs(
+        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+        k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr(),
+        0 if axes is None else ctypes.addressof(axes._c), 0 if axes is None else positions.data_ptr(),
+        _NONE3 if q is None else _rows(q, dim), _rows(k, dim), _rows(v, dim),
+        _NONE3 if axes is None else _position_strides(positions), axes is not None and positions.dtype is torch.int64, batch,
+        k.size(1) if dim == 4 else 0, total, 0 if q is None else q.size(-2), ws.data_ptr(), 16)
+    with _on_device(device):
+        _cabi.check(lib.b2a_cache_append(ctypes.byref(args), _stream_ptr(device)))
+    _remember_workspace("append_cache", ws)
+    return q_out

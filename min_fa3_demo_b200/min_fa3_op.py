@@ -33,6 +33,9 @@ __all__ = [
     "parallel_remote_load_vec",
     "_debug_resolve_launch_grid_shape",
     "check_last_status",
+    "RotaryAxes",
+    "rotary",
+    "append_cache",
 ]
 
 _INT32_MAX = 2**31 - 1
@@ -541,10 +544,22 @@ from .parallel import (TKParallelTensor, _resolve_parallel_context, create_paral
 _RING_EXPORTS = ("backward_varlen_mega_ring", "forward_varlen_mega_ring", "forward_varlen_ring")
 
 
+_ROTARY_EXPORTS = ("RotaryAxes", "rotary")
+_CACHE_EXPORTS = ("append_cache",)
+
+
 def __getattr__(name: str):
-    # The ring module imports helpers from this one, so its entry points are resolved on first
+    # The ring, rotary and cache modules import helpers from this one, so their entry points are resolved on first
     # use (either module may be imported first).
     if name in _RING_EXPORTS:
         from . import ring
         return getattr(ring, name)
+    if name in _ROTARY_EXPORTS:
+        from . import rotary
+        globals()["RotaryAxes"], globals()["rotary"] = rotary.RotaryAxes, rotary.rotary   # a call then finds them at once
+        return globals()[name]
+    if name in _CACHE_EXPORTS:
+        from . import cache
+        globals().update((n, getattr(cache, n)) for n in _CACHE_EXPORTS)
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -1,0 +1,126 @@
+"""Rotary positions with one or several axes (text; height and width of an image; time, height and width of a clip).
+
+No counterpart in the reference, which takes q and k as they are (``bindings.cpp:240-363``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from fractions import Fraction
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _cabi
+from .min_fa3_op import _check, _check_device_capability, _on_device, _SM100, _stream_ptr
+
+__all__ = ["RotaryAxes", "rotary"]
+
+_PI = Fraction("3.14159265358979323846264338327950288419716939937510582")
+_MAX_PAIRS = 64
+
+
+class RotaryAxes:
+    """Which angle each pair of a head's 128 dimensions turns by.
+
+    Pair ``i`` turns by ``positions[axis[i]] * inv_freq[i]``; there are 8, 16, ... or 64 pairs, and the dimensions behind the
+    first ``2 * pairs`` stay as they are.  ``adjacent``: pair ``i`` is dimensions ``(2 i, 2 i + 1)``, otherwise
+    ``(i, i + pairs)``.  Frequencies are taken as the 64-bit floats they are; far positions lose nothing.
+    """
+
+    def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False):
+        inv_freq = [float(f) for f in inv_freq]
+        axis = [0] * len(inv_freq) if axis is None else [int(a) for a in axis]
+        pairs = len(inv_freq)
+        _check(pairs % 8 == 0 and 8 <= pairs <= _MAX_PAIRS,
+               f"the number of pairs must be a multiple of 8 between 8 and {_MAX_PAIRS}, got {pairs}")
+        _check(len(axis) == pairs, f"inv_freq and axis must have the same length. Got {pairs} vs {len(axis)}")
+        _check(all(0 <= a < _MAX_PAIRS for a in axis), f"an axis must be between 0 and {_MAX_PAIRS - 1}")
+        _check(all(abs(f) < float("inf") for f in inv_freq), "inv_freq must be finite")
+        self.axes = max(axis) + 1
+        self.pairs = pairs
+        c = _cabi.RotaryAxes()
+        for i, (f, a) in enumerate(zip(inv_freq, axis)):
+            c.turn[i] = round(Fraction(f) * 2**64 / (2 * _PI)) % 2**64
+            c.axis[i] = a
+        c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
+        self._c = c
+
+    @classmethod
+    def from_sections(cls, sections: Sequence[int], base: float = 10000.0, *, restart: bool = False,
+                      adjacent: bool = False) -> "RotaryAxes":
+        """The first ``sections[0]`` pairs follow axis 0, the next ``sections[1]`` axis 1, and so on.  Pair ``i`` of ``n`` has
+        frequency ``base ** (-i / n)``, counted over all sections, or, with ``restart``, within its own."""
+        _check(all(int(n) >= 0 for n in sections), "sections must not be negative")
+        total = sum(int(n) for n in sections)
+        freq, axis = [], []
+        for a, n in enumerate(int(n) for n in sections):
+            for j in range(n):
+                freq.append(float(base) ** (-(j / n if restart else len(freq) / total)))
+                axis.append(a)
+        return cls(freq, axis, adjacent=adjacent)
+
+
+def _rows(t: torch.Tensor, dim: int) -> Tuple[int, int, int]:
+    """Elements from sequence to sequence, token to token, head to head; 0 where there is only one."""
+    size, stride = t.shape, t.stride()
+    three = tuple(0 if n == 1 else s for n, s in zip(size[:-1], stride[:-1]))
+    return three if dim == 4 else (0, *three)
+
+
+def _check_heads(t: torch.Tensor, name: str, dim: int) -> None:
+    _check(t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.dtype == torch.bfloat16, f"{name} must have dtype torch.bfloat16")
+    _check(t.dim() == dim, f"{name} must have shape " + ("[B, S, H, D]" if dim == 4 else "[total_tokens, H, D]"))
+    _check(t.size(-1) == 128, f"{name} must have head_dim D=128")
+    _check(t.stride(-1) == 1 and not any(s % 8 for s in _rows(t, dim)) and t.data_ptr() % 16 == 0,
+           f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
+
+
+def _check_positions(positions: torch.Tensor, axes: RotaryAxes, shape, device) -> None:
+    _check(isinstance(axes, RotaryAxes), "axes must be a RotaryAxes")
+    _check(positions.device == device, "positions must be on the same CUDA device")
+    _check(positions.dtype in (torch.int32, torch.int64), "positions must have dtype torch.int32 or torch.int64")
+    _check(tuple(positions.shape) == (axes.axes, *shape),
+           f"positions must have shape {[axes.axes, *shape]}. Got {list(positions.shape)}")
+
+
+def _position_strides(positions: torch.Tensor) -> Tuple[int, int, int]:
+    s = positions.stride()
+    return s if len(s) == 3 else (s[0], 0, s[1])
+
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, axes: RotaryAxes, *,
+           inverse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """q and k turned by their positions.
+
+    q ``[B, S, QH, 128]``, k ``[B, S, KVH, 128]`` or None, positions ``[axes, B, S]`` (packed tokens: ``[T, H, 128]`` and
+    ``[axes, T]``), int32 or int64, of any strides (``expand`` one row of positions over a batch).  q and k may be slices of
+    one projection: only the 128 values of a head have to be adjacent.  Returns new contiguous tensors.  ``inverse``
+    turns the other way, which is what the gradients want; ``autograd.rotary`` does it by itself.
+    """
+    dim = q.dim()
+    _check(dim in (3, 4), "q must have shape [B, S, H, D] or [total_tokens, H, D]")
+    _check_heads(q, "q", dim)
+    if k is not None:
+        _check_heads(k, "k", dim)
+        _check(k.device == q.device, "q and k must be on the same CUDA device")
+        _check(k.shape[:-2] == q.shape[:-2], "q and k must have the same tokens")
+    _check_positions(positions, axes, q.shape[:-2], q.device)
+    if q.device.index not in _SM100:
+        _check_device_capability(q.device, "min_fa3_demo_b200 rotary")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    batch, seqlen = (q.size(0), q.size(1)) if dim == 4 else (1, q.size(0))
+    if q.numel() == 0:
+        return q_out, k_out
+    lib = _cabi.load()
+    args = _cabi.RotaryArgs(ctypes.addressof(axes._c), q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
+                            0 if k is None else k_out.data_ptr(), positions.data_ptr(), _rows(q, dim),
+                            (0, 0, 0) if k is None else _rows(k, dim), _position_strides(positions),
+                            positions.dtype is torch.int64, batch, seqlen, q.size(-2), 0 if k is None else k.size(-2),
+                            bool(inverse))
+    with _on_device(q.device):
+        _cabi.check(lib.b2a_rotary(ctypes.byref(args), _stream_ptr(q.device)))
+    return q_out, k_out
