@@ -432,6 +432,41 @@ typedef struct b2a_append_args {
  */
 int b2a_cache_append(const b2a_append_args* args, void* cuda_stream);
 
+typedef struct b2a_tree_args {
+    b2a_cache cache;
+    const int32_t* cache_lens;  /* device int32 [batch]: slots in use before the drafted tokens */
+    const int32_t* cu_seqlens_q; /* device int32 [batch + 1]: packed queries; NULL: seqlen_q a sequence */
+    const void* q;              /* bf16 [total_q, heads_q, 128] */
+    const uint8_t* tree_mask;   /* bytes [batch, seqlen_q, seqlen_q], packed [total_q, seqlen_q]; NULL: a chain */
+    void* out;                  /* bf16 [total_q, heads_q, 128], contiguous */
+    float* lse;                 /* [batch, heads_q, seqlen_q], packed [heads_q, total_q]; b2a_cache_weights reads it */
+    int64_t q_stride[2];        /* elements from token to token, head to head */
+    int64_t mask_stride[2];     /* bytes from sequence to sequence (0 for packed queries), row to row */
+    int32_t batch;
+    int32_t seqlen_q;           /* drafted tokens of a sequence; packed: the most that one has */
+    int32_t total_q;
+    int32_t heads_q;            /* a multiple of heads_k, at most 128 times it */
+    float softmax_scale;        /* 0 = 1/sqrt(128) */
+    float* weights;             /* b2a_cache_weights: fp32 [batch, heads_k, weights_slots] */
+    int64_t weights_stride[2];  /* elements from sequence to sequence, head to head */
+    int32_t weights_slots;
+    void* workspace;            /* device scratch, 16-byte aligned */
+    size_t workspace_bytes;
+} b2a_tree_args;
+
+/* Scratch of b2a_tree_fwd on the current device; looks at cache.heads_k, seqlen_q and heads_q. */
+size_t b2a_tree_fwd_workspace_bytes(const b2a_tree_args* args);
+
+/*
+ * Attention of drafted tokens over the cache.  Drafted token i of sequence b lies in slot cache_lens[b] + i already.  Its row
+ * sees every slot below cache_lens[b] and those drafted tokens u whose mask byte [i][u] is not 0 (no mask: u <= i).  A row
+ * that sees nothing gives out = 0 and lse = -inf; what a row does not see has no part in it, NaN and infinities
+ * included.  Rows behind cu_seqlens_q[batch] are left as they were.  Long sequences are cut along their slots and the
+ * pieces added up in fp32 in a fixed order, so repeated calls give the same bits; the last bits can depend on the other
+ * sequences of the call.
+ */
+int b2a_tree_fwd(const b2a_tree_args* args, void* cuda_stream);
+
 /* ------------------------------------------------------------------------- */
 /* Device status                                                              */
 /* ------------------------------------------------------------------------- */

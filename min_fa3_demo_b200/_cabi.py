@@ -237,6 +237,32 @@ class AppendArgs(Structure):
     ]
 
 
+class TreeArgs(Structure):
+    """Mirror of ``b2a_tree_args``."""
+
+    _fields_ = [
+        ("cache", Cache),
+        ("cache_lens", c_void_p),
+        ("cu_seqlens_q", c_void_p),
+        ("q", c_void_p),
+        ("tree_mask", c_void_p),
+        ("out", c_void_p),
+        ("lse", c_void_p),
+        ("q_stride", c_int64 * 2),
+        ("mask_stride", c_int64 * 2),
+        ("batch", c_int32),
+        ("seqlen_q", c_int32),
+        ("total_q", c_int32),
+        ("heads_q", c_int32),
+        ("softmax_scale", c_float),
+        ("weights", c_void_p),
+        ("weights_stride", c_int64 * 2),
+        ("weights_slots", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 # symbol -> (restype, argtypes); must list every function include/b200attn.h declares.
 SIGNATURES = {
     "b2a_abi_version": (c_int32, []),
@@ -262,6 +288,8 @@ SIGNATURES = {
     "b2a_ring_bwd": (c_int32, [POINTER(RingBwdArgs), c_void_p]),
     "b2a_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
     "b2a_cache_append": (c_int32, [POINTER(AppendArgs), c_void_p]),
+    "b2a_tree_fwd_workspace_bytes": (c_size_t, [POINTER(TreeArgs)]),
+    "b2a_tree_fwd": (c_int32, [POINTER(TreeArgs), c_void_p]),
     "b2a_check_status": (c_int32, [c_void_p, c_void_p]),
     "b2a_set_wait_timeout_ns": (c_int32, [ctypes.c_uint64]),
     "b2a_profile_enable": (c_int32, [c_int32]),

@@ -25,7 +25,7 @@ from .min_fa3_op import (_INT32_MAX, _SM100, _check, _check_device_capability, _
                          _workspace)
 from .rotary import RotaryAxes, _check_heads, _check_positions, _position_strides, _rows
 
-__all__ = ["append_cache"]
+__all__ = ["append_cache", "forward_tree"]
 
 _NONE3 = (0, 0, 0)
 
@@ -142,3 +142,88 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         _cabi.check(lib.b2a_cache_append(ctypes.byref(args), _stream_ptr(device)))
     _remember_workspace("append_cache", ws)
     return q_out
+
+
+def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> Tuple[int, int, Tuple[int, int]]:
+    """Checks what forward_tree and cache_weights share; returns (total_q, most tokens of a sequence, mask strides)."""
+    device = k_cache.device
+    dim = _tokens(q, "q", batch, cu_seqlens_q, device)
+    heads, kvh = q.size(-2), k_cache.size(2)
+    _check(heads > 0 and heads % kvh == 0,
+           f"This demo requires qhead % kvhead == 0 for GQA/MQA. Got qhead={heads}, kvhead={kvh}")
+    _check(heads // kvh <= 128, f"at most 128 query heads may share a KV head. Got qhead={heads}, kvhead={kvh}")
+    if dim == 4:
+        most, total = q.size(1), q.size(0) * q.size(1)
+        _check(max_seqlen_q is None or int(max_seqlen_q) == most, f"max_seqlen_q must be q.size(1). Got {max_seqlen_q} vs {most}")
+        _check(batch == 1 or most == 1 or q.stride(0) == most * q.stride(1), "q must have its sequences one behind the other")
+        shape = (batch, most, most)
+    else:
+        _check(max_seqlen_q is not None and 0 < int(max_seqlen_q) <= _INT32_MAX, "packed q needs a positive max_seqlen_q")
+        most, total = int(max_seqlen_q), q.size(0)
+        shape = (total, most)
+    _check(all(n == 1 or s > 0 for n, s in zip(q.shape, q.stride())), "q must not be expanded")
+    if tree_mask is None:
+        return total, most, (0, 0)
+    _check(tree_mask.device == device, "tree_mask must be on the same CUDA device as the cache")
+    _check(tree_mask.dtype == torch.bool, "tree_mask must have dtype torch.bool")
+    if dim == 4:
+        _check(tuple(tree_mask.shape) == shape, f"tree_mask must have shape {list(shape)}. Got {list(tree_mask.shape)}")
+    else:
+        _check(tree_mask.dim() == 2 and tree_mask.size(0) == total and tree_mask.size(1) >= most,
+               f"tree_mask must have shape [{total}, max_seqlen_q or more]. Got {list(tree_mask.shape)}")
+    _check(tree_mask.size(-1) == 1 or tree_mask.stride(-1) == 1, "the rows of tree_mask must be contiguous")
+    strides = tree_mask.stride()
+    return total, most, (strides[0], strides[1]) if dim == 4 else (0, strides[0])
+
+
+def _token_strides(q: torch.Tensor) -> Tuple[int, int]:
+    """Elements from token to token and from head to head of q seen as one list of tokens."""
+    stride = q.stride()
+    if q.dim() == 4 and q.size(1) == 1:
+        return stride[0], stride[2]
+    return stride[-3], stride[-2]
+
+
+def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
+                 block_table: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[torch.Tensor] = None,
+                 max_seqlen_q: Optional[int] = None, tree_mask: Optional[torch.Tensor] = None, return_lse: bool = False,
+                 out: Optional[torch.Tensor] = None):
+    """Attention of drafted tokens, or of the next token, over the cache.
+
+    q ``[B, n, QH, 128]``, or ``[total_q, QH, 128]`` with ``cu_seqlens_q`` ``[B + 1]`` (int32, on the device) and
+    ``max_seqlen_q``.  Token ``i`` of sequence ``b`` lies in slot ``cache_lens[b] + i`` already (:func:`append_cache`).  It
+    sees all slots before ``cache_lens[b]`` and the new tokens ``u`` with ``tree_mask[b, i, u]`` (bool ``[B, n, n]``; packed
+    ``[total_q, max_seqlen_q]``, a row for each token); without a mask those up to itself: ``n = 1`` is plain decoding.
+    Returns out like q (contiguous) and, with ``return_lse``, the fp32 natural-log LSE ``[B, QH, n]`` (``[QH, total_q]``).  A row
+    that sees nothing gives 0 and -inf.  Rows behind ``cu_seqlens_q[B]`` are not written; ``out`` (contiguous) may be given.
+    Lengths that do not fit and pages that do not exist are reported by ``check_last_status("forward_tree")``.  Repeated
+    calls give the same bits; the last bits can depend on the other sequences of the call.
+    """
+    _check_pair(k_cache, v_cache)
+    device = k_cache.device
+    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", device)
+    _check_table(block_table, k_cache, batch)
+    total, most, mask_stride = _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
+    if device.index not in _SM100:
+        _check_device_capability(device, "min_fa3_demo_b200 forward_tree")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    else:
+        _check(out.device == device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(),
+               "out must be contiguous and have the shape, dtype and device of q")
+    lse = torch.empty((batch, q.size(2), most) if q.dim() == 4 else (q.size(1), total), dtype=torch.float32, device=device)
+    if q.numel() == 0:
+        return (out, lse) if return_lse else out
+    lib = _cabi.load()
+    args = _cabi.TreeArgs(
+        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+        q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), _token_strides(q),
+        mask_stride, batch, most, total, q.size(-2), 0.0)
+    ref = ctypes.byref(args)
+    with _on_device(device):
+        nbytes = lib.b2a_tree_fwd_workspace_bytes(ref)
+        ws = _workspace(nbytes, device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        _cabi.check(lib.b2a_tree_fwd(ref, _stream_ptr(device)))
+    _remember_workspace("forward_tree", ws)
+    return (out, lse) if return_lse else out

@@ -69,8 +69,8 @@ unsigned long long completion_timeout_ns() { return 10ull * wait_timeout_ns(); }
 
 int once_per_device(int device, int slot, int (*fn)()) {
     static std::mutex mu;
-    static bool done[64][8] = {};
-    if (device < 0 || device >= 64 || slot < 0 || slot >= 8) {
+    static bool done[64][16] = {};
+    if (device < 0 || device >= 64 || slot < 0 || slot >= 16) {
         return fail(B2A_ERR_CUDA, "device index %d out of range", device);
     }
     std::lock_guard<std::mutex> lock(mu);
@@ -126,6 +126,31 @@ int make_token_map(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t
     if (res != CUDA_SUCCESS) {
         return fail(B2A_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d",
                     static_cast<int>(res));
+    }
+    return B2A_OK;
+}
+
+int make_strided_map(CUtensorMap* map, const void* base, int dims, const uint64_t* sizes, const int64_t* strides,
+                     uint32_t box_heads, uint32_t box_rows) {
+    EncodeTiledFn encode = get_encode_fn();
+    if (encode == nullptr) {
+        return fail(B2A_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    }
+    cuuint64_t size[4] = {128}, stride[3];
+    for (int i = 0; i < dims - 1; ++i) {
+        size[i + 1] = sizes[dims - 2 - i];
+        stride[i] = static_cast<cuuint64_t>(strides[dims - 2 - i]) * 2;
+        if (size[i + 1] == 1) stride[i] = 256;   // never stepped, and a caller may say anything
+        if (stride[i] == 0 || (stride[i] & 0xF) != 0 || stride[i] >= (1ull << 40)) {
+            return fail(B2A_ERR_INVALID_ARGUMENT, "strides must be positive multiples of 8 elements below 2^39");
+        }
+    }
+    const cuuint32_t box[4] = {64, box_heads, box_rows, 1}, elem_strides[4] = {1, 1, 1, 1};
+    const CUresult res = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, const_cast<void*>(base), size, stride, box,
+                                elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (res != CUDA_SUCCESS) {
+        return fail(B2A_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(res));
     }
     return B2A_OK;
 }

@@ -49,6 +49,11 @@ int current_device_info(DeviceInfo* info);
 int make_token_map(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t heads,
                    uint32_t box_rows, uint32_t box_heads = 1);
 
+// Tiled bf16 tensor map over [rows, heads, 128] (dims 3) or [pages, rows, heads, 128] (dims 4) with given strides in elements,
+// outermost first, a (64 columns, box_heads, box_rows[, 1 page]) box and 128-byte swizzle.
+int make_strided_map(CUtensorMap* map, const void* base, int dims, const uint64_t* sizes, const int64_t* strides,
+                     uint32_t box_heads, uint32_t box_rows);
+
 // Header words at the start of every workspace.
 struct WorkspaceHeader {
     int sched_counter;        // dynamic tile scheduler ticket; -n: no tickets, and n status words, one for each CTA, behind the header

@@ -1,0 +1,836 @@
+// Attention of drafted tokens over a cache: O = softmax(scale Q K^T + mask) V for the few rows that a decoding step has.
+//
+// A row (token t, query head h) sees all slots before the drafted tokens and those drafted tokens its mask names (the
+// ancestors in a tree; without a mask, those up to itself).  The query heads of a K/V head share its stream: tile rows are
+// 128 / group tokens of group heads.  What an item (up to 256 rows of one K/V head against its slots) costs is its slots,
+// 512 bytes each, whatever the number of rows, so the kernel is bound by memory up to some 256 rows and by the softmax beyond.
+//
+// Work: all items' blocks of 128 slots in a row, dealt out in equal runs, a run a CTA (CacheWalk).  An item that crosses the
+// end of a run is finished by tree_combine, in fp32 and in slot order.
+//
+//   warp 0-3, 4-7   softmax warpgroups, one thread a row
+//   warp 8          Q K^T       warp 10   P V       warp 9   plan and TMA loads       warp 11   idle
+//
+// An item of more than 128 rows has two tiles that use each block in turn, as in the forward.  One of at most 128 has only
+// one, and its two warpgroups take turns at the blocks: each has a running maximum, a sum and an O of its own, and they are
+// added up at the end of the piece through tensor memory, which both can read.  So the chain S -> softmax -> P V of one
+// block overlaps the next block's, and a warp that has only a few rows has two blocks' time for each.
+//
+// Tensor memory (512 columns): P of the warpgroups [0,64) [192,256), S [64,192), O [256,384) [384,512).
+//
+// Masked slots: a score is replaced, not added to, so NaN and infinities in K that a row does not see have no effect.  V
+// rows behind the last slot are zeroed in shared memory before the product (0 * NaN is NaN), and so are values of drafted
+// tokens that are not finite; those are added back to the rows that see them at the end.
+#include "b2a_cache.cuh"
+
+#include <cmath>
+
+namespace b2a {
+
+namespace {
+
+constexpr int kTreeThreads = 384;
+constexpr int kTreeStages = 2;
+constexpr int kTreeSlots = 4;       // pieces in flight between the load warp and the others
+constexpr int kTreeQkWarp = 8, kTreeLoadWarp = 9, kTreePvWarp = 10;
+constexpr int kTreeMaxCtas = kFwdStatusWords;
+
+struct TreeParams {
+    CacheQueries c;
+    __nv_bfloat16* out;
+    float* lse;
+    long long lse_seq_stride;    // 0 for packed queries
+    long long lse_head_stride;
+    int tile_tokens;             // 128 / group
+    int box_rows;
+    float scale_log2;
+    unsigned int* status;        // a word for each CTA, behind the header
+    uint32_t timeout_ns;
+    // Pieces that do not cover their item: two a CTA, the one its run begins with and the one it ends with.
+    struct TreeCut* cuts;        // [CTAs]: the item that a run begins inside of
+    float2* part_stat;           // [2 * CTAs][2 tiles][part_rows] (row maximum, row sum)
+    float4* part_o;              // [2 * CTAs][2 tiles][32][part_rows] O before the division
+    int part_rows;
+};
+
+struct TreeCut {
+    long long first, last;       // the item's blocks in the row of all
+    int run;                     // 0: the CTA's run does not begin inside an item
+    int seq, q_begin, tok0, n, head;
+    int pad[2];
+};
+
+struct TreePiece {
+    int valid;
+    int seq, q_begin, n, len, slots, head;
+    int tok0;        // first token
+    int tokens[2];   // of the two tiles
+    int j0, blocks;
+    int part;        // where its part goes; -1: it covers the item
+};
+
+struct __align__(1024) TreeShared {
+    uint8_t q[2][kTileBytes];
+    uint8_t k[kTreeStages][kTileBytes];
+    uint8_t v[kTreeStages][kTileBytes];
+    uint32_t seen[2][2][kTileM][4];   // warpgroup, turn, token: one bit for each slot of the block
+    float2 stat[2][kTileM];           // row maximum and sum of the two warpgroups
+    TreePiece piece[kTreeSlots];
+    uint64_t q_full[2], q_empty[2];
+    uint64_t k_full[kTreeStages], k_empty[kTreeStages];
+    uint64_t v_full[kTreeStages], v_empty[kTreeStages];
+    uint64_t s_full[2], s_empty, p_full[2], pv_done[2];
+    uint64_t seen_full[2];
+    uint64_t both_done, both_read;
+    uint64_t piece_full[kTreeSlots], piece_empty[kTreeSlots];
+    uint32_t not_finite;              // number of the last piece that met a drafted value that is not finite
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+};
+
+constexpr size_t kTreeSmemBytes = sizeof(TreeShared) + 1024;
+static_assert(kTreeSmemBytes <= 227 * 1024, "shared memory of a CTA");
+
+// Whether a block goes to warpgroup x: both tiles take every block, one tile's warpgroups take turns.
+__device__ __forceinline__ bool tree_takes(bool two, int i, int x) { return two || (i & 1) == x; }
+
+__device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreePiece& w, int token, int u) {
+    if (p.c.mask == nullptr) return u <= token;
+    const long long at = p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + token * p.c.mask_stride[1]
+                                                     : (static_cast<long long>(w.q_begin) + token) * p.c.mask_stride[1];
+    return p.c.mask[at + u] != 0;
+}
+
+__device__ __forceinline__ bool bf16_not_finite(uint32_t half) { return (half & 0x7F80u) == 0x7F80u; }
+
+// Values of drafted tokens that are not finite, added to a row that sees them: columns [column, column + 32) of O.
+// Only the sign of the weight, which is positive, matters.
+__device__ __noinline__ void tree_add_not_finite(const TreeParams& p, const TreePiece& w, int token, int column, uint32_t (&t)[32]) {
+    const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
+    for (int u = from; u < to; ++u) {
+        const long long slot = static_cast<long long>(w.len) + u;
+        if (slot >= w.slots || !tree_sees(p, w, token, u)) continue;
+        const int page = p.c.cache.page_of(w.seq, slot);
+        if (page < 0) continue;
+        const __nv_bfloat16* v = p.c.cache.v + page * p.c.cache.v_stride[0] + slot % p.c.cache.page_size * p.c.cache.v_stride[1] +
+                                 w.head * p.c.cache.v_stride[2] + column;
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t bits = __bfloat16_as_ushort(v[i]);
+            if (bf16_not_finite(bits)) t[i] = __float_as_uint(__uint_as_float(t[i]) + __uint_as_float(bits << 16));
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kTreeThreads, 1)
+tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    TreeShared& sh = *reinterpret_cast<TreeShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.q_full[i]), 1);
+            mbar_init(smem_u32(&sh.q_empty[i]), 1);
+            mbar_init(smem_u32(&sh.s_full[i]), 1);
+            mbar_init(smem_u32(&sh.p_full[i]), kTileM);
+            mbar_init(smem_u32(&sh.pv_done[i]), 1);
+            mbar_init(smem_u32(&sh.seen_full[i]), kTileM);
+        }
+        mbar_init(smem_u32(&sh.s_empty), kTileM);
+        mbar_init(smem_u32(&sh.both_done), 2 * kTileM);
+        mbar_init(smem_u32(&sh.both_read), 2 * kTileM);
+        for (int i = 0; i < kTreeStages; ++i) {
+            mbar_init(smem_u32(&sh.k_full[i]), 1);
+            mbar_init(smem_u32(&sh.k_empty[i]), 1);
+            mbar_init(smem_u32(&sh.v_full[i]), 1);
+            mbar_init(smem_u32(&sh.v_empty[i]), 1);
+        }
+        for (int i = 0; i < kTreeSlots; ++i) {
+            mbar_init(smem_u32(&sh.piece_full[i]), 1);
+            mbar_init(smem_u32(&sh.piece_empty[i]), 2 + 8);   // MMA warps and softmax warps
+        }
+        sh.abort_flag = 0;
+        sh.not_finite = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == kTreeQkWarp) {
+        tmem_alloc(smem_u32(&sh.tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+    }
+    let_next_kernel_start();
+    wait_for_previous_kernel();
+    // Each CTA clears and uses a status word of its own, and CTA 0 writes the header (as the forward does).
+    if (threadIdx.x == 0) {
+        p.status[blockIdx.x] = 0u;
+        if (blockIdx.x == 0) reinterpret_cast<int4*>(p.status)[-1] = make_int4(-static_cast<int>(gridDim.x), 0, 0, 0);
+    }
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
+    const WaitCtx wctx{smem_u32(&sh.abort_flag), p.status, p.timeout_ns, 1u};
+
+    if (warp >= 8) {
+        reg_dealloc<72>();
+        if (warp == kTreeLoadWarp) {
+            // ------------------------------------------------------------ plan and loads
+            if (lane == 0) {
+                tma_prefetch_desc(&map_q);
+                tma_prefetch_desc(&map_k);
+                tma_prefetch_desc(&map_v);
+            }
+            CacheWalk walk;
+            walk.start(p.c, blockIdx.x, gridDim.x, lane);
+            if (lane == 0) {
+                TreeCut cut{};
+                if (walk.pos < walk.end && walk.j > 0) {
+                    cut.first = walk.pos - walk.j;
+                    cut.last = cut.first + walk.blocks;
+                    cut.run = walk.run;
+                    cut.seq = walk.seq;
+                    cut.q_begin = walk.s.q_begin;
+                    cut.tok0 = walk.rt * p.c.item_tokens;
+                    cut.n = walk.s.n;
+                    cut.head = walk.head;
+                }
+                p.cuts[blockIdx.x] = cut;
+            }
+            SlotLoader loader{p.box_rows, kSlotBlock / p.box_rows, 0, 0, walk.bad};
+            uint32_t k_it = 0, v_it = 0, q_par = 0;
+            bool ok = true, begun = false;
+            for (uint32_t it = 0; ok; ++it) {
+                const uint32_t at = it % kTreeSlots;
+                ok = mbar_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTreeSlots) & 1u) ^ 1u, 1);
+                if (!ok) break;
+                TreePiece w{};
+                w.valid = walk.pos < walk.end;
+                if (w.valid) {
+                    w.seq = walk.seq;
+                    w.q_begin = walk.s.q_begin;
+                    w.n = walk.s.n;
+                    w.len = walk.s.len;
+                    w.slots = walk.s.slots;
+                    w.head = walk.head;
+                    w.tok0 = walk.rt * p.c.item_tokens;
+                    w.tokens[0] = min(p.tile_tokens, w.n - w.tok0);
+                    w.tokens[1] = max(0, min(p.tile_tokens, w.n - w.tok0 - p.tile_tokens));
+                    w.j0 = walk.j;
+                    w.blocks = walk.piece();
+                    w.part = w.blocks == walk.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (begun ? 1 : 0);
+                    begun = true;
+                }
+                if (lane == 0) {
+                    sh.piece[at] = w;
+                    mbar_arrive(smem_u32(&sh.piece_full[at]));
+                }
+                if (!w.valid) break;
+                auto load_q = [&](int x) {
+                    ok = mbar_wait(wctx, smem_u32(&sh.q_empty[x]), ((q_par >> x) & 1u) ^ 1u, 2);
+                    if (!ok) return;
+                    q_par ^= 1u << x;
+                    if (lane == 0) {
+                        const uint32_t bar = smem_u32(&sh.q_full[x]), dst = smem_u32(&sh.q[x][0]);
+                        const int row = w.q_begin + w.tok0 + x * p.tile_tokens;
+                        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.tile_tokens * p.c.group) * 256u);
+                        tma_load_3d(dst, &map_q, bar, 0, w.head * p.c.group, row);
+                        tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, w.head * p.c.group, row);
+                    }
+                    __syncwarp();
+                };
+                // K of block i is asked for before V of block i - 1: Q K^T is a block ahead of P V.
+                load_q(0);
+                int page_v = 0, row_v = 0;
+                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
+                for (int i = 0; i <= w.blocks && ok; ++i) {
+                    SlotLoader now = loader;
+                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+                    if (i < w.blocks) {
+                        const uint32_t stage = k_it % kTreeStages;
+                        ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
+                        if (!ok) break;
+                        ++k_it;
+                        now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head,
+                                 now.count(w.j0 + i, w.slots), lane);
+                    }
+                    if (i == 0 && w.tokens[1] > 0) {
+                        load_q(1);
+                        if (!ok) break;
+                    }
+                    if (i > 0) {
+                        const uint32_t stage = v_it % kTreeStages;
+                        ok = mbar_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kTreeStages) & 1u) ^ 1u, 4);
+                        if (!ok) break;
+                        ++v_it;
+                        SlotLoader before = now;
+                        before.page = page_v;
+                        before.row = row_v;
+                        before.load(&map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head,
+                                    before.count(w.j0 + i - 1, w.slots), lane);
+                    }
+                    page_v = now.page;
+                    row_v = now.row;
+                }
+                if (!ok) break;
+                walk.advance(p.c, w.blocks);
+            }
+            if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
+        } else if (warp == kTreeQkWarp || warp == kTreePvWarp) {
+            // ------------------------------------------------------------ MMA warps
+            const bool qk = warp == kTreeQkWarp;
+            constexpr uint32_t idesc_qk = make_idesc_bf16(kTileM, kTileN, 0, 0);
+            constexpr uint32_t idesc_pv = make_idesc_bf16(kTileM, kHeadDim, 0, 1);
+            constexpr uint32_t kStageStep = kTileBytes >> 4;
+            const uint32_t q_lo0 = desc_lo_kmajor(smem_u32(&sh.q[0][0]));
+            const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0]));
+            const uint32_t v_lo0 = desc_lo_mnmajor(smem_u32(&sh.v[0][0]));
+            uint32_t kv_it = 0, s_it = 0, par = 0;
+            bool ok = true;
+            for (uint32_t it = 0; ok; ++it) {
+                const uint32_t at = it % kTreeSlots;
+                ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 5);
+                if (!ok) break;
+                const volatile TreePiece& w = sh.piece[at];
+                const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
+                const int blocks = __shfl_sync(0xFFFFFFFFu, w.blocks, 0);
+                const bool two = __shfl_sync(0xFFFFFFFFu, w.tokens[1], 0) > 0;
+                if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+                __syncwarp();
+                if (!valid) break;
+                for (int i = 0; i < blocks && ok; ++i, ++kv_it) {
+                    const uint32_t stage = kv_it % kTreeStages, phase = (kv_it / kTreeStages) & 1u;
+                    if (qk) {
+                        ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), phase, 6);
+                        if (!ok) break;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            if (!tree_takes(two, i, x)) continue;
+                            const int tile = two ? x : 0;
+                            if (i == 0) {
+                                ok = mbar_wait(wctx, smem_u32(&sh.q_full[tile]), (par >> tile) & 1u, 7);
+                                if (!ok) break;
+                                par ^= 1u << tile;
+                            }
+                            // The softmax warps have taken the S before this one out of tensor memory.
+                            ok = mbar_wait(wctx, smem_u32(&sh.s_empty), (s_it & 1u) ^ 1u, 8);
+                            if (!ok) break;
+                            ++s_it;
+                            tc_fence_after_sync();
+                            umma_ss_kk_x8_w(tmem_base + kFwdColS, q_lo0 + tile * kStageStep, k_lo0 + stage * kStageStep, idesc_qk, 0u);
+                            tc_commit_w(smem_u32(&sh.s_full[x]));
+                            if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[tile]));
+                            __syncwarp();
+                        }
+                        tc_commit_w(smem_u32(&sh.k_empty[stage]));
+                    } else {
+                        ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), phase, 9);
+                        if (!ok) break;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            if (!tree_takes(two, i, x)) continue;
+                            ok = mbar_wait(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
+                            if (!ok) break;
+                            par ^= 1u << x;
+                            tc_fence_after_sync();
+                            umma_ts_x8_w(tmem_base + kFwdColO + x * 128u, tmem_base + kFwdColP + x * kFwdColPStep,
+                                         v_lo0 + stage * kStageStep, idesc_pv, i > (two ? 0 : x) ? 1u : 0u);
+                            tc_commit_w(smem_u32(&sh.pv_done[x]));
+                            __syncwarp();
+                        }
+                        tc_commit_w(smem_u32(&sh.v_empty[stage]));
+                    }
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax warpgroups
+        reg_alloc<216>();
+        const int x = warp >> 2;
+        const int quarter = warp & 3;
+        const int r = quarter * 32 + lane;
+        const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_tmem = tmem_base + lane_base + kFwdColS;
+        const uint32_t p_tmem = tmem_base + lane_base + kFwdColP + static_cast<uint32_t>(x) * kFwdColPStep;
+        const uint32_t o_tmem = tmem_base + lane_base + kFwdColO;
+        const float sl2 = p.scale_log2;
+        const int row_token = r / p.c.group;           // of the tile
+        const int row_head = r - row_token * p.c.group;
+        uint32_t s_cnt = 0, pv_cnt = 0, seen_cnt = 0, both_cnt = 0, kv_base = 0;
+        bool ok = true;
+
+        for (uint32_t it = 0; ok; ++it) {
+            const uint32_t at = it % kTreeSlots;
+            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 11);
+            if (!ok) break;
+            const TreePiece& w = sh.piece[at];
+            auto release = [&]() {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+            };
+            if (!w.valid) break;
+            const bool two = w.tokens[1] > 0;
+            const int tile = two ? x : 0;
+            const int tokens = w.tokens[tile];
+            const int rows = tokens * p.c.group;
+            const bool row_valid = r < rows;
+            const bool active = quarter * 32 < rows;      // the warp has a row at all
+            const int token = w.tok0 + tile * p.tile_tokens + row_token;
+            const bool masked = p.c.mask != nullptr;
+
+            float m_used = -INFINITY;   // running reference maximum (raw score units)
+            float l = 0.f;              // running row sum relative to m_used
+            const int first = two ? 0 : x, step = two ? 1 : 2;
+            for (int i = first; i < w.blocks; i += step) {
+                const int base = (w.j0 + i) * kSlotBlock;
+                const bool tail = base + kSlotBlock > w.len;   // drafted tokens, or no slots any more
+                uint32_t* seen = nullptr;
+                if (tail && masked) {
+                    // Which slots of the block each token sees: a warp's lanes are 32 slots.
+                    const int u = base + quarter * 32 + lane - w.len;
+                    seen = &sh.seen[x][seen_cnt & 1u][0][0];
+                    const int from = w.tok0 + tile * p.tile_tokens;
+                    const bool slot_ok = base + quarter * 32 + lane < w.slots;
+#pragma unroll 8
+                    for (int t = 0; t < tokens; ++t) {
+                        const bool yes = slot_ok && (u < 0 || (u < w.n && tree_sees(p, w, from + t, u)));
+                        const uint32_t word = __ballot_sync(0xFFFFFFFFu, yes);
+                        if (lane == 0) seen[t * 4 + quarter] = word;
+                    }
+                    __syncwarp();
+                    mbar_arrive(smem_u32(&sh.seen_full[x]));
+                }
+                ok = mbar_wait(wctx, smem_u32(&sh.s_full[x]), s_cnt & 1u, 12);
+                if (!ok) break;
+                ++s_cnt;
+                tc_fence_after_sync();
+                float s[kTileN];
+                if (active) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t t[32];
+                        tmem_ld_x32(s_tmem + c * 32, t);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(t[e]);
+                    }
+                    tmem_wait_ld();
+                }
+                tc_fence_before_sync();
+                mbar_arrive(smem_u32(&sh.s_empty));
+
+                if (tail) {
+                    if (masked) {
+                        ok = mbar_wait(wctx, smem_u32(&sh.seen_full[x]), seen_cnt & 1u, 13);
+                        if (!ok) break;
+                        ++seen_cnt;
+                    }
+                    // V row r of the block (whichever warpgroup's product with it comes first): behind the last slot
+                    // zeros, and of drafted tokens no value that is not finite.
+                    const int slot = base + r;
+                    const bool look = slot >= w.len && slot < w.slots && (w.n > 1 || masked);
+                    if (!two || x == 0) {
+                        const uint32_t stage = (kv_base + i) % kTreeStages;
+                        ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / kTreeStages) & 1u, 14);
+                        if (!ok) break;
+                        if (look || slot >= w.slots) {
+#pragma unroll 4
+                            for (int c = 0; c < 16; ++c) {
+                                // Another chunk first in each row, so that rows of 128 bytes do not meet in the same banks.
+                                uint4* chunk = reinterpret_cast<uint4*>(&sh.v[stage][(c >> 3) * kHalfTileBytes + r * 128 +
+                                                                                     (((c + r) & 7) * 16)]);
+                                if (!look) {
+                                    *chunk = make_uint4(0u, 0u, 0u, 0u);
+                                    continue;
+                                }
+                                uint4 val = *chunk;
+                                uint32_t words[4] = {val.x, val.y, val.z, val.w};
+                                bool found = false;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if (bf16_not_finite(words[e])) words[e] &= 0xFFFF0000u, found = true;
+                                    if (bf16_not_finite(words[e] >> 16)) words[e] &= 0xFFFFu, found = true;
+                                }
+                                if (found) {
+                                    *chunk = make_uint4(words[0], words[1], words[2], words[3]);
+                                    *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
+                                }
+                            }
+                            fence_proxy_async_smem();
+                        }
+                    }
+                    if (active) {
+                        // One bit per visible slot of 32.
+                        const int lim = min(w.slots, w.len + token + 1) - base;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t bits;
+                            if (masked) {
+                                bits = seen[min(row_token, tokens - 1) * 4 + c];
+                            } else {
+                                const int vis = min(max(lim - c * 32, 0), 32);
+                                bits = vis == 32 ? 0xFFFFFFFFu : (1u << vis) - 1u;
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                if (!((bits >> e) & 1u)) s[c * 32 + e] = -INFINITY;
+                            }
+                        }
+                    }
+                }
+
+                const bool begins = i == first;
+                bool pv_pending = !begins;
+                auto wait_pv = [&]() -> bool {
+                    if (!mbar_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15)) return false;
+                    ++pv_cnt;
+                    tc_fence_after_sync();
+                    pv_pending = false;
+                    return true;
+                };
+                if (!active) {
+                    // None of the warp's rows exists; it keeps step, and its P and O are never looked at.
+                    if (pv_pending) {
+                        ok = wait_pv();
+                        if (!ok) break;
+                    }
+                    mbar_arrive(smem_u32(&sh.p_full[x]));
+                    continue;
+                }
+                float bm;
+                {
+                    float m[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m[e] = s[e];
+#pragma unroll
+                    for (int e = 8; e < kTileN; ++e) m[e & 7] = fmaxf(m[e & 7], s[e]);
+                    bm = fmaxf(max3(max3(m[0], m[1], m[2]), m[3], m[4]), max3(m[5], m[6], m[7]));
+                }
+                const float m_new = fmaxf(m_used, bm);
+                if (begins) {
+                    m_used = m_new;
+                } else if (__any_sync(0xFFFFFFFFu, (m_new - m_used) * sl2 > kRescaleThreshold)) {
+                    // O is scaled only when the maximum has moved by a factor of 2^8: the division at the end uses the same one.
+                    const float factor = m_new == -INFINITY ? 1.f : fast_exp2((m_used - m_new) * sl2);
+                    l *= factor;
+                    m_used = m_new;
+                    ok = wait_pv();
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t t[32];
+                        tmem_ld_x32(o_tmem + x * 128 + c * 32, t);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) t[e] = __float_as_uint(__uint_as_float(t[e]) * factor);
+                        tmem_st_x32(o_tmem + x * 128 + c * 32, t);
+                    }
+                }
+                const float neg_m = m_used == -INFINITY ? 0.f : -m_used * sl2;
+                const float2 sl2v = make_float2(sl2, sl2), negv = make_float2(neg_m, neg_m);
+                float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t t[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 x0 = fma2(make_float2(s[c * 64 + 2 * e], s[c * 64 + 2 * e + 1]), sl2v, negv);
+                        const float2 x1 = fma2(make_float2(s[c * 64 + 2 * e + 2], s[c * 64 + 2 * e + 3]), sl2v, negv);
+                        const float2 p0 = make_float2(fast_exp2(x0.x), fast_exp2(x0.y));
+                        const float2 p1 = make_float2(fast_exp2(x1.x), fast_exp2(x1.y));
+                        acc0 = add2(acc0, p0);
+                        acc1 = add2(acc1, p1);
+                        // P is rounded to bf16 for the product: 2^-9 of a term on average, as much as the rounding of out.
+                        t[e] = pack_bf16x2(p0.x, p0.y);
+                        t[e + 1] = pack_bf16x2(p1.x, p1.y);
+                    }
+                    if (c == 0 && pv_pending) {
+                        ok = wait_pv();
+                        if (!ok) break;
+                    }
+                    tmem_st_x32(p_tmem + c * 32, t);
+                }
+                if (!ok) break;
+                l += (acc0.x + acc0.y) + (acc1.x + acc1.y);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                mbar_arrive(smem_u32(&sh.p_full[x]));
+            }
+            if (!ok) break;
+            kv_base += w.blocks;
+            if (w.blocks > first) {
+                ok = mbar_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15);
+                if (!ok) break;
+                ++pv_cnt;
+                tc_fence_after_sync();
+            }
+
+            // One tile: the two warpgroups' parts, O = a0 O0 + a1 O1; each does half of the columns.
+            float a0 = 1.f, a1 = 0.f;
+            if (!two) {
+                sh.stat[x][r] = make_float2(m_used, l);
+                tc_fence_before_sync();
+                mbar_arrive(smem_u32(&sh.both_done));
+                ok = mbar_wait(wctx, smem_u32(&sh.both_done), both_cnt & 1u, 16);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const float2 s0 = sh.stat[0][r], s1 = sh.stat[1][r];
+                m_used = fmaxf(s0.x, s1.x);
+                a0 = s0.x == m_used ? 1.f : fast_exp2((s0.x - m_used) * sl2);
+                a1 = s1.x == m_used ? 1.f : fast_exp2((s1.x - m_used) * sl2);
+                l = s0.y * a0 + s1.y * a1;
+                if (w.blocks == 1) a1 = 0.f;
+            }
+            if (active) {
+                const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) == it + 1;
+                // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const bool whole = w.part < 0;
+                if (row_valid && (two || x == 0)) {
+                    if (whole) {
+                        const float lse = l == 0.f ? -INFINITY : (m_used * sl2 + fast_log2(l)) * kLn2;
+                        const int head = w.head * p.c.group + row_head;
+                        p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
+                              (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)] = lse;
+                    } else {
+                        p.part_stat[(static_cast<long long>(w.part) * 2 + tile) * p.part_rows + r] = make_float2(m_used, l);
+                    }
+                }
+                __nv_bfloat16* o_row = p.out + ((static_cast<long long>(w.q_begin) + token) * p.c.heads_q +
+                                                w.head * p.c.group + row_head) * kHeadDim;
+                float4* part = p.part_o + (static_cast<long long>(w.part) * 2 + tile) * 32 * p.part_rows + r;
+                const int from = two ? 0 : 2 * x, to = two ? 4 : 2 * x + 2;
+#pragma unroll 1
+                for (int c = from; c < to; ++c) {
+                    uint32_t t[32];
+                    if (two) {
+                        tmem_ld_x32(o_tmem + x * 128 + c * 32, t);
+                        tmem_wait_ld();
+                    } else {
+                        tmem_ld_x32(o_tmem + c * 32, t);
+                        tmem_wait_ld();
+                        if (w.blocks > 1) {
+                            uint32_t t1[32];
+                            tmem_ld_x32(o_tmem + 128 + c * 32, t1);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                t[e] = __float_as_uint(fmaf(__uint_as_float(t1[e]), a1, __uint_as_float(t[e]) * a0));
+                            }
+                        }
+                    }
+                    if (!row_valid) continue;
+                    if (not_finite) tree_add_not_finite(p, w, token, c * 32, t);
+                    if (whole) {
+                        uint4* dst = reinterpret_cast<uint4*>(o_row + c * 32);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                o[e] = pack_bf16x2(__uint_as_float(t[v * 8 + 2 * e]) * inv, __uint_as_float(t[v * 8 + 2 * e + 1]) * inv);
+                            }
+                            dst[v] = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) {
+                            part[(c * 8 + v) * p.part_rows] = make_float4(__uint_as_float(t[4 * v]), __uint_as_float(t[4 * v + 1]),
+                                                                          __uint_as_float(t[4 * v + 2]), __uint_as_float(t[4 * v + 3]));
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before_sync();
+            if (!two) {
+                // Neither warpgroup's next product may overwrite an O that the other still reads.
+                mbar_arrive(smem_u32(&sh.both_read));
+                ok = mbar_wait(wctx, smem_u32(&sh.both_read), both_cnt & 1u, 17);
+                ++both_cnt;
+                if (!ok) break;
+            }
+            release();
+        }
+    }
+
+    // Common exit: every role arrives here (normally or after an abort).
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kTreeQkWarp) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Adds up the pieces of the items that ends of runs cut, in slot order: O = sum_i w_i O_i / sum_i w_i l_i with
+// w_i = 2^(m_i - max m).  CTA (i, strip) looks after the item that run i + 1 begins inside of, if it is the first to do so,
+// and 32 rows of it.
+// ---------------------------------------------------------------------------------------
+constexpr int kTreeStrip = 32;
+
+__global__ void __launch_bounds__(256)
+tree_combine(const __grid_constant__ TreeParams p) {
+    constexpr int kPitch = kHeadDim + 4;    // bf16; keeps the 8-byte column stores of 16 rows on distinct banks
+    __shared__ __align__(8) __nv_bfloat16 out[kTreeStrip * kPitch];
+    __shared__ float weight[kTreeMaxCtas][kTreeStrip];
+    let_next_kernel_start();
+    wait_for_previous_kernel();
+    const int cta = blockIdx.x + 1;
+    const int strips = (p.part_rows + kTreeStrip - 1) / kTreeStrip;
+    const int tile = blockIdx.y / strips;
+    const int row0 = blockIdx.y % strips * kTreeStrip;
+    const TreeCut cut = p.cuts[cta];
+    if (cut.run == 0 || cut.first < static_cast<long long>(cta - 1) * cut.run) return;   // none, or not the first run inside
+    const int tok0 = cut.tok0 + tile * p.tile_tokens;
+    const int rows = min(min(p.tile_tokens, cut.n - tok0) * p.c.group - row0, kTreeStrip);
+    if (rows <= 0) return;
+    const int pieces = static_cast<int>((cut.last - 1) / cut.run) - (cta - 1) + 1;
+    // The first piece ends run cta - 1 (and may begin it); the others begin their runs.
+    auto part_of = [&](int i) -> long long {
+        const int second = i == 0 && cut.first > static_cast<long long>(cta - 1) * cut.run;
+        return (2ll * (cta - 1 + i) + second) * 2 + tile;
+    };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (warp == 0 && lane < rows) {
+        float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < pieces; ++i) m = fmaxf(m, p.part_stat[part_of(i) * p.part_rows + row0 + lane].x);
+        for (int i = 0; i < pieces; ++i) {
+            const float2 st = p.part_stat[part_of(i) * p.part_rows + row0 + lane];
+            const float f = st.x == m ? 1.f : fast_exp2((st.x - m) * p.scale_log2);
+            weight[i][lane] = f;
+            l = fmaf(st.y, f, l);
+        }
+        const float norm = l == 0.f ? 0.f : 1.f / l;
+        for (int i = 0; i < pieces; ++i) weight[i][lane] *= norm;
+        const int r = row0 + lane, token = tok0 + r / p.c.group;
+        p.lse[cut.seq * p.lse_seq_stride + (cut.head * p.c.group + r % p.c.group) * p.lse_head_stride +
+              (p.c.cu_seqlens_q == nullptr ? token : cut.q_begin + token)] =
+            l == 0.f ? -INFINITY : (m * p.scale_log2 + fast_log2(l)) * kLn2;
+    }
+    __syncthreads();
+    // Lane = row, four of the 32 column quads a warp.
+    if (lane < rows) {
+        float4 acc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int i = 0; i < pieces; ++i) {
+            const float f = weight[i][lane];
+            const float4* o = p.part_o + (part_of(i) * 32 + warp * 4) * p.part_rows + row0 + lane;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float4 v = __ldcs(o + u * p.part_rows);
+                acc[u].x = fmaf(v.x, f, acc[u].x);
+                acc[u].y = fmaf(v.y, f, acc[u].y);
+                acc[u].z = fmaf(v.z, f, acc[u].z);
+                acc[u].w = fmaf(v.w, f, acc[u].w);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            *reinterpret_cast<uint2*>(&out[lane * kPitch + (warp * 4 + u) * 4]) =
+                make_uint2(pack_bf16x2(acc[u].x, acc[u].y), pack_bf16x2(acc[u].z, acc[u].w));
+        }
+    }
+    __syncthreads();
+    // A warp writes one whole 256-byte row per instruction.
+    for (int rr = warp; rr < rows; rr += 8) {
+        const int r = row0 + rr;
+        const long long to = (static_cast<long long>(cut.q_begin) + tok0 + r / p.c.group) * p.c.heads_q +
+                             cut.head * p.c.group + r % p.c.group;
+        *reinterpret_cast<uint2*>(p.out + to * kHeadDim + lane * 4) = *reinterpret_cast<const uint2*>(&out[rr * kPitch + lane * 4]);
+    }
+}
+
+int set_tree_smem() {
+    B2A_CUDA_OK(cudaFuncSetAttribute(tree_attention, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTreeSmemBytes)));
+    return B2A_OK;
+}
+
+struct TreeLayout {
+    int ctas, tile_tokens, tiles, rows;
+    size_t cuts, stat, o, total;   // offsets
+};
+
+TreeLayout tree_layout(const b2a_tree_args& a, int sms) {
+    TreeLayout t{};
+    const int group = a.heads_q / a.cache.heads_k;
+    t.ctas = sms < kTreeMaxCtas ? sms : kTreeMaxCtas;
+    t.tile_tokens = kTileM / group;
+    t.tiles = a.seqlen_q > t.tile_tokens ? 2 : 1;
+    t.rows = (t.tiles == 2 ? t.tile_tokens : a.seqlen_q) * group;
+    t.cuts = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
+    t.stat = t.cuts + align_up(t.ctas * sizeof(TreeCut), 256);
+    t.o = t.stat + align_up(4ull * t.ctas * t.rows * sizeof(float2), 256);
+    t.total = t.o + 4ull * t.ctas * t.rows * kHeadDim * sizeof(float);
+    return t;
+}
+
+}  // namespace
+
+}  // namespace b2a
+
+extern "C" {
+
+size_t b2a_tree_fwd_workspace_bytes(const b2a_tree_args* a) {
+    using namespace b2a;
+    DeviceInfo dev{};
+    if (a == nullptr || a->cache.heads_k < 1 || a->heads_q < a->cache.heads_k || a->heads_q % a->cache.heads_k != 0 ||
+        a->heads_q / a->cache.heads_k > kTileM || a->seqlen_q < 1 || current_device_info(&dev) != B2A_OK) {
+        return 0;   // b2a_tree_fwd reports what is wrong
+    }
+    return tree_layout(*a, dev.sm_count).total;
+}
+
+int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
+    using namespace b2a;
+    B2A_REQUIRE(a != nullptr, "args must not be NULL");
+    TreeParams p{};
+    int rc = make_cache_queries(*a, true, &p.c);
+    if (rc != B2A_OK) return rc;
+    B2A_REQUIRE(a->out != nullptr && (reinterpret_cast<uintptr_t>(a->out) & 0xF) == 0, "out must be a 16-byte aligned device pointer");
+    B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
+                "workspace must be a 16-byte aligned device pointer");
+    DeviceInfo dev{};
+    rc = current_device_info(&dev);
+    if (rc != B2A_OK) return rc;
+    const TreeLayout t = tree_layout(*a, dev.sm_count);
+    if (a->workspace_bytes < t.total) {
+        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, t.total);
+    }
+    p.c.item_tokens = 2 * t.tile_tokens;
+    p.c.min_run = 2;
+    p.box_rows = slot_box_rows(p.c.cache);
+    CUtensorMap map_q, map_k, map_v;
+    const uint64_t q_sizes[2] = {static_cast<uint64_t>(a->total_q), static_cast<uint64_t>(a->heads_q)};
+    rc = make_strided_map(&map_q, a->q, 3, q_sizes, a->q_stride, static_cast<uint32_t>(p.c.group), static_cast<uint32_t>(t.tile_tokens));
+    if (rc == B2A_OK) rc = make_slot_map(&map_k, p.c.cache, true, p.box_rows);
+    if (rc == B2A_OK) rc = make_slot_map(&map_v, p.c.cache, false, p.box_rows);
+    if (rc == B2A_OK) rc = once_per_device(dev.device, 6, set_tree_smem);
+    if (rc != B2A_OK) return rc;
+
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.lse = a->lse;
+    p.lse_head_stride = a->cu_seqlens_q == nullptr ? a->seqlen_q : a->total_q;
+    p.lse_seq_stride = a->cu_seqlens_q == nullptr ? static_cast<long long>(a->heads_q) * a->seqlen_q : 0;
+    p.tile_tokens = t.tile_tokens;
+    p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / std::sqrt(static_cast<float>(kHeadDim))) * kLog2e;
+    p.status = reinterpret_cast<unsigned int*>(reinterpret_cast<WorkspaceHeader*>(ws) + 1);
+    p.timeout_ns = wait_timeout_ns();
+    p.cuts = reinterpret_cast<TreeCut*>(ws + t.cuts);
+    p.part_stat = reinterpret_cast<float2*>(ws + t.stat);
+    p.part_o = reinterpret_cast<float4*>(ws + t.o);
+    p.part_rows = t.rows;
+
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    auto attention = tree_attention;
+    auto combine = tree_combine;
+    B2A_CUDA_OK(launch_early(attention, t.ctas, kTreeThreads, kTreeSmemBytes, stream, map_q, map_k, map_v, p));
+    const int strips = t.tiles * ((t.rows + kTreeStrip - 1) / kTreeStrip);
+    if (t.ctas > 1) B2A_CUDA_OK(launch_early(combine, dim3(t.ctas - 1, strips), 256, 0, stream, p));
+    return B2A_OK;
+}
+
+}  // extern "C"

@@ -36,6 +36,7 @@ __all__ = [
     "RotaryAxes",
     "rotary",
     "append_cache",
+    "forward_tree",
 ]
 
 _INT32_MAX = 2**31 - 1
@@ -545,7 +546,7 @@ _RING_EXPORTS = ("backward_varlen_mega_ring", "forward_varlen_mega_ring", "forwa
 
 
 _ROTARY_EXPORTS = ("RotaryAxes", "rotary")
-_CACHE_EXPORTS = ("append_cache",)
+_CACHE_EXPORTS = ("append_cache", "forward_tree")
 
 
 def __getattr__(name: str):
