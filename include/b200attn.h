@@ -467,6 +467,44 @@ size_t b2a_tree_fwd_workspace_bytes(const b2a_tree_args* args);
  */
 int b2a_tree_fwd(const b2a_tree_args* args, void* cuda_stream);
 
+/* Scratch of b2a_cache_weights. */
+size_t b2a_cache_weights_workspace_bytes(void);
+
+/*
+ * What attention each slot received: weights[b][h][s] += the sum over the rows of K/V head h that see slot s of
+ * exp(softmax_scale q k - lse), with the lse that b2a_tree_fwd gave.  Arguments as there (v, out unused); rows with lse = -inf or
+ * +inf add nothing.  weights_slots may be fewer than the cache has: sequences must then not be longer.  Slots behind a
+ * sequence are left as they were.  Repeated calls add the same bits.
+ */
+int b2a_cache_weights(const b2a_tree_args* args, void* cuda_stream);
+
+typedef struct b2a_evict_args {
+    b2a_cache cache;
+    const int32_t* cache_lens;  /* device int32 [batch] */
+    const float* weights;       /* fp32 [batch, heads_k, weights_slots] */
+    int64_t weights_stride[2];  /* elements from sequence to sequence, head to head */
+    int32_t batch;
+    int32_t weights_slots;
+    int32_t budget;             /* slots that a sequence keeps */
+    int32_t recent;             /* how many of them are its last ones */
+    int32_t* new_lens;          /* device int32 [batch]: min(cache_lens, budget) */
+    float* new_weights;         /* contiguous [batch, heads_k, weights_slots]; 0 behind new_lens */
+    int32_t* index;             /* contiguous [batch, heads_k, budget]: the slot that each slot's contents come from; -1 behind new_lens */
+    void* workspace;
+    size_t workspace_bytes;
+} b2a_evict_args;
+
+/* Scratch of b2a_cache_evict; looks at batch, budget and cache.heads_k. */
+size_t b2a_cache_evict_workspace_bytes(const b2a_evict_args* args);
+
+/*
+ * Cuts sequences that are longer than the budget down to it, in place, for each K/V head by itself: the last `recent` slots stay,
+ * and the budget - recent of the others with the largest weights (equal ones: the lower slot; NaN counts as largest).  Heavy slots
+ * below budget - recent keep their place, the gaps are filled with the heavy ones from behind, in ascending order of both, and
+ * the last ones follow in their order.  Pages must not be shared between sequences.  cache_lens and weights are not changed.
+ */
+int b2a_cache_evict(const b2a_evict_args* args, void* cuda_stream);
+
 /* ------------------------------------------------------------------------- */
 /* Device status                                                              */
 /* ------------------------------------------------------------------------- */

@@ -263,6 +263,26 @@ class TreeArgs(Structure):
     ]
 
 
+class EvictArgs(Structure):
+    """Mirror of ``b2a_evict_args``."""
+
+    _fields_ = [
+        ("cache", Cache),
+        ("cache_lens", c_void_p),
+        ("weights", c_void_p),
+        ("weights_stride", c_int64 * 2),
+        ("batch", c_int32),
+        ("weights_slots", c_int32),
+        ("budget", c_int32),
+        ("recent", c_int32),
+        ("new_lens", c_void_p),
+        ("new_weights", c_void_p),
+        ("index", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 # symbol -> (restype, argtypes); must list every function include/b200attn.h declares.
 SIGNATURES = {
     "b2a_abi_version": (c_int32, []),
@@ -290,6 +310,10 @@ SIGNATURES = {
     "b2a_cache_append": (c_int32, [POINTER(AppendArgs), c_void_p]),
     "b2a_tree_fwd_workspace_bytes": (c_size_t, [POINTER(TreeArgs)]),
     "b2a_tree_fwd": (c_int32, [POINTER(TreeArgs), c_void_p]),
+    "b2a_cache_weights_workspace_bytes": (c_size_t, []),
+    "b2a_cache_weights": (c_int32, [POINTER(TreeArgs), c_void_p]),
+    "b2a_cache_evict_workspace_bytes": (c_size_t, [POINTER(EvictArgs)]),
+    "b2a_cache_evict": (c_int32, [POINTER(EvictArgs), c_void_p]),
     "b2a_check_status": (c_int32, [c_void_p, c_void_p]),
     "b2a_set_wait_timeout_ns": (c_int32, [ctypes.c_uint64]),
     "b2a_profile_enable": (c_int32, [c_int32]),

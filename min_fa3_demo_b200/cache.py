@@ -25,7 +25,7 @@ from .min_fa3_op import (_INT32_MAX, _SM100, _check, _check_device_capability, _
                          _workspace)
 from .rotary import RotaryAxes, _check_heads, _check_positions, _position_strides, _rows
 
-__all__ = ["append_cache", "forward_tree"]
+__all__ = ["append_cache", "forward_tree", "cache_weights", "evict_cache"]
 
 _NONE3 = (0, 0, 0)
 
@@ -227,3 +227,92 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         _cabi.check(lib.b2a_tree_fwd(ref, _stream_ptr(device)))
     _remember_workspace("forward_tree", ws)
     return (out, lse) if return_lse else out
+
+
+def _check_weights(weights: torch.Tensor, batch: int, k_cache: torch.Tensor) -> None:
+    kvh = k_cache.size(2)
+    _check(weights.device == k_cache.device, "weights must be on the same CUDA device as the cache")
+    _check(weights.dtype == torch.float32, "weights must have dtype torch.float32")
+    _check(weights.dim() == 3 and weights.size(0) == batch and weights.size(1) == kvh and weights.size(2) > 0,
+           f"weights must have shape [{batch}, {kvh}, slots]. Got {list(weights.shape)}")
+    _check(weights.size(2) == 1 or weights.stride(2) == 1, "the rows of weights must be contiguous")
+
+
+def cache_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, cache_lens: torch.Tensor, weights: torch.Tensor, *,
+                  block_table: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[torch.Tensor] = None,
+                  max_seqlen_q: Optional[int] = None, tree_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adds to ``weights`` ``[B, KVH, slots]`` (fp32), in place, the attention that each slot received, and returns it.
+
+    ``weights[b, h, s]`` grows by the sum of ``exp(q k / sqrt(128) - lse)`` over the rows of K/V head ``h`` that see slot ``s``; the
+    other arguments, and which slots a row sees, are those of the :func:`forward_tree` call that returned ``lse``.  Rows
+    whose lse is infinite add nothing: to leave out drafted tokens that were not accepted, set theirs to infinity.  Slots behind a
+    sequence are left as they were.  What does not fit is reported by ``check_last_status("cache_weights")``.
+    """
+    _check_cache(k_cache, "k_cache")
+    device = k_cache.device
+    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", device)
+    _check_table(block_table, k_cache, batch)
+    total, most, mask_stride = _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
+    shape = (batch, q.size(2), most) if q.dim() == 4 else (q.size(1), total)
+    _check(lse.device == device and lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == shape,
+           f"lse must be a contiguous torch.float32 tensor of shape {list(shape)} on the same CUDA device as the cache")
+    _check_weights(weights, batch, k_cache)
+    _check(all(n == 1 or s > 0 for n, s in zip(weights.shape, weights.stride())), "weights must not be expanded")
+    if device.index not in _SM100:
+        _check_device_capability(device, "min_fa3_demo_b200 cache_weights")
+    if q.numel() == 0:
+        return weights
+    lib = _cabi.load()
+    args = _cabi.TreeArgs(
+        _cache_fields(k_cache, None, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+        q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), 0, lse.data_ptr(), _token_strides(q), mask_stride, batch,
+        most, total, q.size(-2), 0.0, weights.data_ptr(), weights.stride()[:2], weights.size(2))
+    with _on_device(device):
+        nbytes = lib.b2a_cache_weights_workspace_bytes()
+        ws = _workspace(nbytes, device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        _cabi.check(lib.b2a_cache_weights(ctypes.byref(args), _stream_ptr(device)))
+    _remember_workspace("cache_weights", ws)
+    return weights
+
+
+def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, cache_lens: torch.Tensor, budget: int, *,
+                recent: int = 0, block_table: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts sequences longer than ``budget`` slots down to it, in place, each K/V head by itself.
+
+    The last ``recent`` slots stay, and of the others the ``budget - recent`` with the largest ``weights`` ``[B, KVH, slots]`` (equal
+    ones: the lower slot; NaN counts as largest).  Returns ``(lens, weights, index)``: the new ``cache_lens`` ``[B]``, the
+    weights in the new order (0 behind the new length), and for each slot the slot that its contents come from,
+    ``[B, KVH, budget]`` (int32, -1 behind the new length), for whatever else the caller keeps by slot.  Heavy slots below
+    ``budget - recent`` keep their place, the gaps are filled in ascending order with the heavy ones from behind, and the last
+    ones follow in their order.  Sequences within the budget stay as they are.  Pages must not be shared between sequences.
+    Lengths and pages that do not exist are reported by ``check_last_status("evict_cache")``.
+    """
+    _check_pair(k_cache, v_cache)
+    device = k_cache.device
+    batch = _check_lens(cache_lens, None, "", device)
+    _check_table(block_table, k_cache, batch)
+    _check_weights(weights, batch, k_cache)
+    budget, recent = int(budget), int(recent)
+    _check(0 < budget <= _INT32_MAX, f"budget must be positive. Got {budget}")
+    _check(0 <= recent <= budget, f"recent must be between 0 and the budget. Got {recent}")
+    kvh = k_cache.size(2)
+    _check(batch * kvh <= 65535, f"at most 65535 sequences times KV heads. Got {batch} times {kvh}")
+    if device.index not in _SM100:
+        _check_device_capability(device, "min_fa3_demo_b200 evict_cache")
+    lib = _cabi.load()
+    lens = torch.empty(batch, dtype=torch.int32, device=device)
+    new_weights = torch.empty(weights.shape, dtype=torch.float32, device=device)
+    index = torch.empty((batch, kvh, budget), dtype=torch.int32, device=device)
+    args = _cabi.EvictArgs(
+        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), weights.data_ptr(), weights.stride()[:2], batch,
+        weights.size(2), budget, recent, lens.data_ptr(), new_weights.data_ptr(), index.data_ptr())
+    ref = ctypes.byref(args)
+    with _on_device(device):
+        nbytes = lib.b2a_cache_evict_workspace_bytes(ref)
+        ws = _workspace(nbytes, device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        _cabi.check(lib.b2a_cache_evict(ref, _stream_ptr(device)))
+    _remember_workspace("evict_cache", ws)
+    return lens, new_weights, index

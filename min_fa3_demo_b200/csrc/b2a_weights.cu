@@ -1,0 +1,415 @@
+// What attention the slots of a cache received: w[b, h, slot] += sum over the rows of K/V head h that see the slot of
+// exp(scale q k - lse).
+//
+// The scores are made the other way round than for attention, S^T = K Q^T: a thread has a slot, its row of tensor memory the
+// scores of all query rows with it, and the sum is its own.  No slot is shared by two threads or CTAs, so nothing is reduced
+// between them and repeated calls give the same bits.  K is streamed once where the rows of a sequence fit two tiles of
+// 128 (256 bytes a slot and head: bound by memory for up to some 128 rows, by the exponentials beyond); of more rows, two
+// tiles' worth at a time go over the same few blocks, which then come from L2, and the sums wait in shared memory.
+//
+//   warp 0-3, 4-7   sums, the two groups take turns at the blocks
+//   warp 8          K Q^T       warp 9   plan and TMA loads       warp 10, 11   idle
+//
+// Tensor memory (512 columns): two S^T for each group of warps, 128 columns each.
+#include "b2a_cache.cuh"
+
+#include <cmath>
+
+namespace b2a {
+
+namespace {
+
+constexpr int kWeightThreads = 384;
+constexpr int kWeightKStages = 3, kWeightQSlots = 3;
+constexpr int kWeightChunk = 16;      // blocks that several passes of query tiles go over
+constexpr int kWeightSlots = 4;       // pieces in flight
+constexpr int kWeightMmaWarp = 8, kWeightLoadWarp = 9;
+
+struct WeightParams {
+    CacheQueries c;
+    const float* lse;
+    long long lse_seq_stride, lse_head_stride;
+    float* weights;
+    long long weights_stride[2];
+    int tile_tokens;
+    int box_rows;
+    float scale_log2;
+    unsigned int* status;
+    uint32_t timeout_ns;
+};
+
+struct WeightPiece {
+    int valid;
+    int seq, q_begin, n, len, slots, head;
+    int j0, blocks;      // at most kWeightChunk
+};
+
+struct __align__(1024) WeightShared {
+    uint8_t q[kWeightQSlots][kTileBytes];
+    uint8_t k[kWeightKStages][kTileBytes];
+    float lse2[kWeightQSlots][kTileM];          // lse * log2(e) of a tile's rows
+    uint32_t live[kWeightQSlots][4];            // a bit for each row that exists and has a finite lse: the others give nothing
+    float sums[kWeightChunk][kTileM];
+    WeightPiece piece[kWeightSlots];
+    uint64_t q_full[kWeightQSlots], q_empty[kWeightQSlots];
+    uint64_t k_full[kWeightKStages], k_empty[kWeightKStages];
+    uint64_t s_full[4], s_empty[4];
+    uint64_t piece_full[kWeightSlots], piece_empty[kWeightSlots];
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+};
+
+constexpr size_t kWeightSmemBytes = sizeof(WeightShared) + 1024;
+static_assert(kWeightSmemBytes <= 227 * 1024, "shared memory of a CTA");
+
+__device__ __forceinline__ int weight_tiles(const WeightParams& p, int n) { return (n + p.tile_tokens - 1) / p.tile_tokens; }
+
+__global__ void __launch_bounds__(kWeightThreads, 1)
+tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+             const __grid_constant__ WeightParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    WeightShared& sh = *reinterpret_cast<WeightShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kWeightQSlots; ++i) {
+            mbar_init(smem_u32(&sh.q_full[i]), 1);
+            mbar_init(smem_u32(&sh.q_empty[i]), 1 + 8);      // the products, and the warps that read lse2
+        }
+        for (int i = 0; i < kWeightKStages; ++i) {
+            mbar_init(smem_u32(&sh.k_full[i]), 1);
+            mbar_init(smem_u32(&sh.k_empty[i]), 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&sh.s_full[i]), 1);
+            mbar_init(smem_u32(&sh.s_empty[i]), 4);
+        }
+        for (int i = 0; i < kWeightSlots; ++i) {
+            mbar_init(smem_u32(&sh.piece_full[i]), 1);
+            mbar_init(smem_u32(&sh.piece_empty[i]), 1 + 8);
+        }
+        sh.abort_flag = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == kWeightMmaWarp) {
+        tmem_alloc(smem_u32(&sh.tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+    }
+    let_next_kernel_start();
+    wait_for_previous_kernel();
+    if (threadIdx.x == 0) {
+        p.status[blockIdx.x] = 0u;
+        if (blockIdx.x == 0) reinterpret_cast<int4*>(p.status)[-1] = make_int4(-static_cast<int>(gridDim.x), 0, 0, 0);
+    }
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
+    const WaitCtx wctx{smem_u32(&sh.abort_flag), p.status, p.timeout_ns, 1u};
+
+    // All roles go through the same order: pieces, pairs of query tiles, blocks, tiles of the pair.
+    if (warp == kWeightLoadWarp) {
+        if (lane == 0) {
+            tma_prefetch_desc(&map_q);
+            tma_prefetch_desc(&map_k);
+        }
+        CacheWalk walk;
+        walk.start(p.c, blockIdx.x, gridDim.x, lane);
+        SlotLoader loader{p.box_rows, kSlotBlock / p.box_rows, 0, 0, walk.bad};
+        uint32_t q_it = 0, k_it = 0;
+        bool ok = true;
+        for (uint32_t it = 0; ok; ++it) {
+            const uint32_t at = it % kWeightSlots;
+            ok = mbar_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kWeightSlots) & 1u) ^ 1u, 1);
+            if (!ok) break;
+            WeightPiece w{};
+            w.valid = walk.pos < walk.end;
+            if (w.valid) {
+                w.seq = walk.seq;
+                w.q_begin = walk.s.q_begin;
+                w.n = walk.s.n;
+                w.len = walk.s.len;
+                w.slots = walk.s.slots;
+                w.head = walk.head;
+                w.j0 = walk.j;
+                w.blocks = min(walk.piece(), kWeightChunk);
+            }
+            if (lane == 0) {
+                sh.piece[at] = w;
+                mbar_arrive(smem_u32(&sh.piece_full[at]));
+            }
+            if (!w.valid) break;
+            const int tiles = weight_tiles(p, w.n);
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
+                for (int tile = tile0; tile < min(tile0 + 2, tiles); ++tile, ++q_it) {
+                    const uint32_t slot = q_it % kWeightQSlots;
+                    ok = mbar_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
+                    if (!ok) break;
+                    const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, w.n - tok0) * p.c.group;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int r = c * 32 + lane;
+                        float lse = INFINITY;
+                        if (r < rows) {
+                            const int token = tok0 + r / p.c.group, head = w.head * p.c.group + r % p.c.group;
+                            lse = p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
+                                        (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)];
+                        }
+                        const bool live = !isinf(lse);
+                        sh.lse2[slot][r] = live ? lse * kLog2e : 0.f;
+                        const uint32_t bits = __ballot_sync(0xFFFFFFFFu, live);
+                        if (lane == 0) sh.live[slot][c] = bits;
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        const uint32_t bar = smem_u32(&sh.q_full[slot]), dst = smem_u32(&sh.q[slot][0]);
+                        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.tile_tokens * p.c.group) * 256u);
+                        tma_load_3d(dst, &map_q, bar, 0, w.head * p.c.group, w.q_begin + tok0);
+                        tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, w.head * p.c.group, w.q_begin + tok0);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
+                for (int i = 0; i < w.blocks; ++i, ++k_it) {
+                    const SlotLoader now = loader;
+                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+                    const uint32_t stage = k_it % kWeightKStages;
+                    ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
+                    if (!ok) break;
+                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, now.count(w.j0 + i, w.slots), lane);
+                }
+            }
+            if (!ok) break;
+            walk.advance(p.c, w.blocks);
+        }
+        if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
+    } else if (warp == kWeightMmaWarp) {
+        constexpr uint32_t kStep = kTileBytes >> 4;
+        const uint32_t q_lo0 = desc_lo_kmajor(smem_u32(&sh.q[0][0]));
+        const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0]));
+        uint32_t q_it = 0, k_it = 0;
+        uint32_t s_it[2] = {0, 0};
+        bool ok = true;
+        for (uint32_t it = 0; ok; ++it) {
+            const uint32_t at = it % kWeightSlots;
+            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 4);
+            if (!ok) break;
+            const volatile WeightPiece& w = sh.piece[at];
+            const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
+            const int blocks = __shfl_sync(0xFFFFFFFFu, w.blocks, 0);
+            const int n = __shfl_sync(0xFFFFFFFFu, w.n, 0);
+            if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+            __syncwarp();
+            if (!valid) break;
+            const int tiles = weight_tiles(p, n);
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
+                const int here = min(2, tiles - tile0);
+                for (int i = 0; i < blocks && ok; ++i, ++k_it) {
+                    const uint32_t stage = k_it % kWeightKStages;
+                    ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), (k_it / kWeightKStages) & 1u, 5);
+                    if (!ok) break;
+                    const uint32_t x = i & 1;
+                    for (int t = 0; t < here; ++t) {
+                        const uint32_t slot = (q_it + t) % kWeightQSlots;
+                        if (i == 0) {
+                            ok = mbar_wait(wctx, smem_u32(&sh.q_full[slot]), ((q_it + t) / kWeightQSlots) & 1u, 6);
+                            if (!ok) break;
+                        }
+                        const uint32_t count = x ? s_it[1]++ : s_it[0]++;
+                        const uint32_t buf = 2 * x + (count & 1u);
+                        ok = mbar_wait(wctx, smem_u32(&sh.s_empty[buf]), ((count >> 1) & 1u) ^ 1u, 7);
+                        if (!ok) break;
+                        // As many columns as the tile has rows, in steps of 16.
+                        const int rows = min(p.tile_tokens, n - (tile0 + t) * p.tile_tokens) * p.c.group;
+                        const uint32_t idesc = make_idesc_bf16(kTileM, (rows + 15) & ~15, 0, 0);
+                        tc_fence_after_sync();
+                        umma_ss_kk_x8_w(tmem_base + buf * 128u, k_lo0 + stage * kStep, q_lo0 + slot * kStep, idesc, 0u);
+                        tc_commit_w(smem_u32(&sh.s_full[buf]));
+                        if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[slot]));
+                        __syncwarp();
+                    }
+                    tc_commit_w(smem_u32(&sh.k_empty[stage]));
+                }
+                q_it += here;
+            }
+        }
+    } else if (warp < 8) {
+        const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t s_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const float sl2 = p.scale_log2;
+        uint32_t q_it = 0, s_it = 0;
+        bool ok = true;
+        for (uint32_t it = 0; ok; ++it) {
+            const uint32_t at = it % kWeightSlots;
+            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 8);
+            if (!ok) break;
+            const WeightPiece& w = sh.piece[at];
+            if (!w.valid) break;
+            const int tiles = weight_tiles(p, w.n);
+            float* out = p.weights + w.seq * p.weights_stride[0] + w.head * p.weights_stride[1];
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
+                const int here = min(2, tiles - tile0);
+                const bool last = tile0 + 2 >= tiles;
+                for (int i = x; i < w.blocks; i += 2) {
+                    const int slot = (w.j0 + i) * kSlotBlock + r;
+                    const bool tail = (w.j0 + i + 1) * kSlotBlock > w.len;
+                    float before = 0.f;
+                    if (last && slot < w.slots) before = out[slot];
+                    float sum = tile0 == 0 ? 0.f : sh.sums[i][r];
+                    for (int t = 0; t < here; ++t, ++s_it) {
+                        const uint32_t buf = 2 * x + (s_it & 1u), q_slot = (q_it + t) % kWeightQSlots;
+                        const int tok0 = (tile0 + t) * p.tile_tokens, tokens = min(p.tile_tokens, w.n - tok0);
+                        const int rows = tokens * p.c.group;
+                        // Which columns see this slot: all of them before the drafted tokens.
+                        uint32_t bits[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                        const int u = slot - w.len;
+                        if (tail && u >= 0) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) bits[c] = 0u;
+                            if (slot < w.slots) {
+                                const unsigned char* mask = p.c.mask;
+                                if (mask != nullptr) {
+                                    mask += (p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + tok0 * p.c.mask_stride[1]
+                                                                         : (static_cast<long long>(w.q_begin) + tok0) * p.c.mask_stride[1]) + u;
+                                }
+#pragma unroll 4
+                                for (int k = 0; k < tokens; ++k) {
+                                    if (mask == nullptr ? u > tok0 + k : mask[k * p.c.mask_stride[1]] == 0) continue;
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c) {
+                                        const int lo = min(max(k * p.c.group - 32 * c, 0), 32);
+                                        const int hi = min(max((k + 1) * p.c.group - 32 * c, 0), 32);
+                                        const uint32_t below_hi = hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u;
+                                        const uint32_t below_lo = lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u;
+                                        bits[c] |= below_hi & ~below_lo;
+                                    }
+                                }
+                            }
+                        }
+                        ok = mbar_wait(wctx, smem_u32(&sh.s_full[buf]), (s_it >> 1) & 1u, 9);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            if (c * 32 >= rows) break;
+                            uint32_t s[32];
+                            tmem_ld_x32(s_tmem + buf * 128u + c * 32, s);
+                            tmem_wait_ld();
+                            const uint32_t see = bits[c] & sh.live[q_slot][c];
+                            const bool all = __all_sync(0xFFFFFFFFu, see == 0xFFFFFFFFu);
+                            const float4* lse2 = reinterpret_cast<const float4*>(&sh.lse2[q_slot][c * 32]);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if (c * 32 + e * 4 >= rows) break;
+                                const float4 l4 = lse2[e];
+                                float2 p0 = fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])),
+                                                 make_float2(sl2, sl2), make_float2(-l4.x, -l4.y));
+                                float2 p1 = fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])),
+                                                 make_float2(sl2, sl2), make_float2(-l4.z, -l4.w));
+                                p0 = make_float2(fast_exp2(p0.x), fast_exp2(p0.y));
+                                p1 = make_float2(fast_exp2(p1.x), fast_exp2(p1.y));
+                                if (!all) {
+                                    if (!((see >> (4 * e)) & 1u)) p0.x = 0.f;
+                                    if (!((see >> (4 * e + 1)) & 1u)) p0.y = 0.f;
+                                    if (!((see >> (4 * e + 2)) & 1u)) p1.x = 0.f;
+                                    if (!((see >> (4 * e + 3)) & 1u)) p1.y = 0.f;
+                                }
+                                acc[0] = add2(acc[0], p0);
+                                acc[1] = add2(acc[1], p1);
+                            }
+                        }
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sh.s_empty[buf]));
+                        sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+                    }
+                    if (!ok) break;
+                    if (!last) {
+                        sh.sums[i][r] = sum;
+                    } else if (slot < w.slots) {
+                        out[slot] = before + sum;
+                    }
+                }
+                // A warp without a block here has waited for nothing yet: it may give back no tile that is still to come.
+                for (int t = 0; t < here && ok; ++t, ++q_it) {
+                    const uint32_t q_slot = q_it % kWeightQSlots;
+                    ok = mbar_wait(wctx, smem_u32(&sh.q_full[q_slot]), (q_it / kWeightQSlots) & 1u, 10);
+                    __syncwarp();
+                    if (ok && lane == 0) mbar_arrive(smem_u32(&sh.q_empty[q_slot]));
+                }
+            }
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kWeightMmaWarp) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+int set_weight_smem() {
+    B2A_CUDA_OK(cudaFuncSetAttribute(tree_weights, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kWeightSmemBytes)));
+    return B2A_OK;
+}
+
+constexpr size_t kWeightWorkspace = sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int);
+
+}  // namespace
+
+}  // namespace b2a
+
+extern "C" {
+
+size_t b2a_cache_weights_workspace_bytes(void) { return b2a::kWeightWorkspace; }
+
+int b2a_cache_weights(const b2a_tree_args* a, void* cuda_stream) {
+    using namespace b2a;
+    B2A_REQUIRE(a != nullptr, "args must not be NULL");
+    WeightParams p{};
+    int rc = make_cache_queries(*a, false, &p.c);
+    if (rc != B2A_OK) return rc;
+    B2A_REQUIRE(a->weights != nullptr && a->weights_slots >= 1, "weights must not be NULL or empty");
+    B2A_REQUIRE(a->weights_stride[0] >= 0 && a->weights_stride[1] >= 0, "strides of weights must not be negative");
+    B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
+                "workspace must be a 16-byte aligned device pointer");
+    if (a->workspace_bytes < kWeightWorkspace) {
+        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, kWeightWorkspace);
+    }
+    DeviceInfo dev{};
+    rc = current_device_info(&dev);
+    if (rc != B2A_OK) return rc;
+    p.tile_tokens = kTileM / p.c.group;
+    p.c.item_tokens = a->seqlen_q;               // all rows of a sequence are one item
+    p.c.min_run = 1;
+    p.c.limit_slots = std::min(p.c.limit_slots, a->weights_slots);
+    p.box_rows = slot_box_rows(p.c.cache);
+    CUtensorMap map_q, map_k;
+    const uint64_t q_sizes[2] = {static_cast<uint64_t>(a->total_q), static_cast<uint64_t>(a->heads_q)};
+    rc = make_strided_map(&map_q, a->q, 3, q_sizes, a->q_stride, static_cast<uint32_t>(p.c.group), static_cast<uint32_t>(p.tile_tokens));
+    if (rc == B2A_OK) rc = make_slot_map(&map_k, p.c.cache, true, p.box_rows);
+    if (rc == B2A_OK) rc = once_per_device(dev.device, 7, set_weight_smem);
+    if (rc != B2A_OK) return rc;
+    p.lse = a->lse;
+    p.lse_head_stride = a->cu_seqlens_q == nullptr ? a->seqlen_q : a->total_q;
+    p.lse_seq_stride = a->cu_seqlens_q == nullptr ? static_cast<long long>(a->heads_q) * a->seqlen_q : 0;
+    p.weights = a->weights;
+    p.weights_stride[0] = a->weights_stride[0];
+    p.weights_stride[1] = a->weights_stride[1];
+    p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / std::sqrt(static_cast<float>(kHeadDim))) * kLog2e;
+    p.status = reinterpret_cast<unsigned int*>(static_cast<WorkspaceHeader*>(a->workspace) + 1);
+    p.timeout_ns = wait_timeout_ns();
+    const int ctas = std::min(dev.sm_count, kFwdStatusWords);
+    auto kernel = tree_weights;
+    B2A_CUDA_OK(launch_early(kernel, ctas, kWeightThreads, kWeightSmemBytes, static_cast<cudaStream_t>(cuda_stream), map_q, map_k, p));
+    return B2A_OK;
+}
+
+}  // extern "C"

@@ -37,6 +37,8 @@ __all__ = [
     "rotary",
     "append_cache",
     "forward_tree",
+    "cache_weights",
+    "evict_cache",
 ]
 
 _INT32_MAX = 2**31 - 1
@@ -546,7 +548,7 @@ _RING_EXPORTS = ("backward_varlen_mega_ring", "forward_varlen_mega_ring", "forwa
 
 
 _ROTARY_EXPORTS = ("RotaryAxes", "rotary")
-_CACHE_EXPORTS = ("append_cache", "forward_tree")
+_CACHE_EXPORTS = ("append_cache", "forward_tree", "cache_weights", "evict_cache")
 
 
 def __getattr__(name: str):
