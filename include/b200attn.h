@@ -454,8 +454,8 @@ typedef struct b2a_tree_args {
     size_t workspace_bytes;
 } b2a_tree_args;
 
-/* Scratch of b2a_tree_fwd on the current device; looks at cache.heads_k, seqlen_q and heads_q. */
-size_t b2a_tree_fwd_workspace_bytes(const b2a_tree_args* args);
+/* Scratch of b2a_tree_fwd on the current device; 0 for sizes that it refuses. */
+size_t b2a_tree_fwd_workspace_bytes(int32_t seqlen_q, int32_t heads_q, int32_t heads_k);
 
 /*
  * Attention of drafted tokens over the cache.  Drafted token i of sequence b lies in slot cache_lens[b] + i already.  Its row
@@ -494,8 +494,8 @@ typedef struct b2a_evict_args {
     size_t workspace_bytes;
 } b2a_evict_args;
 
-/* Scratch of b2a_cache_evict; looks at batch, budget and cache.heads_k. */
-size_t b2a_cache_evict_workspace_bytes(const b2a_evict_args* args);
+/* Scratch of b2a_cache_evict; 0 for sizes that it refuses. */
+size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget);
 
 /*
  * Cuts sequences that are longer than the budget down to it, in place, for each K/V head by itself: the last `recent` slots stay,

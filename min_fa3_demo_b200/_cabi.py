@@ -8,6 +8,7 @@ fails loudly instead of silently computing somewhere else.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -283,6 +284,14 @@ class EvictArgs(Structure):
     ]
 
 
+# The same layouts for struct.pack: filling one of the structures above field by field costs 3.6 us a call, packing it 0.3.
+_CACHE_FORMAT = "3Qq3q3q4i"
+ROTARY = struct.Struct("<6Q3q3q3q6i")
+APPEND = struct.Struct(f"<{_CACHE_FORMAT}8Q3q3q3q3q5i4x2Q")
+TREE = struct.Struct(f"<{_CACHE_FORMAT}6Q2q2q4if4xQ2qi4x2Q")
+EVICT = struct.Struct(f"<{_CACHE_FORMAT}2Q2q4i5Q")
+
+
 # symbol -> (restype, argtypes); must list every function include/b200attn.h declares.
 SIGNATURES = {
     "b2a_abi_version": (c_int32, []),
@@ -306,14 +315,14 @@ SIGNATURES = {
     "b2a_ring_fwd": (c_int32, [POINTER(RingFwdArgs), c_void_p]),
     "b2a_ring_bwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "b2a_ring_bwd": (c_int32, [POINTER(RingBwdArgs), c_void_p]),
-    "b2a_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
-    "b2a_cache_append": (c_int32, [POINTER(AppendArgs), c_void_p]),
-    "b2a_tree_fwd_workspace_bytes": (c_size_t, [POINTER(TreeArgs)]),
-    "b2a_tree_fwd": (c_int32, [POINTER(TreeArgs), c_void_p]),
+    "b2a_rotary": (c_int32, [c_void_p, c_void_p]),
+    "b2a_cache_append": (c_int32, [c_void_p, c_void_p]),
+    "b2a_tree_fwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "b2a_tree_fwd": (c_int32, [c_void_p, c_void_p]),
     "b2a_cache_weights_workspace_bytes": (c_size_t, []),
-    "b2a_cache_weights": (c_int32, [POINTER(TreeArgs), c_void_p]),
-    "b2a_cache_evict_workspace_bytes": (c_size_t, [POINTER(EvictArgs)]),
-    "b2a_cache_evict": (c_int32, [POINTER(EvictArgs), c_void_p]),
+    "b2a_cache_weights": (c_int32, [c_void_p, c_void_p]),
+    "b2a_cache_evict_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "b2a_cache_evict": (c_int32, [c_void_p, c_void_p]),
     "b2a_check_status": (c_int32, [c_void_p, c_void_p]),
     "b2a_set_wait_timeout_ns": (c_int32, [ctypes.c_uint64]),
     "b2a_profile_enable": (c_int32, [c_int32]),

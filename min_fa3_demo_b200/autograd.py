@@ -172,8 +172,8 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
     # Gradients come in any layout (expanded, transposed) and may be lazily negated.
     t = t.resolve_neg()
-    rows = [s for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
-    return t if t.stride(-1) == 1 and not any(s % 8 for s in rows) and t.data_ptr() % 16 == 0 else t.contiguous()
+    st = t.stride()
+    return t if st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0 and t.data_ptr() & 15 == 0 else t.contiguous()
 
 
 class _Rotary(torch.autograd.Function):
@@ -187,15 +187,18 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        # A rotation's gradient is the rotation back, whatever q and k were; through the same function, so that it can be
-        # differentiated again.
+        # A rotation's gradient is the rotation back, whatever q and k were; with create_graph through the same function, so
+        # that it can be differentiated again.
         positions, = ctx.saved_tensors
-        back = not ctx.inverse
-        if dq is None:
-            if dk is not None:
-                dk, _ = _Rotary.apply(dk, None, positions, ctx.axes, back)
-        else:
-            dq, dk = _Rotary.apply(dq, dk, positions, ctx.axes, back)
+
+        def back(a, b):
+            if torch.is_grad_enabled():
+                return _Rotary.apply(a, b, positions, ctx.axes, not ctx.inverse)
+            return _op.rotary(_rows_in_order(a), None if b is None else _rows_in_order(b), positions, ctx.axes, inverse=not ctx.inverse)
+        if dq is not None:
+            dq, dk = back(dq, dk)
+        elif dk is not None:
+            dk, _ = back(dk, None)
         return dq, dk, None, None, None
 
 

@@ -15,7 +15,6 @@ tables live on the device, so the kernels check them: what does not exist is lef
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -23,11 +22,10 @@ import torch
 from . import _cabi
 from .min_fa3_op import (_INT32_MAX, _SM100, _check, _check_device_capability, _on_device, _remember_workspace, _stream_ptr,
                          _workspace)
-from .rotary import RotaryAxes, _check_heads, _check_positions, _position_strides, _rows
+from .rotary import (_BF16, _INT32, _INT64, _NONE3, RotaryAxes, _are_positions, _check_heads, _check_positions, _is_rows, _like,
+                     _position_strides, _rows)
 
 __all__ = ["append_cache", "forward_tree", "cache_weights", "evict_cache"]
-
-_NONE3 = (0, 0, 0)
 
 
 def _check_cache(cache: torch.Tensor, name: str) -> None:
@@ -36,9 +34,32 @@ def _check_cache(cache: torch.Tensor, name: str) -> None:
     _check(cache.dim() == 4, f"{name} must have shape [pages, page_size, KVH, D]")
     _check(cache.size(3) == 128, f"{name} must have head_dim D=128")
     _check(cache.size(0) > 0 and cache.size(1) > 0 and cache.size(2) > 0, f"{name} must not be empty")
-    _check(cache.stride(3) == 1 and not any(s % 8 for s in _rows(cache, 4)) and cache.data_ptr() % 16 == 0,
+    _check(cache.stride(3) == 1 and not any(s & 7 for s in _rows(cache)) and cache.data_ptr() % 16 == 0,
            f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
     _check(all(n == 1 or s > 0 for n, s in zip(cache.shape, cache.stride())), f"{name} must not be expanded")
+
+
+# As in min_fa3_op: one expression asks whether everything is as it should be, and the checks that say what is wrong are gone
+# through only if not.
+def _is_cache(cache: torch.Tensor, index: int) -> bool:
+    st = cache.stride()
+    return _is_rows(cache, 4, index) and st[1] & 7 == 0 and min(st) > 0 and min(cache.shape) > 0
+
+
+def _is_int32(t: torch.Tensor, index: int, n: int) -> bool:
+    return t.dtype is _INT32 and t.get_device() == index and t.dim() == 1 and t.size(0) == n and t.is_contiguous()
+
+
+def _is_table(block_table: Optional[torch.Tensor], k_cache: torch.Tensor, index: int, batch: int) -> bool:
+    if block_table is None:
+        return k_cache.size(0) >= batch
+    return (block_table.dtype is _INT32 and block_table.get_device() == index and block_table.dim() == 2
+            and block_table.size(0) == batch and block_table.size(1) > 0 and block_table.stride(1) == 1 and k_cache.size(1) & 7 == 0)
+
+
+def _is_call(k_cache, cache_lens, block_table, cu_seqlens, index, batch) -> bool:
+    return (index in _SM100 and batch > 0 and _is_cache(k_cache, index) and _is_int32(cache_lens, index, batch)
+            and _is_table(block_table, k_cache, index, batch) and (cu_seqlens is None or _is_int32(cu_seqlens, index, batch + 1)))
 
 
 def _check_int32(t: torch.Tensor, name: str, shape, device) -> None:
@@ -89,11 +110,34 @@ def _check_lens(cache_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], na
 
 
 def _cache_fields(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: Optional[torch.Tensor]):
-    """``b2a_cache`` as a tuple."""
-    table = (0, 0) if block_table is None else (block_table.data_ptr(), block_table.stride(0))
-    v = (0, _NONE3) if v_cache is None else (v_cache.data_ptr(), _rows(v_cache, 4))
-    return (k_cache.data_ptr(), v[0], *table, _rows(k_cache, 4), v[1], k_cache.size(0), k_cache.size(1), k_cache.size(2),
-            1 if block_table is None else block_table.size(1))
+    """``b2a_cache`` for struct.pack."""
+    pages, size, heads, _ = k_cache.shape
+    at, width, step = (0, 1, 0) if block_table is None else (block_table.data_ptr(), block_table.size(1), block_table.stride(0))
+    if v_cache is None:
+        return (k_cache.data_ptr(), 0, at, step, *_rows(k_cache), 0, 0, 0, pages, size, heads, width)
+    return (k_cache.data_ptr(), v_cache.data_ptr(), at, step, *_rows(k_cache), *_rows(v_cache), pages, size, heads, width)
+
+
+def _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes) -> None:
+    _check_pair(k_cache, v_cache)
+    device = k_cache.device
+    batch = _check_lens(cache_lens, cu_seqlens, "cu_seqlens", device)
+    _check_table(block_table, k_cache, batch)
+    _tokens(k, "k", batch, cu_seqlens, device)
+    _tokens(v, "v", batch, cu_seqlens, device)
+    _check(k.shape == v.shape, "k and v must have the same shape")
+    _check(k.size(-2) == k_cache.size(2), f"k and the cache must have the same KV head count. Got {k.size(-2)} vs {k_cache.size(2)}")
+    _check((positions is None) == (axes is None), "positions and axes go together")
+    _check(q is None or axes is not None, "q is turned by positions, so it needs positions and axes")
+    if axes is not None:
+        _check_positions(positions, axes, k.shape[:-2], device)
+    if q is not None:
+        _tokens(q, "q", batch, cu_seqlens, device)
+        _check(q.shape[:-2] == k.shape[:-2], "q and k must have the same tokens")
+    _check_device_capability(device, "min_fa3_demo_b200 append_cache")
+
+
+_NO_POSITIONS = (0, 0)
 
 
 def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
@@ -108,44 +152,34 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ``cu_seqlens[B]`` go nowhere, and their rows of the returned q are not written.  A token without a slot is left out
     and reported by ``check_last_status("append_cache")``.
     """
-    _check_pair(k_cache, v_cache)
-    device = k_cache.device
-    batch = _check_lens(cache_lens, cu_seqlens, "cu_seqlens", device)
-    _check_table(block_table, k_cache, batch)
-    dim = _tokens(k, "k", batch, cu_seqlens, device)
-    _tokens(v, "v", batch, cu_seqlens, device)
-    _check(k.shape == v.shape, "k and v must have the same shape")
-    _check(k.size(-2) == k_cache.size(2), f"k and the cache must have the same KV head count. Got {k.size(-2)} vs {k_cache.size(2)}")
-    _check((positions is None) == (axes is None), "positions and axes go together")
-    _check(q is None or axes is not None, "q is turned by positions, so it needs positions and axes")
-    if axes is not None:
-        _check_positions(positions, axes, k.shape[:-2], device)
-    if q is not None:
-        _tokens(q, "q", batch, cu_seqlens, device)
-        _check(q.shape[:-2] == k.shape[:-2], "q and k must have the same tokens")
-    if device.index not in _SM100:
-        _check_device_capability(device, "min_fa3_demo_b200 append_cache")
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
+    index, batch, ks = k_cache.get_device(), cache_lens.numel(), k.shape
+    dim, tokens = 4 if cu_seqlens is None else 3, ks[:-2]
+    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens, index, batch) and _is_cache(v_cache, index)
+            and v_cache.shape == k_cache.shape and _is_rows(k, dim, index) and _is_rows(v, dim, index) and v.shape == ks
+            and ks[-2] == k_cache.size(2) and (dim == 3 or ks[0] == batch)
+            and (positions is None if axes is None else positions is not None and _are_positions(positions, axes, tokens, index))
+            and (q is None or (axes is not None and _is_rows(q, dim, index) and q.shape[:-2] == tokens))):
+        _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes)
+    q_out = None if q is None else _like(q)
     if k.numel() == 0:
         return q_out
-    lib = _cabi.load()
+    device = k_cache.device
     ws = _workspace(16, device)
-    total = k.size(0) * k.size(1) if dim == 4 else k.size(0)
-    args = _cabi.AppendArgs(
-        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
-        k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr(),
-        0 if axes is None else ctypes.addressof(axes._c), 0 if axes is None else positions.data_ptr(),
-        _NONE3 if q is None else _rows(q, dim), _rows(k, dim), _rows(v, dim),
-        _NONE3 if axes is None else _position_strides(positions), axes is not None and positions.dtype is torch.int64, batch,
-        k.size(1) if dim == 4 else 0, total, 0 if q is None else q.size(-2), ws.data_ptr(), 16)
+    turned = _NO_POSITIONS if axes is None else (axes._at, positions.data_ptr())
+    args = _cabi.APPEND.pack(
+        *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+        k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr(), *turned,
+        *(_NONE3 if q is None else _rows(q)), *_rows(k), *_rows(v), *(_NONE3 if axes is None else _position_strides(positions)),
+        axes is not None and positions.dtype is _INT64, batch, ks[1] if dim == 4 else 0, ks[0] * ks[1] if dim == 4 else ks[0],
+        0 if q is None else q.size(-2), ws.data_ptr(), 16)
     with _on_device(device):
-        _cabi.check(lib.b2a_cache_append(ctypes.byref(args), _stream_ptr(device)))
+        _cabi.check(_cabi.load().b2a_cache_append(args, _stream_ptr(device)))
     _remember_workspace("append_cache", ws)
     return q_out
 
 
-def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> Tuple[int, int, Tuple[int, int]]:
-    """Checks what forward_tree and cache_weights share; returns (total_q, most tokens of a sequence, mask strides)."""
+def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> None:
+    """Checks what forward_tree and cache_weights share."""
     device = k_cache.device
     dim = _tokens(q, "q", batch, cu_seqlens_q, device)
     heads, kvh = q.size(-2), k_cache.size(2)
@@ -163,7 +197,7 @@ def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> 
         shape = (total, most)
     _check(all(n == 1 or s > 0 for n, s in zip(q.shape, q.stride())), "q must not be expanded")
     if tree_mask is None:
-        return total, most, (0, 0)
+        return
     _check(tree_mask.device == device, "tree_mask must be on the same CUDA device as the cache")
     _check(tree_mask.dtype == torch.bool, "tree_mask must have dtype torch.bool")
     if dim == 4:
@@ -172,16 +206,53 @@ def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> 
         _check(tree_mask.dim() == 2 and tree_mask.size(0) == total and tree_mask.size(1) >= most,
                f"tree_mask must have shape [{total}, max_seqlen_q or more]. Got {list(tree_mask.shape)}")
     _check(tree_mask.size(-1) == 1 or tree_mask.stride(-1) == 1, "the rows of tree_mask must be contiguous")
-    strides = tree_mask.stride()
-    return total, most, (strides[0], strides[1]) if dim == 4 else (0, strides[0])
 
 
 def _token_strides(q: torch.Tensor) -> Tuple[int, int]:
     """Elements from token to token and from head to head of q seen as one list of tokens."""
     stride = q.stride()
-    if q.dim() == 4 and q.size(1) == 1:
+    if len(stride) == 4 and q.size(1) == 1:
         return stride[0], stride[2]
     return stride[-3], stride[-2]
+
+
+def _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index) -> bool:
+    """Whether q and tree_mask are as _check_queries wants them, and simple enough to be told at once."""
+    dim = 4 if cu_seqlens_q is None else 3
+    if not _is_rows(q, dim, index):
+        return False
+    qs, st = q.shape, q.stride()
+    if not (min(st) > 0 and qs[-2] % k_cache.size(2) == 0 and 0 < qs[-2] <= 128 * k_cache.size(2)):
+        return False
+    if dim == 4:
+        most = qs[1]
+        if not (qs[0] == batch and st[0] == most * st[1] and (max_seqlen_q is None or max_seqlen_q == most)):
+            return False
+    else:
+        most = max_seqlen_q
+        if not (type(most) is int and 0 < most <= _INT32_MAX):
+            return False
+    if tree_mask is None:
+        return True
+    size = tree_mask.shape
+    return (tree_mask.dtype is torch.bool and tree_mask.get_device() == index and len(size) == dim - 1 and tree_mask.stride(-1) == 1
+            and (size == (batch, most, most) if dim == 4 else size[0] == qs[0] and size[1] >= most))
+
+
+def _query_sizes(q, max_seqlen_q, tree_mask) -> Tuple[int, int, int, Tuple[int, int]]:
+    """Tokens, the most of a sequence, heads and the strides of the mask."""
+    qs = q.shape
+    if len(qs) == 4:
+        return qs[0] * qs[1], qs[1], qs[2], (0, 0) if tree_mask is None else tree_mask.stride()[:2]
+    return qs[0], int(max_seqlen_q), qs[1], (0, 0) if tree_mask is None else (0, tree_mask.stride(0))
+
+
+def _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask) -> None:
+    _check_pair(k_cache, v_cache)
+    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", k_cache.device)
+    _check_table(block_table, k_cache, batch)
+    _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
+    _check_device_capability(k_cache.device, "min_fa3_demo_b200 forward_tree")
 
 
 def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
@@ -199,32 +270,30 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     Lengths that do not fit and pages that do not exist are reported by ``check_last_status("forward_tree")``.  Repeated
     calls give the same bits; the last bits can depend on the other sequences of the call.
     """
-    _check_pair(k_cache, v_cache)
+    index, batch = k_cache.get_device(), cache_lens.numel()
+    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens_q, index, batch) and _is_cache(v_cache, index)
+            and v_cache.shape == k_cache.shape
+            and _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index)):
+        _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask)
+    total, most, heads, mask_stride = _query_sizes(q, max_seqlen_q, tree_mask)
     device = k_cache.device
-    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", device)
-    _check_table(block_table, k_cache, batch)
-    total, most, mask_stride = _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
-    if device.index not in _SM100:
-        _check_device_capability(device, "min_fa3_demo_b200 forward_tree")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = _like(q)
     else:
         _check(out.device == device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(),
                "out must be contiguous and have the shape, dtype and device of q")
-    lse = torch.empty((batch, q.size(2), most) if q.dim() == 4 else (q.size(1), total), dtype=torch.float32, device=device)
-    if q.numel() == 0:
+    lse = torch.empty((batch, heads, most) if cu_seqlens_q is None else (heads, total), dtype=torch.float32, device=device)
+    if total == 0:
         return (out, lse) if return_lse else out
     lib = _cabi.load()
-    args = _cabi.TreeArgs(
-        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-        q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), _token_strides(q),
-        mask_stride, batch, most, total, q.size(-2), 0.0)
-    ref = ctypes.byref(args)
     with _on_device(device):
-        nbytes = lib.b2a_tree_fwd_workspace_bytes(ref)
+        nbytes = lib.b2a_tree_fwd_workspace_bytes(most, heads, k_cache.size(2))
         ws = _workspace(nbytes, device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        _cabi.check(lib.b2a_tree_fwd(ref, _stream_ptr(device)))
+        args = _cabi.TREE.pack(
+            *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+            q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), *_token_strides(q),
+            *mask_stride, batch, most, total, heads, 0.0, 0, 0, 0, 0, ws.data_ptr(), nbytes)
+        _cabi.check(lib.b2a_tree_fwd(args, _stream_ptr(device)))
     _remember_workspace("forward_tree", ws)
     return (out, lse) if return_lse else out
 
@@ -238,6 +307,22 @@ def _check_weights(weights: torch.Tensor, batch: int, k_cache: torch.Tensor) -> 
     _check(weights.size(2) == 1 or weights.stride(2) == 1, "the rows of weights must be contiguous")
 
 
+def _are_weights(weights: torch.Tensor, batch: int, k_cache: torch.Tensor, index: int) -> bool:
+    size = weights.shape
+    return (weights.dtype is torch.float32 and weights.get_device() == index and len(size) == 3 and size[0] == batch
+            and size[1] == k_cache.size(2) and size[2] > 0 and weights.stride(2) == 1 and min(weights.stride()) > 0)
+
+
+def _check_cache_weights(q, k_cache, cache_lens, weights, block_table, cu_seqlens_q, max_seqlen_q, tree_mask) -> None:
+    _check_cache(k_cache, "k_cache")
+    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", k_cache.device)
+    _check_table(block_table, k_cache, batch)
+    _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
+    _check_weights(weights, batch, k_cache)
+    _check(all(n == 1 or s > 0 for n, s in zip(weights.shape, weights.stride())), "weights must not be expanded")
+    _check_device_capability(k_cache.device, "min_fa3_demo_b200 cache_weights")
+
+
 def cache_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, cache_lens: torch.Tensor, weights: torch.Tensor, *,
                   block_table: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[torch.Tensor] = None,
                   max_seqlen_q: Optional[int] = None, tree_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -248,32 +333,41 @@ def cache_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, cac
     whose lse is infinite add nothing: to leave out drafted tokens that were not accepted, set theirs to infinity.  Slots behind a
     sequence are left as they were.  What does not fit is reported by ``check_last_status("cache_weights")``.
     """
-    _check_cache(k_cache, "k_cache")
-    device = k_cache.device
-    batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", device)
-    _check_table(block_table, k_cache, batch)
-    total, most, mask_stride = _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
-    shape = (batch, q.size(2), most) if q.dim() == 4 else (q.size(1), total)
-    _check(lse.device == device and lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == shape,
-           f"lse must be a contiguous torch.float32 tensor of shape {list(shape)} on the same CUDA device as the cache")
-    _check_weights(weights, batch, k_cache)
-    _check(all(n == 1 or s > 0 for n, s in zip(weights.shape, weights.stride())), "weights must not be expanded")
-    if device.index not in _SM100:
-        _check_device_capability(device, "min_fa3_demo_b200 cache_weights")
-    if q.numel() == 0:
+    index, batch = k_cache.get_device(), cache_lens.numel()
+    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens_q, index, batch)
+            and _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index)
+            and _are_weights(weights, batch, k_cache, index)):
+        _check_cache_weights(q, k_cache, cache_lens, weights, block_table, cu_seqlens_q, max_seqlen_q, tree_mask)
+    total, most, heads, mask_stride = _query_sizes(q, max_seqlen_q, tree_mask)
+    shape = (batch, heads, most) if cu_seqlens_q is None else (heads, total)
+    if not (lse.get_device() == index and lse.dtype is torch.float32 and lse.is_contiguous() and lse.shape == shape):
+        raise RuntimeError(f"lse must be a contiguous torch.float32 tensor of shape {list(shape)} on the same CUDA device as the cache")
+    if total == 0:
         return weights
+    device = k_cache.device
     lib = _cabi.load()
-    args = _cabi.TreeArgs(
-        _cache_fields(k_cache, None, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-        q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), 0, lse.data_ptr(), _token_strides(q), mask_stride, batch,
-        most, total, q.size(-2), 0.0, weights.data_ptr(), weights.stride()[:2], weights.size(2))
     with _on_device(device):
         nbytes = lib.b2a_cache_weights_workspace_bytes()
         ws = _workspace(nbytes, device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        _cabi.check(lib.b2a_cache_weights(ctypes.byref(args), _stream_ptr(device)))
+        args = _cabi.TREE.pack(
+            *_cache_fields(k_cache, None, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+            q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), 0, lse.data_ptr(), *_token_strides(q), *mask_stride,
+            batch, most, total, heads, 0.0, weights.data_ptr(), weights.stride(0), weights.stride(1), weights.size(2), ws.data_ptr(),
+            nbytes)
+        _cabi.check(lib.b2a_cache_weights(args, _stream_ptr(device)))
     _remember_workspace("cache_weights", ws)
     return weights
+
+
+def _check_evict(k_cache, v_cache, weights, cache_lens, budget, recent, block_table) -> None:
+    _check_pair(k_cache, v_cache)
+    batch = _check_lens(cache_lens, None, "", k_cache.device)
+    _check_table(block_table, k_cache, batch)
+    _check_weights(weights, batch, k_cache)
+    _check(0 < budget <= _INT32_MAX, f"budget must be positive. Got {budget}")
+    _check(0 <= recent <= budget, f"recent must be between 0 and the budget. Got {recent}")
+    _check(batch * k_cache.size(2) <= 65535, f"at most 65535 sequences times KV heads. Got {batch} times {k_cache.size(2)}")
+    _check_device_capability(k_cache.device, "min_fa3_demo_b200 evict_cache")
 
 
 def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, cache_lens: torch.Tensor, budget: int, *,
@@ -289,30 +383,24 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     ones follow in their order.  Sequences within the budget stay as they are.  Pages must not be shared between sequences.
     Lengths and pages that do not exist are reported by ``check_last_status("evict_cache")``.
     """
-    _check_pair(k_cache, v_cache)
-    device = k_cache.device
-    batch = _check_lens(cache_lens, None, "", device)
-    _check_table(block_table, k_cache, batch)
-    _check_weights(weights, batch, k_cache)
     budget, recent = int(budget), int(recent)
-    _check(0 < budget <= _INT32_MAX, f"budget must be positive. Got {budget}")
-    _check(0 <= recent <= budget, f"recent must be between 0 and the budget. Got {recent}")
-    kvh = k_cache.size(2)
-    _check(batch * kvh <= 65535, f"at most 65535 sequences times KV heads. Got {batch} times {kvh}")
-    if device.index not in _SM100:
-        _check_device_capability(device, "min_fa3_demo_b200 evict_cache")
+    index, batch = k_cache.get_device(), cache_lens.numel()
+    if not (_is_call(k_cache, cache_lens, block_table, None, index, batch) and _is_cache(v_cache, index)
+            and v_cache.shape == k_cache.shape and _are_weights(weights, batch, k_cache, index)
+            and 0 <= recent <= budget <= _INT32_MAX and budget > 0 and batch * k_cache.size(2) <= 65535):
+        _check_evict(k_cache, v_cache, weights, cache_lens, budget, recent, block_table)
+    kvh, device = k_cache.size(2), k_cache.device
+    lens = torch.empty_like(cache_lens)
+    new_weights = _like(weights)
+    order = torch.empty((batch, kvh, budget), dtype=_INT32, device=device)
     lib = _cabi.load()
-    lens = torch.empty(batch, dtype=torch.int32, device=device)
-    new_weights = torch.empty(weights.shape, dtype=torch.float32, device=device)
-    index = torch.empty((batch, kvh, budget), dtype=torch.int32, device=device)
-    args = _cabi.EvictArgs(
-        _cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), weights.data_ptr(), weights.stride()[:2], batch,
-        weights.size(2), budget, recent, lens.data_ptr(), new_weights.data_ptr(), index.data_ptr())
-    ref = ctypes.byref(args)
     with _on_device(device):
-        nbytes = lib.b2a_cache_evict_workspace_bytes(ref)
+        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget)
         ws = _workspace(nbytes, device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        _cabi.check(lib.b2a_cache_evict(ref, _stream_ptr(device)))
+        args = _cabi.EVICT.pack(
+            *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), weights.data_ptr(), weights.stride(0),
+            weights.stride(1), batch, weights.size(2), budget, recent, lens.data_ptr(), new_weights.data_ptr(), order.data_ptr(),
+            ws.data_ptr(), nbytes)
+        _cabi.check(lib.b2a_cache_evict(args, _stream_ptr(device)))
     _remember_workspace("evict_cache", ws)
-    return lens, new_weights, index
+    return lens, new_weights, order

@@ -307,10 +307,9 @@ evict_shift(const EvictParams p) {
 
 extern "C" {
 
-size_t b2a_cache_evict_workspace_bytes(const b2a_evict_args* a) {
-    using namespace b2a;
-    if (a == nullptr || a->batch < 1 || a->budget < 1 || a->cache.heads_k < 1) return 0;   // b2a_cache_evict reports what is wrong
-    return 256 + static_cast<size_t>(a->batch) * a->cache.heads_k * a->budget * sizeof(int);
+size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget) {
+    if (batch < 1 || heads_k < 1 || budget < 1) return 0;   // b2a_cache_evict reports what is wrong
+    return 256 + static_cast<size_t>(batch) * heads_k * budget * sizeof(int);
 }
 
 int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
@@ -330,7 +329,7 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     B2A_REQUIRE(rows <= 65535, "at most 65535 sequences times K/V heads, got %lld", rows);
     B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
                 "workspace must be a 16-byte aligned device pointer");
-    const size_t need = b2a_cache_evict_workspace_bytes(a);
+    const size_t need = b2a_cache_evict_workspace_bytes(a->batch, a->cache.heads_k, a->budget);
     if (a->workspace_bytes < need) {
         return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, need);
     }

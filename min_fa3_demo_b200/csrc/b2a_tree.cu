@@ -753,13 +753,12 @@ struct TreeLayout {
     size_t cuts, stat, o, total;   // offsets
 };
 
-TreeLayout tree_layout(const b2a_tree_args& a, int sms) {
+TreeLayout tree_layout(int seqlen_q, int group, int sms) {
     TreeLayout t{};
-    const int group = a.heads_q / a.cache.heads_k;
     t.ctas = sms < kTreeMaxCtas ? sms : kTreeMaxCtas;
     t.tile_tokens = kTileM / group;
-    t.tiles = a.seqlen_q > t.tile_tokens ? 2 : 1;
-    t.rows = (t.tiles == 2 ? t.tile_tokens : a.seqlen_q) * group;
+    t.tiles = seqlen_q > t.tile_tokens ? 2 : 1;
+    t.rows = (t.tiles == 2 ? t.tile_tokens : seqlen_q) * group;
     t.cuts = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
     t.stat = t.cuts + align_up(t.ctas * sizeof(TreeCut), 256);
     t.o = t.stat + align_up(4ull * t.ctas * t.rows * sizeof(float2), 256);
@@ -773,14 +772,14 @@ TreeLayout tree_layout(const b2a_tree_args& a, int sms) {
 
 extern "C" {
 
-size_t b2a_tree_fwd_workspace_bytes(const b2a_tree_args* a) {
+size_t b2a_tree_fwd_workspace_bytes(int32_t seqlen_q, int32_t heads_q, int32_t heads_k) {
     using namespace b2a;
     DeviceInfo dev{};
-    if (a == nullptr || a->cache.heads_k < 1 || a->heads_q < a->cache.heads_k || a->heads_q % a->cache.heads_k != 0 ||
-        a->heads_q / a->cache.heads_k > kTileM || a->seqlen_q < 1 || current_device_info(&dev) != B2A_OK) {
+    if (seqlen_q < 1 || heads_k < 1 || heads_q < heads_k || heads_q % heads_k != 0 || heads_q / heads_k > kTileM ||
+        current_device_info(&dev) != B2A_OK) {
         return 0;   // b2a_tree_fwd reports what is wrong
     }
-    return tree_layout(*a, dev.sm_count).total;
+    return tree_layout(seqlen_q, heads_q / heads_k, dev.sm_count).total;
 }
 
 int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
@@ -795,7 +794,7 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     DeviceInfo dev{};
     rc = current_device_info(&dev);
     if (rc != B2A_OK) return rc;
-    const TreeLayout t = tree_layout(*a, dev.sm_count);
+    const TreeLayout t = tree_layout(a->seqlen_q, p.c.group, dev.sm_count);
     if (a->workspace_bytes < t.total) {
         return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, t.total);
     }

@@ -18,6 +18,7 @@ __all__ = ["RotaryAxes", "rotary"]
 
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510582")
 _MAX_PAIRS = 64
+_NONE3 = (0, 0, 0)
 
 
 class RotaryAxes:
@@ -44,7 +45,7 @@ class RotaryAxes:
             c.turn[i] = round(Fraction(f) * 2**64 / (2 * _PI)) % 2**64
             c.axis[i] = a
         c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
-        self._c = c
+        self._c, self._at = c, ctypes.addressof(c)
 
     @classmethod
     def from_sections(cls, sections: Sequence[int], base: float = 10000.0, *, restart: bool = False,
@@ -61,11 +62,26 @@ class RotaryAxes:
         return cls(freq, axis, adjacent=adjacent)
 
 
-def _rows(t: torch.Tensor, dim: int) -> Tuple[int, int, int]:
+_BF16, _INT32, _INT64 = torch.bfloat16, torch.int32, torch.int64
+
+
+def _rows(t: torch.Tensor) -> Tuple[int, int, int]:
     """Elements from sequence to sequence, token to token, head to head; 0 where there is only one."""
-    size, stride = t.shape, t.stride()
-    three = tuple(0 if n == 1 else s for n, s in zip(size[:-1], stride[:-1]))
-    return three if dim == 4 else (0, *three)
+    st = t.stride()
+    three = st[:3] if len(st) == 4 else (0, st[0], st[1])
+    if (three[0] | three[1] | three[2]) & 7:
+        size = t.shape if len(st) == 4 else (1, *t.shape)
+        three = tuple(0 if n == 1 else s for n, s in zip(size, three))
+    return three
+
+
+def _is_rows(t: torch.Tensor, dim: int, index: int) -> bool:
+    """Whether t is heads of 128 adjacent values, 16 bytes aligned (in one expression; _check_heads says what is wrong)."""
+    if t.dtype is not _BF16 or t.get_device() != index:
+        return False
+    size, st = t.shape, t.stride()
+    return (len(size) == dim and size[-1] == 128 and st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0
+            and t.data_ptr() & 15 == 0)
 
 
 def _check_heads(t: torch.Tensor, name: str, dim: int) -> None:
@@ -73,7 +89,7 @@ def _check_heads(t: torch.Tensor, name: str, dim: int) -> None:
     _check(t.dtype == torch.bfloat16, f"{name} must have dtype torch.bfloat16")
     _check(t.dim() == dim, f"{name} must have shape " + ("[B, S, H, D]" if dim == 4 else "[total_tokens, H, D]"))
     _check(t.size(-1) == 128, f"{name} must have head_dim D=128")
-    _check(t.stride(-1) == 1 and not any(s % 8 for s in _rows(t, dim)) and t.data_ptr() % 16 == 0,
+    _check(t.stride(-1) == 1 and not any(s & 7 for s in _rows(t)) and t.data_ptr() % 16 == 0,
            f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
 
 
@@ -85,10 +101,29 @@ def _check_positions(positions: torch.Tensor, axes: RotaryAxes, shape, device) -
            f"positions must have shape {[axes.axes, *shape]}. Got {list(positions.shape)}")
 
 
+def _are_positions(positions: torch.Tensor, axes: RotaryAxes, shape, index: int) -> bool:
+    return (type(axes) is RotaryAxes and positions.get_device() == index and positions.dtype in (_INT64, _INT32)
+            and positions.shape == (axes.axes, *shape))
+
+
 def _position_strides(positions: torch.Tensor) -> Tuple[int, int, int]:
     s = positions.stride()
     return s if len(s) == 3 else (s[0], 0, s[1])
 
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _check_rotary(q, k, positions, axes, dim) -> None:
+    _check(dim in (3, 4), "q must have shape [B, S, H, D] or [total_tokens, H, D]")
+    _check_heads(q, "q", dim)
+    if k is not None:
+        _check_heads(k, "k", dim)
+        _check(k.device == q.device, "q and k must be on the same CUDA device")
+        _check(k.shape[:-2] == q.shape[:-2], "q and k must have the same tokens")
+    _check_positions(positions, axes, q.shape[:-2], q.device)
+    _check_device_capability(q.device, "min_fa3_demo_b200 rotary")
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, axes: RotaryAxes, *,
@@ -100,27 +135,20 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     one projection: only the 128 values of a head have to be adjacent.  Returns new contiguous tensors.  ``inverse``
     turns the other way, which is what the gradients want; ``autograd.rotary`` does it by itself.
     """
-    dim = q.dim()
-    _check(dim in (3, 4), "q must have shape [B, S, H, D] or [total_tokens, H, D]")
-    _check_heads(q, "q", dim)
-    if k is not None:
-        _check_heads(k, "k", dim)
-        _check(k.device == q.device, "q and k must be on the same CUDA device")
-        _check(k.shape[:-2] == q.shape[:-2], "q and k must have the same tokens")
-    _check_positions(positions, axes, q.shape[:-2], q.device)
-    if q.device.index not in _SM100:
-        _check_device_capability(q.device, "min_fa3_demo_b200 rotary")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    batch, seqlen = (q.size(0), q.size(1)) if dim == 4 else (1, q.size(0))
+    dim, index, qs = q.dim(), q.get_device(), q.shape
+    tokens = qs[:-2]
+    if not (dim in (3, 4) and _is_rows(q, dim, index) and (k is None or (_is_rows(k, dim, index) and k.shape[:-2] == tokens))
+            and _are_positions(positions, axes, tokens, index) and index in _SM100):
+        _check_rotary(q, k, positions, axes, dim)
+    q_out = _like(q)
+    k_out = None if k is None else _like(k)
     if q.numel() == 0:
         return q_out, k_out
-    lib = _cabi.load()
-    args = _cabi.RotaryArgs(ctypes.addressof(axes._c), q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
-                            0 if k is None else k_out.data_ptr(), positions.data_ptr(), _rows(q, dim),
-                            (0, 0, 0) if k is None else _rows(k, dim), _position_strides(positions),
-                            positions.dtype is torch.int64, batch, seqlen, q.size(-2), 0 if k is None else k.size(-2),
-                            bool(inverse))
-    with _on_device(q.device):
-        _cabi.check(lib.b2a_rotary(ctypes.byref(args), _stream_ptr(q.device)))
+    args = _cabi.ROTARY.pack(
+        axes._at, q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
+        positions.data_ptr(), *_rows(q), *(_NONE3 if k is None else _rows(k)), *_position_strides(positions),
+        positions.dtype is _INT64, qs[0] if dim == 4 else 1, tokens[-1], qs[-2], 0 if k is None else k.size(-2), bool(inverse))
+    device = q.device
+    with _on_device(device):
+        _cabi.check(_cabi.load().b2a_rotary(args, _stream_ptr(device)))
     return q_out, k_out
