@@ -226,25 +226,38 @@ inline int make_slot_map(CUtensorMap* map, const CacheView& c, bool keys, int bo
     return make_strided_map(map, keys ? c.k : c.v, 4, sizes, strides, 1, static_cast<uint32_t>(box_rows));
 }
 
-// Loads blocks of slots by one warp: a lane for each box of the block.  A lane looks up its page a block ahead, so that the
-// block table's latency is not on the path.
+// Loads blocks of slots by one warp: a lane for each box of the block.  A lane asks for its page a block ahead and looks at the
+// answer only when it needs it, so that neither the block table's latency nor a division is on the path.
 struct SlotLoader {
-    int box_rows, boxes, page, row;
-    int bad;                 // this lane met a page that does not exist
+    int box_rows, boxes;
+    uint32_t per_page;       // 2^32 / page_size, rounded up: the high half of slot * per_page is slot / page_size or one more
+    int page, row;
+    int bad;                 // this lane met a page that does not exist (TMA fills such a box with zeros)
+
+    __device__ __forceinline__ SlotLoader(const CacheView& c, int rows)
+        : box_rows(rows), boxes(kSlotBlock / rows), per_page(0xFFFFFFFFu / static_cast<uint32_t>(c.page_size) + 1u), page(0), row(0), bad(0) {}
 
     __device__ __forceinline__ void look_up(const CacheView& c, int seq, int block, int slots, int lane) {
-        if (lane >= boxes) return;
         const int slot = block * kSlotBlock + lane * box_rows;
-        if (slot >= slots) return;
-        row = c.block_table == nullptr ? slot : slot % c.page_size;
-        page = c.page_of(seq, slot);
-        bad |= page < 0;     // TMA fills such a box with zeros
+        if (lane >= boxes || slot >= slots) return;
+        if (c.block_table == nullptr) {
+            page = seq;
+            row = slot;
+            return;
+        }
+        int at = static_cast<int>(__umulhi(static_cast<uint32_t>(slot), per_page));
+        row = slot - at * c.page_size;
+        if (row < 0) {
+            --at;
+            row += c.page_size;
+        }
+        page = c.block_table[seq * c.table_stride + at];
     }
     // Boxes of a block that hold slots.
     __device__ __forceinline__ int count(int block, int slots) const {
         return min(boxes, max(0, (slots - block * kSlotBlock + box_rows - 1) / box_rows));
     }
-    __device__ __forceinline__ void load(const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int n, int lane) const {
+    __device__ __forceinline__ void load(const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int n, int lane) {
         if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * static_cast<uint32_t>(box_rows) * 256u);
         __syncwarp();
         if (lane < n) {
@@ -253,6 +266,9 @@ struct SlotLoader {
             tma_load_4d(at + kHalfTileBytes, map, bar, 64, head, row, page);
         }
         __syncwarp();
+    }
+    __device__ __forceinline__ void check(const CacheView& c, int n, int lane) {
+        bad |= lane < n && static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages);
     }
 };
 

@@ -9,7 +9,7 @@
 // end of a run is finished by tree_combine, in fp32 and in slot order.
 //
 //   warp 0-3, 4-7   softmax warpgroups, one thread a row
-//   warp 8          Q K^T       warp 10   P V       warp 9   plan and TMA loads       warp 11   idle
+//   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of Q and K       warp 11   loads of V
 //
 // An item of more than 128 rows has two tiles that use each block in turn, as in the forward.  One of at most 128 has only
 // one, and its two warpgroups take turns at the blocks: each has a running maximum, a sum and an O of its own, and they are
@@ -32,7 +32,7 @@ namespace {
 constexpr int kTreeThreads = 384;
 constexpr int kTreeStages = 2;
 constexpr int kTreeSlots = 4;       // pieces in flight between the load warp and the others
-constexpr int kTreeQkWarp = 8, kTreeLoadWarp = 9, kTreePvWarp = 10;
+constexpr int kTreeQkWarp = 8, kTreeLoadWarp = 9, kTreePvWarp = 10, kTreeVWarp = 11;
 constexpr int kTreeMaxCtas = kFwdStatusWords;
 
 struct TreeParams {
@@ -94,29 +94,42 @@ static_assert(kTreeSmemBytes <= 227 * 1024, "shared memory of a CTA");
 // Whether a block goes to warpgroup x: both tiles take every block, one tile's warpgroups take turns.
 __device__ __forceinline__ bool tree_takes(bool two, int i, int x) { return two || (i & 1) == x; }
 
+__device__ __forceinline__ const unsigned char* tree_mask_row(const TreeParams& p, const TreePiece& w, int token) {
+    return p.c.mask + (p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + token * p.c.mask_stride[1]
+                                                   : (static_cast<long long>(w.q_begin) + token) * p.c.mask_stride[1]);
+}
+
 __device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreePiece& w, int token, int u) {
-    if (p.c.mask == nullptr) return u <= token;
-    const long long at = p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + token * p.c.mask_stride[1]
-                                                     : (static_cast<long long>(w.q_begin) + token) * p.c.mask_stride[1];
-    return p.c.mask[at + u] != 0;
+    return p.c.mask == nullptr ? u <= token : tree_mask_row(p, w, token)[u] != 0;
 }
 
 __device__ __forceinline__ bool bf16_not_finite(uint32_t half) { return (half & 0x7F80u) == 0x7F80u; }
 
 // Values of drafted tokens that are not finite, added to a row that sees them: columns [column, column + 32) of O.
 // Only the sign of the weight, which is positive, matters.
-__device__ __noinline__ void tree_add_not_finite(const TreeParams& p, const TreePiece& w, int token, int column, uint32_t (&t)[32]) {
+__device__ __forceinline__ void tree_add_not_finite(const TreeParams& p, const TreePiece& w, int token, int column, uint32_t (&t)[32]) {
     const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
+#pragma unroll 1
     for (int u = from; u < to; ++u) {
         const long long slot = static_cast<long long>(w.len) + u;
         if (slot >= w.slots || !tree_sees(p, w, token, u)) continue;
         const int page = p.c.cache.page_of(w.seq, slot);
         if (page < 0) continue;
-        const __nv_bfloat16* v = p.c.cache.v + page * p.c.cache.v_stride[0] + slot % p.c.cache.page_size * p.c.cache.v_stride[1] +
-                                 w.head * p.c.cache.v_stride[2] + column;
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t bits = __bfloat16_as_ushort(v[i]);
-            if (bf16_not_finite(bits)) t[i] = __float_as_uint(__uint_as_float(t[i]) + __uint_as_float(bits << 16));
+        const uint4* v = reinterpret_cast<const uint4*>(p.c.cache.v + page * p.c.cache.v_stride[0] +
+                                                        slot % p.c.cache.page_size * p.c.cache.v_stride[1] +
+                                                        w.head * p.c.cache.v_stride[2] + column);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 eight = v[i];
+            const uint32_t words[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = i * 8 + e * 2;
+                if (bf16_not_finite(words[e])) t[at] = __float_as_uint(__uint_as_float(t[at]) + __uint_as_float(words[e] << 16));
+                if (bf16_not_finite(words[e] >> 16)) {
+                    t[at + 1] = __float_as_uint(__uint_as_float(t[at + 1]) + __uint_as_float(words[e] & 0xFFFF0000u));
+                }
+            }
         }
     }
 }
@@ -148,7 +161,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         for (int i = 0; i < kTreeSlots; ++i) {
             mbar_init(smem_u32(&sh.piece_full[i]), 1);
-            mbar_init(smem_u32(&sh.piece_empty[i]), 2 + 8);   // MMA warps and softmax warps
+            mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 8);   // MMA warps, V's load warp and softmax warps
         }
         sh.abort_flag = 0;
         sh.not_finite = 0;
@@ -197,9 +210,11 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 }
                 p.cuts[blockIdx.x] = cut;
             }
-            SlotLoader loader{p.box_rows, kSlotBlock / p.box_rows, 0, 0, walk.bad};
-            uint32_t k_it = 0, v_it = 0, q_par = 0;
+            SlotLoader loader(p.c.cache, p.box_rows);
+            loader.bad = walk.bad;
+            uint32_t k_it = 0, q_par = 0;
             bool ok = true, begun = false;
+            PH_DECL(3)   // 0 other, 1 wait for K's stage, 2 issue K
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTreeSlots;
                 ok = mbar_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTreeSlots) & 1u) ^ 1u, 1);
@@ -239,43 +254,57 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     }
                     __syncwarp();
                 };
-                // K of block i is asked for before V of block i - 1: Q K^T is a block ahead of P V.
                 load_q(0);
-                int page_v = 0, row_v = 0;
                 loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-                for (int i = 0; i <= w.blocks && ok; ++i) {
+                for (int i = 0; i < w.blocks && ok; ++i, ++k_it) {
                     SlotLoader now = loader;
                     if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-                    if (i < w.blocks) {
-                        const uint32_t stage = k_it % kTreeStages;
-                        ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
-                        if (!ok) break;
-                        ++k_it;
-                        now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head,
-                                 now.count(w.j0 + i, w.slots), lane);
-                    }
-                    if (i == 0 && w.tokens[1] > 0) {
-                        load_q(1);
-                        if (!ok) break;
-                    }
-                    if (i > 0) {
-                        const uint32_t stage = v_it % kTreeStages;
-                        ok = mbar_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kTreeStages) & 1u) ^ 1u, 4);
-                        if (!ok) break;
-                        ++v_it;
-                        SlotLoader before = now;
-                        before.page = page_v;
-                        before.row = row_v;
-                        before.load(&map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head,
-                                    before.count(w.j0 + i - 1, w.slots), lane);
-                    }
-                    page_v = now.page;
-                    row_v = now.row;
+                    const int boxes = now.count(w.j0 + i, w.slots);
+                    const uint32_t stage = k_it % kTreeStages;
+                    PH_MARK(0);
+                    ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
+                    if (!ok) break;
+                    PH_MARK(1);
+                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
+                    PH_MARK(2);
+                    now.check(p.c.cache, boxes, lane);
+                    loader.bad |= now.bad;
+                    if (i == 0 && w.tokens[1] > 0) load_q(1);
                 }
                 if (!ok) break;
                 walk.advance(p.c, w.blocks);
             }
             if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
+            PH_PRINT("tree load", 3);
+        } else if (warp == kTreeVWarp) {
+            // ------------------------------------------------------------ loads of V
+            SlotLoader loader(p.c.cache, p.box_rows);
+            uint32_t v_it = 0;
+            bool ok = true;
+            PH_DECL(3)   // 0 other, 1 wait for V's stage, 2 issue V
+            for (uint32_t it = 0; ok; ++it) {
+                const uint32_t at = it % kTreeSlots;
+                ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 4);
+                if (!ok) break;
+                const TreePiece w = sh.piece[at];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+                if (!w.valid) break;
+                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
+                for (int i = 0; i < w.blocks; ++i, ++v_it) {
+                    SlotLoader now = loader;
+                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+                    const int boxes = now.count(w.j0 + i, w.slots);
+                    const uint32_t stage = v_it % kTreeStages;
+                    PH_MARK(0);
+                    ok = mbar_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kTreeStages) & 1u) ^ 1u, 18);
+                    if (!ok) break;
+                    PH_MARK(1);
+                    now.load(&map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
+                    PH_MARK(2);
+                }
+            }
+            PH_PRINT("tree load", 3);
         } else if (warp == kTreeQkWarp || warp == kTreePvWarp) {
             // ------------------------------------------------------------ MMA warps
             const bool qk = warp == kTreeQkWarp;
@@ -287,6 +316,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const uint32_t v_lo0 = desc_lo_mnmajor(smem_u32(&sh.v[0][0]));
             uint32_t kv_it = 0, s_it = 0, par = 0;
             bool ok = true;
+            PH_DECL(4)   // 0 other, 1 wait K (V), 2 wait S (P), 3 issue
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTreeSlots;
                 ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 5);
@@ -300,9 +330,11 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (!valid) break;
                 for (int i = 0; i < blocks && ok; ++i, ++kv_it) {
                     const uint32_t stage = kv_it % kTreeStages, phase = (kv_it / kTreeStages) & 1u;
+                    PH_MARK(0);
                     if (qk) {
                         ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), phase, 6);
                         if (!ok) break;
+                        PH_MARK(1);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             if (!tree_takes(two, i, x)) continue;
@@ -315,33 +347,39 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             // The softmax warps have taken the S before this one out of tensor memory.
                             ok = mbar_wait(wctx, smem_u32(&sh.s_empty), (s_it & 1u) ^ 1u, 8);
                             if (!ok) break;
+                            PH_MARK(2);
                             ++s_it;
                             tc_fence_after_sync();
                             umma_ss_kk_x8_w(tmem_base + kFwdColS, q_lo0 + tile * kStageStep, k_lo0 + stage * kStageStep, idesc_qk, 0u);
                             tc_commit_w(smem_u32(&sh.s_full[x]));
                             if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[tile]));
                             __syncwarp();
+                            PH_MARK(3);
                         }
                         tc_commit_w(smem_u32(&sh.k_empty[stage]));
                     } else {
                         ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), phase, 9);
                         if (!ok) break;
+                        PH_MARK(1);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             if (!tree_takes(two, i, x)) continue;
                             ok = mbar_wait(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
                             if (!ok) break;
+                            PH_MARK(2);
                             par ^= 1u << x;
                             tc_fence_after_sync();
                             umma_ts_x8_w(tmem_base + kFwdColO + x * 128u, tmem_base + kFwdColP + x * kFwdColPStep,
                                          v_lo0 + stage * kStageStep, idesc_pv, i > (two ? 0 : x) ? 1u : 0u);
                             tc_commit_w(smem_u32(&sh.pv_done[x]));
                             __syncwarp();
+                            PH_MARK(3);
                         }
                         tc_commit_w(smem_u32(&sh.v_empty[stage]));
                     }
                 }
             }
+            PH_PRINT("tree mma", 4);
         }
     } else {
         // ---------------------------------------------------------------- softmax warpgroups
@@ -358,6 +396,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const int row_head = r - row_token * p.c.group;
         uint32_t s_cnt = 0, pv_cnt = 0, seen_cnt = 0, both_cnt = 0, kv_base = 0;
         bool ok = true;
+        PH_DECL(6)   // 0 other, 1 which slots are seen, 2 wait S, 3 take S, 4 V rows and mask, 5 softmax
 
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kTreeSlots;
@@ -385,23 +424,33 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const int base = (w.j0 + i) * kSlotBlock;
                 const bool tail = base + kSlotBlock > w.len;   // drafted tokens, or no slots any more
                 uint32_t* seen = nullptr;
+                PH_MARK(0);
                 if (tail && masked) {
-                    // Which slots of the block each token sees: a warp's lanes are 32 slots.
-                    const int u = base + quarter * 32 + lane - w.len;
+                    // Which slots of the block each token sees: a warp's lanes are 32 slots.  Eight tokens' bytes at a time.
+                    const int slot = base + quarter * 32 + lane, u = slot - w.len;
+                    const bool ask = slot < w.slots && u >= 0 && u < w.n, always = u < 0 && slot < w.slots;
+                    const unsigned char* byte = tree_mask_row(p, w, w.tok0 + tile * p.tile_tokens) + (ask ? u : 0);
                     seen = &sh.seen[x][seen_cnt & 1u][0][0];
-                    const int from = w.tok0 + tile * p.tile_tokens;
-                    const bool slot_ok = base + quarter * 32 + lane < w.slots;
-#pragma unroll 8
-                    for (int t = 0; t < tokens; ++t) {
-                        const bool yes = slot_ok && (u < 0 || (u < w.n && tree_sees(p, w, from + t, u)));
-                        const uint32_t word = __ballot_sync(0xFFFFFFFFu, yes);
-                        if (lane == 0) seen[t * 4 + quarter] = word;
+                    for (int t0 = 0; t0 < tokens; t0 += 8) {
+                        uint32_t yes[8];
+#pragma unroll
+                        for (int t = 0; t < 8; ++t) {
+                            yes[t] = always ? 1u : 0u;
+                            if (ask && t0 + t < tokens) yes[t] = byte[(t0 + t) * p.c.mask_stride[1]];
+                        }
+#pragma unroll
+                        for (int t = 0; t < 8; ++t) {
+                            const uint32_t word = __ballot_sync(0xFFFFFFFFu, yes[t] != 0u);
+                            if (lane == 0 && t0 + t < tokens) seen[(t0 + t) * 4 + quarter] = word;
+                        }
                     }
                     __syncwarp();
                     mbar_arrive(smem_u32(&sh.seen_full[x]));
                 }
+                PH_MARK(1);
                 ok = mbar_wait(wctx, smem_u32(&sh.s_full[x]), s_cnt & 1u, 12);
                 if (!ok) break;
+                PH_MARK(2);
                 ++s_cnt;
                 tc_fence_after_sync();
                 float s[kTileN];
@@ -417,6 +466,17 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 }
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&sh.s_empty));
+                PH_MARK(3);
+
+                const bool begins = i == first;
+                bool pv_pending = !begins;
+                auto wait_pv = [&]() -> bool {
+                    if (!mbar_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15)) return false;
+                    ++pv_cnt;
+                    tc_fence_after_sync();
+                    pv_pending = false;
+                    return true;
+                };
 
                 if (tail) {
                     if (masked) {
@@ -429,34 +489,45 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     const int slot = base + r;
                     const bool look = slot >= w.len && slot < w.slots && (w.n > 1 || masked);
                     if (!two || x == 0) {
+                        // A barrier tells the last phase from the one before it, no more: the V that lay in this stage two
+                        // blocks ago has to have come, which the product with it proves.
+                        if (pv_pending) {
+                            ok = wait_pv();
+                            if (!ok) break;
+                        }
                         const uint32_t stage = (kv_base + i) % kTreeStages;
                         ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / kTreeStages) & 1u, 14);
                         if (!ok) break;
-                        if (look || slot >= w.slots) {
-#pragma unroll 4
-                            for (int c = 0; c < 16; ++c) {
-                                // Another chunk first in each row, so that rows of 128 bytes do not meet in the same banks.
-                                uint4* chunk = reinterpret_cast<uint4*>(&sh.v[stage][(c >> 3) * kHalfTileBytes + r * 128 +
-                                                                                     (((c + r) & 7) * 16)]);
-                                if (!look) {
-                                    *chunk = make_uint4(0u, 0u, 0u, 0u);
-                                    continue;
-                                }
-                                uint4 val = *chunk;
-                                uint32_t words[4] = {val.x, val.y, val.z, val.w};
-                                bool found = false;
+                        // Another chunk first in each row, so that rows of 128 bytes do not meet in the same banks.
+                        uint8_t* row = &sh.v[stage][r * 128];
+                        auto chunk = [&](int c) { return reinterpret_cast<uint4*>(row + (c >> 3) * kHalfTileBytes + (((c + r) & 7) * 16)); };
+                        if (slot >= w.slots) {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    if (bf16_not_finite(words[e])) words[e] &= 0xFFFF0000u, found = true;
-                                    if (bf16_not_finite(words[e] >> 16)) words[e] &= 0xFFFFu, found = true;
-                                }
-                                if (found) {
-                                    *chunk = make_uint4(words[0], words[1], words[2], words[3]);
-                                    *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
+                            for (int c = 0; c < 16; ++c) *chunk(c) = make_uint4(0u, 0u, 0u, 0u);
+                        } else if (look) {
+                            uint32_t ones = 0;      // an exponent of all ones carries into its half's sign bit
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                const uint4 v = *chunk(c);
+                                ones |= ((v.x & 0x7F807F80u) + 0x00800080u) | ((v.y & 0x7F807F80u) + 0x00800080u) |
+                                        ((v.z & 0x7F807F80u) + 0x00800080u) | ((v.w & 0x7F807F80u) + 0x00800080u);
+                            }
+                            if ((ones & 0x80008000u) != 0u) {
+                                *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
+#pragma unroll 1
+                                for (int c = 0; c < 16; ++c) {
+                                    const uint4 v = *chunk(c);
+                                    uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        if (bf16_not_finite(words[e])) words[e] &= 0xFFFF0000u;
+                                        if (bf16_not_finite(words[e] >> 16)) words[e] &= 0xFFFFu;
+                                    }
+                                    *chunk(c) = make_uint4(words[0], words[1], words[2], words[3]);
                                 }
                             }
-                            fence_proxy_async_smem();
                         }
+                        fence_proxy_async_smem();
                     }
                     if (active) {
                         // One bit per visible slot of 32.
@@ -478,15 +549,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     }
                 }
 
-                const bool begins = i == first;
-                bool pv_pending = !begins;
-                auto wait_pv = [&]() -> bool {
-                    if (!mbar_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15)) return false;
-                    ++pv_cnt;
-                    tc_fence_after_sync();
-                    pv_pending = false;
-                    return true;
-                };
+                PH_MARK(4);
                 if (!active) {
                     // None of the warp's rows exists; it keeps step, and its P and O are never looked at.
                     if (pv_pending) {
@@ -508,8 +571,9 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const float m_new = fmaxf(m_used, bm);
                 if (begins) {
                     m_used = m_new;
-                } else if (__any_sync(0xFFFFFFFFu, (m_new - m_used) * sl2 > kRescaleThreshold)) {
-                    // O is scaled only when the maximum has moved by a factor of 2^8: the division at the end uses the same one.
+                } else if (__any_sync(0xFFFFFFFFu, row_valid && (m_new - m_used) * sl2 > kRescaleThreshold)) {
+                    // O is scaled only when the maximum has moved by a factor of 2^8: the division at the end uses the same
+                    // one.  Rows of the tile that do not exist have no say: what lies there differs from call to call.
                     const float factor = m_new == -INFINITY ? 1.f : fast_exp2((m_used - m_new) * sl2);
                     l *= factor;
                     m_used = m_new;
@@ -554,6 +618,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 tmem_wait_st();
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&sh.p_full[x]));
+                PH_MARK(5);
             }
             if (!ok) break;
             kv_base += w.blocks;
@@ -651,6 +716,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
             release();
         }
+        PH_PRINT("tree softmax", 6);
     }
 
     // Common exit: every role arrives here (normally or after an abort).
@@ -673,7 +739,6 @@ __global__ void __launch_bounds__(256)
 tree_combine(const __grid_constant__ TreeParams p) {
     constexpr int kPitch = kHeadDim + 4;    // bf16; keeps the 8-byte column stores of 16 rows on distinct banks
     __shared__ __align__(8) __nv_bfloat16 out[kTreeStrip * kPitch];
-    __shared__ float weight[kTreeMaxCtas][kTreeStrip];
     let_next_kernel_start();
     wait_for_previous_kernel();
     const int cta = blockIdx.x + 1;
@@ -692,23 +757,27 @@ tree_combine(const __grid_constant__ TreeParams p) {
         return (2ll * (cta - 1 + i) + second) * 2 + tile;
     };
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (warp == 0 && lane < rows) {
-        float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, norm = 0.f;
+    if (lane < rows) {
+#pragma unroll 4
         for (int i = 0; i < pieces; ++i) m = fmaxf(m, p.part_stat[part_of(i) * p.part_rows + row0 + lane].x);
+    }
+    // Each warp finds the row's weights by itself.
+    auto weight_of = [&](const float2& st) { return st.x == m ? 1.f : fast_exp2((st.x - m) * p.scale_log2); };
+    if (lane < rows) {
+#pragma unroll 4
         for (int i = 0; i < pieces; ++i) {
             const float2 st = p.part_stat[part_of(i) * p.part_rows + row0 + lane];
-            const float f = st.x == m ? 1.f : fast_exp2((st.x - m) * p.scale_log2);
-            weight[i][lane] = f;
-            l = fmaf(st.y, f, l);
+            l = fmaf(st.y, weight_of(st), l);
         }
-        const float norm = l == 0.f ? 0.f : 1.f / l;
-        for (int i = 0; i < pieces; ++i) weight[i][lane] *= norm;
-        const int r = row0 + lane, token = tok0 + r / p.c.group;
-        p.lse[cut.seq * p.lse_seq_stride + (cut.head * p.c.group + r % p.c.group) * p.lse_head_stride +
-              (p.c.cu_seqlens_q == nullptr ? token : cut.q_begin + token)] =
-            l == 0.f ? -INFINITY : (m * p.scale_log2 + fast_log2(l)) * kLn2;
+        norm = l == 0.f ? 0.f : 1.f / l;
+        if (warp == 0) {
+            const int r = row0 + lane, token = tok0 + r / p.c.group;
+            p.lse[cut.seq * p.lse_seq_stride + (cut.head * p.c.group + r % p.c.group) * p.lse_head_stride +
+                  (p.c.cu_seqlens_q == nullptr ? token : cut.q_begin + token)] =
+                l == 0.f ? -INFINITY : (m * p.scale_log2 + fast_log2(l)) * kLn2;
+        }
     }
-    __syncthreads();
     // Lane = row, four of the 32 column quads a warp.
     if (lane < rows) {
         float4 acc[4];
@@ -716,7 +785,7 @@ tree_combine(const __grid_constant__ TreeParams p) {
         for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
         for (int i = 0; i < pieces; ++i) {
-            const float f = weight[i][lane];
+            const float f = weight_of(p.part_stat[part_of(i) * p.part_rows + row0 + lane]) * norm;
             const float4* o = p.part_o + (part_of(i) * 32 + warp * 4) * p.part_rows + row0 + lane;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {

@@ -47,7 +47,8 @@ struct WeightPiece {
 struct __align__(1024) WeightShared {
     uint8_t q[kWeightQSlots][kTileBytes];
     uint8_t k[kWeightKStages][kTileBytes];
-    float lse2[kWeightQSlots][kTileM];          // lse * log2(e) of a tile's rows
+    float minus_lse2[kWeightQSlots][kTileM];    // -lse * log2(e) of a tile's rows
+    uint4 token_columns[kTileM];                // the columns of a tile's token
     uint32_t live[kWeightQSlots][4];            // a bit for each row that exists and has a finite lse: the others give nothing
     float sums[kWeightChunk][kTileM];
     WeightPiece piece[kWeightSlots];
@@ -62,7 +63,59 @@ struct __align__(1024) WeightShared {
 constexpr size_t kWeightSmemBytes = sizeof(WeightShared) + 1024;
 static_assert(kWeightSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
+// Of 32 columns those from a number on (which may be anything).
+__host__ __device__ __forceinline__ uint32_t columns_from(int from) {
+    return from <= 0 ? 0xFFFFFFFFu : from >= 32 ? 0u : 0xFFFFFFFFu << from;
+}
+
 __device__ __forceinline__ int weight_tiles(const WeightParams& p, int n) { return (n + p.tile_tokens - 1) / p.tile_tokens; }
+
+// 2^x for two values on the FMA pipe, within 2.3e-7: n = round(x) from the low bits of x + 1.5 * 2^23, and 2^(x - n) by a
+// polynomial of degree 5 whose largest relative error on [-0.5, 0.5] a linear program made smallest (6.8e-8 before rounding; the
+// constant term is held at 1, so that x <= -127 gives exactly 0).  NaN stays NaN.
+__device__ __forceinline__ float2 exp2_fma2(float2 x) {
+    constexpr float kMagic = 12582912.f;
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(x.x) : "f"(x.x));   // -127
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(x.y) : "f"(x.y));
+    const float2 t = add2(x, make_float2(kMagic, kMagic));
+    const float2 f = fma2(add2(t, make_float2(-kMagic, -kMagic)), make_float2(-1.f, -1.f), x);
+    float2 p = fma2(f, make_float2(0.0013202981790527701f, 0.0013202981790527701f),
+                    make_float2(0.009674952365458012f, 0.009674952365458012f));
+    p = fma2(p, f, make_float2(0.055510472506284714f, 0.055510472506284714f));
+    p = fma2(p, f, make_float2(0.24022166430950165f, 0.24022166430950165f));
+    p = fma2(p, f, make_float2(0.6931465864181519f, 0.6931465864181519f));
+    p = fma2(p, f, make_float2(1.f, 1.f));
+    return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
+                               __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000)));
+}
+
+// Which of the 8 four-column groups of 32 columns take two of their exponentials from the FMA pipe (bit e: group e).
+#ifndef B2A_WEIGHT_FMA_MASK
+#define B2A_WEIGHT_FMA_MASK 0xFFu
+#endif
+
+// Adds exp2(scale s + minus_lse2) of 32 columns, those of which `see` has a bit.
+template <bool kAll>
+__device__ __forceinline__ void weight_sum(const uint32_t (&s)[32], const float4* minus_lse2, float sl2, uint32_t see, float2 (&acc)[4]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float4 l4 = minus_lse2[e];
+        float2 p0 = fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), make_float2(sl2, sl2),
+                         make_float2(l4.x, l4.y));
+        float2 p1 = fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), make_float2(sl2, sl2),
+                         make_float2(l4.z, l4.w));
+        p0 = make_float2(fast_exp2(p0.x), fast_exp2(p0.y));
+        p1 = ((B2A_WEIGHT_FMA_MASK >> e) & 1u) ? exp2_fma2(p1) : make_float2(fast_exp2(p1.x), fast_exp2(p1.y));
+        if (!kAll) {
+            if (!((see >> (4 * e)) & 1u)) p0.x = 0.f;
+            if (!((see >> (4 * e + 1)) & 1u)) p0.y = 0.f;
+            if (!((see >> (4 * e + 2)) & 1u)) p1.x = 0.f;
+            if (!((see >> (4 * e + 3)) & 1u)) p1.y = 0.f;
+        }
+        acc[(2 * e) & 3] = add2(acc[(2 * e) & 3], p0);
+        acc[(2 * e + 1) & 3] = add2(acc[(2 * e + 1) & 3], p1);
+    }
+}
 
 __global__ void __launch_bounds__(kWeightThreads, 1)
 tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -74,7 +127,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kWeightQSlots; ++i) {
             mbar_init(smem_u32(&sh.q_full[i]), 1);
-            mbar_init(smem_u32(&sh.q_empty[i]), 1 + 8);      // the products, and the warps that read lse2
+            mbar_init(smem_u32(&sh.q_empty[i]), 1 + 8);      // the products, and the warps that read minus_lse2
         }
         for (int i = 0; i < kWeightKStages; ++i) {
             mbar_init(smem_u32(&sh.k_full[i]), 1);
@@ -97,6 +150,12 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         tmem_relinquish();
         tc_fence_before_sync();
     }
+    for (int k = threadIdx.x; k < p.tile_tokens; k += kWeightThreads) {
+        uint32_t columns[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) columns[c] = columns_from(k * p.c.group - 32 * c) & ~columns_from((k + 1) * p.c.group - 32 * c);
+        sh.token_columns[k] = make_uint4(columns[0], columns[1], columns[2], columns[3]);
+    }
     let_next_kernel_start();
     wait_for_previous_kernel();
     if (threadIdx.x == 0) {
@@ -116,7 +175,8 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         CacheWalk walk;
         walk.start(p.c, blockIdx.x, gridDim.x, lane);
-        SlotLoader loader{p.box_rows, kSlotBlock / p.box_rows, 0, 0, walk.bad};
+        SlotLoader loader(p.c.cache, p.box_rows);
+        loader.bad = walk.bad;
         uint32_t q_it = 0, k_it = 0;
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
@@ -141,44 +201,55 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             }
             if (!w.valid) break;
             const int tiles = weight_tiles(p, w.n);
-            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
-                for (int tile = tile0; tile < min(tile0 + 2, tiles); ++tile, ++q_it) {
-                    const uint32_t slot = q_it % kWeightQSlots;
-                    ok = mbar_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
-                    if (!ok) break;
-                    const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, w.n - tok0) * p.c.group;
+            auto load_tile = [&](int tile) {
+                const uint32_t slot = q_it % kWeightQSlots;
+                const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, w.n - tok0) * p.c.group;
+                // Read before the wait, which is for the last warp to be done with the tile that lies there.
+                float lse[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int r = c * 32 + lane;
-                        float lse = INFINITY;
-                        if (r < rows) {
-                            const int token = tok0 + r / p.c.group, head = w.head * p.c.group + r % p.c.group;
-                            lse = p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
-                                        (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)];
-                        }
-                        const bool live = !isinf(lse);
-                        sh.lse2[slot][r] = live ? lse * kLog2e : 0.f;
-                        const uint32_t bits = __ballot_sync(0xFFFFFFFFu, live);
-                        if (lane == 0) sh.live[slot][c] = bits;
+                for (int c = 0; c < 4; ++c) {
+                    const int r = c * 32 + lane;
+                    lse[c] = INFINITY;
+                    if (r < rows) {
+                        const int token = tok0 + r / p.c.group, head = w.head * p.c.group + r % p.c.group;
+                        lse[c] = p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
+                                       (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)];
                     }
-                    __syncwarp();
-                    if (lane == 0) {
-                        const uint32_t bar = smem_u32(&sh.q_full[slot]), dst = smem_u32(&sh.q[slot][0]);
-                        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.tile_tokens * p.c.group) * 256u);
-                        tma_load_3d(dst, &map_q, bar, 0, w.head * p.c.group, w.q_begin + tok0);
-                        tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, w.head * p.c.group, w.q_begin + tok0);
-                    }
-                    __syncwarp();
                 }
-                if (!ok) break;
+                ok = mbar_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
+                if (!ok) return;
+                ++q_it;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const bool live = !isinf(lse[c]);
+                    sh.minus_lse2[slot][c * 32 + lane] = live ? -lse[c] * kLog2e : 0.f;
+                    const uint32_t bits = __ballot_sync(0xFFFFFFFFu, live);
+                    if (lane == 0) sh.live[slot][c] = bits;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    const uint32_t bar = smem_u32(&sh.q_full[slot]), dst = smem_u32(&sh.q[slot][0]);
+                    mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.tile_tokens * p.c.group) * 256u);
+                    tma_load_3d(dst, &map_q, bar, 0, w.head * p.c.group, w.q_begin + tok0);
+                    tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, w.head * p.c.group, w.q_begin + tok0);
+                }
+                __syncwarp();
+            };
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
                 loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-                for (int i = 0; i < w.blocks; ++i, ++k_it) {
-                    const SlotLoader now = loader;
+                load_tile(tile0);
+                for (int i = 0; i < w.blocks && ok; ++i, ++k_it) {
+                    SlotLoader now = loader;
                     if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+                    const int boxes = now.count(w.j0 + i, w.slots);
                     const uint32_t stage = k_it % kWeightKStages;
                     ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
                     if (!ok) break;
-                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, now.count(w.j0 + i, w.slots), lane);
+                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
+                    now.check(p.c.cache, boxes, lane);
+                    loader.bad |= now.bad;
+                    // The pair's second tile may have to wait for a slot: the first blocks are on their way by then.
+                    if (tile0 + 1 < tiles && i == min(kWeightKStages, w.blocks) - 1) load_tile(tile0 + 1);
                 }
             }
             if (!ok) break;
@@ -192,6 +263,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         uint32_t q_it = 0, k_it = 0;
         uint32_t s_it[2] = {0, 0};
         bool ok = true;
+        PH_DECL(5)   // 0 other, 1 wait K, 2 wait Q, 3 wait S, 4 issue
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
             ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 4);
@@ -208,8 +280,10 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const int here = min(2, tiles - tile0);
                 for (int i = 0; i < blocks && ok; ++i, ++k_it) {
                     const uint32_t stage = k_it % kWeightKStages;
+                    PH_MARK(0);
                     ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), (k_it / kWeightKStages) & 1u, 5);
                     if (!ok) break;
+                    PH_MARK(1);
                     const uint32_t x = i & 1;
                     for (int t = 0; t < here; ++t) {
                         const uint32_t slot = (q_it + t) % kWeightQSlots;
@@ -217,10 +291,12 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                             ok = mbar_wait(wctx, smem_u32(&sh.q_full[slot]), ((q_it + t) / kWeightQSlots) & 1u, 6);
                             if (!ok) break;
                         }
+                        PH_MARK(2);
                         const uint32_t count = x ? s_it[1]++ : s_it[0]++;
                         const uint32_t buf = 2 * x + (count & 1u);
                         ok = mbar_wait(wctx, smem_u32(&sh.s_empty[buf]), ((count >> 1) & 1u) ^ 1u, 7);
                         if (!ok) break;
+                        PH_MARK(3);
                         // As many columns as the tile has rows, in steps of 16.
                         const int rows = min(p.tile_tokens, n - (tile0 + t) * p.tile_tokens) * p.c.group;
                         const uint32_t idesc = make_idesc_bf16(kTileM, (rows + 15) & ~15, 0, 0);
@@ -229,18 +305,21 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         tc_commit_w(smem_u32(&sh.s_full[buf]));
                         if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[slot]));
                         __syncwarp();
+                        PH_MARK(4);
                     }
                     tc_commit_w(smem_u32(&sh.k_empty[stage]));
                 }
                 q_it += here;
             }
         }
+        PH_PRINT("weights mma", 5);
     } else if (warp < 8) {
         const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t s_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const float sl2 = p.scale_log2;
         uint32_t q_it = 0, s_it = 0;
         bool ok = true;
+        PH_DECL(4)   // 0 other, 1 wait S, 2 sums
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
             ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 8);
@@ -262,69 +341,65 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         const uint32_t buf = 2 * x + (s_it & 1u), q_slot = (q_it + t) % kWeightQSlots;
                         const int tok0 = (tile0 + t) * p.tile_tokens, tokens = min(p.tile_tokens, w.n - tok0);
                         const int rows = tokens * p.c.group;
-                        // Which columns see this slot: all of them before the drafted tokens.
-                        uint32_t bits[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                        // Which columns see this slot: all of them if it lies before the drafted tokens.
+                        uint4 some = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
                         const int u = slot - w.len;
                         if (tail && u >= 0) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) bits[c] = 0u;
-                            if (slot < w.slots) {
-                                const unsigned char* mask = p.c.mask;
-                                if (mask != nullptr) {
-                                    mask += (p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + tok0 * p.c.mask_stride[1]
-                                                                         : (static_cast<long long>(w.q_begin) + tok0) * p.c.mask_stride[1]) + u;
-                                }
-#pragma unroll 4
+                            some = make_uint4(0u, 0u, 0u, 0u);
+                            if (slot < w.slots && p.c.mask == nullptr) {
+                                const int from = max(0, u - tok0) * p.c.group;   // the first column that does
+                                some = make_uint4(columns_from(from), columns_from(from - 32), columns_from(from - 64), columns_from(from - 96));
+                            } else if (slot < w.slots) {
+                                const unsigned char* mask = p.c.mask + u +
+                                    (p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + tok0 * p.c.mask_stride[1]
+                                                                 : (static_cast<long long>(w.q_begin) + tok0) * p.c.mask_stride[1]);
+#pragma unroll 8
                                 for (int k = 0; k < tokens; ++k) {
-                                    if (mask == nullptr ? u > tok0 + k : mask[k * p.c.mask_stride[1]] == 0) continue;
-#pragma unroll
-                                    for (int c = 0; c < 4; ++c) {
-                                        const int lo = min(max(k * p.c.group - 32 * c, 0), 32);
-                                        const int hi = min(max((k + 1) * p.c.group - 32 * c, 0), 32);
-                                        const uint32_t below_hi = hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u;
-                                        const uint32_t below_lo = lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u;
-                                        bits[c] |= below_hi & ~below_lo;
+                                    const uint4 columns = sh.token_columns[k];
+                                    if (mask[k * p.c.mask_stride[1]] != 0) {
+                                        some.x |= columns.x;
+                                        some.y |= columns.y;
+                                        some.z |= columns.z;
+                                        some.w |= columns.w;
                                     }
                                 }
                             }
                         }
+                        PH_MARK(0);
                         ok = mbar_wait(wctx, smem_u32(&sh.s_full[buf]), (s_it >> 1) & 1u, 9);
                         if (!ok) break;
+                        PH_MARK(1);
                         tc_fence_after_sync();
-                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                        float2 acc[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.f, 0.f);
+                        const uint4 live = *reinterpret_cast<const uint4*>(&sh.live[q_slot][0]);
+                        const uint32_t see[4] = {some.x & live.x, some.y & live.y, some.z & live.z, some.w & live.w};
+                        const uint32_t from = s_tmem + buf * 128u;
+                        const float4* lse2 = reinterpret_cast<const float4*>(&sh.minus_lse2[q_slot][0]);
+                        // The next 32 columns are on their way out of tensor memory while these are added up.
+                        uint32_t s0[32], s1[32];
+                        tmem_ld_x32(from, s0);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            if (c * 32 >= rows) break;
-                            uint32_t s[32];
-                            tmem_ld_x32(s_tmem + buf * 128u + c * 32, s);
-                            tmem_wait_ld();
-                            const uint32_t see = bits[c] & sh.live[q_slot][c];
-                            const bool all = __all_sync(0xFFFFFFFFu, see == 0xFFFFFFFFu);
-                            const float4* lse2 = reinterpret_cast<const float4*>(&sh.lse2[q_slot][c * 32]);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                if (c * 32 + e * 4 >= rows) break;
-                                const float4 l4 = lse2[e];
-                                float2 p0 = fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])),
-                                                 make_float2(sl2, sl2), make_float2(-l4.x, -l4.y));
-                                float2 p1 = fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])),
-                                                 make_float2(sl2, sl2), make_float2(-l4.z, -l4.w));
-                                p0 = make_float2(fast_exp2(p0.x), fast_exp2(p0.y));
-                                p1 = make_float2(fast_exp2(p1.x), fast_exp2(p1.y));
-                                if (!all) {
-                                    if (!((see >> (4 * e)) & 1u)) p0.x = 0.f;
-                                    if (!((see >> (4 * e + 1)) & 1u)) p0.y = 0.f;
-                                    if (!((see >> (4 * e + 2)) & 1u)) p1.x = 0.f;
-                                    if (!((see >> (4 * e + 3)) & 1u)) p1.y = 0.f;
+                            if (c * 32 < rows) {
+                                tmem_wait_ld();
+                                if ((c + 1) * 32 < rows) {
+                                    if (c & 1) tmem_ld_x32(from + (c + 1) * 32, s0); else tmem_ld_x32(from + (c + 1) * 32, s1);
                                 }
-                                acc[0] = add2(acc[0], p0);
-                                acc[1] = add2(acc[1], p1);
+                                if (__all_sync(0xFFFFFFFFu, see[c] == 0xFFFFFFFFu)) {
+                                    weight_sum<true>(c & 1 ? s1 : s0, lse2 + c * 8, sl2, see[c], acc);
+                                } else {
+                                    weight_sum<false>(c & 1 ? s1 : s0, lse2 + c * 8, sl2, see[c], acc);
+                                }
                             }
                         }
+                        const float2 both = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&sh.s_empty[buf]));
-                        sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+                        sum += both.x + both.y;
+                        PH_MARK(2);
                     }
                     if (!ok) break;
                     if (!last) {
@@ -345,6 +420,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
         }
+        PH_PRINT("weights", 3);
     }
 
     tc_fence_before_sync();

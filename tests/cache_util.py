@@ -21,7 +21,7 @@ class Cache:
     """
 
     def __init__(self, seed, seqs, slots, kvh, page=0, layout="plain", device="cuda"):
-        gen = torch.Generator().manual_seed(seed)
+        gen = torch.Generator().manual_seed(seed + 77777)     # a stream of its own: no key equals a query
         self.kvh, self.page, self.seqs = kvh, page, seqs
         width = 1 if page == 0 else -(-slots // page)
         size = slots if page == 0 else page
@@ -95,16 +95,18 @@ def ancestors(rng, count):
 
 
 def tree_attention(q, k, v, seen):
-    """One sequence in 64 bits: q [n, QH, 128], k, v [slots, KVH, 128], seen [n, slots] -> out [n, QH, 128], lse [QH, n].
-    What a row does not see has no part in it, whatever it is."""
+    """One sequence in 64 bits: q [n, QH, 128], k, v [slots, KVH, 128], seen [n, slots] -> out [n, QH, 128], lse [QH, n], and
+    the root of the sum of the squares of out's terms.  What a row does not see has no part in it, whatever it is."""
     group = q.size(1) // k.size(1)
     q, k, v = q.double(), k.double(), v.double()
-    out, lse = torch.zeros_like(q), torch.full((q.size(1), q.size(0)), -math.inf, dtype=torch.float64)
+    out, spread, lse = torch.zeros_like(q), torch.zeros_like(q), torch.full((q.size(1), q.size(0)), -math.inf, dtype=torch.float64)
     for i in range(q.size(0)):
         if not seen[i].any():
             continue
         ki, vi = k[seen[i]].repeat_interleave(group, 1), v[seen[i]].repeat_interleave(group, 1)
         s = torch.einsum("hd,shd->hs", q[i], ki) / math.sqrt(128)
         lse[:, i] = s.logsumexp(1)
-        out[i] = torch.einsum("hs,shd->hd", s.softmax(1), vi)
-    return out, lse
+        p = s.softmax(1)
+        out[i] = torch.einsum("hs,shd->hd", p, vi)
+        spread[i] = torch.einsum("hs,shd->hd", p * p, vi * vi).sqrt()
+    return out, lse, spread
