@@ -62,6 +62,12 @@ inline int make_cache_view(const b2a_cache& c, int batch, bool needs_v, CacheVie
     return B2A_OK;
 }
 
+// mbar_wait for a whole warp, with one answer for all its lanes: a lane that gave up alone would leave the others waiting for it at
+// the next warp-wide instruction.
+__device__ __forceinline__ bool warp_wait(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t tag) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(ctx, bar, parity, tag));
+}
+
 // ---------------------------------------------------------------------------------------
 // Work of the kernels that stream the cache once: all blocks of 128 slots of all (sequence, group of query tokens, K/V head),
 // in this order, are dealt out to the CTAs in runs of equal length.  The lengths are on the device, so every CTA finds its

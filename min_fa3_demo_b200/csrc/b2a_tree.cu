@@ -21,7 +21,7 @@
 // Masked slots: a score is replaced, not added to, so NaN and infinities in K that a row does not see have no effect.  V
 // rows behind the last slot are zeroed in shared memory before the product (0 * NaN is NaN), and so are values of drafted
 // tokens that are not finite; those are added back to the rows that see them at the end.
-#include "b2a_cache.cuh"
+#include "b2a_tree.cuh"
 
 #include <cmath>
 
@@ -33,41 +33,6 @@ constexpr int kTreeThreads = 384;
 constexpr int kTreeStages = 2;
 constexpr int kTreeSlots = 4;       // pieces in flight between the load warp and the others
 constexpr int kTreeQkWarp = 8, kTreeLoadWarp = 9, kTreePvWarp = 10, kTreeVWarp = 11;
-constexpr int kTreeMaxCtas = kFwdStatusWords;
-
-struct TreeParams {
-    CacheQueries c;
-    __nv_bfloat16* out;
-    float* lse;
-    long long lse_seq_stride;    // 0 for packed queries
-    long long lse_head_stride;
-    int tile_tokens;             // 128 / group
-    int box_rows;
-    float scale_log2;
-    unsigned int* status;        // a word for each CTA, behind the header
-    uint32_t timeout_ns;
-    // Pieces that do not cover their item: two a CTA, the one its run begins with and the one it ends with.
-    struct TreeCut* cuts;        // [CTAs]: the item that a run begins inside of
-    float2* part_stat;           // [2 * CTAs][2 tiles][part_rows] (row maximum, row sum)
-    float4* part_o;              // [2 * CTAs][2 tiles][32][part_rows] O before the division
-    int part_rows;
-};
-
-struct TreeCut {
-    long long first, last;       // the item's blocks in the row of all
-    int run;                     // 0: the CTA's run does not begin inside an item
-    int seq, q_begin, tok0, n, head;
-    int pad[2];
-};
-
-struct TreePiece {
-    int valid;
-    int seq, q_begin, n, len, slots, head;
-    int tok0;        // first token
-    int tokens[2];   // of the two tiles
-    int j0, blocks;
-    int part;        // where its part goes; -1: it covers the item
-};
 
 struct __align__(1024) TreeShared {
     uint8_t q[2][kTileBytes];
@@ -93,17 +58,6 @@ static_assert(kTreeSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
 // Whether a block goes to warpgroup x: both tiles take every block, one tile's warpgroups take turns.
 __device__ __forceinline__ bool tree_takes(bool two, int i, int x) { return two || (i & 1) == x; }
-
-__device__ __forceinline__ const unsigned char* tree_mask_row(const TreeParams& p, const TreePiece& w, int token) {
-    return p.c.mask + (p.c.cu_seqlens_q == nullptr ? w.seq * p.c.mask_stride[0] + token * p.c.mask_stride[1]
-                                                   : (static_cast<long long>(w.q_begin) + token) * p.c.mask_stride[1]);
-}
-
-__device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreePiece& w, int token, int u) {
-    return p.c.mask == nullptr ? u <= token : tree_mask_row(p, w, token)[u] != 0;
-}
-
-__device__ __forceinline__ bool bf16_not_finite(uint32_t half) { return (half & 0x7F80u) == 0x7F80u; }
 
 // Values of drafted tokens that are not finite, added to a row that sees them: columns [column, column + 32) of O.
 // Only the sign of the weight, which is positive, matters.
@@ -196,20 +150,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
             CacheWalk walk;
             walk.start(p.c, blockIdx.x, gridDim.x, lane);
-            if (lane == 0) {
-                TreeCut cut{};
-                if (walk.pos < walk.end && walk.j > 0) {
-                    cut.first = walk.pos - walk.j;
-                    cut.last = cut.first + walk.blocks;
-                    cut.run = walk.run;
-                    cut.seq = walk.seq;
-                    cut.q_begin = walk.s.q_begin;
-                    cut.tok0 = walk.rt * p.c.item_tokens;
-                    cut.n = walk.s.n;
-                    cut.head = walk.head;
-                }
-                p.cuts[blockIdx.x] = cut;
-            }
+            if (lane == 0) p.cuts[blockIdx.x] = tree_cut(p, walk);
             SlotLoader loader(p.c.cache, p.box_rows);
             loader.bad = walk.bad;
             uint32_t k_it = 0, q_par = 0;
@@ -217,32 +158,17 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             PH_DECL(3)   // 0 other, 1 wait for K's stage, 2 issue K
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTreeSlots;
-                ok = mbar_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTreeSlots) & 1u) ^ 1u, 1);
+                ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTreeSlots) & 1u) ^ 1u, 1);
                 if (!ok) break;
-                TreePiece w{};
-                w.valid = walk.pos < walk.end;
-                if (w.valid) {
-                    w.seq = walk.seq;
-                    w.q_begin = walk.s.q_begin;
-                    w.n = walk.s.n;
-                    w.len = walk.s.len;
-                    w.slots = walk.s.slots;
-                    w.head = walk.head;
-                    w.tok0 = walk.rt * p.c.item_tokens;
-                    w.tokens[0] = min(p.tile_tokens, w.n - w.tok0);
-                    w.tokens[1] = max(0, min(p.tile_tokens, w.n - w.tok0 - p.tile_tokens));
-                    w.j0 = walk.j;
-                    w.blocks = walk.piece();
-                    w.part = w.blocks == walk.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (begun ? 1 : 0);
-                    begun = true;
-                }
+                const TreePiece w = tree_piece(p, walk, begun);
+                begun = true;
                 if (lane == 0) {
                     sh.piece[at] = w;
                     mbar_arrive(smem_u32(&sh.piece_full[at]));
                 }
                 if (!w.valid) break;
                 auto load_q = [&](int x) {
-                    ok = mbar_wait(wctx, smem_u32(&sh.q_empty[x]), ((q_par >> x) & 1u) ^ 1u, 2);
+                    ok = warp_wait(wctx, smem_u32(&sh.q_empty[x]), ((q_par >> x) & 1u) ^ 1u, 2);
                     if (!ok) return;
                     q_par ^= 1u << x;
                     if (lane == 0) {
@@ -262,7 +188,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     const int boxes = now.count(w.j0 + i, w.slots);
                     const uint32_t stage = k_it % kTreeStages;
                     PH_MARK(0);
-                    ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
+                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
                     if (!ok) break;
                     PH_MARK(1);
                     now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
@@ -278,33 +204,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             PH_PRINT("tree load", 3);
         } else if (warp == kTreeVWarp) {
             // ------------------------------------------------------------ loads of V
-            SlotLoader loader(p.c.cache, p.box_rows);
-            uint32_t v_it = 0;
-            bool ok = true;
-            PH_DECL(3)   // 0 other, 1 wait for V's stage, 2 issue V
-            for (uint32_t it = 0; ok; ++it) {
-                const uint32_t at = it % kTreeSlots;
-                ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 4);
-                if (!ok) break;
-                const TreePiece w = sh.piece[at];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
-                if (!w.valid) break;
-                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-                for (int i = 0; i < w.blocks; ++i, ++v_it) {
-                    SlotLoader now = loader;
-                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-                    const int boxes = now.count(w.j0 + i, w.slots);
-                    const uint32_t stage = v_it % kTreeStages;
-                    PH_MARK(0);
-                    ok = mbar_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kTreeStages) & 1u) ^ 1u, 18);
-                    if (!ok) break;
-                    PH_MARK(1);
-                    now.load(&map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
-                    PH_MARK(2);
-                }
-            }
-            PH_PRINT("tree load", 3);
+            tree_load_v<kTreeSlots, kTreeStages>(p, sh, &map_v, wctx, lane);
         } else if (warp == kTreeQkWarp || warp == kTreePvWarp) {
             // ------------------------------------------------------------ MMA warps
             const bool qk = warp == kTreeQkWarp;
@@ -319,7 +219,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             PH_DECL(4)   // 0 other, 1 wait K (V), 2 wait S (P), 3 issue
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTreeSlots;
-                ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 5);
+                ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 5);
                 if (!ok) break;
                 const volatile TreePiece& w = sh.piece[at];
                 const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
@@ -340,7 +240,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             if (!tree_takes(two, i, x)) continue;
                             const int tile = two ? x : 0;
                             if (i == 0) {
-                                ok = mbar_wait(wctx, smem_u32(&sh.q_full[tile]), (par >> tile) & 1u, 7);
+                                ok = warp_wait(wctx, smem_u32(&sh.q_full[tile]), (par >> tile) & 1u, 7);
                                 if (!ok) break;
                                 par ^= 1u << tile;
                             }
@@ -400,7 +300,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kTreeSlots;
-            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 11);
+            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTreeSlots) & 1u, 11);
             if (!ok) break;
             const TreePiece& w = sh.piece[at];
             auto release = [&]() {
@@ -480,7 +380,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
                 if (tail) {
                     if (masked) {
-                        ok = mbar_wait(wctx, smem_u32(&sh.seen_full[x]), seen_cnt & 1u, 13);
+                        ok = warp_wait(wctx, smem_u32(&sh.seen_full[x]), seen_cnt & 1u, 13);
                         if (!ok) break;
                         ++seen_cnt;
                     }
@@ -496,35 +396,11 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             if (!ok) break;
                         }
                         const uint32_t stage = (kv_base + i) % kTreeStages;
-                        ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / kTreeStages) & 1u, 14);
+                        ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / kTreeStages) & 1u, 14);
                         if (!ok) break;
-                        // Another chunk first in each row, so that rows of 128 bytes do not meet in the same banks.
-                        uint8_t* row = &sh.v[stage][r * 128];
-                        auto chunk = [&](int c) { return reinterpret_cast<uint4*>(row + (c >> 3) * kHalfTileBytes + (((c + r) & 7) * 16)); };
-                        if (slot >= w.slots) {
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) *chunk(c) = make_uint4(0u, 0u, 0u, 0u);
-                        } else if (look) {
-                            uint32_t ones = 0;      // an exponent of all ones carries into its half's sign bit
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) {
-                                const uint4 v = *chunk(c);
-                                ones |= ((v.x & 0x7F807F80u) + 0x00800080u) | ((v.y & 0x7F807F80u) + 0x00800080u) |
-                                        ((v.z & 0x7F807F80u) + 0x00800080u) | ((v.w & 0x7F807F80u) + 0x00800080u);
-                            }
-                            if ((ones & 0x80008000u) != 0u) {
+                        if (slot >= w.slots || look) {
+                            if (tree_clean_row(&sh.v[stage][r * 128], r, slot >= w.slots)) {
                                 *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
-#pragma unroll 1
-                                for (int c = 0; c < 16; ++c) {
-                                    const uint4 v = *chunk(c);
-                                    uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        if (bf16_not_finite(words[e])) words[e] &= 0xFFFF0000u;
-                                        if (bf16_not_finite(words[e] >> 16)) words[e] &= 0xFFFFu;
-                                    }
-                                    *chunk(c) = make_uint4(words[0], words[1], words[2], words[3]);
-                                }
                             }
                         }
                         fence_proxy_async_smem();
@@ -589,7 +465,8 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         tmem_st_x32(o_tmem + x * 128 + c * 32, t);
                     }
                 }
-                const float neg_m = m_used == -INFINITY ? 0.f : -m_used * sl2;
+                // P stays below 1 however far the maximum has moved since, so that no product with a finite V overflows.
+                const float neg_m = m_used == -INFINITY ? 0.f : -m_used * sl2 - kRescaleThreshold;
                 const float2 sl2v = make_float2(sl2, sl2), negv = make_float2(neg_m, neg_m);
                 float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -635,7 +512,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 sh.stat[x][r] = make_float2(m_used, l);
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&sh.both_done));
-                ok = mbar_wait(wctx, smem_u32(&sh.both_done), both_cnt & 1u, 16);
+                ok = warp_wait(wctx, smem_u32(&sh.both_done), both_cnt & 1u, 16);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const float2 s0 = sh.stat[0][r], s1 = sh.stat[1][r];
@@ -652,7 +529,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const bool whole = w.part < 0;
                 if (row_valid && (two || x == 0)) {
                     if (whole) {
-                        const float lse = l == 0.f ? -INFINITY : (m_used * sl2 + fast_log2(l)) * kLn2;
+                        const float lse = l == 0.f ? -INFINITY : (m_used * sl2 + kRescaleThreshold + fast_log2(l)) * kLn2;
                         const int head = w.head * p.c.group + row_head;
                         p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
                               (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)] = lse;
@@ -710,7 +587,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (!two) {
                 // Neither warpgroup's next product may overwrite an O that the other still reads.
                 mbar_arrive(smem_u32(&sh.both_read));
-                ok = mbar_wait(wctx, smem_u32(&sh.both_read), both_cnt & 1u, 17);
+                ok = warp_wait(wctx, smem_u32(&sh.both_read), both_cnt & 1u, 17);
                 ++both_cnt;
                 if (!ok) break;
             }
@@ -775,7 +652,7 @@ tree_combine(const __grid_constant__ TreeParams p) {
             const int r = row0 + lane, token = tok0 + r / p.c.group;
             p.lse[cut.seq * p.lse_seq_stride + (cut.head * p.c.group + r % p.c.group) * p.lse_head_stride +
                   (p.c.cu_seqlens_q == nullptr ? token : cut.q_begin + token)] =
-                l == 0.f ? -INFINITY : (m * p.scale_log2 + fast_log2(l)) * kLn2;
+                l == 0.f ? -INFINITY : (m * p.scale_log2 + kRescaleThreshold + fast_log2(l)) * kLn2;
         }
     }
     // Lane = row, four of the 32 column quads a warp.
@@ -818,20 +695,23 @@ int set_tree_smem() {
 }
 
 struct TreeLayout {
-    int ctas, tile_tokens, tiles, rows;
-    size_t cuts, stat, o, total;   // offsets
+    int ctas, tile_tokens, tiles, rows;   // rows of a tile; few rows: of an item, which is one tile
+    bool few;
+    size_t cuts, stat, o, total;          // offsets
 };
 
 TreeLayout tree_layout(int seqlen_q, int group, int sms) {
     TreeLayout t{};
     t.ctas = sms < kTreeMaxCtas ? sms : kTreeMaxCtas;
-    t.tile_tokens = kTileM / group;
+    t.few = static_cast<long long>(seqlen_q) * group <= kFewRows;
+    t.tile_tokens = t.few ? seqlen_q : kTileM / group;
     t.tiles = seqlen_q > t.tile_tokens ? 2 : 1;
     t.rows = (t.tiles == 2 ? t.tile_tokens : seqlen_q) * group;
     t.cuts = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
     t.stat = t.cuts + align_up(t.ctas * sizeof(TreeCut), 256);
-    t.o = t.stat + align_up(4ull * t.ctas * t.rows * sizeof(float2), 256);
-    t.total = t.o + 4ull * t.ctas * t.rows * kHeadDim * sizeof(float);
+    const size_t parts = 2ull * t.ctas * (t.few ? 1 : 2) * t.rows;
+    t.o = t.stat + align_up(parts * sizeof(float2), 256);
+    t.total = t.o + parts * kHeadDim * sizeof(float);
     return t;
 }
 
@@ -867,7 +747,7 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     if (a->workspace_bytes < t.total) {
         return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, t.total);
     }
-    p.c.item_tokens = 2 * t.tile_tokens;
+    p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
     p.c.min_run = 2;
     p.box_rows = slot_box_rows(p.c.cache);
     CUtensorMap map_q, map_k, map_v;
@@ -875,7 +755,7 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     rc = make_strided_map(&map_q, a->q, 3, q_sizes, a->q_stride, static_cast<uint32_t>(p.c.group), static_cast<uint32_t>(t.tile_tokens));
     if (rc == B2A_OK) rc = make_slot_map(&map_k, p.c.cache, true, p.box_rows);
     if (rc == B2A_OK) rc = make_slot_map(&map_v, p.c.cache, false, p.box_rows);
-    if (rc == B2A_OK) rc = once_per_device(dev.device, 6, set_tree_smem);
+    if (rc == B2A_OK && !t.few) rc = once_per_device(dev.device, 6, set_tree_smem);
     if (rc != B2A_OK) return rc;
 
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -893,6 +773,7 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     p.part_rows = t.rows;
 
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (t.few) return launch_tree_few(map_q, map_k, map_v, p, t.ctas, dev, stream);
     auto attention = tree_attention;
     auto combine = tree_combine;
     B2A_CUDA_OK(launch_early(attention, t.ctas, kTreeThreads, kTreeSmemBytes, stream, map_q, map_k, map_v, p));

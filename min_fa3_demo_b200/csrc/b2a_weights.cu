@@ -181,7 +181,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
-            ok = mbar_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kWeightSlots) & 1u) ^ 1u, 1);
+            ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kWeightSlots) & 1u) ^ 1u, 1);
             if (!ok) break;
             WeightPiece w{};
             w.valid = walk.pos < walk.end;
@@ -216,7 +216,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                                        (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)];
                     }
                 }
-                ok = mbar_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
+                ok = warp_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
                 if (!ok) return;
                 ++q_it;
 #pragma unroll
@@ -243,7 +243,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
                     const int boxes = now.count(w.j0 + i, w.slots);
                     const uint32_t stage = k_it % kWeightKStages;
-                    ok = mbar_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
+                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
                     if (!ok) break;
                     now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
                     now.check(p.c.cache, boxes, lane);
@@ -266,7 +266,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         PH_DECL(5)   // 0 other, 1 wait K, 2 wait Q, 3 wait S, 4 issue
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
-            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 4);
+            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 4);
             if (!ok) break;
             const volatile WeightPiece& w = sh.piece[at];
             const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
@@ -281,20 +281,20 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 for (int i = 0; i < blocks && ok; ++i, ++k_it) {
                     const uint32_t stage = k_it % kWeightKStages;
                     PH_MARK(0);
-                    ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), (k_it / kWeightKStages) & 1u, 5);
+                    ok = warp_wait(wctx, smem_u32(&sh.k_full[stage]), (k_it / kWeightKStages) & 1u, 5);
                     if (!ok) break;
                     PH_MARK(1);
                     const uint32_t x = i & 1;
                     for (int t = 0; t < here; ++t) {
                         const uint32_t slot = (q_it + t) % kWeightQSlots;
                         if (i == 0) {
-                            ok = mbar_wait(wctx, smem_u32(&sh.q_full[slot]), ((q_it + t) / kWeightQSlots) & 1u, 6);
+                            ok = warp_wait(wctx, smem_u32(&sh.q_full[slot]), ((q_it + t) / kWeightQSlots) & 1u, 6);
                             if (!ok) break;
                         }
                         PH_MARK(2);
                         const uint32_t count = x ? s_it[1]++ : s_it[0]++;
                         const uint32_t buf = 2 * x + (count & 1u);
-                        ok = mbar_wait(wctx, smem_u32(&sh.s_empty[buf]), ((count >> 1) & 1u) ^ 1u, 7);
+                        ok = warp_wait(wctx, smem_u32(&sh.s_empty[buf]), ((count >> 1) & 1u) ^ 1u, 7);
                         if (!ok) break;
                         PH_MARK(3);
                         // As many columns as the tile has rows, in steps of 16.
@@ -322,7 +322,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         PH_DECL(4)   // 0 other, 1 wait S, 2 sums
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
-            ok = mbar_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 8);
+            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 8);
             if (!ok) break;
             const WeightPiece& w = sh.piece[at];
             if (!w.valid) break;
@@ -366,7 +366,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                             }
                         }
                         PH_MARK(0);
-                        ok = mbar_wait(wctx, smem_u32(&sh.s_full[buf]), (s_it >> 1) & 1u, 9);
+                        ok = warp_wait(wctx, smem_u32(&sh.s_full[buf]), (s_it >> 1) & 1u, 9);
                         if (!ok) break;
                         PH_MARK(1);
                         tc_fence_after_sync();
@@ -411,7 +411,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 // A warp without a block here has waited for nothing yet: it may give back no tile that is still to come.
                 for (int t = 0; t < here && ok; ++t, ++q_it) {
                     const uint32_t q_slot = q_it % kWeightQSlots;
-                    ok = mbar_wait(wctx, smem_u32(&sh.q_full[q_slot]), (q_it / kWeightQSlots) & 1u, 10);
+                    ok = warp_wait(wctx, smem_u32(&sh.q_full[q_slot]), (q_it / kWeightQSlots) & 1u, 10);
                     __syncwarp();
                     if (ok && lane == 0) mbar_arrive(smem_u32(&sh.q_empty[q_slot]));
                 }
