@@ -495,7 +495,7 @@ typedef struct b2a_evict_args {
 } b2a_evict_args;
 
 /* Scratch of b2a_cache_evict; 0 for sizes that it refuses. */
-size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget);
+size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget, int32_t weights_slots);
 
 /*
  * Cuts sequences that are longer than the budget down to it, in place, for each K/V head by itself: the last `recent` slots stay,

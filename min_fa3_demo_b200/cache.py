@@ -395,7 +395,7 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     order = torch.empty((batch, kvh, budget), dtype=_INT32, device=device)
     lib = _cabi.load()
     with _on_device(device):
-        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget)
+        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget, weights.size(2))
         ws = _workspace(nbytes, device)
         args = _cabi.EVICT.pack(
             *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), weights.data_ptr(), weights.stride(0),

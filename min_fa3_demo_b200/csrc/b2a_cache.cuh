@@ -18,15 +18,33 @@ struct CacheView {
     int page_size;
     int heads;
     int table_width;
+    unsigned int per_page;      // 2^32 / page_size, rounded up
 
-    __device__ __forceinline__ long long capacity() const {   // slots of a sequence
-        return block_table == nullptr ? page_size : static_cast<long long>(page_size) * table_width;
+    __device__ __forceinline__ int capacity() const {   // slots of a sequence
+        return block_table == nullptr ? page_size : page_size * table_width;
     }
-    // Page of a slot; -1: there is none.
-    __device__ __forceinline__ int page_of(int seq, long long slot) const {
+    // A slot's number in the block table, and its row there, without a division: the high half of slot * per_page is the
+    // quotient or one more.
+    __device__ __forceinline__ int entry_of(int slot, int* row) const {
+        int at = static_cast<int>(__umulhi(static_cast<unsigned int>(slot), per_page));
+        *row = slot - at * page_size;
+        if (*row < 0) {
+            --at;
+            *row += page_size;
+        }
+        return at;
+    }
+    // Page of a slot, and its row; -1: there is none.
+    __device__ __forceinline__ int page_of(int seq, long long slot, int* row) const {
         if (slot < 0 || slot >= capacity()) return -1;
-        const int page = block_table == nullptr ? seq : block_table[seq * table_stride + slot / page_size];
+        *row = static_cast<int>(slot);
+        if (block_table == nullptr) return seq;
+        const int page = block_table[seq * table_stride + entry_of(static_cast<int>(slot), row)];
         return page >= 0 && page < pages ? page : -1;
+    }
+    // Where a slot's head lies in K (V), in elements; -1: nowhere.
+    __device__ __forceinline__ long long at(const long long (&stride)[3], int page, int row, int head) const {
+        return page < 0 ? -1 : page * stride[0] + row * stride[1] + head * stride[2];
     }
 };
 
@@ -59,6 +77,7 @@ inline int make_cache_view(const b2a_cache& c, int batch, bool needs_v, CacheVie
     view->page_size = c.page_size;
     view->heads = c.heads_k;
     view->table_width = c.table_width;
+    view->per_page = c.page_size == 1 ? 0xFFFFFFFFu : 0xFFFFFFFFu / static_cast<unsigned int>(c.page_size) + 1u;
     return B2A_OK;
 }
 
@@ -110,7 +129,7 @@ __device__ __forceinline__ CacheSeq cache_seq(const CacheQueries& p, int b) {
     }
     s.bad = begin < 0 || end < begin || end > p.total_q || end - begin > p.seqlen_q;
     const long long n = s.bad ? 0 : end - begin;
-    const long long cap = min(p.cache.capacity(), static_cast<long long>(p.limit_slots));
+    const long long cap = min(p.cache.capacity(), p.limit_slots);
     s.q_begin = static_cast<int>(begin);
     s.n = static_cast<int>(n);
     s.len = static_cast<int>(min(max(len, 0ll), cap));
@@ -236,12 +255,10 @@ inline int make_slot_map(CUtensorMap* map, const CacheView& c, bool keys, int bo
 // answer only when it needs it, so that neither the block table's latency nor a division is on the path.
 struct SlotLoader {
     int box_rows, boxes;
-    uint32_t per_page;       // 2^32 / page_size, rounded up: the high half of slot * per_page is slot / page_size or one more
     int page, row;
     int bad;                 // this lane met a page that does not exist (TMA fills such a box with zeros)
 
-    __device__ __forceinline__ SlotLoader(const CacheView& c, int rows)
-        : box_rows(rows), boxes(kSlotBlock / rows), per_page(0xFFFFFFFFu / static_cast<uint32_t>(c.page_size) + 1u), page(0), row(0), bad(0) {}
+    __device__ __forceinline__ explicit SlotLoader(int rows) : box_rows(rows), boxes(kSlotBlock / rows), page(0), row(0), bad(0) {}
 
     __device__ __forceinline__ void look_up(const CacheView& c, int seq, int block, int slots, int lane) {
         const int slot = block * kSlotBlock + lane * box_rows;
@@ -251,12 +268,7 @@ struct SlotLoader {
             row = slot;
             return;
         }
-        int at = static_cast<int>(__umulhi(static_cast<uint32_t>(slot), per_page));
-        row = slot - at * c.page_size;
-        if (row < 0) {
-            --at;
-            row += c.page_size;
-        }
+        const int at = c.entry_of(slot, &row);
         page = c.block_table[seq * c.table_stride + at];
     }
     // Boxes of a block that hold slots.

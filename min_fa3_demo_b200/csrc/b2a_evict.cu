@@ -20,6 +20,7 @@ namespace b2a {
 namespace {
 
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectKeys = 45056;           // candidates whose keys fit in shared memory: 176 KiB beside the histogram's 33
 constexpr int kMoveThreads = 256;
 constexpr int kFillSlots = kMoveThreads;     // slots of a CTA of evict_fill
 constexpr int kShiftRows = 64;               // rows in registers: 8 warps times 8
@@ -38,11 +39,12 @@ struct EvictParams {
     int* index;                    // [batch, heads, budget]
     int* movers;                   // [batch, heads, budget]
     WorkspaceHeader* header;
+    uint32_t* stays;               // [batch * heads][slots / 32], where the keys do not fit in shared memory
+    int* bad;                      // [batch]: the sequence's length or a page of it does not exist
+    int report;                    // which launch writes the header: 0 evict_select, 1 evict_fill, 2 evict_shift
 };
 
-__device__ __forceinline__ long long evict_cap(const EvictParams& p) {
-    return min(p.cache.capacity(), static_cast<long long>(p.slots));
-}
+__device__ __forceinline__ long long evict_cap(const EvictParams& p) { return min(p.cache.capacity(), p.slots); }
 
 __device__ __forceinline__ int evict_len(const EvictParams& p, int seq) {
     return static_cast<int>(min(max(static_cast<long long>(p.cache_lens[seq]), 0ll), evict_cap(p)));
@@ -55,21 +57,31 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
 }
 
-// Lengths and pages: CTA 0 finds out whether all exist and writes the header, so that no launch has to clear it.
-__device__ __forceinline__ void check_evict(const EvictParams& p, int* flag) {
-    if (threadIdx.x == 0) *flag = 0;
-    __syncthreads();
-    for (int b = 0; b < p.batch; ++b) {
-        const long long len = p.cache_lens[b];
-        if (len < 0 || len > evict_cap(p)) *flag = 1;
-        if (p.cache.block_table == nullptr) continue;
-        const int pages = (evict_len(p, b) + p.cache.page_size - 1) / p.cache.page_size;
-        for (int i = threadIdx.x; i < pages; i += kSelectThreads) {
-            if (p.cache.page_of(b, static_cast<long long>(i) * p.cache.page_size) < 0) *flag = 1;
+// Whether a sequence's length and pages exist; by one CTA.
+__device__ __forceinline__ void check_evict(const EvictParams& p, int seq) {
+    const long long len = p.cache_lens[seq];
+    int bad = len < 0 || len > evict_cap(p);
+    if (p.cache.block_table != nullptr) {
+        const int pages = (evict_len(p, seq) + p.cache.page_size - 1) / p.cache.page_size;
+        for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+            int row;
+            if (p.cache.page_of(seq, static_cast<long long>(i) * p.cache.page_size, &row) < 0) bad = 1;
         }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) *p.header = WorkspaceHeader{0, 0, *flag ? kStatusBadArg << 24 : 0u, 0};
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) p.bad[seq] = bad;
+}
+
+// The header, written whole by one CTA of the last launch, so that no launch has to clear it.  (Where only evict_select runs,
+// nothing moves, and the lengths are all there is to check.)
+__device__ __forceinline__ void report_evict(const EvictParams& p, int launch) {
+    if (p.report != launch || blockIdx.x != 0 || blockIdx.y != 0) return;
+    int bad = 0;
+    for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+        bad |= launch == 0 ? p.cache_lens[b] < 0 || p.cache_lens[b] > evict_cap(p) : p.bad[b];
+    }
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) *p.header = WorkspaceHeader{0, 0, bad ? kStatusBadArg << 24 : 0u, 0};
 }
 
 // Exclusive sums of a value of each warp, in every thread; the total in *total.
@@ -88,12 +100,16 @@ __device__ __forceinline__ int warps_before(int mine, int warp, int lane, int* s
     return __shfl_sync(0xFFFFFFFFu, upto - v, warp);
 }
 
+// in_shared: the keys of all candidates fit in shared memory; otherwise each pass reads the weights again.  Loops stay rolled up: a
+// CTA goes through each once, and instructions that come from memory cost more than they save (keys in registers, eight passes
+// over 16 each unrolled: 53 us where this takes TIME).
 __global__ void __launch_bounds__(kSelectThreads)
-evict_select(const EvictParams p) {
+evict_select(const EvictParams p, const int in_shared) {
+    extern __shared__ uint32_t keys[];
     __shared__ int count[256][32];
     __shared__ int bin_sum[256];
     __shared__ int per_warp[32];
-    __shared__ int found[2];
+    __shared__ int found[3];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     let_next_kernel_start();
     wait_for_previous_kernel();
@@ -103,6 +119,24 @@ evict_select(const EvictParams p) {
     const float* w = p.weights + seq * p.weights_stride[0] + head * p.weights_stride[1];
     float* new_w = p.new_weights + static_cast<long long>(blockIdx.x) * p.slots;
     int* index = p.index + static_cast<long long>(blockIdx.x) * p.budget;
+    const int old = p.budget - p.recent;         // slots for the heaviest
+    const int candidates = len - p.recent;       // more than old, if the sequence is too long
+    // A warp has a run of slots, so that sums over warps keep their order.
+    const int run = ((candidates + 31) / 32 + 31) / 32 * 32;
+    const int first = min(warp * run, candidates), last = min(first + run, candidates);
+    uint32_t* stays = in_shared ? keys + candidates : p.stays + static_cast<long long>(blockIdx.x) * ((p.slots + 31) / 32);
+    if (in_shared && len > p.budget) {
+        // Only the warp itself reads them again.
+#pragma unroll 4
+        for (int j = first + lane; j < last; j += 32) keys[j] = weight_key(w[j]);
+        __syncwarp();
+    }
+    auto each = [&](auto&& take) {               // take(first of 32 slots, this lane's key)
+#pragma unroll 1
+        for (int j0 = first; j0 < last; j0 += 32) {
+            take(j0, j0 + lane >= last ? 0u : in_shared ? keys[j0 + lane] : weight_key(w[j0 + lane]));
+        }
+    };
     if (head == 0 && threadIdx.x == 0) p.new_lens[seq] = keep;
     for (int j = keep + threadIdx.x; j < p.slots; j += kSelectThreads) new_w[j] = 0.f;
     for (int j = keep + threadIdx.x; j < p.budget; j += kSelectThreads) index[j] = -1;
@@ -112,8 +146,6 @@ evict_select(const EvictParams p) {
             index[j] = j;
         }
     } else {
-        const int old = p.budget - p.recent;         // slots for the heaviest
-        const int candidates = len - p.recent;       // more than old
         // The last ones, in their order.
         for (int j = old + threadIdx.x; j < keep; j += kSelectThreads) {
             new_w[j] = w[j + len - keep];
@@ -125,11 +157,9 @@ evict_select(const EvictParams p) {
         for (int shift = 24; shift >= 0 && old > 0; shift -= 8) {
             for (int i = threadIdx.x; i < 256 * 32; i += kSelectThreads) count[i >> 5][i & 31] = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int j = threadIdx.x; j < candidates; j += kSelectThreads) {
-                const uint32_t k = weight_key(w[j]);
-                if (shift == 24 || (k >> (shift + 8)) == key) atomicAdd(&count[(k >> shift) & 255u][lane], 1);
-            }
+            each([&](int j0, uint32_t k) {
+                if (j0 + lane < last && (shift == 24 || (k >> (shift + 8)) == key)) atomicAdd(&count[(k >> shift) & 255u][lane], 1);
+            });
             __syncthreads();
             if (threadIdx.x < 256) {
                 int sum = 0;
@@ -155,6 +185,7 @@ evict_select(const EvictParams p) {
                         if (above + n >= need) {
                             found[0] = bin;
                             found[1] = need - above;
+                            found[2] = n;
                             break;
                         }
                         above += n;
@@ -166,111 +197,117 @@ evict_select(const EvictParams p) {
             need = found[1];
         }
         if (old > 0) {
-            // A warp has a run of slots, so that sums over warps keep their order.
-            const int run = ((candidates + 31) / 32 + 31) / 32 * 32;
-            const int first = min(warp * run, candidates), last = min(first + run, candidates);
-            int equal = 0, total;
-            for (int j0 = first; j0 < last; j0 += 32) {
-                const bool eq = j0 + lane < last && weight_key(w[j0 + lane]) == key;
-                equal += __popc(__ballot_sync(0xFFFFFFFFu, eq));
-            }
-            const int equal_before = warps_before(equal, warp, lane, per_warp, &total);
-            // Twice over the run: count the kept slots behind the heaviest's place, then list them.
-            int* movers = p.movers + static_cast<long long>(blockIdx.x) * p.budget;
             const unsigned below = (1u << lane) - 1u;
-            int at = 0, gap = 0;
-            for (int pass = 0; pass < 2; ++pass) {
-                int eq_seen = equal_before, n = 0, gaps = 0;
-                for (int j0 = first; j0 < last; j0 += 32) {
-                    const int j = j0 + lane;
-                    const uint32_t k = j < last ? weight_key(w[j]) : 0u;
-                    const bool eq = j < last && k == key;
+            int equal_before = 0, total;
+            const bool ties = need < found[2];             // not all slots of the last key stay: the lower ones do
+            if (ties) {
+                int equal = 0;
+                each([&](int j0, uint32_t k) { equal += __popc(__ballot_sync(0xFFFFFFFFu, j0 + lane < last && k == key)); });
+                equal_before = warps_before(equal, warp, lane, per_warp, &total);
+            }
+            // A bit for each slot that stays; those behind the heaviest's place and the gaps in it are counted.
+            int moves = 0, gaps = 0;
+            each([&](int j0, uint32_t k) {
+                bool yes = j0 + lane < last && k >= key;
+                if (ties) {
+                    const bool eq = j0 + lane < last && k == key;
                     const unsigned eqs = __ballot_sync(0xFFFFFFFFu, eq);
-                    const bool kept = j < last && (k > key || (eq && eq_seen + __popc(eqs & below) < need));
-                    eq_seen += __popc(eqs);
-                    const unsigned moves = __ballot_sync(0xFFFFFFFFu, kept && j >= old);
-                    if (pass == 1 && kept && j >= old) movers[at + n + __popc(moves & below)] = j;
-                    n += __popc(moves);
-                    gaps += __popc(__ballot_sync(0xFFFFFFFFu, !kept && j < last && j < old));
+                    yes = yes && (!eq || equal_before + __popc(eqs & below) < need);
+                    equal_before += __popc(eqs);
                 }
-                if (pass == 0) {
-                    at = warps_before(n, warp, lane, per_warp, &total);
-                    gap = warps_before(gaps, warp, lane, per_warp, &total);
-                }
+                const unsigned stay = __ballot_sync(0xFFFFFFFFu, yes);
+                const unsigned here = old - j0 >= 32 ? 0xFFFFFFFFu : old <= j0 ? 0u : (1u << (old - j0)) - 1u;
+                if (lane == 0) stays[j0 >> 5] = stay;
+                moves += __popc(stay & ~here);
+                gaps += __popc(~stay & here);
+            });
+            int at = warps_before(moves, warp, lane, per_warp, &total);
+            int gap = warps_before(gaps, warp, lane, per_warp, &total);
+            int* movers = p.movers + static_cast<long long>(blockIdx.x) * p.budget;
+#pragma unroll 1
+            for (int j0 = max(first, old & ~31); j0 < last; j0 += 32) {
+                const unsigned all = stays[j0 >> 5] & (old <= j0 ? 0xFFFFFFFFu : 0xFFFFFFFFu << (old - j0));
+                if ((all >> lane) & 1u) movers[at + __popc(all & below)] = j0 + lane;
+                at += __popc(all);
             }
             __threadfence_block();
             __syncthreads();
-            int eq_seen = equal_before;
-            for (int j0 = first; j0 < last && j0 < old; j0 += 32) {
-                const int j = j0 + lane;
-                const uint32_t k = j < last ? weight_key(w[j]) : 0u;
-                const bool eq = j < last && k == key;
-                const unsigned eqs = __ballot_sync(0xFFFFFFFFu, eq);
-                const bool kept = j < last && (k > key || (eq && eq_seen + __popc(eqs & below) < need));
-                eq_seen += __popc(eqs);
-                const bool here = j < last && j < old;
-                const unsigned gaps = __ballot_sync(0xFFFFFFFFu, here && !kept);
-                if (here) {
-                    const int from = kept ? j : movers[gap + __popc(gaps & below)];
-                    index[j] = from;
-                    new_w[j] = w[from];
+#pragma unroll 2
+            for (int j0 = first; j0 < min(last, old); j0 += 32) {
+                const unsigned stay = stays[j0 >> 5];
+                if (j0 + lane < old) {
+                    const int from = (stay >> lane) & 1u ? j0 + lane : movers[gap + __popc(~stay & below)];
+                    index[j0 + lane] = from;
+                    new_w[j0 + lane] = w[from];
                 }
-                gap += __popc(gaps);
+                gap += __popc(~stay);                       // the last group's count is not used again
             }
         }
     }
-    if (blockIdx.x == 0) check_evict(p, found);
+    if (head == 0) check_evict(p, seq);
+    report_evict(p, 0);
 }
 
-// Rows of K and V of one slot: the lower half of a warp has K, the upper V, 16 bytes a lane.
-__device__ __forceinline__ uint4* evict_row(const EvictParams& p, int seq, int head, int slot, int lane) {
-    const int page = p.cache.page_of(seq, slot);
-    if (page < 0) return nullptr;
-    const long long* st = lane < 16 ? p.cache.k_stride : p.cache.v_stride;
-    return reinterpret_cast<uint4*>((lane < 16 ? p.cache.k : p.cache.v) + page * st[0] + slot % p.cache.page_size * st[1] +
-                                    head * st[2] + (lane & 15) * 8);
+// Moves up to 32 rows of K and V by one warp: a lane finds out where one row comes from and goes to, all at once, and then the
+// warp copies row by row, kAtOnce on their way, the lower half of its lanes K, the upper V, 16 bytes each.
+template <int kAtOnce, typename Sync>
+__device__ __forceinline__ void evict_move(const EvictParams& p, int seq, int head, bool moves, int from, int to, int lane, Sync&& sync) {
+    long long src[2] = {-1, -1}, dst[2] = {-1, -1};
+    if (moves) {
+        int row;
+        int page = p.cache.page_of(seq, from, &row);
+        src[0] = p.cache.at(p.cache.k_stride, page, row, head);
+        src[1] = p.cache.at(p.cache.v_stride, page, row, head);
+        page = p.cache.page_of(seq, to, &row);
+        dst[0] = p.cache.at(p.cache.k_stride, page, row, head);
+        dst[1] = p.cache.at(p.cache.v_stride, page, row, head);
+        if (src[0] < 0 || dst[0] < 0) moves = false;
+    }
+    unsigned left = __ballot_sync(0xFFFFFFFFu, moves);
+    __nv_bfloat16* base = (lane < 16 ? p.cache.k : p.cache.v) + (lane & 15) * 8;
+    do {
+        uint4 data[kAtOnce];
+        __nv_bfloat16* put[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            put[i] = nullptr;
+            if (left != 0u) {
+                const int at = __ffs(left) - 1;
+                left &= left - 1u;
+                const long long k_src = __shfl_sync(0xFFFFFFFFu, src[0], at), v_src = __shfl_sync(0xFFFFFFFFu, src[1], at);
+                const long long k_dst = __shfl_sync(0xFFFFFFFFu, dst[0], at), v_dst = __shfl_sync(0xFFFFFFFFu, dst[1], at);
+                put[i] = base + (lane < 16 ? k_dst : v_dst);
+                data[i] = *reinterpret_cast<const uint4*>(base + (lane < 16 ? k_src : v_src));
+            }
+        }
+        sync();
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (put[i] != nullptr) *reinterpret_cast<uint4*>(put[i]) = data[i];
+        }
+    } while (left != 0u);
 }
 
 __global__ void __launch_bounds__(kMoveThreads)
 evict_fill(const EvictParams p) {
     let_next_kernel_start();
     wait_for_previous_kernel();
+    report_evict(p, 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int which = blockIdx.y, seq = which / p.cache.heads, head = which - seq * p.cache.heads;
     if (evict_len(p, seq) <= p.budget) return;
     const int old = p.budget - p.recent;
-    const int j0 = blockIdx.x * kFillSlots + warp * 32;
-    if (j0 >= old) return;
-    const int from = j0 + lane < old ? p.index[static_cast<long long>(which) * p.budget + j0 + lane] : j0 + lane;
-    unsigned moves = __ballot_sync(0xFFFFFFFFu, from != j0 + lane);
-    while (moves != 0u) {
-        // Four rows at a time on the way.
-        uint4 data[4];
-        uint4* to[4];
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            to[i] = nullptr;
-            if (moves != 0u) {
-                const int at = __ffs(moves) - 1;
-                moves &= moves - 1u;
-                const uint4* src = evict_row(p, seq, head, __shfl_sync(0xFFFFFFFFu, from, at), lane);
-                to[i] = src == nullptr ? nullptr : evict_row(p, seq, head, j0 + at, lane);
-                if (to[i] != nullptr) data[i] = *src;
-                ++n;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (to[i] != nullptr) *to[i] = data[i];
-        }
-    }
+    const int j = blockIdx.x * kFillSlots + threadIdx.x;
+    if (blockIdx.x * kFillSlots + warp * 32 >= old) return;
+    const int from = j < old ? p.index[static_cast<long long>(which) * p.budget + j] : j;
+    evict_move<8>(p, seq, head, from != j, from, j, lane, [] {});
 }
 
 __global__ void __launch_bounds__(kMoveThreads)
 evict_shift(const EvictParams p) {
     let_next_kernel_start();
     wait_for_previous_kernel();
+    report_evict(p, 2);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int which = blockIdx.y, seq = which / p.cache.heads, head = which - seq * p.cache.heads;
     const int by = evict_len(p, seq) - p.budget;
@@ -281,24 +318,21 @@ evict_shift(const EvictParams p) {
     const int first = overlap ? 0 : blockIdx.x * kShiftRows, last = overlap ? p.recent : min(first + kShiftRows, p.recent);
     // Upwards: a chunk is written when all of it has been read, and what it overwrites lies below the next one's source.
     for (int r0 = first; r0 < last; r0 += kShiftRows) {
-        uint4 data[8];
-        uint4* to[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = r0 + warp * 8 + i;
-            to[i] = nullptr;
-            if (r < last) {
-                const uint4* src = evict_row(p, seq, head, old + r + by, lane);
-                to[i] = src == nullptr ? nullptr : evict_row(p, seq, head, old + r, lane);
-                if (to[i] != nullptr) data[i] = *src;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (to[i] != nullptr) *to[i] = data[i];
-        }
+        const int r = r0 + warp * 8 + lane;
+        evict_move<8>(p, seq, head, lane < 8 && r < last, old + r + by, old + r, lane, [] { __syncthreads(); });
     }
+}
+
+// Workspace: the header, a word for each sequence, the movers, and a bit for each slot.
+size_t evict_movers_at(int batch) { return align_up(sizeof(WorkspaceHeader) + batch * sizeof(int), 256); }
+size_t evict_stays_at(int batch, size_t rows, int budget) { return evict_movers_at(batch) + align_up(rows * budget * sizeof(int), 256); }
+
+size_t select_smem(long long candidates) { return (candidates + (candidates + 31) / 32) * sizeof(uint32_t); }   // keys, and a bit for each
+
+int set_select_smem() {
+    B2A_CUDA_OK(cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(select_smem(kSelectKeys))));
+    return B2A_OK;
 }
 
 }  // namespace
@@ -307,9 +341,10 @@ evict_shift(const EvictParams p) {
 
 extern "C" {
 
-size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget) {
-    if (batch < 1 || heads_k < 1 || budget < 1) return 0;   // b2a_cache_evict reports what is wrong
-    return 256 + static_cast<size_t>(batch) * heads_k * budget * sizeof(int);
+size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget, int32_t weights_slots) {
+    if (batch < 1 || heads_k < 1 || budget < 1 || weights_slots < 1) return 0;   // b2a_cache_evict reports what is wrong
+    const size_t rows = static_cast<size_t>(batch) * heads_k;
+    return b2a::evict_stays_at(batch, rows, budget) + rows * ((static_cast<size_t>(weights_slots) + 31) / 32) * sizeof(uint32_t);
 }
 
 int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
@@ -329,7 +364,7 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     B2A_REQUIRE(rows <= 65535, "at most 65535 sequences times K/V heads, got %lld", rows);
     B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
                 "workspace must be a 16-byte aligned device pointer");
-    const size_t need = b2a_cache_evict_workspace_bytes(a->batch, a->cache.heads_k, a->budget);
+    const size_t need = b2a_cache_evict_workspace_bytes(a->batch, a->cache.heads_k, a->budget, a->weights_slots);
     if (a->workspace_bytes < need) {
         return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, need);
     }
@@ -348,18 +383,26 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     p.new_weights = a->new_weights;
     p.index = a->index;
     p.header = static_cast<WorkspaceHeader*>(a->workspace);
-    p.movers = reinterpret_cast<int*>(static_cast<uint8_t*>(a->workspace) + 256);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.bad = reinterpret_cast<int*>(ws + sizeof(WorkspaceHeader));
+    p.movers = reinterpret_cast<int*>(ws + evict_movers_at(a->batch));
+    p.stays = reinterpret_cast<uint32_t*>(ws + evict_stays_at(a->batch, static_cast<size_t>(rows), a->budget));
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const long long most = std::min<long long>(p.cache.block_table == nullptr ? p.cache.page_size
+                                                                              : static_cast<long long>(p.cache.page_size) * p.cache.table_width,
+                                               p.slots);
+    const bool in_shared = most - p.recent <= kSelectKeys;
+    rc = once_per_device(dev.device, 11, set_select_smem);
+    if (rc != B2A_OK) return rc;
+    const int old = p.budget - p.recent;
+    p.report = most <= p.budget ? 0 : p.recent > 0 ? 2 : 1;
     auto select = evict_select;
     auto fill = evict_fill;
     auto shift = evict_shift;
-    B2A_CUDA_OK(launch_early(select, static_cast<unsigned int>(rows), kSelectThreads, 0, stream, p));
+    B2A_CUDA_OK(launch_early(select, static_cast<unsigned int>(rows), kSelectThreads,
+                             in_shared && most > p.recent ? select_smem(most - p.recent) : 0, stream, p, in_shared ? 1 : 0));
     // Nothing moves where no sequence can be longer than the budget.
-    if (std::min<long long>(p.cache.block_table == nullptr ? p.cache.page_size : static_cast<long long>(p.cache.page_size) * p.cache.table_width,
-                            p.slots) <= p.budget) {
-        return B2A_OK;
-    }
-    const int old = p.budget - p.recent;
+    if (most <= p.budget) return B2A_OK;
     if (old > 0) {
         B2A_CUDA_OK(launch_early(fill, dim3((old + kFillSlots - 1) / kFillSlots, rows), kMoveThreads, 0, stream, p));
     }

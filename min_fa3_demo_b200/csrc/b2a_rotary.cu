@@ -85,20 +85,20 @@ __device__ __forceinline__ void check_append(const RotaryParams& p) {
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
-    for (int b = threadIdx.x; b < p.batch; b += kRotaryThreads) {
+    for (int b = threadIdx.x >> 5; b < p.batch; b += kRotaryThreads / 32) {      // a warp a sequence, a lane a page
         const long long first = p.cache_lens[b];
         const int begin = p.cu_seqlens == nullptr ? 0 : p.cu_seqlens[b];
         const int end = p.cu_seqlens == nullptr ? p.seqlen : p.cu_seqlens[b + 1];
-        if (begin < 0 || end < begin || (p.cu_seqlens != nullptr && end > p.total) || first < 0) {
+        const long long last = first + (static_cast<long long>(end) - begin);
+        if (begin < 0 || end < begin || (p.cu_seqlens != nullptr && end > p.total) || first < 0 || last > p.cache.capacity()) {
             bad = 1;
             continue;
         }
-        if (first + (end - begin) > p.cache.capacity()) {
-            bad = 1;
-        } else if (p.cache.block_table != nullptr) {
-            for (long long slot = first; slot < first + (end - begin); slot += p.cache.page_size - slot % p.cache.page_size) {
-                if (p.cache.page_of(b, slot) < 0) bad = 1;
-            }
+        if (p.cache.block_table == nullptr || last == first) continue;
+        int row;
+        const int entry = p.cache.entry_of(static_cast<int>(first), &row);
+        for (long long slot = (entry + (threadIdx.x & 31ll)) * p.cache.page_size; slot < last; slot += 32ll * p.cache.page_size) {
+            if (p.cache.page_of(b, slot, &row) < 0) bad = 1;
         }
     }
     __syncthreads();
@@ -119,11 +119,10 @@ rotary_tokens(const RotaryParams p) {
     if (warp < kTokens) {
         TokenPlace at = find_token(p, token0 + warp, lane);
         if (kAppend && at.valid) {
-            const long long slot = static_cast<long long>(p.cache_lens[at.seq]) + at.number;
-            const int page = p.cache.page_of(at.seq, slot);
-            const long long row = slot % p.cache.page_size;
-            at.k_at = page < 0 ? -1 : page * p.cache.k_stride[0] + row * p.cache.k_stride[1];
-            at.v_at = page < 0 ? -1 : page * p.cache.v_stride[0] + row * p.cache.v_stride[1];
+            int row;
+            const int page = p.cache.page_of(at.seq, static_cast<long long>(p.cache_lens[at.seq]) + at.number, &row);
+            at.k_at = p.cache.at(p.cache.k_stride, page, row, 0);
+            at.v_at = p.cache.at(p.cache.v_stride, page, row, 0);
         }
         if (lane == 0) place[warp] = at;
     }

@@ -67,11 +67,10 @@ __device__ __forceinline__ void tree_add_not_finite(const TreeParams& p, const T
     for (int u = from; u < to; ++u) {
         const long long slot = static_cast<long long>(w.len) + u;
         if (slot >= w.slots || !tree_sees(p, w, token, u)) continue;
-        const int page = p.c.cache.page_of(w.seq, slot);
+        int row;
+        const int page = p.c.cache.page_of(w.seq, slot, &row);
         if (page < 0) continue;
-        const uint4* v = reinterpret_cast<const uint4*>(p.c.cache.v + page * p.c.cache.v_stride[0] +
-                                                        slot % p.c.cache.page_size * p.c.cache.v_stride[1] +
-                                                        w.head * p.c.cache.v_stride[2] + column);
+        const uint4* v = reinterpret_cast<const uint4*>(p.c.cache.v + p.c.cache.at(p.c.cache.v_stride, page, row, w.head) + column);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 eight = v[i];
@@ -151,7 +150,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             CacheWalk walk;
             walk.start(p.c, blockIdx.x, gridDim.x, lane);
             if (lane == 0) p.cuts[blockIdx.x] = tree_cut(p, walk);
-            SlotLoader loader(p.c.cache, p.box_rows);
+            SlotLoader loader(p.box_rows);
             loader.bad = walk.bad;
             uint32_t k_it = 0, q_par = 0;
             bool ok = true, begun = false;

@@ -82,7 +82,7 @@ __device__ __forceinline__ TreePiece tree_piece(const TreeParams& p, const Cache
 // Loads of V by one warp: the blocks of all pieces, one behind the other.
 template <int kSlots, int kStages, typename Shared>
 __device__ __forceinline__ void tree_load_v(const TreeParams& p, Shared& sh, const CUtensorMap* map, const WaitCtx& wctx, int lane) {
-    SlotLoader loader(p.c.cache, p.box_rows);
+    SlotLoader loader(p.box_rows);
     uint32_t v_it = 0;
     bool ok = true;
     PH_DECL(3)   // 0 other, 1 wait for V's stage, 2 issue V

@@ -194,7 +194,7 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
         CacheWalk walk;
         walk.start(p.c, blockIdx.x, gridDim.x, lane);
         if (lane == 0) p.cuts[blockIdx.x] = tree_cut(p, walk);
-        SlotLoader loader(p.c.cache, p.box_rows);
+        SlotLoader loader(p.box_rows);
         loader.bad = walk.bad;
         uint32_t k_it = 0;
         bool ok = true;
@@ -556,11 +556,10 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
                     for (int u = from; u < to; ++u) {
                         const long long slot = static_cast<long long>(w.len) + u;
-                        const int page = slot < w.slots ? p.c.cache.page_of(w.seq, slot) : -1;
+                        int row;
+                        const int page = slot < w.slots ? p.c.cache.page_of(w.seq, slot, &row) : -1;
                         if (page < 0) continue;
-                        const uint32_t bits = __bfloat16_as_ushort(p.c.cache.v[page * p.c.cache.v_stride[0] +
-                                                                               slot % p.c.cache.page_size * p.c.cache.v_stride[1] +
-                                                                               w.head * p.c.cache.v_stride[2] + r]);
+                        const uint32_t bits = __bfloat16_as_ushort(p.c.cache.v[p.c.cache.at(p.c.cache.v_stride, page, row, w.head) + r]);
                         if (!bf16_not_finite(bits)) continue;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {

@@ -175,7 +175,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         CacheWalk walk;
         walk.start(p.c, blockIdx.x, gridDim.x, lane);
-        SlotLoader loader(p.c.cache, p.box_rows);
+        SlotLoader loader(p.box_rows);
         loader.bad = walk.bad;
         uint32_t q_it = 0, k_it = 0;
         bool ok = true;
