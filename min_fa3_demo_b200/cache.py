@@ -39,27 +39,41 @@ def _check_cache(cache: torch.Tensor, name: str) -> None:
     _check(all(n == 1 or s > 0 for n, s in zip(cache.shape, cache.stride())), f"{name} must not be expanded")
 
 
-# As in min_fa3_op: one expression asks whether everything is as it should be, and the checks that say what is wrong are gone
-# through only if not.
-def _is_cache(cache: torch.Tensor, index: int) -> bool:
-    st = cache.stride()
-    return _is_rows(cache, 4, index) and st[1] & 7 == 0 and min(st) > 0 and min(cache.shape) > 0
-
-
+# As in min_fa3_op, a call first asks in few expressions whether everything is as it should be, and goes through the checks that say
+# what is wrong only if not.  Here the same functions also collect what struct.pack wants, so that shapes, strides and addresses
+# are asked for once (16 sequences, one token: forward_tree 19 us of host work without, HOST with).
 def _is_int32(t: torch.Tensor, index: int, n: int) -> bool:
     return t.dtype is _INT32 and t.get_device() == index and t.dim() == 1 and t.size(0) == n and t.is_contiguous()
 
 
-def _is_table(block_table: Optional[torch.Tensor], k_cache: torch.Tensor, index: int, batch: int) -> bool:
+def _simple_cache(k, v, cache_lens, block_table, index: int, batch: int):
+    """``b2a_cache`` for struct.pack, or None where something is wrong or needs a closer look."""
+    ks, kst, kp = k.shape, k.stride(), k.data_ptr()
+    if len(ks) != 4 or k.dtype is not _BF16 or index not in _SM100 or not _is_int32(cache_lens, index, batch):
+        return None
+    pages, size, heads, dim = ks
+    k0, k1, k2, k3 = kst
+    if v is None:
+        vp = v0 = v1 = v2 = 0
+    else:
+        if v.dtype is not _BF16 or v.get_device() != index or v.shape != ks:
+            return None
+        vp, vst = v.data_ptr(), v.stride()
+        v0, v1, v2, v3 = vst
+        if v3 != 1 or v0 * v1 * v2 == 0:
+            return None
+    if (dim != 128 or k3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & 7 or (kp | vp) & 15 or k0 * k1 * k2 * pages * size * heads == 0
+            or batch == 0):
+        return None
     if block_table is None:
-        return k_cache.size(0) >= batch
-    return (block_table.dtype is _INT32 and block_table.get_device() == index and block_table.dim() == 2
-            and block_table.size(0) == batch and block_table.size(1) > 0 and block_table.stride(1) == 1 and k_cache.size(1) & 7 == 0)
-
-
-def _is_call(k_cache, cache_lens, block_table, cu_seqlens, index, batch) -> bool:
-    return (index in _SM100 and batch > 0 and _is_cache(k_cache, index) and _is_int32(cache_lens, index, batch)
-            and _is_table(block_table, k_cache, index, batch) and (cu_seqlens is None or _is_int32(cu_seqlens, index, batch + 1)))
+        return (kp, vp, 0, 0, k0, k1, k2, v0, v1, v2, pages, size, heads, 1) if pages >= batch else None
+    if block_table.dtype is not _INT32 or block_table.get_device() != index or block_table.dim() != 2 or size & 7:
+        return None
+    rows, width = block_table.shape
+    t0, t1 = block_table.stride()
+    if rows != batch or width == 0 or t1 != 1:
+        return None
+    return (kp, vp, block_table.data_ptr(), t0, k0, k1, k2, v0, v1, v2, pages, size, heads, width)
 
 
 def _check_int32(t: torch.Tensor, name: str, shape, device) -> None:
@@ -110,12 +124,11 @@ def _check_lens(cache_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], na
 
 
 def _cache_fields(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: Optional[torch.Tensor]):
-    """``b2a_cache`` for struct.pack."""
+    """``b2a_cache`` for struct.pack, of a cache that has been checked."""
     pages, size, heads, _ = k_cache.shape
     at, width, step = (0, 1, 0) if block_table is None else (block_table.data_ptr(), block_table.size(1), block_table.stride(0))
-    if v_cache is None:
-        return (k_cache.data_ptr(), 0, at, step, *_rows(k_cache), 0, 0, 0, pages, size, heads, width)
-    return (k_cache.data_ptr(), v_cache.data_ptr(), at, step, *_rows(k_cache), *_rows(v_cache), pages, size, heads, width)
+    v = (0, _NONE3) if v_cache is None else (v_cache.data_ptr(), _rows(v_cache))
+    return (k_cache.data_ptr(), v[0], at, step, *_rows(k_cache), *v[1], pages, size, heads, width)
 
 
 def _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes) -> None:
@@ -154,12 +167,13 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     """
     index, batch, ks = k_cache.get_device(), cache_lens.numel(), k.shape
     dim, tokens = 4 if cu_seqlens is None else 3, ks[:-2]
-    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens, index, batch) and _is_cache(v_cache, index)
-            and v_cache.shape == k_cache.shape and _is_rows(k, dim, index) and _is_rows(v, dim, index) and v.shape == ks
-            and ks[-2] == k_cache.size(2) and (dim == 3 or ks[0] == batch)
+    fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
+    if not (fields is not None and _is_rows(k, dim, index) and _is_rows(v, dim, index) and v.shape == ks
+            and ks[-2] == fields[12] and (ks[0] == batch if dim == 4 else _is_int32(cu_seqlens, index, batch + 1))
             and (positions is None if axes is None else positions is not None and _are_positions(positions, axes, tokens, index))
             and (q is None or (axes is not None and _is_rows(q, dim, index) and q.shape[:-2] == tokens))):
         _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes)
+        fields = _cache_fields(k_cache, v_cache, block_table)
     q_out = None if q is None else _like(q)
     if k.numel() == 0:
         return q_out
@@ -167,7 +181,7 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ws = _workspace(16, device)
     turned = _NO_POSITIONS if axes is None else (axes._at, positions.data_ptr())
     args = _cabi.APPEND.pack(
-        *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+        *fields, cache_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
         k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr(), *turned,
         *(_NONE3 if q is None else _rows(q)), *_rows(k), *_rows(v), *(_NONE3 if axes is None else _position_strides(positions)),
         axes is not None and positions.dtype is _INT64, batch, ks[1] if dim == 4 else 0, ks[0] * ks[1] if dim == 4 else ks[0],
@@ -208,43 +222,51 @@ def _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache) -> 
     _check(tree_mask.size(-1) == 1 or tree_mask.stride(-1) == 1, "the rows of tree_mask must be contiguous")
 
 
-def _token_strides(q: torch.Tensor) -> Tuple[int, int]:
-    """Elements from token to token and from head to head of q seen as one list of tokens."""
-    stride = q.stride()
-    if len(stride) == 4 and q.size(1) == 1:
-        return stride[0], stride[2]
-    return stride[-3], stride[-2]
-
-
-def _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index) -> bool:
-    """Whether q and tree_mask are as _check_queries wants them, and simple enough to be told at once."""
-    dim = 4 if cu_seqlens_q is None else 3
-    if not _is_rows(q, dim, index):
-        return False
+def _simple_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, kvh, index):
+    """(address of the mask, tokens, the most of a sequence, heads, strides of q and of the mask), or None where something is
+    wrong or needs a closer look."""
+    if q.dtype is not _BF16 or q.get_device() != index or q.data_ptr() & 15:
+        return None
     qs, st = q.shape, q.stride()
-    if not (min(st) > 0 and qs[-2] % k_cache.size(2) == 0 and 0 < qs[-2] <= 128 * k_cache.size(2)):
-        return False
-    if dim == 4:
-        most = qs[1]
-        if not (qs[0] == batch and st[0] == most * st[1] and (max_seqlen_q is None or max_seqlen_q == most)):
-            return False
+    if cu_seqlens_q is None:
+        if len(qs) != 4:
+            return None
+        seqs, most, heads, dim = qs
+        s_seq, s_tok, s_head, s_dim = st
+        total = seqs * most
+        if seqs != batch or s_seq != most * s_tok or not (max_seqlen_q is None or max_seqlen_q == most):
+            return None
     else:
+        if len(qs) != 3 or type(max_seqlen_q) is not int or not 0 < max_seqlen_q <= _INT32_MAX or not _is_int32(cu_seqlens_q, index, batch + 1):
+            return None
+        total, heads, dim = qs
+        s_tok, s_head, s_dim = st
         most = max_seqlen_q
-        if not (type(most) is int and 0 < most <= _INT32_MAX):
-            return False
+    if dim != 128 or s_dim != 1 or (s_tok | s_head) & 7 or s_tok * s_head == 0 or heads % kvh or not 0 < heads <= 128 * kvh:
+        return None
     if tree_mask is None:
-        return True
-    size = tree_mask.shape
-    return (tree_mask.dtype is torch.bool and tree_mask.get_device() == index and len(size) == dim - 1 and tree_mask.stride(-1) == 1
-            and (size == (batch, most, most) if dim == 4 else size[0] == qs[0] and size[1] >= most))
+        return 0, total, most, heads, s_tok, s_head, 0, 0
+    if tree_mask.dtype is not torch.bool or tree_mask.get_device() != index:
+        return None
+    size, st = tree_mask.shape, tree_mask.stride()
+    if st[-1] != 1:
+        return None
+    if cu_seqlens_q is None:
+        return (tree_mask.data_ptr(), total, most, heads, s_tok, s_head, st[0], st[1]) if size == (batch, most, most) else None
+    if len(size) != 2 or size[0] != total or size[1] < most:
+        return None
+    return tree_mask.data_ptr(), total, most, heads, s_tok, s_head, 0, st[0]
 
 
-def _query_sizes(q, max_seqlen_q, tree_mask) -> Tuple[int, int, int, Tuple[int, int]]:
-    """Tokens, the most of a sequence, heads and the strides of the mask."""
-    qs = q.shape
+def _query_fields(q, max_seqlen_q, tree_mask):
+    """What _simple_queries returns, of arguments that have been checked."""
+    qs, st = q.shape, q.stride()
+    at = 0 if tree_mask is None else tree_mask.data_ptr()
     if len(qs) == 4:
-        return qs[0] * qs[1], qs[1], qs[2], (0, 0) if tree_mask is None else tree_mask.stride()[:2]
-    return qs[0], int(max_seqlen_q), qs[1], (0, 0) if tree_mask is None else (0, tree_mask.stride(0))
+        mask = (0, 0) if tree_mask is None else tree_mask.stride()[:2]
+        token = st[0] if qs[1] == 1 else st[1]
+        return at, qs[0] * qs[1], qs[1], qs[2], token, st[2], *mask
+    return at, qs[0], int(max_seqlen_q), qs[1], st[0], st[1], 0, 0 if tree_mask is None else tree_mask.stride(0)
 
 
 def _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask) -> None:
@@ -271,28 +293,30 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     calls give the same bits; the last bits can depend on the other sequences of the call.
     """
     index, batch = k_cache.get_device(), cache_lens.numel()
-    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens_q, index, batch) and _is_cache(v_cache, index)
-            and v_cache.shape == k_cache.shape
-            and _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index)):
+    fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
+    query = fields and _simple_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, fields[12], index)
+    if query is None:
         _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask)
-    total, most, heads, mask_stride = _query_sizes(q, max_seqlen_q, tree_mask)
+        fields, query = _cache_fields(k_cache, v_cache, block_table), _query_fields(q, max_seqlen_q, tree_mask)
+    mask, total, most, heads, s_tok, s_head, m_seq, m_row = query
     device = k_cache.device
     if out is None:
         out = _like(q)
     else:
         _check(out.device == device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(),
                "out must be contiguous and have the shape, dtype and device of q")
-    lse = torch.empty((batch, heads, most) if cu_seqlens_q is None else (heads, total), dtype=torch.float32, device=device)
+    if cu_seqlens_q is None:
+        cu, lse = 0, torch.empty_strided((batch, heads, most), (heads * most, most, 1), dtype=torch.float32, device=device)
+    else:
+        cu, lse = cu_seqlens_q.data_ptr(), torch.empty_strided((heads, total), (total, 1), dtype=torch.float32, device=device)
     if total == 0:
         return (out, lse) if return_lse else out
     lib = _cabi.load()
     with _on_device(device):
-        nbytes = lib.b2a_tree_fwd_workspace_bytes(most, heads, k_cache.size(2))
+        nbytes = lib.b2a_tree_fwd_workspace_bytes(most, heads, fields[12])
         ws = _workspace(nbytes, device)
-        args = _cabi.TREE.pack(
-            *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-            q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), *_token_strides(q),
-            *mask_stride, batch, most, total, heads, 0.0, 0, 0, 0, 0, ws.data_ptr(), nbytes)
+        args = _cabi.TREE.pack(*fields, cache_lens.data_ptr(), cu, q.data_ptr(), mask, out.data_ptr(), lse.data_ptr(), s_tok, s_head,
+                               m_seq, m_row, batch, most, total, heads, 0.0, 0, 0, 0, 0, ws.data_ptr(), nbytes)
         _cabi.check(lib.b2a_tree_fwd(args, _stream_ptr(device)))
     _remember_workspace("forward_tree", ws)
     return (out, lse) if return_lse else out
@@ -307,10 +331,10 @@ def _check_weights(weights: torch.Tensor, batch: int, k_cache: torch.Tensor) -> 
     _check(weights.size(2) == 1 or weights.stride(2) == 1, "the rows of weights must be contiguous")
 
 
-def _are_weights(weights: torch.Tensor, batch: int, k_cache: torch.Tensor, index: int) -> bool:
-    size = weights.shape
+def _are_weights(weights: torch.Tensor, batch: int, kvh: int, index: int) -> bool:
+    size, st = weights.shape, weights.stride()
     return (weights.dtype is torch.float32 and weights.get_device() == index and len(size) == 3 and size[0] == batch
-            and size[1] == k_cache.size(2) and size[2] > 0 and weights.stride(2) == 1 and min(weights.stride()) > 0)
+            and size[1] == kvh and size[2] > 0 and st[2] == 1 and st[0] * st[1] > 0)
 
 
 def _check_cache_weights(q, k_cache, cache_lens, weights, block_table, cu_seqlens_q, max_seqlen_q, tree_mask) -> None:
@@ -321,6 +345,9 @@ def _check_cache_weights(q, k_cache, cache_lens, weights, block_table, cu_seqlen
     _check_weights(weights, batch, k_cache)
     _check(all(n == 1 or s > 0 for n, s in zip(weights.shape, weights.stride())), "weights must not be expanded")
     _check_device_capability(k_cache.device, "min_fa3_demo_b200 cache_weights")
+
+
+_WEIGHTS_WORKSPACE = 1024     # b2a_cache_weights_workspace_bytes
 
 
 def cache_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, cache_lens: torch.Tensor, weights: torch.Tensor, *,
@@ -334,26 +361,25 @@ def cache_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, cac
     sequence are left as they were.  What does not fit is reported by ``check_last_status("cache_weights")``.
     """
     index, batch = k_cache.get_device(), cache_lens.numel()
-    if not (_is_call(k_cache, cache_lens, block_table, cu_seqlens_q, index, batch)
-            and _are_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache, index)
-            and _are_weights(weights, batch, k_cache, index)):
+    fields = _simple_cache(k_cache, None, cache_lens, block_table, index, batch)
+    query = fields and _simple_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, fields[12], index)
+    if query is None or not _are_weights(weights, batch, fields[12], index):
         _check_cache_weights(q, k_cache, cache_lens, weights, block_table, cu_seqlens_q, max_seqlen_q, tree_mask)
-    total, most, heads, mask_stride = _query_sizes(q, max_seqlen_q, tree_mask)
-    shape = (batch, heads, most) if cu_seqlens_q is None else (heads, total)
+        fields, query = _cache_fields(k_cache, None, block_table), _query_fields(q, max_seqlen_q, tree_mask)
+    mask, total, most, heads, s_tok, s_head, m_seq, m_row = query
+    shape, cu = ((batch, heads, most), 0) if cu_seqlens_q is None else ((heads, total), cu_seqlens_q.data_ptr())
     if not (lse.get_device() == index and lse.dtype is torch.float32 and lse.is_contiguous() and lse.shape == shape):
         raise RuntimeError(f"lse must be a contiguous torch.float32 tensor of shape {list(shape)} on the same CUDA device as the cache")
     if total == 0:
         return weights
     device = k_cache.device
     lib = _cabi.load()
+    w_seq, w_head, _ = weights.stride()
     with _on_device(device):
-        nbytes = lib.b2a_cache_weights_workspace_bytes()
-        ws = _workspace(nbytes, device)
-        args = _cabi.TREE.pack(
-            *_cache_fields(k_cache, None, block_table), cache_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-            q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), 0, lse.data_ptr(), *_token_strides(q), *mask_stride,
-            batch, most, total, heads, 0.0, weights.data_ptr(), weights.stride(0), weights.stride(1), weights.size(2), ws.data_ptr(),
-            nbytes)
+        ws = _workspace(_WEIGHTS_WORKSPACE, device)
+        args = _cabi.TREE.pack(*fields, cache_lens.data_ptr(), cu, q.data_ptr(), mask, 0, lse.data_ptr(), s_tok, s_head, m_seq, m_row,
+                               batch, most, total, heads, 0.0, weights.data_ptr(), w_seq, w_head, weights.size(2), ws.data_ptr(),
+                               _WEIGHTS_WORKSPACE)
         _cabi.check(lib.b2a_cache_weights(args, _stream_ptr(device)))
     _remember_workspace("cache_weights", ws)
     return weights
@@ -385,22 +411,22 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     """
     budget, recent = int(budget), int(recent)
     index, batch = k_cache.get_device(), cache_lens.numel()
-    if not (_is_call(k_cache, cache_lens, block_table, None, index, batch) and _is_cache(v_cache, index)
-            and v_cache.shape == k_cache.shape and _are_weights(weights, batch, k_cache, index)
-            and 0 <= recent <= budget <= _INT32_MAX and budget > 0 and batch * k_cache.size(2) <= 65535):
+    fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
+    if not (fields is not None and _are_weights(weights, batch, fields[12], index) and 0 <= recent <= budget <= _INT32_MAX
+            and budget > 0 and batch * fields[12] <= 65535):
         _check_evict(k_cache, v_cache, weights, cache_lens, budget, recent, block_table)
-    kvh, device = k_cache.size(2), k_cache.device
+        fields = _cache_fields(k_cache, v_cache, block_table)
+    kvh, device, slots = fields[12], k_cache.device, weights.size(2)
     lens = torch.empty_like(cache_lens)
     new_weights = _like(weights)
-    order = torch.empty((batch, kvh, budget), dtype=_INT32, device=device)
+    order = torch.empty_strided((batch, kvh, budget), (kvh * budget, budget, 1), dtype=_INT32, device=device)
     lib = _cabi.load()
+    w_seq, w_head, _ = weights.stride()
     with _on_device(device):
-        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget, weights.size(2))
+        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget, slots)
         ws = _workspace(nbytes, device)
-        args = _cabi.EVICT.pack(
-            *_cache_fields(k_cache, v_cache, block_table), cache_lens.data_ptr(), weights.data_ptr(), weights.stride(0),
-            weights.stride(1), batch, weights.size(2), budget, recent, lens.data_ptr(), new_weights.data_ptr(), order.data_ptr(),
-            ws.data_ptr(), nbytes)
+        args = _cabi.EVICT.pack(*fields, cache_lens.data_ptr(), weights.data_ptr(), w_seq, w_head, batch, slots, budget, recent,
+                                lens.data_ptr(), new_weights.data_ptr(), order.data_ptr(), ws.data_ptr(), nbytes)
         _cabi.check(lib.b2a_cache_evict(args, _stream_ptr(device)))
     _remember_workspace("evict_cache", ws)
     return lens, new_weights, order
