@@ -254,14 +254,18 @@ inline int make_slot_map(CUtensorMap* map, const CacheView& c, bool keys, int bo
 // Loads blocks of slots by one warp: a lane for each box of the block.  A lane asks for its page a block ahead and looks at the
 // answer only when it needs it, so that neither the block table's latency nor a division is on the path.
 struct SlotLoader {
-    int box_rows, boxes;
+    int shift, boxes;        // rows of a box, a power of two
     int page, row;
     int bad;                 // this lane met a page that does not exist (TMA fills such a box with zeros)
 
-    __device__ __forceinline__ explicit SlotLoader(int rows) : box_rows(rows), boxes(kSlotBlock / rows), page(0), row(0), bad(0) {}
+    __device__ __forceinline__ explicit SlotLoader(int box_rows) {
+        shift = __ffs(box_rows) - 1;
+        boxes = kSlotBlock >> shift;
+        page = row = bad = 0;
+    }
 
     __device__ __forceinline__ void look_up(const CacheView& c, int seq, int block, int slots, int lane) {
-        const int slot = block * kSlotBlock + lane * box_rows;
+        const int slot = block * kSlotBlock + (lane << shift);
         if (lane >= boxes || slot >= slots) return;
         if (c.block_table == nullptr) {
             page = seq;
@@ -273,13 +277,13 @@ struct SlotLoader {
     }
     // Boxes of a block that hold slots.
     __device__ __forceinline__ int count(int block, int slots) const {
-        return min(boxes, max(0, (slots - block * kSlotBlock + box_rows - 1) / box_rows));
+        return min(boxes, max(0, (slots - block * kSlotBlock + (1 << shift) - 1) >> shift));
     }
     __device__ __forceinline__ void load(const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int n, int lane) {
-        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * static_cast<uint32_t>(box_rows) * 256u);
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n << shift) * 256u);
         __syncwarp();
         if (lane < n) {
-            const uint32_t at = dst + static_cast<uint32_t>(lane * box_rows) * 128u;
+            const uint32_t at = dst + static_cast<uint32_t>(lane << shift) * 128u;
             tma_load_4d(at, map, bar, 0, head, row, page);
             tma_load_4d(at + kHalfTileBytes, map, bar, 64, head, row, page);
         }

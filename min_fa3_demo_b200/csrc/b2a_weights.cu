@@ -7,10 +7,12 @@
 // 128 (256 bytes a slot and head: bound by memory for up to some 128 rows, by the exponentials beyond); of more rows, two
 // tiles' worth at a time go over the same few blocks, which then come from L2, and the sums wait in shared memory.
 //
-//   warp 0-3, 4-7   sums, the two groups take turns at the blocks
-//   warp 8          K Q^T       warp 9   plan and TMA loads       warp 10, 11   idle
+//   warp 0-15   sums, in four groups that take turns at the blocks (with two, a scheduler's two warps did not keep its
+//               special-function unit busy: 256 rows of 32 heads against 16,000 slots TWO us, with four FOUR)
+//   warp 16     K Q^T       warp 17   plan, loads of K       warp 18   loads of Q and its lse: pages of 16 slots cost a warp some
+//               1,000 clk a block to ask for, which Q must not wait behind
 //
-// Tensor memory (512 columns): two S^T for each group of warps, 128 columns each.
+// Tensor memory (512 columns): an S^T of 128 columns for each group of warps.
 #include "b2a_cache.cuh"
 
 #include <cmath>
@@ -19,11 +21,13 @@ namespace b2a {
 
 namespace {
 
-constexpr int kWeightThreads = 384;
-constexpr int kWeightKStages = 3, kWeightQSlots = 3;
+constexpr int kWeightGroups = 4;       // of four warps each, which take turns at the blocks
+constexpr int kWeightThreads = 128 * kWeightGroups + 96;
+constexpr int kWeightKStages = kWeightGroups, kWeightQSlots = 2;
+constexpr int kWeightPass = 2;        // query tiles that go over a chunk's blocks together
 constexpr int kWeightChunk = 16;      // blocks that several passes of query tiles go over
 constexpr int kWeightSlots = 4;       // pieces in flight
-constexpr int kWeightMmaWarp = 8, kWeightLoadWarp = 9;
+constexpr int kWeightMmaWarp = 4 * kWeightGroups, kWeightLoadWarp = kWeightMmaWarp + 1, kWeightQWarp = kWeightMmaWarp + 2;
 
 struct WeightParams {
     CacheQueries c;
@@ -54,7 +58,7 @@ struct __align__(1024) WeightShared {
     WeightPiece piece[kWeightSlots];
     uint64_t q_full[kWeightQSlots], q_empty[kWeightQSlots];
     uint64_t k_full[kWeightKStages], k_empty[kWeightKStages];
-    uint64_t s_full[4], s_empty[4];
+    uint64_t s_full[kWeightGroups], s_empty[kWeightGroups];
     uint64_t piece_full[kWeightSlots], piece_empty[kWeightSlots];
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -89,16 +93,16 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
                                __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000)));
 }
 
-// Which of the 8 four-column groups of 32 columns take two of their exponentials from the FMA pipe (bit e: group e).
+// Which of the 4 four-column groups of 16 columns take two of their exponentials from the FMA pipe (bit e: group e).
 #ifndef B2A_WEIGHT_FMA_MASK
-#define B2A_WEIGHT_FMA_MASK 0xFFu
+#define B2A_WEIGHT_FMA_MASK 0x0u
 #endif
 
-// Adds exp2(scale s + minus_lse2) of 32 columns, those of which `see` has a bit.
+// Adds exp2(scale s + minus_lse2) of 16 columns, those of which `see` has a bit.
 template <bool kAll>
-__device__ __forceinline__ void weight_sum(const uint32_t (&s)[32], const float4* minus_lse2, float sl2, uint32_t see, float2 (&acc)[4]) {
+__device__ __forceinline__ void weight_sum(const uint32_t (&s)[16], const float4* minus_lse2, float sl2, uint32_t see, float2 (&acc)[4]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
         const float4 l4 = minus_lse2[e];
         float2 p0 = fma2(make_float2(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1])), make_float2(sl2, sl2),
                          make_float2(l4.x, l4.y));
@@ -127,19 +131,19 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kWeightQSlots; ++i) {
             mbar_init(smem_u32(&sh.q_full[i]), 1);
-            mbar_init(smem_u32(&sh.q_empty[i]), 1 + 8);      // the products, and the warps that read minus_lse2
+            mbar_init(smem_u32(&sh.q_empty[i]), 1 + 4 * kWeightGroups);      // the products, and the warps that read minus_lse2
         }
         for (int i = 0; i < kWeightKStages; ++i) {
             mbar_init(smem_u32(&sh.k_full[i]), 1);
             mbar_init(smem_u32(&sh.k_empty[i]), 1);
         }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kWeightGroups; ++i) {
             mbar_init(smem_u32(&sh.s_full[i]), 1);
             mbar_init(smem_u32(&sh.s_empty[i]), 4);
         }
         for (int i = 0; i < kWeightSlots; ++i) {
             mbar_init(smem_u32(&sh.piece_full[i]), 1);
-            mbar_init(smem_u32(&sh.piece_empty[i]), 1 + 8);
+            mbar_init(smem_u32(&sh.piece_empty[i]), 2 + 4 * kWeightGroups);
         }
         sh.abort_flag = 0;
         fence_mbar_init();
@@ -167,17 +171,17 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
     const WaitCtx wctx{smem_u32(&sh.abort_flag), p.status, p.timeout_ns, 1u};
 
-    // All roles go through the same order: pieces, pairs of query tiles, blocks, tiles of the pair.
+    // All roles go through the same order: pieces, pairs of query tiles, fours of blocks, tiles of the pair, blocks.  So each group of
+    // warps has its turn before the next product for the same one.
     if (warp == kWeightLoadWarp) {
         if (lane == 0) {
-            tma_prefetch_desc(&map_q);
             tma_prefetch_desc(&map_k);
         }
         CacheWalk walk;
         walk.start(p.c, blockIdx.x, gridDim.x, lane);
         SlotLoader loader(p.box_rows);
         loader.bad = walk.bad;
-        uint32_t q_it = 0, k_it = 0;
+        uint32_t k_it = 0;
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kWeightSlots;
@@ -200,8 +204,39 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 mbar_arrive(smem_u32(&sh.piece_full[at]));
             }
             if (!w.valid) break;
+            const int passes = (weight_tiles(p, w.n) + kWeightPass - 1) / kWeightPass;
+            for (int pass = 0; pass < passes && ok; ++pass) {
+                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
+                for (int i = 0; i < w.blocks; ++i, ++k_it) {
+                    SlotLoader now = loader;
+                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+                    const int boxes = now.count(w.j0 + i, w.slots);
+                    const uint32_t stage = k_it % kWeightKStages;
+                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
+                    if (!ok) break;
+                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
+                    now.check(p.c.cache, boxes, lane);
+                    loader.bad |= now.bad;
+                }
+            }
+            if (!ok) break;
+            walk.advance(p.c, w.blocks);
+        }
+        if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
+    } else if (warp == kWeightQWarp) {
+        if (lane == 0) tma_prefetch_desc(&map_q);
+        uint32_t q_it = 0;
+        bool ok = true;
+        for (uint32_t it = 0; ok; ++it) {
+            const uint32_t at = it % kWeightSlots;
+            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kWeightSlots) & 1u, 11);
+            if (!ok) break;
+            const WeightPiece w = sh.piece[at];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+            if (!w.valid) break;
             const int tiles = weight_tiles(p, w.n);
-            auto load_tile = [&](int tile) {
+            for (int tile = 0; tile < tiles; ++tile) {
                 const uint32_t slot = q_it % kWeightQSlots;
                 const int tok0 = tile * p.tile_tokens, rows = min(p.tile_tokens, w.n - tok0) * p.c.group;
                 // Read before the wait, which is for the last warp to be done with the tile that lies there.
@@ -217,7 +252,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     }
                 }
                 ok = warp_wait(wctx, smem_u32(&sh.q_empty[slot]), ((q_it / kWeightQSlots) & 1u) ^ 1u, 2);
-                if (!ok) return;
+                if (!ok) break;
                 ++q_it;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -234,34 +269,15 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, w.head * p.c.group, w.q_begin + tok0);
                 }
                 __syncwarp();
-            };
-            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
-                loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-                load_tile(tile0);
-                for (int i = 0; i < w.blocks && ok; ++i, ++k_it) {
-                    SlotLoader now = loader;
-                    if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-                    const int boxes = now.count(w.j0 + i, w.slots);
-                    const uint32_t stage = k_it % kWeightKStages;
-                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kWeightKStages) & 1u) ^ 1u, 3);
-                    if (!ok) break;
-                    now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
-                    now.check(p.c.cache, boxes, lane);
-                    loader.bad |= now.bad;
-                    // The pair's second tile may have to wait for a slot: the first blocks are on their way by then.
-                    if (tile0 + 1 < tiles && i == min(kWeightKStages, w.blocks) - 1) load_tile(tile0 + 1);
-                }
             }
-            if (!ok) break;
-            walk.advance(p.c, w.blocks);
         }
-        if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
     } else if (warp == kWeightMmaWarp) {
         constexpr uint32_t kStep = kTileBytes >> 4;
         const uint32_t q_lo0 = desc_lo_kmajor(smem_u32(&sh.q[0][0]));
         const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0]));
         uint32_t q_it = 0, k_it = 0;
-        uint32_t s_it[2] = {0, 0};
+        uint32_t par = 0;       // bit x: phase of group x's S^T
+        uint32_t first_group = 0;   // that takes a piece's first block: the turns go on from piece to piece
         bool ok = true;
         PH_DECL(5)   // 0 other, 1 wait K, 2 wait Q, 3 wait S, 4 issue
         for (uint32_t it = 0; ok; ++it) {
@@ -276,48 +292,55 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             __syncwarp();
             if (!valid) break;
             const int tiles = weight_tiles(p, n);
-            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
-                const int here = min(2, tiles - tile0);
-                for (int i = 0; i < blocks && ok; ++i, ++k_it) {
-                    const uint32_t stage = k_it % kWeightKStages;
-                    PH_MARK(0);
-                    ok = warp_wait(wctx, smem_u32(&sh.k_full[stage]), (k_it / kWeightKStages) & 1u, 5);
-                    if (!ok) break;
-                    PH_MARK(1);
-                    const uint32_t x = i & 1;
-                    for (int t = 0; t < here; ++t) {
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += kWeightPass) {
+                const int here = min(kWeightPass, tiles - tile0);
+                for (int i0 = 0; i0 < blocks && ok; i0 += kWeightGroups) {
+                    const int count = min(kWeightGroups, blocks - i0);
+                    for (int t = 0; t < here && ok; ++t) {
                         const uint32_t slot = (q_it + t) % kWeightQSlots;
-                        if (i == 0) {
+                        PH_MARK(0);
+                        if (i0 == 0) {
                             ok = warp_wait(wctx, smem_u32(&sh.q_full[slot]), ((q_it + t) / kWeightQSlots) & 1u, 6);
                             if (!ok) break;
                         }
                         PH_MARK(2);
-                        const uint32_t count = x ? s_it[1]++ : s_it[0]++;
-                        const uint32_t buf = 2 * x + (count & 1u);
-                        ok = warp_wait(wctx, smem_u32(&sh.s_empty[buf]), ((count >> 1) & 1u) ^ 1u, 7);
-                        if (!ok) break;
-                        PH_MARK(3);
                         // As many columns as the tile has rows, in steps of 16.
                         const int rows = min(p.tile_tokens, n - (tile0 + t) * p.tile_tokens) * p.c.group;
                         const uint32_t idesc = make_idesc_bf16(kTileM, (rows + 15) & ~15, 0, 0);
-                        tc_fence_after_sync();
-                        umma_ss_kk_x8_w(tmem_base + buf * 128u, k_lo0 + stage * kStep, q_lo0 + slot * kStep, idesc, 0u);
-                        tc_commit_w(smem_u32(&sh.s_full[buf]));
-                        if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[slot]));
-                        __syncwarp();
-                        PH_MARK(4);
+                        for (int j = 0; j < count; ++j) {
+                            const uint32_t x = (first_group + i0 + j) % kWeightGroups;
+                            const uint32_t stage = (k_it + j) % kWeightKStages;
+                            PH_MARK(0);
+                            if (t == 0) {
+                                ok = warp_wait(wctx, smem_u32(&sh.k_full[stage]), ((k_it + j) / kWeightKStages) & 1u, 5);
+                                if (!ok) break;
+                            }
+                            PH_MARK(1);
+                            ok = warp_wait(wctx, smem_u32(&sh.s_empty[x]), ((par >> x) & 1u) ^ 1u, 7);
+                            if (!ok) break;
+                            par ^= 1u << x;
+                            PH_MARK(3);
+                            tc_fence_after_sync();
+                            umma_ss_kk_x8_w(tmem_base + x * 128u, k_lo0 + stage * kStep, q_lo0 + slot * kStep, idesc, 0u);
+                            tc_commit_w(smem_u32(&sh.s_full[x]));
+                            if (t == here - 1) tc_commit_w(smem_u32(&sh.k_empty[stage]));
+                            __syncwarp();
+                            PH_MARK(4);
+                        }
+                        if (ok && i0 + count == blocks) tc_commit_w(smem_u32(&sh.q_empty[slot]));
                     }
-                    tc_commit_w(smem_u32(&sh.k_empty[stage]));
+                    k_it += count;
                 }
                 q_it += here;
             }
+            first_group += blocks;
         }
         PH_PRINT("weights mma", 5);
-    } else if (warp < 8) {
+    } else {
         const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t s_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const float sl2 = p.scale_log2;
-        uint32_t q_it = 0, s_it = 0;
+        uint32_t q_it = 0, s_it = 0, first_group = 0;
         bool ok = true;
         PH_DECL(4)   // 0 other, 1 wait S, 2 sums
         for (uint32_t it = 0; ok; ++it) {
@@ -327,18 +350,19 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const WeightPiece& w = sh.piece[at];
             if (!w.valid) break;
             const int tiles = weight_tiles(p, w.n);
+            const int mine = (x - first_group) % kWeightGroups;      // this group's first block
             float* out = p.weights + w.seq * p.weights_stride[0] + w.head * p.weights_stride[1];
-            for (int tile0 = 0; tile0 < tiles && ok; tile0 += 2) {
-                const int here = min(2, tiles - tile0);
-                const bool last = tile0 + 2 >= tiles;
-                for (int i = x; i < w.blocks; i += 2) {
+            for (int tile0 = 0; tile0 < tiles && ok; tile0 += kWeightPass) {
+                const int here = min(kWeightPass, tiles - tile0);
+                const bool last = tile0 + kWeightPass >= tiles;
+                for (int i = mine; i < w.blocks; i += kWeightGroups) {
                     const int slot = (w.j0 + i) * kSlotBlock + r;
                     const bool tail = (w.j0 + i + 1) * kSlotBlock > w.len;
                     float before = 0.f;
                     if (last && slot < w.slots) before = out[slot];
                     float sum = tile0 == 0 ? 0.f : sh.sums[i][r];
                     for (int t = 0; t < here; ++t, ++s_it) {
-                        const uint32_t buf = 2 * x + (s_it & 1u), q_slot = (q_it + t) % kWeightQSlots;
+                        const uint32_t q_slot = (q_it + t) % kWeightQSlots;
                         const int tok0 = (tile0 + t) * p.tile_tokens, tokens = min(p.tile_tokens, w.n - tok0);
                         const int rows = tokens * p.c.group;
                         // Which columns see this slot: all of them if it lies before the drafted tokens.
@@ -366,7 +390,7 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                             }
                         }
                         PH_MARK(0);
-                        ok = warp_wait(wctx, smem_u32(&sh.s_full[buf]), (s_it >> 1) & 1u, 9);
+                        ok = warp_wait(wctx, smem_u32(&sh.s_full[x]), s_it & 1u, 9);
                         if (!ok) break;
                         PH_MARK(1);
                         tc_fence_after_sync();
@@ -375,29 +399,31 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.f, 0.f);
                         const uint4 live = *reinterpret_cast<const uint4*>(&sh.live[q_slot][0]);
                         const uint32_t see[4] = {some.x & live.x, some.y & live.y, some.z & live.z, some.w & live.w};
-                        const uint32_t from = s_tmem + buf * 128u;
+                        const uint32_t from = s_tmem + x * 128u;
                         const float4* lse2 = reinterpret_cast<const float4*>(&sh.minus_lse2[q_slot][0]);
-                        // The next 32 columns are on their way out of tensor memory while these are added up.
-                        uint32_t s0[32], s1[32];
-                        tmem_ld_x32(from, s0);
+                        // The next 16 columns are on their way out of tensor memory while these are added up.
+                        uint32_t s0[16], s1[16];
+                        tmem_ld_x16(from, s0);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            if (c * 32 < rows) {
+                        for (int c = 0; c < 8; ++c) {
+                            if (c * 16 < rows) {
                                 tmem_wait_ld();
-                                if ((c + 1) * 32 < rows) {
-                                    if (c & 1) tmem_ld_x32(from + (c + 1) * 32, s0); else tmem_ld_x32(from + (c + 1) * 32, s1);
-                                }
-                                if (__all_sync(0xFFFFFFFFu, see[c] == 0xFFFFFFFFu)) {
-                                    weight_sum<true>(c & 1 ? s1 : s0, lse2 + c * 8, sl2, see[c], acc);
+                                if ((c + 1) * 16 < rows) tmem_ld_x16(from + (c + 1) * 16, c & 1 ? s0 : s1);
+                                const uint32_t bits = (see[c >> 1] >> ((c & 1) * 16)) & 0xFFFFu;
+                                if (__all_sync(0xFFFFFFFFu, bits == 0xFFFFu)) {
+                                    weight_sum<true>(c & 1 ? s1 : s0, lse2 + c * 4, sl2, bits, acc);
                                 } else {
-                                    weight_sum<false>(c & 1 ? s1 : s0, lse2 + c * 8, sl2, see[c], acc);
+                                    weight_sum<false>(c & 1 ? s1 : s0, lse2 + c * 4, sl2, bits, acc);
                                 }
                             }
                         }
                         const float2 both = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
                         tc_fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&sh.s_empty[buf]));
+                        if (lane == 0) {
+                            mbar_arrive(smem_u32(&sh.s_empty[x]));
+                            if (i + kWeightGroups >= w.blocks) mbar_arrive(smem_u32(&sh.q_empty[q_slot]));   // its last block
+                        }
                         sum += both.x + both.y;
                         PH_MARK(2);
                     }
@@ -408,15 +434,16 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         out[slot] = before + sum;
                     }
                 }
-                // A warp without a block here has waited for nothing yet: it may give back no tile that is still to come.
-                for (int t = 0; t < here && ok; ++t, ++q_it) {
-                    const uint32_t q_slot = q_it % kWeightQSlots;
-                    ok = warp_wait(wctx, smem_u32(&sh.q_full[q_slot]), (q_it / kWeightQSlots) & 1u, 10);
-                    __syncwarp();
+                // A group without a block here has waited for nothing yet: it may give back no tile that is still to come.
+                for (int t = 0; t < here && mine >= w.blocks && ok; ++t) {
+                    const uint32_t q_slot = (q_it + t) % kWeightQSlots;
+                    ok = warp_wait(wctx, smem_u32(&sh.q_full[q_slot]), ((q_it + t) / kWeightQSlots) & 1u, 10);
                     if (ok && lane == 0) mbar_arrive(smem_u32(&sh.q_empty[q_slot]));
                 }
+                q_it += here;
             }
             if (!ok) break;
+            first_group += w.blocks;
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
         }
