@@ -171,7 +171,8 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 # ------------------------------------------------------------------------------------------
 def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
     # Gradients come in any layout (expanded, transposed) and may be lazily negated.
-    t = t.resolve_neg()
+    if t.is_neg():
+        t = t.resolve_neg()
     st = t.stride()
     return t if st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0 and t.data_ptr() & 15 == 0 else t.contiguous()
 

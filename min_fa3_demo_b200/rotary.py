@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 from fractions import Fraction
+from math import isfinite
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -16,9 +17,16 @@ from .min_fa3_op import _check, _check_device_capability, _on_device, _SM100, _s
 
 __all__ = ["RotaryAxes", "rotary"]
 
-_PI = Fraction("3.14159265358979323846264338327950288419716939937510582")
+_TURN = round(2**192 / (2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")))
 _MAX_PAIRS = 64
 _NONE3 = (0, 0, 0)
+
+
+def _turn(freq: float) -> int:
+    """``freq / (2 pi)`` in units of 2^-64 modulo a turn: a float is an integer over a power of two."""
+    num, den = freq.as_integer_ratio()
+    shift = 127 + den.bit_length()                      # 2^128, which _TURN has too much, times den
+    return ((num * _TURN + (1 << shift - 1)) >> shift) % 2**64
 
 
 class RotaryAxes:
@@ -37,13 +45,12 @@ class RotaryAxes:
                f"the number of pairs must be a multiple of 8 between 8 and {_MAX_PAIRS}, got {pairs}")
         _check(len(axis) == pairs, f"inv_freq and axis must have the same length. Got {pairs} vs {len(axis)}")
         _check(all(0 <= a < _MAX_PAIRS for a in axis), f"an axis must be between 0 and {_MAX_PAIRS - 1}")
-        _check(all(abs(f) < float("inf") for f in inv_freq), "inv_freq must be finite")
+        _check(all(isfinite(f) for f in inv_freq), "inv_freq must be finite")
         self.axes = max(axis) + 1
         self.pairs = pairs
         c = _cabi.RotaryAxes()
-        for i, (f, a) in enumerate(zip(inv_freq, axis)):
-            c.turn[i] = round(Fraction(f) * 2**64 / (2 * _PI)) % 2**64
-            c.axis[i] = a
+        c.turn[:pairs] = [_turn(f) for f in inv_freq]
+        c.axis[:pairs] = axis
         c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
         self._c, self._at = c, ctypes.addressof(c)
 
@@ -135,19 +142,37 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     one projection: only the 128 values of a head have to be adjacent.  Returns new contiguous tensors.  ``inverse``
     turns the other way, which is what the gradients want; ``autograd.rotary`` does it by itself.
     """
-    dim, index, qs = q.dim(), q.get_device(), q.shape
-    tokens = qs[:-2]
-    if not (dim in (3, 4) and _is_rows(q, dim, index) and (k is None or (_is_rows(k, dim, index) and k.shape[:-2] == tokens))
-            and _are_positions(positions, axes, tokens, index) and index in _SM100):
+    index, qs, q_at = q.get_device(), q.shape, q.data_ptr()
+    dim = len(qs)
+    # As in min_fa3_op: a few expressions ask whether everything is as it should be, and _check_rotary says what is not.
+    fine = (dim in (3, 4) and index in _SM100 and q.dtype is _BF16 and type(axes) is RotaryAxes
+            and positions.dtype in (_INT64, _INT32) and positions.get_device() == index and positions.dim() == dim - 1)
+    if fine:
+        q_step, batch, seqlen, heads_q = q.stride(), 1 if dim == 3 else qs[0], qs[-3], qs[-2]
+        q_rows = (0, q_step[0], q_step[1]) if dim == 3 else q_step[:3]
+        fine = (qs[-1] == 128 and q_step[-1] == 1 and (q_rows[0] | q_rows[1] | q_rows[2]) & 7 == 0 and q_at & 15 == 0
+                and positions.shape == ((axes.axes, seqlen) if dim == 3 else (axes.axes, batch, seqlen)))
+    k_at, k_rows, heads_k = 0, _NONE3, 0
+    if fine and k is not None:
+        ks, k_step, k_at = k.shape, k.stride(), k.data_ptr()
+        fine = len(ks) == dim and k.dtype is _BF16 and k.get_device() == index and k_at & 15 == 0 and ks[-3] == seqlen
+        if fine:
+            heads_k = ks[-2]
+            k_rows = (0, k_step[0], k_step[1]) if dim == 3 else k_step[:3]
+            fine = (ks[-1] == 128 and k_step[-1] == 1 and (k_rows[0] | k_rows[1] | k_rows[2]) & 7 == 0
+                    and (dim == 3 or ks[0] == batch))
+    if not fine:
         _check_rotary(q, k, positions, axes, dim)
+        q_rows, batch, seqlen, heads_q = _rows(q), 1 if dim == 3 else qs[0], qs[-3], qs[-2]
+        if k is not None:
+            k_at, k_rows, heads_k = k.data_ptr(), _rows(k), k.size(-2)
     q_out = _like(q)
     k_out = None if k is None else _like(k)
-    if q.numel() == 0:
+    if batch * seqlen * heads_q == 0:
         return q_out, k_out
-    args = _cabi.ROTARY.pack(
-        axes._at, q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
-        positions.data_ptr(), *_rows(q), *(_NONE3 if k is None else _rows(k)), *_position_strides(positions),
-        positions.dtype is _INT64, qs[0] if dim == 4 else 1, tokens[-1], qs[-2], 0 if k is None else k.size(-2), bool(inverse))
+    args = _cabi.ROTARY.pack(axes._at, q_at, k_at, q_out.data_ptr(), 0 if k is None else k_out.data_ptr(), positions.data_ptr(),
+                             *q_rows, *k_rows, *_position_strides(positions), positions.dtype is _INT64, batch, seqlen, heads_q,
+                             heads_k, bool(inverse))
     device = q.device
     with _on_device(device):
         _cabi.check(_cabi.load().b2a_rotary(args, _stream_ptr(device)))
