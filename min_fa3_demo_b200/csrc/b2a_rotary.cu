@@ -106,7 +106,7 @@ __device__ __forceinline__ void check_append(const RotaryParams& p) {
 }
 
 template <bool kAppend, int kTokens>
-__global__ void __launch_bounds__(kRotaryThreads)
+__global__ void __launch_bounds__(kRotaryThreads, 5)
 rotary_tokens(const RotaryParams p) {
     constexpr int kWarpsPerToken = kRotaryThreads / 32 / kTokens;
     __shared__ __align__(16) float2 cos_sin[kTokens][64];
@@ -116,6 +116,29 @@ rotary_tokens(const RotaryParams p) {
     let_next_kernel_start();
     wait_for_previous_kernel();
 
+    // A thread's 16 dimensions: for halves [8 c, 8 c + 8) of each while there are pairs, behind them 16 in a row; for
+    // neighbours 8 of the lower and 8 of the upper 64, so that eight threads load 128 bytes in a row.
+    const int c = lane & 7;
+    const bool turned = c * 8 < p.pairs;                  // halves only
+    const int lo = p.adjacent || turned ? 8 * c : 16 * c;
+    const int hi = p.adjacent ? 64 + 8 * c : turned ? p.pairs + 8 * c : 16 * c + 8;
+    const int mine = warp / kWarpsPerToken, token = token0 + mine;
+    const int heads = p.heads[0] + p.heads[1] + p.heads[2];
+    const int seq = p.cu_seqlens == nullptr ? token / p.seqlen : 0, number = token - seq * p.seqlen;
+    auto which_of = [&](int h) { return h < p.heads[0] ? 0 : h < p.heads[0] + p.heads[1] ? 1 : 2; };
+    auto head_of = [&](int h, int which) { return h - (which > 0 ? p.heads[0] : 0) - (which > 1 ? p.heads[1] : 0); };
+    auto source = [&](int h) {
+        const int which = which_of(h);
+        return p.src[which] + seq * p.stride[which][0] + number * p.stride[which][1] + head_of(h, which) * p.stride[which][2];
+    };
+    // The first head's values are on their way while the angles are computed.
+    int h = (warp % kWarpsPerToken) * 4 + (lane >> 3);
+    uint4 a{}, b{};
+    if (token < p.total && h < heads) {
+        const __nv_bfloat16* src = source(h);
+        a = *reinterpret_cast<const uint4*>(src + lo);
+        b = *reinterpret_cast<const uint4*>(src + hi);
+    }
     if (warp < kTokens) {
         TokenPlace at = find_token(p, token0 + warp, lane);
         if (kAppend && at.valid) {
@@ -143,47 +166,33 @@ rotary_tokens(const RotaryParams p) {
     }
     __syncthreads();
 
-    const int mine = warp / kWarpsPerToken;
     const TokenPlace at = place[mine];
-    const int token = token0 + mine;
     if (at.valid) {
-        // A thread's 16 dimensions: for halves [8 c, 8 c + 8) of each while there are pairs, behind them 16 in a row; for
-        // neighbours 8 of the lower and 8 of the upper 64, so that eight threads load 128 bytes in a row.
-        const int c = lane & 7;
-        const bool turned = c * 8 < p.pairs;                  // halves only
-        const int lo = p.adjacent || turned ? 8 * c : 16 * c;
-        const int hi = p.adjacent ? 64 + 8 * c : turned ? p.pairs + 8 * c : 16 * c + 8;
         float2 cs[8];
-        bool turn_lo = turned, turn_hi = turned;
-        if (p.adjacent) {
-            turn_lo = 4 * c < p.pairs;
-            turn_hi = 32 + 4 * c < p.pairs;
-        }
+        const bool turn_lo = 4 * c < p.pairs, turn_hi = 32 + 4 * c < p.pairs;      // neighbours only
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int pair = p.adjacent ? (e < 4 ? 4 * c + e : 28 + 4 * c + e) : 8 * c + e;
             cs[e] = pair < p.pairs ? cos_sin[mine][pair] : make_float2(1.f, 0.f);
         }
-        const int heads = p.heads[0] + p.heads[1] + p.heads[2];
-        const long long token_in_seq = p.cu_seqlens == nullptr ? at.number : token;
-        const long long seq = p.cu_seqlens == nullptr ? at.seq : 0;
-#pragma unroll 2
-        for (int h = (warp % kWarpsPerToken) * 4 + (lane >> 3); h < heads; h += 4 * kWarpsPerToken) {
-            const int which = h < p.heads[0] ? 0 : h < p.heads[0] + p.heads[1] ? 1 : 2;
-            const int head = h - (which > 0 ? p.heads[0] : 0) - (which > 1 ? p.heads[1] : 0);
-            const __nv_bfloat16* src = p.src[which] + seq * p.stride[which][0] + token_in_seq * p.stride[which][1] +
-                                       head * p.stride[which][2];
+#pragma unroll 1
+        while (h < heads) {
+            const int which = which_of(h), head = head_of(h, which);
             __nv_bfloat16* dst;
             if (kAppend && which > 0) {
                 const long long row = which == 1 ? at.k_at : at.v_at;
-                if (row < 0) continue;
-                dst = which == 1 ? p.cache.k + row + head * p.cache.k_stride[2] : p.cache.v + row + head * p.cache.v_stride[2];
+                dst = row < 0 ? nullptr
+                      : which == 1 ? p.cache.k + row + head * p.cache.k_stride[2] : p.cache.v + row + head * p.cache.v_stride[2];
             } else {
                 dst = p.dst[which] + (static_cast<long long>(token) * p.heads[which] + head) * kHeadDim;
             }
-            uint4 a = *reinterpret_cast<const uint4*>(src + lo);
-            uint4 b = *reinterpret_cast<const uint4*>(src + hi);
             uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+            h += 4 * kWarpsPerToken;
+            if (h < heads) {
+                const __nv_bfloat16* src = source(h);
+                a = *reinterpret_cast<const uint4*>(src + lo);
+                b = *reinterpret_cast<const uint4*>(src + hi);
+            }
             if (which < 2) {
                 if (p.adjacent) {
 #pragma unroll
@@ -202,8 +211,10 @@ rotary_tokens(const RotaryParams p) {
                     }
                 }
             }
-            *reinterpret_cast<uint4*>(dst + lo) = make_uint4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<uint4*>(dst + hi) = make_uint4(y[0], y[1], y[2], y[3]);
+            if (dst != nullptr) {
+                *reinterpret_cast<uint4*>(dst + lo) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(dst + hi) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
         }
     }
     if (kAppend && blockIdx.x == 0) check_append(p);
