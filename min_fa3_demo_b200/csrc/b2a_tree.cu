@@ -30,20 +30,23 @@ namespace b2a {
 namespace {
 
 constexpr int kTreeThreads = 384;
-constexpr int kTreeStages = 2;
 constexpr int kTreeSlots = 4;       // pieces in flight between the load warp and the others
 constexpr int kTreeQkWarp = 8, kTreeLoadWarp = 9, kTreePvWarp = 10, kTreeVWarp = 11;
 
+// kTwo: items may have two tiles.  Where none has, the second tile's room goes to another stage of K (trees of up to 32 tokens, 32
+// over 8 heads, 16 sequences of up to 8,000 slots: 90 us without, 87 with, 89.5 if it goes to V).
+template <bool kTwo>
 struct __align__(1024) TreeShared {
-    uint8_t q[2][kTileBytes];
-    uint8_t k[kTreeStages][kTileBytes];
-    uint8_t v[kTreeStages][kTileBytes];
+    static constexpr int kTiles = kTwo ? 2 : 1, kK = kTwo ? 2 : 3, kV = 2;
+    uint8_t q[kTiles][kTileBytes];
+    uint8_t k[kK][kTileBytes];
+    uint8_t v[kV][kTileBytes];
     uint32_t seen[2][2][kTileM][4];   // warpgroup, turn, token: one bit for each slot of the block
     float2 stat[2][kTileM];           // row maximum and sum of the two warpgroups
     TreePiece piece[kTreeSlots];
     uint64_t q_full[2], q_empty[2];
-    uint64_t k_full[kTreeStages], k_empty[kTreeStages];
-    uint64_t v_full[kTreeStages], v_empty[kTreeStages];
+    uint64_t k_full[kK], k_empty[kK];
+    uint64_t v_full[kV], v_empty[kV];
     uint64_t s_full[2], s_empty, p_full[2], pv_done[2];
     uint64_t seen_full[2];
     uint64_t both_done, both_read;
@@ -53,8 +56,9 @@ struct __align__(1024) TreeShared {
     uint32_t abort_flag;
 };
 
-constexpr size_t kTreeSmemBytes = sizeof(TreeShared) + 1024;
-static_assert(kTreeSmemBytes <= 227 * 1024, "shared memory of a CTA");
+template <bool kTwo>
+constexpr size_t tree_smem_bytes() { return sizeof(TreeShared<kTwo>) + 1024; }
+static_assert(tree_smem_bytes<true>() <= 227 * 1024 && tree_smem_bytes<false>() <= 227 * 1024, "shared memory of a CTA");
 
 // Whether a block goes to warpgroup x: both tiles take every block, one tile's warpgroups take turns.
 __device__ __forceinline__ bool tree_takes(bool two, int i, int x) { return two || (i & 1) == x; }
@@ -87,11 +91,13 @@ __device__ __forceinline__ void tree_add_not_finite(const TreeParams& p, const T
     }
 }
 
+template <bool kTwo>
 __global__ void __launch_bounds__(kTreeThreads, 1)
 tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeParams p) {
     extern __shared__ uint8_t smem_raw[];
-    TreeShared& sh = *reinterpret_cast<TreeShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    using Shared = TreeShared<kTwo>;
+    Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -106,9 +112,11 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         mbar_init(smem_u32(&sh.s_empty), kTileM);
         mbar_init(smem_u32(&sh.both_done), 2 * kTileM);
         mbar_init(smem_u32(&sh.both_read), 2 * kTileM);
-        for (int i = 0; i < kTreeStages; ++i) {
+        for (int i = 0; i < Shared::kK; ++i) {
             mbar_init(smem_u32(&sh.k_full[i]), 1);
             mbar_init(smem_u32(&sh.k_empty[i]), 1);
+        }
+        for (int i = 0; i < Shared::kV; ++i) {
             mbar_init(smem_u32(&sh.v_full[i]), 1);
             mbar_init(smem_u32(&sh.v_empty[i]), 1);
         }
@@ -185,16 +193,16 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     SlotLoader now = loader;
                     if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
                     const int boxes = now.count(w.j0 + i, w.slots);
-                    const uint32_t stage = k_it % kTreeStages;
+                    const uint32_t stage = k_it % Shared::kK;
                     PH_MARK(0);
-                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / kTreeStages) & 1u) ^ 1u, 3);
+                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
                     if (!ok) break;
                     PH_MARK(1);
                     now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
                     PH_MARK(2);
                     now.check(p.c.cache, boxes, lane);
                     loader.bad |= now.bad;
-                    if (i == 0 && w.tokens[1] > 0) load_q(1);
+                    if (kTwo && i == 0 && w.tokens[1] > 0) load_q(1);
                 }
                 if (!ok) break;
                 walk.advance(p.c, w.blocks);
@@ -203,7 +211,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             PH_PRINT("tree load", 3);
         } else if (warp == kTreeVWarp) {
             // ------------------------------------------------------------ loads of V
-            tree_load_v<kTreeSlots, kTreeStages>(p, sh, &map_v, wctx, lane);
+            tree_load_v<kTreeSlots, Shared::kV>(p, sh, &map_v, wctx, lane);
         } else if (warp == kTreeQkWarp || warp == kTreePvWarp) {
             // ------------------------------------------------------------ MMA warps
             const bool qk = warp == kTreeQkWarp;
@@ -223,12 +231,12 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const volatile TreePiece& w = sh.piece[at];
                 const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
                 const int blocks = __shfl_sync(0xFFFFFFFFu, w.blocks, 0);
-                const bool two = __shfl_sync(0xFFFFFFFFu, w.tokens[1], 0) > 0;
+                const bool two = kTwo && __shfl_sync(0xFFFFFFFFu, w.tokens[1], 0) > 0;
                 if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
                 __syncwarp();
                 if (!valid) break;
                 for (int i = 0; i < blocks && ok; ++i, ++kv_it) {
-                    const uint32_t stage = kv_it % kTreeStages, phase = (kv_it / kTreeStages) & 1u;
+                    const uint32_t stages = qk ? Shared::kK : Shared::kV, stage = kv_it % stages, phase = (kv_it / stages) & 1u;
                     PH_MARK(0);
                     if (qk) {
                         ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), phase, 6);
@@ -307,7 +315,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
             };
             if (!w.valid) break;
-            const bool two = w.tokens[1] > 0;
+            const bool two = kTwo && w.tokens[1] > 0;
             const int tile = two ? x : 0;
             const int tokens = w.tokens[tile];
             const int rows = tokens * p.c.group;
@@ -394,8 +402,8 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             ok = wait_pv();
                             if (!ok) break;
                         }
-                        const uint32_t stage = (kv_base + i) % kTreeStages;
-                        ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / kTreeStages) & 1u, 14);
+                        const uint32_t stage = (kv_base + i) % Shared::kV;
+                        ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / Shared::kV) & 1u, 14);
                         if (!ok) break;
                         if (slot >= w.slots || look) {
                             if (tree_clean_row(&sh.v[stage][r * 128], r, slot >= w.slots)) {
@@ -688,8 +696,10 @@ tree_combine(const __grid_constant__ TreeParams p) {
     }
 }
 
+template <bool kTwo>
 int set_tree_smem() {
-    B2A_CUDA_OK(cudaFuncSetAttribute(tree_attention, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTreeSmemBytes)));
+    B2A_CUDA_OK(cudaFuncSetAttribute(tree_attention<kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(tree_smem_bytes<kTwo>())));
     return B2A_OK;
 }
 
@@ -754,7 +764,8 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     rc = make_strided_map(&map_q, a->q, 3, q_sizes, a->q_stride, static_cast<uint32_t>(p.c.group), static_cast<uint32_t>(t.tile_tokens));
     if (rc == B2A_OK) rc = make_slot_map(&map_k, p.c.cache, true, p.box_rows);
     if (rc == B2A_OK) rc = make_slot_map(&map_v, p.c.cache, false, p.box_rows);
-    if (rc == B2A_OK && !t.few) rc = once_per_device(dev.device, 6, set_tree_smem);
+    if (rc == B2A_OK && t.tiles == 2) rc = once_per_device(dev.device, 6, set_tree_smem<true>);
+    if (rc == B2A_OK && t.tiles == 1 && !t.few) rc = once_per_device(dev.device, 12, set_tree_smem<false>);
     if (rc != B2A_OK) return rc;
 
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -773,9 +784,10 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
 
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     if (t.few) return launch_tree_few(map_q, map_k, map_v, p, t.ctas, dev, stream);
-    auto attention = tree_attention;
+    auto attention = t.tiles == 2 ? tree_attention<true> : tree_attention<false>;
+    const size_t smem = t.tiles == 2 ? tree_smem_bytes<true>() : tree_smem_bytes<false>();
     auto combine = tree_combine;
-    B2A_CUDA_OK(launch_early(attention, t.ctas, kTreeThreads, kTreeSmemBytes, stream, map_q, map_k, map_v, p));
+    B2A_CUDA_OK(launch_early(attention, t.ctas, kTreeThreads, smem, stream, map_q, map_k, map_v, p));
     const int strips = t.tiles * ((t.rows + kTreeStrip - 1) / kTreeStrip);
     if (t.ctas > 1) B2A_CUDA_OK(launch_early(combine, dim3(t.ctas - 1, strips), 256, 0, stream, p));
     return B2A_OK;
