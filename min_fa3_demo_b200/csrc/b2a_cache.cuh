@@ -91,7 +91,8 @@ __device__ __forceinline__ bool warp_wait(const WaitCtx& ctx, uint32_t bar, uint
 // Work of the kernels that stream the cache once: all blocks of 128 slots of all (sequence, group of query tokens, K/V head),
 // in this order, are dealt out to the CTAs in runs of equal length.  The lengths are on the device, so every CTA finds its
 // own run: one warp adds up the sequences' blocks, a lane a sequence.  Nothing is handed out while the kernel runs, and no
-// list has to be made by a launch before it.
+// list has to be made by a launch before it.  Behind an item's blocks come a few that stand for what its masks, its sums
+// and its results cost; a run that begins among those begins with the next item.
 // ---------------------------------------------------------------------------------------
 constexpr int kSlotBlock = 128;
 
@@ -108,6 +109,7 @@ struct CacheQueries {
     int group;                  // query heads of a K/V head
     int item_tokens;            // query tokens of an item
     int min_run;                // fewest blocks of a run
+    int item_extra;             // what beginning and ending an item costs, in blocks
     int limit_slots;            // slots behind these do not exist (weights with fewer of them than the cache)
 };
 
@@ -157,7 +159,7 @@ __device__ __forceinline__ long long cache_seq_blocks(const CacheQueries& p, con
     } else {
         for (int rt = 0; rt < items; ++rt) blocks += cache_item_blocks(p, s, rt);
     }
-    return blocks * p.cache.heads;
+    return (blocks + static_cast<long long>(items) * p.item_extra) * p.cache.heads;
 }
 
 // A CTA's run [pos, end) and where in it the walk is.  Every lane of the warp holds the same.
@@ -209,19 +211,23 @@ struct CacheWalk {
         long long off = pos - before;
         rt = 0;
         blocks = cache_item_blocks(p, s, 0);
-        while (off >= static_cast<long long>(blocks) * p.cache.heads) {
-            off -= static_cast<long long>(blocks) * p.cache.heads;
+        while (off >= static_cast<long long>(blocks + p.item_extra) * p.cache.heads) {
+            off -= static_cast<long long>(blocks + p.item_extra) * p.cache.heads;
             blocks = cache_item_blocks(p, s, ++rt);
         }
-        head = static_cast<int>(off / blocks);
-        j = static_cast<int>(off - static_cast<long long>(head) * blocks);
+        head = static_cast<int>(off / (blocks + p.item_extra));
+        j = static_cast<int>(off - static_cast<long long>(head) * (blocks + p.item_extra));
+        if (j >= blocks) advance(p, 0);
     }
+    __device__ __forceinline__ long long item_begin() const { return pos - j; }
     // Blocks [j, j + piece()) of the item are the next piece.
     __device__ __forceinline__ int piece() const { return static_cast<int>(min(static_cast<long long>(blocks - j), end - pos)); }
     __device__ __forceinline__ void advance(const CacheQueries& p, int count) {
         pos += count;
         j += count;
-        if (j < blocks || pos >= end) return;
+        if (j < blocks) return;
+        pos += blocks + p.item_extra - j;
+        if (pos >= end) return;
         j = 0;
         if (++head < p.cache.heads) return;
         head = 0;

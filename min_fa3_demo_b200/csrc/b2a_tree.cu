@@ -161,14 +161,13 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             SlotLoader loader(p.box_rows);
             loader.bad = walk.bad;
             uint32_t k_it = 0, q_par = 0;
-            bool ok = true, begun = false;
+            bool ok = true;
             PH_DECL(3)   // 0 other, 1 wait for K's stage, 2 issue K
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTreeSlots;
                 ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTreeSlots) & 1u) ^ 1u, 1);
                 if (!ok) break;
-                const TreePiece w = tree_piece(p, walk, begun);
-                begun = true;
+                const TreePiece w = tree_piece(p, walk);
                 if (lane == 0) {
                     sh.piece[at] = w;
                     mbar_arrive(smem_u32(&sh.piece_full[at]));
@@ -758,6 +757,10 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     }
     p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
     p.c.min_run = 2;
+    // A few blocks' time goes into an item's masks, sums and results, so that runs of equal numbers of blocks differ in how many
+    // items end in them.  0, 2, 4, 6, 8 blocks (us): one token, 16 sequences of up to 8,001 slots, 58.5, 57.5, 57.2, 57.0, 57.3;
+    // trees of up to 32 tokens 87.2, 83.5, 81.2, 80.6, 80.5; of 64, 64 over 8 heads, 179, 175, 172, 168, 173.
+    p.c.item_extra = t.few ? 4 : 6;
     p.box_rows = slot_box_rows(p.c.cache);
     CUtensorMap map_q, map_k, map_v;
     const uint64_t q_sizes[2] = {static_cast<uint64_t>(a->total_q), static_cast<uint64_t>(a->heads_q)};

@@ -46,7 +46,7 @@ struct TreePiece {
 __device__ __forceinline__ TreeCut tree_cut(const TreeParams& p, const CacheWalk& walk) {
     TreeCut cut{};
     if (walk.pos < walk.end && walk.j > 0) {
-        cut.first = walk.pos - walk.j;
+        cut.first = walk.item_begin();
         cut.last = cut.first + walk.blocks;
         cut.run = walk.run;
         cut.seq = walk.seq;
@@ -58,8 +58,8 @@ __device__ __forceinline__ TreeCut tree_cut(const TreeParams& p, const CacheWalk
     return cut;
 }
 
-// The walk's next piece; `begun`: there was one before it.
-__device__ __forceinline__ TreePiece tree_piece(const TreeParams& p, const CacheWalk& walk, bool begun) {
+// The walk's next piece.
+__device__ __forceinline__ TreePiece tree_piece(const TreeParams& p, const CacheWalk& walk) {
     TreePiece w{};
     w.valid = walk.pos < walk.end;
     if (w.valid) {
@@ -74,7 +74,9 @@ __device__ __forceinline__ TreePiece tree_piece(const TreeParams& p, const Cache
         w.tokens[1] = max(0, min(p.tile_tokens, w.n - w.tok0 - p.tile_tokens));
         w.j0 = walk.j;
         w.blocks = walk.piece();
-        w.part = w.blocks == walk.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (begun ? 1 : 0);
+        // The item that the run begins inside of (or with), or another one, which then crosses the run's end.
+        const bool other = walk.item_begin() > static_cast<long long>(blockIdx.x) * walk.run;
+        w.part = w.blocks == walk.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (other ? 1 : 0);
     }
     return w;
 }

@@ -203,7 +203,7 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const uint32_t at = it % kFewSlots;
             ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kFewSlots) & 1u) ^ 1u, 1);
             if (!ok) break;
-            const TreePiece w = tree_piece(p, walk, it > 0);
+            const TreePiece w = tree_piece(p, walk);
             if (lane == 0) {
                 sh.piece[at] = w;
                 mbar_arrive(smem_u32(&sh.piece_full[at]));
