@@ -13,6 +13,7 @@
 //                  memory: 512 bytes in and out a row.
 //   evict_shift    moves the last rows down.  They may overlap their destination, so then one CTA a head goes upwards, a
 //                  chunk in registers at a time.  After evict_fill, whose sources it may overwrite.
+// Where only a few rows can move, evict_select does both itself.
 #include "b2a_cache.cuh"
 
 namespace b2a {
@@ -23,6 +24,7 @@ constexpr int kSelectThreads = 1024;
 constexpr int kSelectKeys = 45056;           // candidates whose keys fit in shared memory: 176 KiB beside the histogram's 33
 constexpr int kMoveThreads = 256;
 constexpr int kFillSlots = kMoveThreads;     // slots of a CTA of evict_fill
+constexpr int kInsideRows = 512;             // up to which evict_select moves the rows itself
 constexpr int kShiftRows = 64;               // rows in registers: 8 warps times 8
 
 struct EvictParams {
@@ -41,7 +43,8 @@ struct EvictParams {
     WorkspaceHeader* header;
     uint32_t* stays;               // [batch * heads][slots / 32], where the keys do not fit in shared memory
     int* bad;                      // [batch]: the sequence's length or a page of it does not exist
-    int report;                    // which launch writes the header: 0 evict_select, 1 evict_fill, 2 evict_shift
+    int report;                    // which launch writes the header: 0 evict_select, 1 evict_fill, 2 evict_shift, -1 see inside
+    int inside;                    // few rows move: evict_select moves them, and `bad` holds a status word for each sequence
 };
 
 __device__ __forceinline__ long long evict_cap(const EvictParams& p) { return min(p.cache.capacity(), p.slots); }
@@ -69,7 +72,7 @@ __device__ __forceinline__ void check_evict(const EvictParams& p, int seq) {
         }
     }
     bad = __syncthreads_or(bad);
-    if (threadIdx.x == 0) p.bad[seq] = bad;
+    if (threadIdx.x == 0) p.bad[seq] = bad ? kStatusBadArg << 24 : 0;
 }
 
 // The header, written whole by one CTA of the last launch, so that no launch has to clear it.  (Where only evict_select runs,
@@ -100,9 +103,49 @@ __device__ __forceinline__ int warps_before(int mine, int warp, int lane, int* s
     return __shfl_sync(0xFFFFFFFFu, upto - v, warp);
 }
 
+// Moves up to 32 rows of K and V by one warp: a lane finds out where one row comes from and goes to, all at once, and then the
+// warp copies row by row, kAtOnce on their way, the lower half of its lanes K, the upper V, 16 bytes each.
+template <int kAtOnce, typename Sync>
+__device__ __forceinline__ void evict_move(const EvictParams& p, int seq, int head, bool moves, int from, int to, int lane, Sync&& sync) {
+    long long src[2] = {-1, -1}, dst[2] = {-1, -1};
+    if (moves) {
+        int row;
+        int page = p.cache.page_of(seq, from, &row);
+        src[0] = p.cache.at(p.cache.k_stride, page, row, head);
+        src[1] = p.cache.at(p.cache.v_stride, page, row, head);
+        page = p.cache.page_of(seq, to, &row);
+        dst[0] = p.cache.at(p.cache.k_stride, page, row, head);
+        dst[1] = p.cache.at(p.cache.v_stride, page, row, head);
+        if (src[0] < 0 || dst[0] < 0) moves = false;
+    }
+    unsigned left = __ballot_sync(0xFFFFFFFFu, moves);
+    __nv_bfloat16* base = (lane < 16 ? p.cache.k : p.cache.v) + (lane & 15) * 8;
+    do {
+        uint4 data[kAtOnce];
+        __nv_bfloat16* put[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            put[i] = nullptr;
+            if (left != 0u) {
+                const int at = __ffs(left) - 1;
+                left &= left - 1u;
+                const long long k_src = __shfl_sync(0xFFFFFFFFu, src[0], at), v_src = __shfl_sync(0xFFFFFFFFu, src[1], at);
+                const long long k_dst = __shfl_sync(0xFFFFFFFFu, dst[0], at), v_dst = __shfl_sync(0xFFFFFFFFu, dst[1], at);
+                put[i] = base + (lane < 16 ? k_dst : v_dst);
+                data[i] = *reinterpret_cast<const uint4*>(base + (lane < 16 ? k_src : v_src));
+            }
+        }
+        sync();
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (put[i] != nullptr) *reinterpret_cast<uint4*>(put[i]) = data[i];
+        }
+    } while (left != 0u);
+}
+
 // in_shared: the keys of all candidates fit in shared memory; otherwise each pass reads the weights again.  Loops stay rolled up: a
 // CTA goes through each once, and instructions that come from memory cost more than they save (keys in registers, eight passes
-// over 16 each unrolled: 53 us where this takes TIME).
+// over 16 each unrolled: 53 us where this takes 32, 16,000 slots of 64 heads).
 __global__ void __launch_bounds__(kSelectThreads)
 evict_select(const EvictParams p, const int in_shared) {
     extern __shared__ uint32_t keys[];
@@ -246,46 +289,22 @@ evict_select(const EvictParams p, const int in_shared) {
     }
     if (head == 0) check_evict(p, seq);
     report_evict(p, 0);
-}
-
-// Moves up to 32 rows of K and V by one warp: a lane finds out where one row comes from and goes to, all at once, and then the
-// warp copies row by row, kAtOnce on their way, the lower half of its lanes K, the upper V, 16 bytes each.
-template <int kAtOnce, typename Sync>
-__device__ __forceinline__ void evict_move(const EvictParams& p, int seq, int head, bool moves, int from, int to, int lane, Sync&& sync) {
-    long long src[2] = {-1, -1}, dst[2] = {-1, -1};
-    if (moves) {
-        int row;
-        int page = p.cache.page_of(seq, from, &row);
-        src[0] = p.cache.at(p.cache.k_stride, page, row, head);
-        src[1] = p.cache.at(p.cache.v_stride, page, row, head);
-        page = p.cache.page_of(seq, to, &row);
-        dst[0] = p.cache.at(p.cache.k_stride, page, row, head);
-        dst[1] = p.cache.at(p.cache.v_stride, page, row, head);
-        if (src[0] < 0 || dst[0] < 0) moves = false;
+    if (!p.inside) return;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.header = WorkspaceHeader{-p.batch, 0, 0u, 0};
+    const int by = len - p.budget;
+    if (by <= 0) return;
+    // What evict_fill and evict_shift do, by this CTA.
+    __threadfence_block();
+    __syncthreads();
+    for (int j0 = warp * 32; j0 < old; j0 += kSelectThreads) {
+        const int j = j0 + lane, from = j < old ? index[j] : j;
+        if (__any_sync(0xFFFFFFFFu, from != j)) evict_move<4>(p, seq, head, from != j, from, j, lane, [] {});
     }
-    unsigned left = __ballot_sync(0xFFFFFFFFu, moves);
-    __nv_bfloat16* base = (lane < 16 ? p.cache.k : p.cache.v) + (lane & 15) * 8;
-    do {
-        uint4 data[kAtOnce];
-        __nv_bfloat16* put[kAtOnce];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            put[i] = nullptr;
-            if (left != 0u) {
-                const int at = __ffs(left) - 1;
-                left &= left - 1u;
-                const long long k_src = __shfl_sync(0xFFFFFFFFu, src[0], at), v_src = __shfl_sync(0xFFFFFFFFu, src[1], at);
-                const long long k_dst = __shfl_sync(0xFFFFFFFFu, dst[0], at), v_dst = __shfl_sync(0xFFFFFFFFu, dst[1], at);
-                put[i] = base + (lane < 16 ? k_dst : v_dst);
-                data[i] = *reinterpret_cast<const uint4*>(base + (lane < 16 ? k_src : v_src));
-            }
-        }
-        sync();
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            if (put[i] != nullptr) *reinterpret_cast<uint4*>(put[i]) = data[i];
-        }
-    } while (left != 0u);
+    __syncthreads();
+    for (int r0 = 0; r0 < p.recent; r0 += kSelectThreads / 8) {
+        const int r = r0 + warp * 4 + lane;
+        evict_move<4>(p, seq, head, lane < 4 && r < p.recent, old + r + by, old + r, lane, [] { __syncthreads(); });
+    }
 }
 
 __global__ void __launch_bounds__(kMoveThreads)
@@ -395,14 +414,17 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     rc = once_per_device(dev.device, 11, set_select_smem);
     if (rc != B2A_OK) return rc;
     const int old = p.budget - p.recent;
-    p.report = most <= p.budget ? 0 : p.recent > 0 ? 2 : 1;
+    // Where few rows move, one launch instead of three (one slot of 4,097 leaves 16 sequences, 64 recent ones: 28.8 us with three
+    // launches, 14.3 with one).
+    p.inside = most > p.budget && most - p.budget + p.recent <= kInsideRows && p.batch <= kFwdStatusWords;
+    p.report = p.inside ? -1 : most <= p.budget ? 0 : p.recent > 0 ? 2 : 1;
     auto select = evict_select;
     auto fill = evict_fill;
     auto shift = evict_shift;
     B2A_CUDA_OK(launch_early(select, static_cast<unsigned int>(rows), kSelectThreads,
                              in_shared && most > p.recent ? select_smem(most - p.recent) : 0, stream, p, in_shared ? 1 : 0));
     // Nothing moves where no sequence can be longer than the budget.
-    if (most <= p.budget) return B2A_OK;
+    if (most <= p.budget || p.inside) return B2A_OK;
     if (old > 0) {
         B2A_CUDA_OK(launch_early(fill, dim3((old + kFillSlots - 1) / kFillSlots, rows), kMoveThreads, 0, stream, p));
     }

@@ -7,8 +7,8 @@
 // 128 (256 bytes a slot and head: bound by memory for up to some 128 rows, by the exponentials beyond); of more rows, two
 // tiles' worth at a time go over the same few blocks, which then come from L2, and the sums wait in shared memory.
 //
-//   warp 0-15   sums, in four groups that take turns at the blocks (with two, a scheduler's two warps did not keep its
-//               special-function unit busy: 256 rows of 32 heads against 16,000 slots TWO us, with four FOUR)
+//   warp 0-15   sums, in four groups that take turns at the blocks: bound by the special-function unit, 1,040 clk a tile of 128 x 128
+//               (two groups 1,280; every second or fourth pair of exponentials as a polynomial on the FMA pipe made it slower)
 //   warp 16     K Q^T       warp 17   plan, loads of K       warp 18   loads of Q and its lse: pages of 16 slots cost a warp some
 //               1,000 clk a block to ask for, which Q must not wait behind
 //
@@ -74,30 +74,6 @@ __host__ __device__ __forceinline__ uint32_t columns_from(int from) {
 
 __device__ __forceinline__ int weight_tiles(const WeightParams& p, int n) { return (n + p.tile_tokens - 1) / p.tile_tokens; }
 
-// 2^x for two values on the FMA pipe, within 2.3e-7: n = round(x) from the low bits of x + 1.5 * 2^23, and 2^(x - n) by a
-// polynomial of degree 5 whose largest relative error on [-0.5, 0.5] a linear program made smallest (6.8e-8 before rounding; the
-// constant term is held at 1, so that x <= -127 gives exactly 0).  NaN stays NaN.
-__device__ __forceinline__ float2 exp2_fma2(float2 x) {
-    constexpr float kMagic = 12582912.f;
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(x.x) : "f"(x.x));   // -127
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(x.y) : "f"(x.y));
-    const float2 t = add2(x, make_float2(kMagic, kMagic));
-    const float2 f = fma2(add2(t, make_float2(-kMagic, -kMagic)), make_float2(-1.f, -1.f), x);
-    float2 p = fma2(f, make_float2(0.0013202981790527701f, 0.0013202981790527701f),
-                    make_float2(0.009674952365458012f, 0.009674952365458012f));
-    p = fma2(p, f, make_float2(0.055510472506284714f, 0.055510472506284714f));
-    p = fma2(p, f, make_float2(0.24022166430950165f, 0.24022166430950165f));
-    p = fma2(p, f, make_float2(0.6931465864181519f, 0.6931465864181519f));
-    p = fma2(p, f, make_float2(1.f, 1.f));
-    return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
-                               __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000)));
-}
-
-// Which of the 4 four-column groups of 16 columns take two of their exponentials from the FMA pipe (bit e: group e).
-#ifndef B2A_WEIGHT_FMA_MASK
-#define B2A_WEIGHT_FMA_MASK 0x0u
-#endif
-
 // Adds exp2(scale s + minus_lse2) of 16 columns, those of which `see` has a bit.
 template <bool kAll>
 __device__ __forceinline__ void weight_sum(const uint32_t (&s)[16], const float4* minus_lse2, float sl2, uint32_t see, float2 (&acc)[4]) {
@@ -109,7 +85,7 @@ __device__ __forceinline__ void weight_sum(const uint32_t (&s)[16], const float4
         float2 p1 = fma2(make_float2(__uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3])), make_float2(sl2, sl2),
                          make_float2(l4.z, l4.w));
         p0 = make_float2(fast_exp2(p0.x), fast_exp2(p0.y));
-        p1 = ((B2A_WEIGHT_FMA_MASK >> e) & 1u) ? exp2_fma2(p1) : make_float2(fast_exp2(p1.x), fast_exp2(p1.y));
+        p1 = make_float2(fast_exp2(p1.x), fast_exp2(p1.y));
         if (!kAll) {
             if (!((see >> (4 * e)) & 1u)) p0.x = 0.f;
             if (!((see >> (4 * e + 1)) & 1u)) p0.y = 0.f;
