@@ -414,8 +414,8 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     rc = once_per_device(dev.device, 11, set_select_smem);
     if (rc != B2A_OK) return rc;
     const int old = p.budget - p.recent;
-    // Where few rows move, one launch instead of three (one slot of 4,097 leaves 16 sequences, 64 recent ones: 28.8 us with three
-    // launches, 14.3 with one).
+    // Where few rows move, one launch instead of three.  Us with one and with three, 8 heads, 4,096 slots kept; of 4 sequences 65 rows
+    // move: 12.4, 15.4; 512: 19.5, 18.3; 1,024: 26.3, 21.6; of 16 sequences 12.4, 19.2; 26.3, 30.0; 34.7, 37.9.
     p.inside = most > p.budget && most - p.budget + p.recent <= kInsideRows && p.batch <= kFwdStatusWords;
     p.report = p.inside ? -1 : most <= p.budget ? 0 : p.recent > 0 ? 2 : 1;
     auto select = evict_select;

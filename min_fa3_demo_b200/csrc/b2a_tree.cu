@@ -756,7 +756,7 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
         return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, t.total);
     }
     p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
-    p.c.min_run = 2;
+    p.c.min_run = 2;     // blocks (1, 2, 4 of them: a tree of 8 tokens over 700 slots, 32 heads over 8, 15.5, 14.9, 15.9 us)
     // A few blocks' time goes into an item's masks, sums and results, so that runs of equal numbers of blocks differ in how many
     // items end in them.  0, 2, 4, 6, 8 blocks (us): one token, 16 sequences of up to 8,001 slots, 58.5, 57.5, 57.2, 57.0, 57.3;
     // trees of up to 32 tokens 87.2, 83.5, 81.2, 80.6, 80.5; of 64, 64 over 8 heads, 179, 175, 172, 168, 173.

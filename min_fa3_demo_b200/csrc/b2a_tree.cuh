@@ -156,8 +156,14 @@ __device__ __forceinline__ bool tree_clean_row(uint8_t* row, int r, bool behind)
     return true;
 }
 
-// b2a_tree_few.cu: the kernels for calls of at most kFewRows rows an item.  map_q's box holds all of an item's.
-constexpr int kFewRows = 64;
+// b2a_tree_few.cu: the kernels for calls of at most kFewRows rows an item.  map_q's box holds all of an item's.  Us with them and
+// with those of b2a_tree.cu, 32 heads over 8, sequences x slots:
+//              1 x 16,384     64 x 2,048      16 x 16,384     4 x 400        32 x 1,000
+//    4 rows    24.7  31.5     99.1  113.2     171.6  174.6    12.4  16.0     35.2  42.8
+//   16         25.9  32.1    104.2  119.1     175.2  178.9    14.1  16.9     38.7  45.8
+//   32         30.8  33.4    121.1  122.2     185.3  182.3    16.5  17.4     50.0  47.1
+//   64         45.0  41.6    190.3  142.5     251.3  186.0    22.2  19.9     78.5  53.7
+constexpr int kFewRows = 32;
 int launch_tree_few(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, int ctas,
                     const DeviceInfo& dev, cudaStream_t stream);
 

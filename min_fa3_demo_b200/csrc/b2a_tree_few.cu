@@ -1,11 +1,11 @@
-// Attention of drafted tokens over a cache for items of at most 64 rows (tokens times query heads of a K/V head): plain
+// Attention of drafted tokens over a cache for items of at most 32 rows (tokens times query heads of a K/V head): plain
 // decoding, and small trees.  The mathematics, the work's order and the masks are those of b2a_tree.cu; the products are made the
 // other way round.
 //
 // S^T = K Q^T has a lane of tensor memory for each slot and a column for each row, so that all 128 threads of a warpgroup share
 // the softmax of a few rows, where a thread for each row would leave most of them idle and one warp with 128 exponentials a
 // row and block.  P^T goes to shared memory in bf16, and O^T += V^T P^T has a lane for each dimension and a column for each row.
-// Both products are 128 x N x 128 with N = 16, 32 or 64.
+// Both products are 128 x N x 128 with N = 16 or 32.
 //
 // Softmax across threads: a row's probabilities are taken relative to a reference in shared memory which all slots of a block
 // have to share.  It need not be the maximum: P in bf16 and the sums in fp32 have the exponents of fp32, so any bound will
@@ -33,7 +33,7 @@ constexpr float kFewAbove = 64.f;     // log2 units: how far above the score tha
 template <int N>
 struct __align__(1024) FewShared {
     // More rows leave room for fewer blocks.
-    static constexpr int kQ = N == 16 ? 2 : 1, kK = N == 64 ? 2 : 3, kV = 3;
+    static constexpr int kQ = N == 16 ? 2 : 1, kK = 3, kV = 3;
     uint8_t q[kQ][N * 256];           // two halves of [N rows][128 bytes]
     uint8_t p[2][N * 256];            // P^T of the warpgroups, likewise
     uint8_t k[kK][kTileBytes];
@@ -44,7 +44,7 @@ struct __align__(1024) FewShared {
     int out_at[N];                    // and which row of out it is
     float top[2][4][N];               // of each warp: maxima, then sums
     float2 stat[2][N];                // reference and sum of the two warpgroups
-    unsigned long long token_rows[N]; // the rows of a token
+    uint32_t token_rows[N];           // the rows of a token
     TreePiece piece[kFewSlots];
     uint64_t q_full[kQ], q_empty[kQ];
     uint64_t k_full[kK], k_empty[kK];
@@ -60,7 +60,7 @@ struct __align__(1024) FewShared {
 
 template <int N>
 constexpr size_t few_smem_bytes() { return sizeof(FewShared<N>) + 1024; }
-static_assert(few_smem_bytes<16>() <= 227 * 1024 && few_smem_bytes<32>() <= 227 * 1024 && few_smem_bytes<64>() <= 227 * 1024, "");
+static_assert(few_smem_bytes<16>() <= 227 * 1024 && few_smem_bytes<32>() <= 227 * 1024, "");
 
 // N columns of tensor memory.
 template <int N>
@@ -77,27 +77,22 @@ __device__ __forceinline__ void few_ld(uint32_t taddr, uint32_t (&r)[N]) {
 }
 
 // Sums of N columns over the lanes of a warp, halving the columns as it halves the lanes: lane j ends with the sum of column
-// j % N (of j and j + 32 in v[0] and v[1] for N = 64).
+// j % N.
 template <int N>
 __device__ __forceinline__ void few_column_sums(float (&v)[N], int lane) {
-    constexpr int kLanes = N < 32 ? N : 32;
     if constexpr (N == 16) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], 16);
     }
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) {
+    for (int d = N / 2; d > 0; d >>= 1) {
         const bool upper = (lane & d) != 0;
 #pragma unroll
-        for (int g = 0; g < N / kLanes; ++g) {
-#pragma unroll
-            for (int i = 0; i < d; ++i) {
-                const float low = v[g * kLanes + i], high = v[g * kLanes + i + d];
-                v[g * kLanes + i] = (upper ? high : low) + __shfl_xor_sync(0xFFFFFFFFu, upper ? low : high, d);
-            }
+        for (int i = 0; i < d; ++i) {
+            const float low = v[i], high = v[i + d];
+            v[i] = (upper ? high : low) + __shfl_xor_sync(0xFFFFFFFFu, upper ? low : high, d);
         }
     }
-    if constexpr (N == 64) v[1] = v[32];
 }
 
 // The eight k-steps of a 128 x N x 128 product, B with two halves of N rows of 128 bytes.
@@ -158,7 +153,7 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
     for (int i = threadIdx.x; i < Shared::kQ * N * 16; i += kFewThreads) reinterpret_cast<uint4*>(&sh.q[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
     if (threadIdx.x < N) {
         const int first = threadIdx.x * p.c.group, last = first + p.c.group;
-        const unsigned long long to = last >= 64 ? ~0ull : (1ull << last) - 1, from = first >= 64 ? ~0ull : (1ull << first) - 1;
+        const uint32_t to = last >= 32 ? ~0u : (1u << last) - 1, from = first >= 32 ? ~0u : (1u << first) - 1;
         sh.token_rows[threadIdx.x] = to & ~from;
         const int token = threadIdx.x / p.c.group, head = threadIdx.x - token * p.c.group;
         sh.lse_at[threadIdx.x] = head * p.lse_head_stride + token;
@@ -181,9 +176,6 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
     const WaitCtx wctx{smem_u32(&sh.abort_flag), p.status, p.timeout_ns, 1u};
 
-    // 64 rows need more registers for the softmax than an even share.
-    if (warp >= 8) {
-    if constexpr (N == 64) reg_dealloc<72>();
     if (warp == kFewLoadWarp) {
         // ---------------------------------------------------------------- plan, loads of Q and K
         if (lane == 0) {
@@ -302,10 +294,8 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
             }
         }
         PH_PRINT("few mma", 4);
-    }
     } else {
         // ---------------------------------------------------------------- softmax
-        if constexpr (N == 64) reg_alloc<216>();
         const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;      // r: slot of the block, dimension of O^T
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_tmem = tmem_base + lane_base + x * N, o_tmem = tmem_base + lane_base + 2 * N;
@@ -350,12 +340,12 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     return true;
                 };
                 // Rows that see this slot: all of them if it lies before the drafted tokens.
-                unsigned long long see = ~0ull;
+                uint32_t see = ~0u;
                 if (tail && slot >= w.len) {
                     const int u = slot - w.len;
                     see = 0;
                     if (slot < w.slots && p.c.mask == nullptr) {
-                        see = u * p.c.group >= 64 ? 0ull : ~0ull << (u * p.c.group);
+                        see = u * p.c.group >= 32 ? 0u : ~0u << (u * p.c.group);
                     } else if (slot < w.slots && u < w.n) {
                         const unsigned char* byte = tree_mask_row(p, w, 0) + u;
 #pragma unroll 8
@@ -392,10 +382,10 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                         }
                     }
                     fence_proxy_async_smem();
-                    if (__any_sync(0xFFFFFFFFu, see != ~0ull)) {
+                    if (__any_sync(0xFFFFFFFFu, see != ~0u)) {
 #pragma unroll
                         for (int c = 0; c < N; ++c) {
-                            if (!((see >> c) & 1ull)) s[c] = 0xFF800000u;    // -inf
+                            if (!((see >> c) & 1u)) s[c] = 0xFF800000u;    // -inf
                         }
                     }
                 }
@@ -520,7 +510,6 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
             ok = meet();                         // nobody still reads maxima
             if (!ok) break;
             if (lane < N) sh.top[x][quarter][lane] = sum[0];
-            if constexpr (N == 64) sh.top[x][quarter][32 + lane] = sum[1];
             ok = meet();
             if (!ok) break;
             if (r < N) {
@@ -670,12 +659,9 @@ int launch_tree_few(const CUtensorMap& map_q, const CUtensorMap& map_k, const CU
     if (p.part_rows <= 16) {
         rc = once_per_device(dev.device, 8, set_few_smem<16>);
         if (rc == B2A_OK) rc = launch_few<16>(map_q, map_k, map_v, p, ctas, stream);
-    } else if (p.part_rows <= 32) {
+    } else {
         rc = once_per_device(dev.device, 9, set_few_smem<32>);
         if (rc == B2A_OK) rc = launch_few<32>(map_q, map_k, map_v, p, ctas, stream);
-    } else {
-        rc = once_per_device(dev.device, 10, set_few_smem<64>);
-        if (rc == B2A_OK) rc = launch_few<64>(map_q, map_k, map_v, p, ctas, stream);
     }
     if (rc != B2A_OK || ctas == 1) return rc;
     auto combine = tree_combine_few;

@@ -24,7 +24,8 @@ namespace {
 constexpr int kWeightGroups = 4;       // of four warps each, which take turns at the blocks
 constexpr int kWeightThreads = 128 * kWeightGroups + 96;
 constexpr int kWeightKStages = kWeightGroups, kWeightQSlots = 2;
-constexpr int kWeightPass = 2;        // query tiles that go over a chunk's blocks together
+constexpr int kWeightPass = 2;        // query tiles that go over a chunk's blocks together (256 tokens, 64 heads over 8, 32,768 slots: 188 us
+                                      // with two, 192 with one; as many as have room)
 constexpr int kWeightChunk = 16;      // blocks that several passes of query tiles go over
 constexpr int kWeightSlots = 4;       // pieces in flight
 constexpr int kWeightMmaWarp = 4 * kWeightGroups, kWeightLoadWarp = kWeightMmaWarp + 1, kWeightQWarp = kWeightMmaWarp + 2;

@@ -106,6 +106,17 @@ def test_numbers_of_drafted_tokens(count, tree):
     ragged.check(*ragged.call())
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("rows", [15, 16, 17, 31, 32, 33, 127, 128, 129, 256, 257])
+def test_rows_of_an_item(rows, tree):
+    """Where the kernel changes: 16, 32, 128 and 256 rows, one of a token each, and as heads of one token."""
+    batch = Batch(rows, [0, 200, 1000], [rows, rows, rows // 2], 1, 1, 16, "plain", tree, slack=3)
+    batch.check(*batch.call())
+    if rows <= 128:
+        one = Batch(rows, [0, 127, 700], [1, 1, 1], rows, 1, 0, "plain", tree)
+        one.check(*one.call())
+
+
 @pytest.mark.parametrize("lens,counts,heads", [([20000], [1], (8, 8)), ([20000], [5], (32, 8)), ([9000, 17, 4000, 1], [40, 40, 40, 40], (8, 1)),
                                                ([33000], [70], (8, 1)), ([300] * 150, [2] * 150, (8, 2)), ([30] * 700, [1] * 700, (2, 1))])
 def test_long_caches_and_many_sequences(lens, counts, heads):
