@@ -163,7 +163,7 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     sequence ``b`` goes to slot ``cache_lens[b] + i``.  With ``axes`` and ``positions`` ``[axes, B, n]`` (``[axes, total]``)
     k is turned as :func:`rotary` turns it; q, if given, likewise, and is returned.  Packed tokens behind
     ``cu_seqlens[B]`` go nowhere, and their rows of the returned q are not written.  A token without a slot is left out
-    and reported by ``check_last_status("append_cache")``.
+    and reported by ``check_last_status("append_cache")``.  No two tokens may be given the same slot by shared pages.
     """
     index, batch, ks = k_cache.get_device(), cache_lens.numel(), k.shape
     dim, tokens = 4 if cu_seqlens is None else 3, ks[:-2]
@@ -284,7 +284,7 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     """Attention of drafted tokens, or of the next token, over the cache.
 
     q ``[B, n, QH, 128]``, or ``[total_q, QH, 128]`` with ``cu_seqlens_q`` ``[B + 1]`` (int32, on the device) and
-    ``max_seqlen_q``.  Token ``i`` of sequence ``b`` lies in slot ``cache_lens[b] + i`` already (:func:`append_cache`).  It
+    ``max_seqlen_q`` (its sequences one behind the other).  Token ``i`` of sequence ``b`` lies in slot ``cache_lens[b] + i`` already (:func:`append_cache`).  It
     sees all slots before ``cache_lens[b]`` and the new tokens ``u`` with ``tree_mask[b, i, u]`` (bool ``[B, n, n]``; packed
     ``[total_q, max_seqlen_q]``, a row for each token); without a mask those up to itself: ``n = 1`` is plain decoding.
     Returns out like q (contiguous) and, with ``return_lse``, the fp32 natural-log LSE ``[B, QH, n]`` (``[QH, total_q]``).  A row

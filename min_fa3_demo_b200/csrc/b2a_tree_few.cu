@@ -9,7 +9,7 @@
 //
 // Softmax across threads: a row's probabilities are taken relative to a reference in shared memory which all slots of a block
 // have to share.  It need not be the maximum: P in bf16 and the sums in fp32 have the exponents of fp32, so any bound will
-// do that lies no more than 2^64 above some score.  A piece begins with that much above its first slot's, and a block asks once
+// do that lies no more than 2^32 above some score (V down to 2^-90 then keeps its products normal).  A piece begins with that much above its first slot's, and a block asks once
 // whether any score is larger (one barrier of the warpgroup); only then are the maxima over the threads looked for.  No
 // probability is above 1, so no product with a finite V overflows.  Each thread adds up its own slots' probabilities; the sums
 // meet at the end of the piece.
@@ -28,7 +28,7 @@ namespace {
 constexpr int kFewThreads = 384;
 constexpr int kFewSlots = 4;
 constexpr int kFewQkWarp = 8, kFewLoadWarp = 9, kFewPvWarp = 10, kFewVWarp = 11;
-constexpr float kFewAbove = 64.f;     // log2 units: how far above the score that it was taken from a reference lies
+constexpr float kFewAbove = 32.f;     // log2 units: how far above the score that it was taken from a reference lies
 
 template <int N>
 struct __align__(1024) FewShared {

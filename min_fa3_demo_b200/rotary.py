@@ -87,7 +87,7 @@ def _is_rows(t: torch.Tensor, dim: int, index: int) -> bool:
     if t.dtype is not _BF16 or t.get_device() != index:
         return False
     size, st = t.shape, t.stride()
-    return (len(size) == dim and size[-1] == 128 and st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0
+    return (len(size) == dim and size[-1] == 128 and size[-2] > 0 and st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0
             and t.data_ptr() & 15 == 0)
 
 
@@ -96,6 +96,7 @@ def _check_heads(t: torch.Tensor, name: str, dim: int) -> None:
     _check(t.dtype == torch.bfloat16, f"{name} must have dtype torch.bfloat16")
     _check(t.dim() == dim, f"{name} must have shape " + ("[B, S, H, D]" if dim == 4 else "[total_tokens, H, D]"))
     _check(t.size(-1) == 128, f"{name} must have head_dim D=128")
+    _check(t.size(-2) > 0, f"{name} must have heads")
     _check(t.stride(-1) == 1 and not any(s & 7 for s in _rows(t)) and t.data_ptr() % 16 == 0,
            f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
 
@@ -150,7 +151,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if fine:
         q_step, batch, seqlen, heads_q = q.stride(), 1 if dim == 3 else qs[0], qs[-3], qs[-2]
         q_rows = (0, q_step[0], q_step[1]) if dim == 3 else q_step[:3]
-        fine = (qs[-1] == 128 and q_step[-1] == 1 and (q_rows[0] | q_rows[1] | q_rows[2]) & 7 == 0 and q_at & 15 == 0
+        fine = (qs[-1] == 128 and q_step[-1] == 1 and (q_rows[0] | q_rows[1] | q_rows[2]) & 7 == 0 and q_at & 15 == 0 and heads_q > 0
                 and positions.shape == ((axes.axes, seqlen) if dim == 3 else (axes.axes, batch, seqlen)))
     k_at, k_rows, heads_k = 0, _NONE3, 0
     if fine and k is not None:
@@ -159,7 +160,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         if fine:
             heads_k = ks[-2]
             k_rows = (0, k_step[0], k_step[1]) if dim == 3 else k_step[:3]
-            fine = (ks[-1] == 128 and k_step[-1] == 1 and (k_rows[0] | k_rows[1] | k_rows[2]) & 7 == 0
+            fine = (ks[-1] == 128 and k_step[-1] == 1 and heads_k > 0 and (k_rows[0] | k_rows[1] | k_rows[2]) & 7 == 0
                     and (dim == 3 or ks[0] == batch))
     if not fine:
         _check_rotary(q, k, positions, axes, dim)
@@ -168,7 +169,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             k_at, k_rows, heads_k = k.data_ptr(), _rows(k), k.size(-2)
     q_out = _like(q)
     k_out = None if k is None else _like(k)
-    if batch * seqlen * heads_q == 0:
+    if batch * seqlen == 0:
         return q_out, k_out
     args = _cabi.ROTARY.pack(axes._at, q_at, k_at, q_out.data_ptr(), 0 if k is None else k_out.data_ptr(), positions.data_ptr(),
                              *q_rows, *k_rows, *_position_strides(positions), positions.dtype is _INT64, batch, seqlen, heads_q,

@@ -201,6 +201,8 @@ REFUSALS = [
     ("rotary", dict(q=lambda: t(3, 5, 4, 64)), "q must have head_dim D=128"),
     ("rotary", dict(q=lambda: t(3, 5, 4, 256)[..., ::2]), "with adjacent values in a head"),
     ("rotary", dict(q=lambda: t(3, 5, 4, 132)[..., :128]), "other strides multiples of 8"),
+    ("rotary", dict(q=lambda: t(3, 5, 0, 128)), "q must have heads"), ("rotary", dict(k=lambda: t(3, 5, 0, 128)), "k must have heads"),
+    ("append", dict(q=lambda: t(3, 5, 0, 128)), "q must have heads"),
     ("rotary", dict(k=lambda: t(3, 6, 2, 128)), "q and k must have the same tokens"),
     ("rotary", dict(k=lambda: t(15, 2, 128)), "k must have shape [B, S, H, D]"),
     ("rotary", dict(k=lambda: t(3, 5, 2, 128, device="cuda:1")), "q and k must be on the same CUDA device"),

@@ -140,6 +140,43 @@ def test_what_does_not_exist_is_left_out_and_reported(what):
     assert torch.equal(cache.k.cpu()[pages[:20], rows[:20]], before.cpu()[pages[torch.tensor(place)], rows[torch.tensor(place)]])
 
 
+@pytest.mark.parametrize("recent", [0, 4])
+@pytest.mark.parametrize("what", ["too long", "negative length", "page too high", "negative page"])
+def test_what_does_not_exist_where_many_rows_move(what, recent):
+    """As above, with rows moved by launches of their own."""
+    cache = Cache(14, 2, 1280, 1, 16)
+    weights = draw(15, 2, 1, cache.slots)
+    lens = [900, 1200]
+    if what == "too long":
+        lens[1] = cache.slots + 1
+    elif what == "negative length":
+        lens[1] = -1
+    else:
+        cache.table[1, 2] = cache.k.size(0) if what == "page too high" else -3
+    before = cache.k.cpu()
+    out = min_fa3_op.evict_cache(cache.k, cache.v, weights.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 200, recent=recent,
+                                 block_table=cache.table)
+    with pytest.raises(RuntimeError, match="device-side check failed"):
+        min_fa3_op.check_last_status("evict_cache")
+    place = torch.tensor(order(weights[0, 0].tolist(), 900, 200, recent))
+    assert torch.equal(out[2][0, 0].cpu().long(), place)
+    pages, rows = cache.index(0)
+    assert torch.equal(cache.k.cpu()[pages[:200], rows[:200]], before[pages[place], rows[place]])
+
+
+@pytest.mark.parametrize("seqs", [252, 253, 300])
+def test_many_sequences(seqs):
+    """Up to 252 sequences report in words of their own."""
+    cache = Cache(seqs, seqs, 24, 1, 8)
+    check(cache, draw(seqs, seqs, 1, cache.slots), [(b * 7) % 25 for b in range(seqs)], 11, 3)
+
+
+@pytest.mark.parametrize("budget", [48, 49, 1000])
+def test_a_budget_that_no_sequence_exceeds(budget):
+    cache = Cache(budget, 2, 48, 2, 16)
+    check(cache, draw(budget, 2, 2, cache.slots), [48, 0], budget, min(budget, 20))
+
+
 def test_graph_and_another_stream():
     cache = Cache(12, 2, 200, 2, 16)
     weights, lens = draw(13, 2, 2, cache.slots).cuda(), torch.tensor([200, 150], dtype=torch.int32).cuda()

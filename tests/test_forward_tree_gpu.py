@@ -147,6 +147,18 @@ def test_growing_scores():
     assert (lse[0].double().cpu() - ref_lse).abs().max().item() <= 150 * 2**-21
 
 
+@pytest.mark.parametrize("count", [1, 7, 30, 70])
+def test_tiny_values(count):
+    """V of 2^-70: probabilities are relative to a bound up to 2^32 above some score, so a product may be as small as 2^-102, and
+    what is lost below 2^-126 is at most 2^-126 a slot of 2^-32 or more in all: 2^-94 * 240, which is 2^-16 of 2^-70.  Each of the two
+    results is rounded once."""
+    batch = Batch(count, [210], [count], 4, 1, 16, slack=20)
+    want = batch.call()[0].double()
+    batch.cache.v *= 2.0**-70
+    out = batch.call()[0].double() * 2.0**70
+    assert ((out - want).abs() <= 2 * BF16_HALF_STEP * want.abs() + 2**-15).all()
+
+
 def test_rows_that_see_nothing():
     batch = Batch(10, [0, 5, 0], [6, 6, 6], 8, 2, 16)
     for b, i in ((0, 0), (0, 5), (1, 2), (2, 3)):
@@ -226,6 +238,27 @@ def test_strided_queries_and_masks(view):
     wide = torch.ones(2, 12, 40, dtype=torch.bool).cuda()
     wide[:, :9, 5:14] = batch.tree_mask
     batch.check(*batch.call(tree_mask=wide[:, :9, 5:14]))
+
+
+@pytest.mark.parametrize("count", [1, 6, 40])
+def test_pages_that_several_sequences_share(count):
+    """A common beginning, stored once, and a page that a sequence's table names twice."""
+    batch = Batch(count, [150, 170, 150], [count] * 3, 8, 2, 16)
+    for b in (1, 2):
+        batch.cache.table[b, :4] = batch.cache.table[0, :4]
+        batch.cache.place[b][:64] = batch.cache.place[0][:64]
+    batch.cache.table[2, 5] = batch.cache.table[2, 1]
+    batch.cache.place[2][80:96] = batch.cache.place[2][16:32]
+    batch.check(*batch.call())
+
+
+def test_out_over_q():
+    """out may be q itself: what is read of a row is read before it is written."""
+    for count in (1, 9, 60, 150):
+        batch = Batch(count, [3000, 40], [count, count], 4, 1, 16)
+        want, want_lse = batch.call()
+        out, lse = batch.call(out=batch.q)
+        assert out is batch.q and torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
 def test_padded_batch_keeps_the_rows_behind_it():
