@@ -16,6 +16,7 @@
 //
 // The two warpgroups take turns at the blocks, each with a reference, a sum and an O^T of its own.  A block needs some 1,000 clk
 // from K to the end of its product with V, and up to six stages of 32 KiB are on their way: bound by memory.
+// One token, 32 heads over 8: 16 sequences of 16,384 slots 1.07 GB in 171 us, 6.3 TB/s; of up to 8,001 slots 293 MB in 57 us, 5.1 TB/s.
 //
 //   warp 0-3, 4-7   softmax
 //   warp 8          K Q^T       warp 10   V^T P^T       warp 9   plan, loads of Q and K       warp 11   loads of V

@@ -7,8 +7,10 @@
 // 128 (256 bytes a slot and head: bound by memory for up to some 128 rows, by the exponentials beyond); of more rows, two
 // tiles' worth at a time go over the same few blocks, which then come from L2, and the sums wait in shared memory.
 //
-//   warp 0-15   sums, in four groups that take turns at the blocks: bound by the special-function unit, 1,040 clk a tile of 128 x 128
-//               (two groups 1,280; every second or fourth pair of exponentials as a polynomial on the FMA pipe made it slower)
+//   warp 0-15   sums, in four groups that take turns at the blocks: bound by the special-function unit, which they keep 83% busy
+//               (2,048 tokens, 32 heads over 8, 16,384 slots before them: 377 us; two groups take 1.2 times as long; every second or
+//               fourth pair of exponentials as a polynomial on the FMA pipe made it slower).  One token, 16 sequences of up to
+//               8,001 slots: 152 MB in 30.5 us, 5.0 TB/s
 //   warp 16     K Q^T       warp 17   plan, loads of K       warp 18   loads of Q and its lse: pages of 16 slots cost a warp some
 //               1,000 clk a block to ask for, which Q must not wait behind
 //
@@ -24,8 +26,8 @@ namespace {
 constexpr int kWeightGroups = 4;       // of four warps each, which take turns at the blocks
 constexpr int kWeightThreads = 128 * kWeightGroups + 96;
 constexpr int kWeightKStages = kWeightGroups, kWeightQSlots = 2;
-constexpr int kWeightPass = 2;        // query tiles that go over a chunk's blocks together (256 tokens, 64 heads over 8, 32,768 slots: 188 us
-                                      // with two, 192 with one; as many as have room)
+constexpr int kWeightPass = 2;        // query tiles that go over a chunk's blocks together (256 tokens, 64 heads over 8, 32,768 slots: 169 us
+                                      // with two, 172 with one; two have room)
 constexpr int kWeightChunk = 16;      // blocks that several passes of query tiles go over
 constexpr int kWeightSlots = 4;       // pieces in flight
 constexpr int kWeightMmaWarp = 4 * kWeightGroups, kWeightLoadWarp = kWeightMmaWarp + 1, kWeightQWarp = kWeightMmaWarp + 2;
@@ -378,18 +380,25 @@ tree_weights(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         const uint32_t see[4] = {some.x & live.x, some.y & live.y, some.z & live.z, some.w & live.w};
                         const uint32_t from = s_tmem + x * 128u;
                         const float4* lse2 = reinterpret_cast<const float4*>(&sh.minus_lse2[q_slot][0]);
-                        // The next 16 columns are on their way out of tensor memory while these are added up.
+                        // The next 16 columns are on their way out of tensor memory while these are added up.  A tile that every
+                        // slot of the warp sees whole has no bits to look at (256 tokens, 64 heads over 8, 32,768 slots: 188 us
+                        // without this, 169 with).
                         uint32_t s0[16], s1[16];
                         tmem_ld_x16(from, s0);
+                        if (rows > 112 && __all_sync(0xFFFFFFFFu, (see[0] & see[1] & see[2] & see[3]) == 0xFFFFFFFFu)) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            if (c * 16 < rows) {
+                            for (int c = 0; c < 8; ++c) {
                                 tmem_wait_ld();
-                                if ((c + 1) * 16 < rows) tmem_ld_x16(from + (c + 1) * 16, c & 1 ? s0 : s1);
-                                const uint32_t bits = (see[c >> 1] >> ((c & 1) * 16)) & 0xFFFFu;
-                                if (__all_sync(0xFFFFFFFFu, bits == 0xFFFFu)) {
-                                    weight_sum<true>(c & 1 ? s1 : s0, lse2 + c * 4, sl2, bits, acc);
-                                } else {
+                                if (c < 7) tmem_ld_x16(from + (c + 1) * 16, c & 1 ? s0 : s1);
+                                weight_sum<true>(c & 1 ? s1 : s0, lse2 + c * 4, sl2, 0xFFFFu, acc);
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                if (c * 16 < rows) {
+                                    tmem_wait_ld();
+                                    if ((c + 1) * 16 < rows) tmem_ld_x16(from + (c + 1) * 16, c & 1 ? s0 : s1);
+                                    const uint32_t bits = see[c >> 1] >> ((c & 1) * 16);
                                     weight_sum<false>(c & 1 ? s1 : s0, lse2 + c * 4, sl2, bits, acc);
                                 }
                             }
