@@ -9,14 +9,15 @@
 //
 // Softmax across threads: a row's probabilities are taken relative to a reference in shared memory which all slots of a block
 // have to share.  It need not be the maximum: P in bf16 and the sums in fp32 have the exponents of fp32, so any bound will
-// do that lies no more than 2^32 above some score (V down to 2^-90 then keeps its products normal).  A piece begins with that much above its first slot's, and a block asks once
-// whether any score is larger (one barrier of the warpgroup); only then are the maxima over the threads looked for.  No
-// probability is above 1, so no product with a finite V overflows.  Each thread adds up its own slots' probabilities; the sums
-// meet at the end of the piece.
+// do that lies no more than 2^32 above some score (V down to 2^-90 then keeps its products normal).  A piece begins with that
+// much above its first slot's, and a block asks once whether any score is larger (one barrier of the warpgroup); only then
+// are the maxima over the threads looked for.  No probability is above 1, so no product with a finite V overflows.  Each
+// thread adds up its own slots' probabilities; the sums meet at the end of the piece.
 //
 // The two warpgroups take turns at the blocks, each with a reference, a sum and an O^T of its own.  A block needs some 1,000 clk
 // from K to the end of its product with V, and up to six stages of 32 KiB are on their way: bound by memory.
-// One token, 32 heads over 8: 16 sequences of 16,384 slots 1.07 GB in 171 us, 6.3 TB/s; of up to 8,001 slots 293 MB in 57 us, 5.1 TB/s.
+// One token, 32 heads over 8, 16 sequences of 16,384 slots: 1.07 GB in 171 us, 6.3 TB/s; of up to 8,001 slots: 293 MB in 57 us,
+// 5.1 TB/s.
 //
 //   warp 0-3, 4-7   softmax
 //   warp 8          K Q^T       warp 10   V^T P^T       warp 9   plan, loads of Q and K       warp 11   loads of V
