@@ -14,7 +14,7 @@
 //   evict_shift    moves the last rows down.  They may overlap their destination, so then one CTA a head goes upwards, a
 //                  chunk in registers at a time.  After evict_fill, whose sources it may overwrite.
 // Where only a few rows can move, evict_select does both itself.
-// 8 sequences of up to 16,000 slots, 8 heads, cut to 4,000 with 250 recent ones: 59 us; each by itself, with cold caches, 32, 24 (128 MB
+// 8 sequences of up to 16,000 slots, 8 heads, cut to 4,000 with 250 recent ones: 57 us; each by itself, with cold caches, 23, 24 (128 MB
 // moved, 5.3 TB/s) and 12.
 #include "b2a_cache.cuh"
 
@@ -147,7 +147,7 @@ __device__ __forceinline__ void evict_move(const EvictParams& p, int seq, int he
 
 // in_shared: the keys of all candidates fit in shared memory; otherwise each pass reads the weights again.  Loops stay rolled up: a
 // CTA goes through each once, and instructions that come from memory cost more than they save (keys in registers, eight passes
-// over 16 each unrolled: 53 us where this takes 32, 16,000 slots of 64 heads).
+// over 16 each unrolled: 53 us where rolled ones took 32, 16,000 slots of 64 heads).
 __global__ void __launch_bounds__(kSelectThreads)
 evict_select(const EvictParams p, const int in_shared) {
     extern __shared__ uint32_t keys[];
@@ -240,6 +240,10 @@ evict_select(const EvictParams p, const int in_shared) {
             __syncthreads();
             key = (key << 8) | static_cast<uint32_t>(found[0]);
             need = found[1];
+            if (need == found[2]) {              // all with these digits stay: the others do not matter (mostly so after three)
+                key <<= shift;
+                break;
+            }
         }
         if (old > 0) {
             const unsigned below = (1u << lane) - 1u;
@@ -417,7 +421,7 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     if (rc != B2A_OK) return rc;
     const int old = p.budget - p.recent;
     // Where few rows move, one launch instead of three.  Us with one and with three, 8 heads, 4,096 slots kept; of 4 sequences 65 rows
-    // move: 12.4, 15.4; 512: 19.5, 18.3; 1,024: 26.3, 21.6; of 16 sequences 12.4, 19.2; 26.3, 30.0; 34.7, 37.9.
+    // move: 10.1, 13.2; 512: 18.6, 17.5; 1,024: 25.2, 20.5; of 16 sequences 10.2, 17.9; 24.5, 29.0; 33.3, 36.4.
     p.inside = most > p.budget && most - p.budget + p.recent <= kInsideRows && p.batch <= kFwdStatusWords;
     p.report = p.inside ? -1 : most <= p.budget ? 0 : p.recent > 0 ? 2 : 1;
     auto select = evict_select;
