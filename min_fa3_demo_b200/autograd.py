@@ -208,7 +208,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """Differentiable :func:`min_fa3_op.rotary`: q and k (or None) turned by positions of one or several axes.
 
     In a CUDA graph, forward and backward are captured together, while no graph of the same leaves that was recorded outside
-    is alive: the engine would make the capture wait for that one's stream."""
+    is alive: the engine would make the capture wait for that one's stream, which ends the capture with an error."""
     return _Rotary.apply(q, k, positions, axes, False)
 
 

@@ -4,7 +4,8 @@ Same function names, argument meaning, output shapes and error behaviour as the 
 (``min_fa3_op.py`` and the pybind layer ``bindings.cpp`` /
 ``csrc/backward/min_fa3_bwd_bindings.cu``), so a caller switches by changing the import.
 PyTorch is used only for device memory and streams; every computation is a call through
-the C ABI declared in ``include/b200attn.h``.  Without the CUDA library the import of the
+the C ABI declared in ``include/b200attn.h``.  ``rotary``, ``append_cache``, ``forward_tree``, ``cache_weights`` and
+``evict_cache`` (``rotary.py``, ``cache.py``) are additions of the same kind for decoding.  Without the CUDA library the import of the
 entry points still works (for CPU-side argument checks) but every compute call raises.
 """
 
