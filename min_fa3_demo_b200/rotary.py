@@ -52,7 +52,12 @@ class RotaryAxes:
         c.turn[:pairs] = [_turn(f) for f in inv_freq]
         c.axis[:pairs] = axis
         c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
-        self._c, self._at = c, ctypes.addressof(c)
+        self._c = c
+
+    @property
+    def _at(self) -> int:
+        # Asked for at each call: a copy or an unpickled object has a structure of its own, elsewhere.
+        return ctypes.addressof(self._c)
 
     @classmethod
     def from_sections(cls, sections: Sequence[int], base: float = 10000.0, *, restart: bool = False,
