@@ -53,7 +53,9 @@ struct __align__(1024) TreeShared {
     uint64_t seen_full[2];
     uint64_t both_done, both_read;
     uint64_t piece_full[kTreeSlots], piece_empty[kTreeSlots];
-    uint32_t not_finite;              // number of the last piece that met a drafted value that is not finite
+    // Number of the last piece, of the even ones and of the odd ones, that met a drafted value that is not finite.  Of two tiles
+    // the first one's warpgroup may be a piece ahead of the other's, and no more: they take S from one place in turn.
+    uint32_t not_finite[2];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -127,7 +129,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 8);   // MMA warps, V's load warp and softmax warps
         }
         sh.abort_flag = 0;
-        sh.not_finite = 0;
+        sh.not_finite[0] = sh.not_finite[1] = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -408,7 +410,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         if (!ok) break;
                         if (slot >= w.slots || look) {
                             if (tree_clean_row(&sh.v[stage][r * 128], r, slot >= w.slots)) {
-                                *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
+                                *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[it & 1u]) = it + 1;
                             }
                         }
                         fence_proxy_async_smem();
@@ -531,7 +533,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (w.blocks == 1) a1 = 0.f;
             }
             if (active) {
-                const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) == it + 1;
+                const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[it & 1u]) == it + 1;
                 // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const bool whole = w.part < 0;
