@@ -141,7 +141,7 @@ __device__ __forceinline__ CacheSeq cache_seq(const CacheQueries& p, int b) {
 }
 
 __device__ __forceinline__ int cache_items(const CacheQueries& p, const CacheSeq& s) {
-    return (s.n + p.item_tokens - 1) / p.item_tokens;
+    return s.n > 0 ? (s.n - 1) / p.item_tokens + 1 : 0;     // item_tokens may be any bound that a caller gave
 }
 
 // Blocks that item `rt` of a sequence sees; at least one, so that rows that see nothing are written too.
