@@ -170,11 +170,16 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 # Rotary positions
 # ------------------------------------------------------------------------------------------
 def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
-    # Gradients come in any layout (expanded, transposed) and may be lazily negated.
+    # Gradients come in any layout (expanded, transposed, at any address of a larger buffer), may be lazily negated, and a zero
+    # tensor has no memory at all.  contiguous() would return a tensor as it is whose address alone is wrong.
+    if t._is_zerotensor():
+        return torch.zeros(t.shape, dtype=t.dtype, device=t.device)
     if t.is_neg():
         t = t.resolve_neg()
     st = t.stride()
-    return t if st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0 and t.data_ptr() & 15 == 0 else t.contiguous()
+    if len(st) < 3 or (st[-1] == 1 and (st[0] | st[1] | st[-2]) & 7 == 0 and t.data_ptr() & 15 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 class _Rotary(torch.autograd.Function):
