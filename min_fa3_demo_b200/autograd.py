@@ -196,6 +196,8 @@ class _Rotary(torch.autograd.Function):
         # A rotation's gradient is the rotation back, whatever q and k were; with create_graph through the same function, so
         # that it can be differentiated again.
         positions, = ctx.saved_tensors
+        need_q, need_k = ctx.needs_input_grad[:2]
+        dq, dk = dq if need_q else None, dk if need_k else None
 
         def back(a, b):
             if torch.is_grad_enabled():

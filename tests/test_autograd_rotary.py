@@ -43,3 +43,24 @@ def test_cpu_tensors_and_other_shapes_are_refused_with_words():
         ag.rotary(torch.zeros(3, 2, 128, dtype=BF16), None, torch.zeros(1, 3, dtype=torch.int64), axes)
     for t in (torch.zeros(128, dtype=BF16), torch.zeros(2, 128, dtype=BF16)):
         assert ag._rows_in_order(t) is t                   # the call's own checks say what is wrong
+
+
+@pytest.mark.parametrize("need_q,need_k", [(True, True), (True, False), (False, True)])
+def test_only_gradients_that_are_asked_for_are_turned(monkeypatch, need_q, need_k):
+    turned = []
+
+    def rotary(q, k, positions, axes, *, inverse=False):
+        turned.append([h.size(-2) for h in (q, k) if h is not None])
+        return q * 2, None if k is None else k * 2
+    monkeypatch.setattr(ag, "_require_cuda", lambda t, name: None)
+    monkeypatch.setattr(ag._op, "rotary", rotary)
+    monkeypatch.setattr(ag, "_plain_tensors", lambda tensors: True, raising=False)
+    q, k = torch.randn(3, 4, 128, requires_grad=need_q), torch.randn(3, 2, 128, requires_grad=need_k)
+    axes = ag._op.RotaryAxes([1.0] * 8)
+    for create_graph in (False, True):
+        del turned[:]
+        out, out_k = ag.rotary(q, k, torch.zeros(1, 3, dtype=torch.int64), axes)
+        leaves = [t for t, need in ((q, need_q), (k, need_k)) if need]
+        grads = torch.autograd.grad(out.sum() + out_k.sum(), leaves, create_graph=create_graph)
+        assert turned == [[4, 2], [h for h, need in ((4, need_q), (2, need_k)) if need]]
+        assert all(torch.equal(g, torch.full_like(g, 2)) for g in grads)
