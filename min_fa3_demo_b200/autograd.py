@@ -16,7 +16,7 @@ module does the pairing once:
                                                    completion counter, copies local K/V into the
                                                    arena, and performs the zero + barrier protocol
 
-The dense operators are registered with ``torch.library.custom_op`` (namespace ``b200attn``)
+The dense operators and ``rotary`` are registered with ``torch.library.custom_op`` (namespace ``b200attn``)
 with fake (meta) implementations, so they trace under ``torch.compile`` / fake tensors; there
 is no CPU implementation — calling them with CPU tensors raises.  Gradients are first order: those of
 ``attention`` refuse to be differentiated again, those of the other two carry no graph; ``rotary``'s can be differentiated again.
@@ -182,14 +182,45 @@ def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, turn: Sequence[int], axis: Sequence[int],
+            adjacent: bool, inverse: bool) -> List[torch.Tensor]:
+    _require_cuda(q, "q")
+    out = _op.rotary(_rows_in_order(q), None if k is None else _rows_in_order(k), positions,
+                     _op.RotaryAxes._from_plain(turn, axis, adjacent), inverse=inverse)
+    return [t for t in out if t is not None]
+
+
+_rotary_op = torch.library.custom_op("b200attn::rotary", _rotary, mutates_args=())
+
+
+@_rotary_op.register_fake
+def _(q, k, positions, turn, axis, adjacent, inverse):
+    return [t.new_empty(t.shape) for t in (q, k) if t is not None]
+
+
+def _turned(q, k, positions, axes, inverse: bool, plain: bool):
+    if plain:
+        return _op.rotary(_rows_in_order(q), None if k is None else _rows_in_order(k), positions, axes, inverse=inverse)
+    if not isinstance(axes, _op.RotaryAxes):
+        raise RuntimeError("axes must be a RotaryAxes")
+    turn, axis, adjacent = axes._plain
+    out = torch.ops.b200attn.rotary(q, k, positions, turn, axis, adjacent, inverse)
+    return out[0], None if k is None else out[1]
+
+
 class _Rotary(torch.autograd.Function):
+    # Where nothing looks on, the operator's body is called as it is, as in _Attention.  A call is so short that _plain_call would
+    # be felt (4 us of 105, forward and backward): grad mode is off here anyhow, _rows_in_order sees to negated and zero tensors, and
+    # the backward of a plain forward only asks whether somebody traces it.
     @staticmethod
     def forward(ctx, q, k, positions, axes, inverse: bool):
-        _require_cuda(q, "q")
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.axes, ctx.inverse = axes, inverse
-        return _op.rotary(_rows_in_order(q), None if k is None else _rows_in_order(k), positions, axes, inverse=inverse)
+        ctx.plain = plain = (type(q) in _PLAIN_TYPES and q.is_cuda and type(positions) in _PLAIN_TYPES
+                             and (k is None or type(k) in _PLAIN_TYPES) and not torch.compiler.is_compiling()
+                             and _LOOKER_CHECKS is not None and not any([check() for check in _LOOKER_CHECKS]))
+        return _turned(q, k, positions, axes, inverse, plain)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -198,16 +229,16 @@ class _Rotary(torch.autograd.Function):
         positions, = ctx.saved_tensors
         need_q, need_k = ctx.needs_input_grad[:2]
         dq, dk = dq if need_q else None, dk if need_k else None
-
-        def back(a, b):
-            if torch.is_grad_enabled():
-                return _Rotary.apply(a, b, positions, ctx.axes, not ctx.inverse)
-            return _op.rotary(_rows_in_order(a), None if b is None else _rows_in_order(b), positions, ctx.axes, inverse=not ctx.inverse)
-        if dq is not None:
-            dq, dk = back(dq, dk)
-        elif dk is not None:
-            dk, _ = back(dk, None)
-        return dq, dk, None, None, None
+        first, second = (dk, None) if dq is None else (dq, dk)
+        if first is None:
+            return None, None, None, None, None
+        if torch.is_grad_enabled():
+            turned = _Rotary.apply(first, second, positions, ctx.axes, not ctx.inverse)
+        else:
+            plain = (ctx.plain and type(first) in _PLAIN_TYPES and (second is None or type(second) in _PLAIN_TYPES)
+                     and _LOOKER_CHECKS[1]() is None)
+            turned = _turned(first, second, positions, ctx.axes, not ctx.inverse, plain)
+        return (None, turned[0], None, None, None) if dq is None else (*turned, None, None, None)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, axes: "_op.RotaryAxes"

@@ -53,6 +53,19 @@ class RotaryAxes:
         c.axis[:pairs] = axis
         c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
         self._c = c
+        # The same as plain values, which an operator's schema can hold: turns as signed numbers of 64 bits.
+        self._plain = ([t - 2**64 if t >= 2**63 else t for t in c.turn[:pairs]], axis, bool(adjacent))
+
+    @classmethod
+    def _from_plain(cls, turn: Sequence[int], axis: Sequence[int], adjacent: bool) -> "RotaryAxes":
+        self = cls.__new__(cls)
+        self.axes, self.pairs = max(axis) + 1, len(axis)
+        self._c = c = _cabi.RotaryAxes()
+        c.turn[:self.pairs] = [t % 2**64 for t in turn]
+        c.axis[:self.pairs] = axis
+        c.pairs, c.axes, c.adjacent = self.pairs, self.axes, int(adjacent)
+        self._plain = (list(turn), list(axis), bool(adjacent))
+        return self
 
     @property
     def _at(self) -> int:

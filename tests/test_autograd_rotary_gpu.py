@@ -37,3 +37,34 @@ def test_addresses_that_are_not_aligned_and_zero_tensors():
     zero = torch._efficientzerotensor(out.shape, dtype=out.dtype, device=out.device)
     grad, = torch.autograd.grad(out, leaf, zero)
     assert grad.shape == q.shape and not grad.any()
+
+
+def test_fake_tensors_and_a_traced_step():
+    """As ``attention``: a compiled step has the operator in its graph, and gives the bits of the ordinary one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q, k = (torch.empty(2, 33, h, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True) for h in (4, 2))
+        out, out_k = autograd.rotary(q, k, torch.empty(3, 2, 33, dtype=torch.int64, device="cuda"), AXES)
+        grads = torch.autograd.grad((out, out_k), (q, k), (out, out_k))
+        assert [t.shape for t in (out, out_k, *grads)] == [q.shape, k.shape] * 2
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (randn(gen, 2, 33, h, 128).cuda().requires_grad_() for h in (4, 2, 2))
+    positions = torch.randint(0, 9000, (3, 2, 33), generator=gen).cuda()
+
+    # Three tensors: a compiled autograd.Function whose arguments are one tensor twice loses a gradient, whatever it computes.
+    def step(a, b, c):
+        out, out_k = autograd.rotary(a * 2, b, positions, AXES)
+        return autograd.attention(out, out_k, c, True, deterministic=True)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+    want, ours = step(q, k, v), compiled(q, k, v)
+    assert torch.equal(ours, want)
+    for a, b in zip(torch.autograd.grad(ours, (q, k, v), torch.ones_like(ours)), torch.autograd.grad(want, (q, k, v), torch.ones_like(want))):
+        assert torch.equal(a, b)
+
+
+def test_profilers_see_the_operator():
+    q = torch.zeros(5, 4, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    positions = torch.zeros(3, 5, dtype=torch.int64, device="cuda")
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        autograd.rotary(q, None, positions, AXES)[0].sum().backward()
+    assert "b200attn::rotary" in {e.key for e in prof.key_averages()}
