@@ -467,6 +467,14 @@ size_t b2a_tree_fwd_workspace_bytes(int32_t seqlen_q, int32_t heads_q, int32_t h
  */
 int b2a_tree_fwd(const b2a_tree_args* args, void* cuda_stream);
 
+/*
+ * b2a_tree_fwd with the pieces' results (up to 38 MB) in a buffer of their own, 16-byte aligned, of b2a_tree_fwd_workspace_bytes -
+ * b2a_tree_fwd_kept_workspace_bytes.  The workspace, whose status b2a_check_status reads, then has only the latter size; the
+ * buffer may be reused in stream order after the call.
+ */
+int b2a_tree_fwd_with_scratch(const b2a_tree_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream);
+size_t b2a_tree_fwd_kept_workspace_bytes(void);
+
 /* Scratch of b2a_cache_weights. */
 size_t b2a_cache_weights_workspace_bytes(void);
 
@@ -504,6 +512,10 @@ size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t b
  * the last ones follow in their order.  Pages must not be shared between sequences.  cache_lens and weights are not changed.
  */
 int b2a_cache_evict(const b2a_evict_args* args, void* cuda_stream);
+
+/* b2a_cache_evict with all but the status in a buffer of its own, as b2a_tree_fwd_with_scratch. */
+int b2a_cache_evict_with_scratch(const b2a_evict_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream);
+size_t b2a_cache_evict_kept_workspace_bytes(int32_t batch);
 
 /* ------------------------------------------------------------------------- */
 /* Device status                                                              */

@@ -319,10 +319,14 @@ SIGNATURES = {
     "b2a_cache_append": (c_int32, [c_void_p, c_void_p]),
     "b2a_tree_fwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
     "b2a_tree_fwd": (c_int32, [c_void_p, c_void_p]),
+    "b2a_tree_fwd_with_scratch": (c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "b2a_tree_fwd_kept_workspace_bytes": (c_size_t, []),
     "b2a_cache_weights_workspace_bytes": (c_size_t, []),
     "b2a_cache_weights": (c_int32, [c_void_p, c_void_p]),
     "b2a_cache_evict_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "b2a_cache_evict": (c_int32, [c_void_p, c_void_p]),
+    "b2a_cache_evict_with_scratch": (c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "b2a_cache_evict_kept_workspace_bytes": (c_size_t, [c_int32]),
     "b2a_check_status": (c_int32, [c_void_p, c_void_p]),
     "b2a_set_wait_timeout_ns": (c_int32, [ctypes.c_uint64]),
     "b2a_profile_enable": (c_int32, [c_int32]),

@@ -15,13 +15,14 @@ tables live on the device, so the kernels check them: what does not exist is lef
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _cabi
-from .min_fa3_op import (_INT32_MAX, _SM100, _check, _check_device_capability, _on_device, _remember_workspace, _stream_ptr,
-                         _workspace)
+from .min_fa3_op import (_INT32_MAX, _SCRATCH_KEPT, _SM100, _check, _check_device_capability, _on_device, _remember_workspace,
+                         _stream_ptr, _workspace)
 from .rotary import (_BF16, _INT32, _INT64, _NONE3, RotaryAxes, _are_positions, _check_heads, _check_positions, _is_rows, _like,
                      _position_strides, _rows)
 
@@ -277,6 +278,25 @@ def _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens
     _check_device_capability(k_cache.device, "min_fa3_demo_b200 forward_tree")
 
 
+# The pieces' results (up to 38 MB) and evict_cache's lists have a buffer of their own, as in min_fa3_op: the workspace outlives the
+# call.  The second allocation costs the host 1.5 us a call, of which sizes that are asked for once give back 0.5.
+_TREE_KEPT = 13312            # b2a_tree_fwd_kept_workspace_bytes
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_bytes(lib, index: int, most: int, heads: int, kvh: int) -> Tuple[int, int]:
+    """Bytes of the workspace that is kept, and of the buffer that is not; with that device current."""
+    nbytes = lib.b2a_tree_fwd_workspace_bytes(most, heads, kvh)
+    return (nbytes, 0) if nbytes <= _SCRATCH_KEPT else (_TREE_KEPT, nbytes - _TREE_KEPT)
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_bytes(lib, batch: int, kvh: int, budget: int, slots: int) -> Tuple[int, int]:
+    nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget, slots)
+    kept = nbytes if nbytes <= _SCRATCH_KEPT else lib.b2a_cache_evict_kept_workspace_bytes(batch)
+    return kept, nbytes - kept
+
+
 def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
                  block_table: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[torch.Tensor] = None,
                  max_seqlen_q: Optional[int] = None, tree_mask: Optional[torch.Tensor] = None, return_lse: bool = False,
@@ -313,11 +333,15 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         return (out, lse) if return_lse else out
     lib = _cabi.load()
     with _on_device(device):
-        nbytes = lib.b2a_tree_fwd_workspace_bytes(most, heads, fields[12])
+        nbytes, more = _tree_bytes(lib, index, most, heads, fields[12])
         ws = _workspace(nbytes, device)
         args = _cabi.TREE.pack(*fields, cache_lens.data_ptr(), cu, q.data_ptr(), mask, out.data_ptr(), lse.data_ptr(), s_tok, s_head,
                                m_seq, m_row, batch, most, total, heads, 0.0, 0, 0, 0, 0, ws.data_ptr(), nbytes)
-        _cabi.check(lib.b2a_tree_fwd(args, _stream_ptr(device)))
+        if more:
+            scratch = ws.new_empty(more)
+            _cabi.check(lib.b2a_tree_fwd_with_scratch(args, scratch.data_ptr(), more, _stream_ptr(device)))
+        else:
+            _cabi.check(lib.b2a_tree_fwd(args, _stream_ptr(device)))
     _remember_workspace("forward_tree", ws)
     return (out, lse) if return_lse else out
 
@@ -423,10 +447,14 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     lib = _cabi.load()
     w_seq, w_head, _ = weights.stride()
     with _on_device(device):
-        nbytes = lib.b2a_cache_evict_workspace_bytes(batch, kvh, budget, slots)
+        nbytes, more = _evict_bytes(lib, batch, kvh, budget, slots)
         ws = _workspace(nbytes, device)
         args = _cabi.EVICT.pack(*fields, cache_lens.data_ptr(), weights.data_ptr(), w_seq, w_head, batch, slots, budget, recent,
                                 lens.data_ptr(), new_weights.data_ptr(), order.data_ptr(), ws.data_ptr(), nbytes)
-        _cabi.check(lib.b2a_cache_evict(args, _stream_ptr(device)))
+        if more:
+            scratch = ws.new_empty(more)
+            _cabi.check(lib.b2a_cache_evict_with_scratch(args, scratch.data_ptr(), more, _stream_ptr(device)))
+        else:
+            _cabi.check(lib.b2a_cache_evict(args, _stream_ptr(device)))
     _remember_workspace("evict_cache", ws)
     return lens, new_weights, order

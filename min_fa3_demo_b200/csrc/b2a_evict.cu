@@ -348,9 +348,12 @@ evict_shift(const EvictParams p) {
     }
 }
 
-// Workspace: the header, a word for each sequence, the movers, and a bit for each slot.
-size_t evict_movers_at(int batch) { return align_up(sizeof(WorkspaceHeader) + batch * sizeof(int), 256); }
-size_t evict_stays_at(int batch, size_t rows, int budget) { return evict_movers_at(batch) + align_up(rows * budget * sizeof(int), 256); }
+// Workspace: the header and a word for each sequence, which are kept after a call, then the movers, and a bit for each slot.
+size_t evict_kept(int batch) { return align_up(sizeof(WorkspaceHeader) + batch * sizeof(int), 256); }
+size_t evict_stays_at(size_t rows, int budget) { return align_up(rows * budget * sizeof(int), 256); }
+size_t evict_scratch(size_t rows, int budget, int slots) {
+    return evict_stays_at(rows, budget) + rows * ((static_cast<size_t>(slots) + 31) / 32) * sizeof(uint32_t);
+}
 
 size_t select_smem(long long candidates) { return (candidates + (candidates + 31) / 32) * sizeof(uint32_t); }   // keys, and a bit for each
 
@@ -368,11 +371,22 @@ extern "C" {
 
 size_t b2a_cache_evict_workspace_bytes(int32_t batch, int32_t heads_k, int32_t budget, int32_t weights_slots) {
     if (batch < 1 || heads_k < 1 || budget < 1 || weights_slots < 1) return 0;   // b2a_cache_evict reports what is wrong
-    const size_t rows = static_cast<size_t>(batch) * heads_k;
-    return b2a::evict_stays_at(batch, rows, budget) + rows * ((static_cast<size_t>(weights_slots) + 31) / 32) * sizeof(uint32_t);
+    return b2a::evict_kept(batch) + b2a::evict_scratch(static_cast<size_t>(batch) * heads_k, budget, weights_slots);
 }
 
+size_t b2a_cache_evict_kept_workspace_bytes(int32_t batch) { return batch < 1 ? 0 : b2a::evict_kept(batch); }
+
 int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
+    using namespace b2a;
+    B2A_REQUIRE(a != nullptr, "args must not be NULL");
+    B2A_REQUIRE(a->batch >= 1, "batch must be >= 1, got %d", a->batch);
+    B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
+                "workspace must be a 16-byte aligned device pointer");
+    const size_t kept = evict_kept(a->batch), behind = a->workspace_bytes > kept ? a->workspace_bytes - kept : 0;
+    return b2a_cache_evict_with_scratch(a, static_cast<uint8_t*>(a->workspace) + kept, behind, cuda_stream);
+}
+
+int b2a_cache_evict_with_scratch(const b2a_evict_args* a, void* scratch, size_t scratch_bytes, void* cuda_stream) {
     using namespace b2a;
     B2A_REQUIRE(a != nullptr, "args must not be NULL");
     EvictParams p{};
@@ -389,10 +403,13 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     B2A_REQUIRE(rows <= 65535, "at most 65535 sequences times K/V heads, got %lld", rows);
     B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
                 "workspace must be a 16-byte aligned device pointer");
-    const size_t need = b2a_cache_evict_workspace_bytes(a->batch, a->cache.heads_k, a->budget, a->weights_slots);
-    if (a->workspace_bytes < need) {
-        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, need);
+    B2A_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 0xF) == 0,
+                "scratch must be a 16-byte aligned device pointer");
+    const size_t kept = evict_kept(a->batch), need = evict_scratch(static_cast<size_t>(rows), a->budget, a->weights_slots);
+    if (a->workspace_bytes < kept) {
+        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, kept);
     }
+    if (scratch_bytes < need) return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "scratch has %zu bytes, need %zu", scratch_bytes, need);
     DeviceInfo dev{};
     rc = current_device_info(&dev);
     if (rc != B2A_OK) return rc;
@@ -410,8 +427,8 @@ int b2a_cache_evict(const b2a_evict_args* a, void* cuda_stream) {
     p.header = static_cast<WorkspaceHeader*>(a->workspace);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     p.bad = reinterpret_cast<int*>(ws + sizeof(WorkspaceHeader));
-    p.movers = reinterpret_cast<int*>(ws + evict_movers_at(a->batch));
-    p.stays = reinterpret_cast<uint32_t*>(ws + evict_stays_at(a->batch, static_cast<size_t>(rows), a->budget));
+    p.movers = static_cast<int*>(scratch);
+    p.stays = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(scratch) + evict_stays_at(static_cast<size_t>(rows), a->budget));
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     const long long most = std::min<long long>(p.cache.block_table == nullptr ? p.cache.page_size
                                                                               : static_cast<long long>(p.cache.page_size) * p.cache.table_width,

@@ -89,7 +89,7 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_
 // Room for such words in a fixed-length forward's workspace (a B200 has 148 SMs; the rest is for copy CTAs): 1 KiB with the header.
 constexpr int kFwdStatusWords = 252;
 
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+constexpr size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Upper bound on work-list entries when documents are cut into `rows`-token pieces.
 inline size_t max_entries(int batch, int total_tokens, int rows) {

@@ -544,12 +544,12 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         p.lse[w.seq * p.lse_seq_stride + head * p.lse_head_stride +
                               (p.c.cu_seqlens_q == nullptr ? token : w.q_begin + token)] = lse;
                     } else {
-                        p.part_stat[(static_cast<long long>(w.part) * 2 + tile) * p.part_rows + r] = make_float2(m_used, l);
+                        p.part_stat[(static_cast<long long>(w.part) * Shared::kTiles + tile) * p.part_rows + r] = make_float2(m_used, l);
                     }
                 }
                 __nv_bfloat16* o_row = p.out + ((static_cast<long long>(w.q_begin) + token) * p.c.heads_q +
                                                 w.head * p.c.group + row_head) * kHeadDim;
-                float4* part = p.part_o + (static_cast<long long>(w.part) * 2 + tile) * 32 * p.part_rows + r;
+                float4* part = p.part_o + (static_cast<long long>(w.part) * Shared::kTiles + tile) * 32 * p.part_rows + r;
                 const int from = two ? 0 : 2 * x, to = two ? 4 : 2 * x + 2;
 #pragma unroll 1
                 for (int c = from; c < to; ++c) {
@@ -641,7 +641,7 @@ tree_combine(const __grid_constant__ TreeParams p) {
     // The first piece ends run cta - 1 (and may begin it); the others begin their runs.
     auto part_of = [&](int i) -> long long {
         const int second = i == 0 && cut.first > static_cast<long long>(cta - 1) * cut.run;
-        return (2ll * (cta - 1 + i) + second) * 2 + tile;
+        return (2ll * (cta - 1 + i) + second) * p.part_tiles + tile;
     };
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float m = -INFINITY, l = 0.f, norm = 0.f;
@@ -709,8 +709,12 @@ int set_tree_smem() {
 struct TreeLayout {
     int ctas, tile_tokens, tiles, rows;   // rows of a tile; few rows: of an item, which is one tile
     bool few;
-    size_t cuts, stat, o, total;          // offsets
+    size_t o, scratch;                    // of the pieces' results behind their sums, and of both
 };
+
+// What is kept after a call: header, status words and cuts.
+constexpr size_t kTreeCutsAt = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
+constexpr size_t kTreeKept = align_up(kTreeCutsAt + kTreeMaxCtas * sizeof(TreeCut), 256);
 
 TreeLayout tree_layout(int seqlen_q, int group, int sms) {
     TreeLayout t{};
@@ -719,11 +723,9 @@ TreeLayout tree_layout(int seqlen_q, int group, int sms) {
     t.tile_tokens = t.few ? seqlen_q : kTileM / group;
     t.tiles = seqlen_q > t.tile_tokens ? 2 : 1;
     t.rows = (t.tiles == 2 ? t.tile_tokens : seqlen_q) * group;
-    t.cuts = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
-    t.stat = t.cuts + align_up(t.ctas * sizeof(TreeCut), 256);
-    const size_t parts = 2ull * t.ctas * (t.few ? 1 : 2) * t.rows;
-    t.o = t.stat + align_up(parts * sizeof(float2), 256);
-    t.total = t.o + parts * kHeadDim * sizeof(float);
+    const size_t parts = 2ull * t.ctas * t.tiles * t.rows;
+    t.o = align_up(parts * sizeof(float2), 256);
+    t.scratch = t.o + parts * kHeadDim * sizeof(float);
     return t;
 }
 
@@ -740,10 +742,21 @@ size_t b2a_tree_fwd_workspace_bytes(int32_t seqlen_q, int32_t heads_q, int32_t h
         current_device_info(&dev) != B2A_OK) {
         return 0;   // b2a_tree_fwd reports what is wrong
     }
-    return tree_layout(seqlen_q, heads_q / heads_k, dev.sm_count).total;
+    return kTreeKept + tree_layout(seqlen_q, heads_q / heads_k, dev.sm_count).scratch;
 }
 
+size_t b2a_tree_fwd_kept_workspace_bytes(void) { return b2a::kTreeKept; }
+
 int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
+    using namespace b2a;
+    B2A_REQUIRE(a != nullptr, "args must not be NULL");
+    B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
+                "workspace must be a 16-byte aligned device pointer");
+    const size_t behind = a->workspace_bytes > kTreeKept ? a->workspace_bytes - kTreeKept : 0;
+    return b2a_tree_fwd_with_scratch(a, static_cast<uint8_t*>(a->workspace) + kTreeKept, behind, cuda_stream);
+}
+
+int b2a_tree_fwd_with_scratch(const b2a_tree_args* a, void* scratch, size_t scratch_bytes, void* cuda_stream) {
     using namespace b2a;
     B2A_REQUIRE(a != nullptr, "args must not be NULL");
     TreeParams p{};
@@ -752,12 +765,15 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     B2A_REQUIRE(a->out != nullptr && (reinterpret_cast<uintptr_t>(a->out) & 0xF) == 0, "out must be a 16-byte aligned device pointer");
     B2A_REQUIRE(a->workspace != nullptr && (reinterpret_cast<uintptr_t>(a->workspace) & 0xF) == 0,
                 "workspace must be a 16-byte aligned device pointer");
+    B2A_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 0xF) == 0,
+                "scratch must be a 16-byte aligned device pointer");
     DeviceInfo dev{};
     rc = current_device_info(&dev);
     if (rc != B2A_OK) return rc;
     const TreeLayout t = tree_layout(a->seqlen_q, p.c.group, dev.sm_count);
-    if (a->workspace_bytes < t.total) {
-        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace_bytes, t.total);
+    if (a->workspace_bytes < kTreeKept || scratch_bytes < t.scratch) {
+        return fail(B2A_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes and %zu for the pieces, need %zu and %zu", a->workspace_bytes,
+                    scratch_bytes, kTreeKept, t.scratch);
     }
     p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
     p.c.min_run = 2;     // blocks (1, 2, 4 of them: a tree of 8 tokens over 700 slots, 32 heads over 8, 15.5, 14.9, 15.9 us)
@@ -784,9 +800,10 @@ int b2a_tree_fwd(const b2a_tree_args* a, void* cuda_stream) {
     p.scale_log2 = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / std::sqrt(static_cast<float>(kHeadDim))) * kLog2e;
     p.status = reinterpret_cast<unsigned int*>(reinterpret_cast<WorkspaceHeader*>(ws) + 1);
     p.timeout_ns = wait_timeout_ns();
-    p.cuts = reinterpret_cast<TreeCut*>(ws + t.cuts);
-    p.part_stat = reinterpret_cast<float2*>(ws + t.stat);
-    p.part_o = reinterpret_cast<float4*>(ws + t.o);
+    p.cuts = reinterpret_cast<TreeCut*>(ws + kTreeCutsAt);
+    p.part_stat = reinterpret_cast<float2*>(scratch);
+    p.part_o = reinterpret_cast<float4*>(static_cast<uint8_t*>(scratch) + t.o);
+    p.part_tiles = t.tiles;
     p.part_rows = t.rows;
 
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);

@@ -20,8 +20,9 @@ struct TreeParams {
     uint32_t timeout_ns;
     // Pieces that do not cover their item: two a CTA, the one its run begins with and the one it ends with.
     struct TreeCut* cuts;        // [CTAs]: the item that a run begins inside of
-    float2* part_stat;           // [2 * CTAs][2 tiles][part_rows] (row maximum, row sum); few rows: no tiles, (reference, row sum)
-    float4* part_o;              // [2 * CTAs][2 tiles][32][part_rows] O before the division; few rows: [2 * CTAs][part_rows][32]
+    float2* part_stat;           // [2 * CTAs][part_tiles][part_rows] (row maximum, row sum); few rows: (reference, row sum)
+    float4* part_o;              // [2 * CTAs][part_tiles][32][part_rows] O before the division; few rows: [2 * CTAs][part_rows][32]
+    int part_tiles;
     int part_rows;
 };
 
