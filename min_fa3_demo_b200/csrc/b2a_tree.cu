@@ -463,8 +463,10 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     const float factor = m_new == -INFINITY ? 1.f : fast_exp2((m_used - m_new) * sl2);
                     l *= factor;
                     m_used = m_new;
-                    ok = wait_pv();
-                    if (!ok) break;
+                    if (pv_pending) {         // a block that ends a sequence has waited already
+                        ok = wait_pv();
+                        if (!ok) break;
+                    }
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t t[32];
