@@ -42,6 +42,10 @@ struct CacheView {
         const int page = block_table[seq * table_stride + entry_of(static_cast<int>(slot), row)];
         return page >= 0 && page < pages ? page : -1;
     }
+    __device__ __forceinline__ bool has(int seq, int slot) const {
+        int row;
+        return page_of(seq, slot, &row) >= 0;
+    }
     // Where a slot's head lies in K (V), in elements; -1: nowhere.
     __device__ __forceinline__ long long at(const long long (&stride)[3], int page, int row, int head) const {
         return page < 0 ? -1 : page * stride[0] + row * stride[1] + head * stride[2];
@@ -262,7 +266,7 @@ inline int make_slot_map(CUtensorMap* map, const CacheView& c, bool keys, int bo
 struct SlotLoader {
     int shift, boxes;        // rows of a box, a power of two
     int page, row;
-    int bad;                 // this lane met a page that does not exist (TMA fills such a box with zeros)
+    int bad;                 // this lane met a page that does not exist
 
     __device__ __forceinline__ explicit SlotLoader(int box_rows) {
         shift = __ffs(box_rows) - 1;
@@ -295,8 +299,13 @@ struct SlotLoader {
         }
         __syncwarp();
     }
-    __device__ __forceinline__ void check(const CacheView& c, int n, int lane) {
-        bad |= lane < n && static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages);
+    // Before a block is loaded: whether one of its pages does not exist.  TMA fills such a box with zeros, and its slots must not
+    // take part, so the CTA is told (`missing`, in shared memory, never taken back: its blocks then look up their pages).
+    __device__ __forceinline__ void check(const CacheView& c, int n, int lane, uint32_t* missing) {
+        const int gone = lane < n && static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages);
+        bad |= gone;
+        if (__any_sync(0xFFFFFFFFu, gone) && lane == 0) *reinterpret_cast<volatile uint32_t*>(missing) = 1u;
+        __syncwarp();
     }
 };
 

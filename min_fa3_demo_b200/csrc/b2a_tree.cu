@@ -56,6 +56,7 @@ struct __align__(1024) TreeShared {
     // Number of the last piece, of the even ones and of the odd ones, that met a drafted value that is not finite.  Of two tiles
     // the first one's warpgroup may be a piece ahead of the other's, and no more: they take S from one place in turn.
     uint32_t not_finite[2];
+    uint32_t missing;                 // the CTA has met a page that does not exist
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -130,6 +131,7 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         sh.abort_flag = 0;
         sh.not_finite[0] = sh.not_finite[1] = 0;
+        sh.missing = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -201,10 +203,10 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
                     if (!ok) break;
                     PH_MARK(1);
+                    now.check(p.c.cache, boxes, lane, &sh.missing);
+                    loader.bad |= now.bad;
                     now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
                     PH_MARK(2);
-                    now.check(p.c.cache, boxes, lane);
-                    loader.bad |= now.bad;
                     if (kTwo && i == 0 && w.tokens[1] > 0) load_q(1);
                 }
                 if (!ok) break;
@@ -415,22 +417,33 @@ tree_attention(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         }
                         fence_proxy_async_smem();
                     }
-                    if (active) {
-                        // One bit per visible slot of 32.
-                        const int lim = min(w.slots, w.len + token + 1) - base;
+                }
+                if (active && tail) {
+                    // One bit per visible slot of 32.
+                    const int lim = min(w.slots, w.len + token + 1) - base;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t bits;
-                            if (masked) {
-                                bits = seen[min(row_token, tokens - 1) * 4 + c];
-                            } else {
-                                const int vis = min(max(lim - c * 32, 0), 32);
-                                bits = vis == 32 ? 0xFFFFFFFFu : (1u << vis) - 1u;
-                            }
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t bits;
+                        if (masked) {
+                            bits = seen[min(row_token, tokens - 1) * 4 + c];
+                        } else {
+                            const int vis = min(max(lim - c * 32, 0), 32);
+                            bits = vis == 32 ? 0xFFFFFFFFu : (1u << vis) - 1u;
+                        }
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                if (!((bits >> e) & 1u)) s[c * 32 + e] = -INFINITY;
-                            }
+                        for (int e = 0; e < 32; ++e) {
+                            if (!((bits >> e) & 1u)) s[c * 32 + e] = -INFINITY;
+                        }
+                    }
+                }
+                // Asked by the whole warp: the flag may go up, for a block still to come, between two lanes' looks.
+                if (__builtin_expect(__any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u), 0)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t bits = __ballot_sync(0xFFFFFFFFu, p.c.cache.has(w.seq, base + c * 32 + lane));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            if (!((bits >> e) & 1u)) s[c * 32 + e] = -INFINITY;
                         }
                     }
                 }

@@ -56,6 +56,7 @@ struct __align__(1024) FewShared {
     uint64_t piece_full[kFewSlots], piece_empty[kFewSlots];
     uint32_t moves[2][2];             // of each warpgroup, in turn: number of the last block that had to move a reference
     uint32_t not_finite;
+    uint32_t missing;                 // the CTA has met a page that does not exist
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -148,6 +149,7 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         sh.abort_flag = 0;
         sh.not_finite = 0;
+        sh.missing = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -223,10 +225,10 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
                 if (!ok) break;
                 PH_MARK(1);
+                now.check(p.c.cache, boxes, lane, &sh.missing);
+                loader.bad |= now.bad;
                 now.load(&map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
                 PH_MARK(2);
-                now.check(p.c.cache, boxes, lane);
-                loader.bad |= now.bad;
             }
             if (!ok) break;
             walk.advance(p.c, w.blocks);
@@ -363,6 +365,8 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 ++block_cnt;
                 PH_MARK(1);
                 tc_fence_after_sync();
+                // One answer for the warp: the flag may go up, for a block still to come, between two lanes' looks.
+                const bool missing = __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u);
                 uint32_t s[N];
                 few_ld<N>(s_tmem, s);
                 tmem_wait_ld();
@@ -384,11 +388,12 @@ tree_attention_few(const __grid_constant__ CUtensorMap map_q, const __grid_const
                         }
                     }
                     fence_proxy_async_smem();
-                    if (__any_sync(0xFFFFFFFFu, see != ~0u)) {
+                }
+                if (missing && !p.c.cache.has(w.seq, slot)) see = 0;
+                if ((tail || missing) && __any_sync(0xFFFFFFFFu, see != ~0u)) {
 #pragma unroll
-                        for (int c = 0; c < N; ++c) {
-                            if (!((see >> c) & 1u)) s[c] = 0xFF800000u;    // -inf
-                        }
+                    for (int c = 0; c < N; ++c) {
+                        if (!((see >> c) & 1u)) s[c] = 0xFF800000u;    // -inf
                     }
                 }
                 PH_MARK(3);
