@@ -351,7 +351,7 @@ int b2a_ring_bwd(const b2a_ring_bwd_args* args, void* cuda_stream);
 /*
  * Which angle each pair of a head's dimensions turns by: pair i by positions[axis[i]] times its frequency.  The
  * frequency is given as the fraction of a turn a position makes, round(f / (2 pi) * 2^64) mod 2^64: the low 64 bits of
- * position * turn are then the fraction of a turn that is left, exact however far the position is.
+ * position * turn are then the fraction of a turn that is left, off by half of 2^-64 of a turn for each position at most.
  * pairs is a multiple of 8, at most 64; the dimensions behind the first 2 * pairs stay as they are.
  */
 typedef struct b2a_rotary_axes {

@@ -6,7 +6,9 @@
 //
 // Far positions: a product of a position of a million and a frequency in 32 bits is off by 0.06.  The frequency comes as the
 // fraction of a turn that one position makes, in units of 2^-64, so that position * turn mod 2^64 is the fraction of a turn
-// that is left over; its upper 32 bits go to sincospif.  One 64-bit integer product, no reduction, an angle within 4e-9.
+// that is left over; its upper 32 bits go to sincospif, as a float.  One 64-bit integer product, no reduction.  The float's 24 bits
+// leave the angle within 1.1e-7 for positions up to 2^36; the frequency's own rounding, half of 2^-64 of a turn, adds 1.7e-19 for each
+// position (2^45: 6e-6, a bf16 result's rounding is 4e-3).
 //
 // Bound by memory: 256 bytes in and out a token and head.  A CTA takes a few tokens, computes their angles once into shared
 // memory, and its threads then go over the heads, eight to a head with two 16-byte loads each.  32,760 tokens of 32 + 8 heads: 672 MB

@@ -34,7 +34,8 @@ class RotaryAxes:
 
     Pair ``i`` turns by ``positions[axis[i]] * inv_freq[i]``; there are 8, 16, ... or 64 pairs, and the dimensions behind the
     first ``2 * pairs`` stay as they are.  ``adjacent``: pair ``i`` is dimensions ``(2 i, 2 i + 1)``, otherwise
-    ``(i, i + pairs)``.  Frequencies are taken as the 64-bit floats they are; far positions lose nothing.
+    ``(i, i + pairs)``.  Frequencies are taken as the 64-bit floats they are.  An angle is within 1.1e-7 for
+    positions up to 2^36, and 1.7e-19 times the position more beyond (2^45: 6e-6).
     """
 
     def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False):
