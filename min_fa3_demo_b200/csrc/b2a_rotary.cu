@@ -12,8 +12,8 @@
 //
 // Bound by memory: 256 bytes in and out a token and head.  A CTA takes a few tokens, computes their angles once into shared
 // memory, and its threads then go over the heads, eight to a head with two 16-byte loads each.  32,760 tokens of 32 + 8 heads: 672 MB
-// in 110 us, 6.1 TB/s; 8 x 1,024 of 16 + 16: 134 MB in 28 us, 4.9 TB/s; 8,192 new tokens of 4 sequences with q, k and v, 32 + 8 + 8
-// heads, into pages of 16 slots: 139 MB in 28 us.
+// in 110 us, 6.1 TB/s; 8 x 1,024 of 16 + 16: 134 MB in 28 us, 4.9 TB/s; 5,647 new tokens of 4 sequences with q, k and v, 32 + 8 + 8
+// heads, into pages of 16 slots: 139 MB in 28.7 us.
 #include "b2a_cache.cuh"
 
 namespace b2a {

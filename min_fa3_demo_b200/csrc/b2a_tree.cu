@@ -5,7 +5,7 @@
 // 128 / group tokens of group heads.  What an item (up to 256 rows of one K/V head against its slots) costs is its slots,
 // 512 bytes each, whatever the number of rows, so the kernel is bound by memory up to some 256 rows and by the softmax beyond.
 // 16 sequences of 16,384 slots, 8 K/V heads, 64 rows: 1.07 GB in 186 us, 5.8 TB/s; 16 of up to 8,000 slots in pages of 16, up
-// to 128 rows: 353 MB in 80 us, 4.4 TB/s; 8 of up to 16,000 slots, 512 rows: 147 GFLOP in 167 us, 0.88 PFLOP/s.
+// to 128 rows: 353 MB in 81 us, 4.4 TB/s; 8 of up to 16,000 slots, 512 rows: 147 GFLOP in 168 us, 0.88 PFLOP/s.
 //
 // Work: all items' blocks of 128 slots in a row, dealt out in equal runs, a run a CTA (CacheWalk).  An item that crosses the
 // end of a run is finished by tree_combine, in fp32 and in slot order.

@@ -10,7 +10,7 @@
 //   warp 0-15   sums, in four groups that take turns at the blocks: bound by the special-function unit, which they keep 83% busy
 //               (2,048 tokens, 32 heads over 8, 16,384 slots before them: 377 us; two groups take 1.2 times as long; every second or
 //               fourth pair of exponentials as a polynomial on the FMA pipe made it slower).  One token, 16 sequences of up to
-//               8,001 slots: 152 MB in 30.5 us, 5.0 TB/s
+//               8,001 slots: 152 MB in 31.2 us, 4.9 TB/s
 //   warp 16     K Q^T       warp 17   plan, loads of K       warp 18   loads of Q and its lse: pages of 16 slots cost a warp some
 //               1,000 clk a block to ask for, which Q must not wait behind
 //
