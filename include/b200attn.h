@@ -458,12 +458,12 @@ typedef struct b2a_tree_args {
 size_t b2a_tree_fwd_workspace_bytes(int32_t seqlen_q, int32_t heads_q, int32_t heads_k);
 
 /*
- * Attention of drafted tokens over the cache.  Drafted token i of sequence b lies in slot cache_lens[b] + i already.  Its row
- * sees every slot below cache_lens[b] and those drafted tokens u whose mask byte [i][u] is not 0 (no mask: u <= i).  A row
- * that sees nothing gives out = 0 and lse = -inf; what a row does not see has no part in it, NaN and infinities
- * included, and nobody sees slots whose page does not exist (the status word says so).  Rows behind cu_seqlens_q[batch] are left as they were.  Long sequences are cut along their slots and the
- * pieces added up in fp32 in a fixed order, so repeated calls give the same bits; the last bits can depend on the other
- * sequences of the call.
+ * Attention of drafted tokens over the cache.  Drafted token i of sequence b lies in slot cache_lens[b] + i already.  Its
+ * row sees every slot below cache_lens[b] and those drafted tokens u whose mask byte [i][u] is not 0 (no mask: u <= i).  A
+ * row that sees nothing gives out = 0 and lse = -inf; what a row does not see has no part in it, NaN and infinities
+ * included, and nobody sees slots whose page does not exist (the status word says so).  Rows behind cu_seqlens_q[batch]
+ * are left as they were.  Long sequences are cut along their slots and the pieces added up in fp32 in a fixed order, so
+ * repeated calls give the same bits; the last bits can depend on the other sequences of the call.
  */
 int b2a_tree_fwd(const b2a_tree_args* args, void* cuda_stream);
 
@@ -480,9 +480,10 @@ size_t b2a_cache_weights_workspace_bytes(void);
 
 /*
  * What attention each slot received: weights[b][h][s] += the sum over the rows of K/V head h that see slot s of
- * exp(softmax_scale q k - lse), with the lse that b2a_tree_fwd gave.  Arguments as there (v, out unused); rows with lse = -inf or
- * +inf add nothing, and slots whose page does not exist receive nothing.  weights_slots may be fewer than the cache has: sequences must then not be longer.  Slots behind a
- * sequence are left as they were.  Repeated calls add the same bits.
+ * exp(softmax_scale q k - lse), with the lse that b2a_tree_fwd gave.  Arguments as there (v, out unused); rows with lse =
+ * -inf or +inf add nothing, and slots whose page does not exist receive nothing. weights_slots may be fewer than the cache
+ * has: sequences must then not be longer.  Slots behind a sequence are left as they were.  Repeated calls add the same
+ * bits.
  */
 int b2a_cache_weights(const b2a_tree_args* args, void* cuda_stream);
 

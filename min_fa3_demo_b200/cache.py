@@ -433,9 +433,9 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     weights in the new order (0 behind the new length), and for each slot the slot that its contents come from,
     ``[B, KVH, budget]`` (int32, -1 behind the new length), for whatever else the caller keeps by slot.  Heavy slots below
     ``budget - recent`` keep their place, the gaps are filled in ascending order with the heavy ones from behind, and the last
-    ones follow in their order.  Give ``weights`` no more slots than the longest sequence may have: where
-    ``slots - budget + recent`` is at most 512 one launch does it all.  Sequences within the budget stay as they are.  Pages must not be shared between sequences.
-    Lengths and pages that do not exist are reported by ``check_last_status("evict_cache")``.
+    ones follow in their order.  Give ``weights`` no more slots than the longest sequence may have: where ``slots - budget +
+    recent`` is at most 512 one launch does it all.  Sequences within the budget stay as they are.  Pages must not be shared
+    between sequences.  Lengths and pages that do not exist are reported by ``check_last_status("evict_cache")``.
     """
     budget, recent = int(budget), int(recent)
     index, batch = k_cache.get_device(), cache_lens.numel()
