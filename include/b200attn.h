@@ -360,6 +360,7 @@ typedef struct b2a_rotary_axes {
     int32_t pairs;
     int32_t axes;               /* rows of positions */
     int32_t adjacent;           /* pair i: dimensions (2 i, 2 i + 1); otherwise (i, i + pairs) */
+    float magnitude;            /* what turned pairs are multiplied by; 0 = 1 */
 } b2a_rotary_axes;
 
 typedef struct b2a_rotary_args {
@@ -380,7 +381,7 @@ typedef struct b2a_rotary_args {
     int32_t inverse;            /* 1: by the negative angles, which is the gradient's rotation */
 } b2a_rotary_args;
 
-/* q and k turned by their positions: y1 = x1 cos a - x2 sin a, y2 = x2 cos a + x1 sin a for each pair (x1, x2). */
+/* q and k turned by their positions: y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a) for each pair (x1, x2), m the magnitude. */
 int b2a_rotary(const b2a_rotary_args* args, void* cuda_stream);
 
 /*
@@ -474,6 +475,35 @@ int b2a_tree_fwd(const b2a_tree_args* args, void* cuda_stream);
  */
 int b2a_tree_fwd_with_scratch(const b2a_tree_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream);
 size_t b2a_tree_fwd_kept_workspace_bytes(void);
+
+/*
+ * A cache in 8 bits: b2a_cache with k and v in e4m3 (float8_e4m3fn), strides in elements and multiples of 16, and with scales. A value of
+ * slot s stands for itself times the scale of its head and of block s / block (within its page): a block's scale lies in fp32
+ * [pages, ceil(page_size / block), heads_k].  Scales are positive and finite.
+ */
+typedef struct b2a_cache_scales {
+    float* k;
+    float* v;
+    int64_t k_stride[3];        /* elements from page to page, block to block, head to head */
+    int64_t v_stride[3];
+    int32_t block;              /* slots of a scale: a power of two, 16 or more; with a block table it divides page_size */
+} b2a_cache_scales;
+
+/*
+ * b2a_cache_append into a cache in 8 bits.  A block that its first new token begins gets the smallest power of two as its scale with which
+ * the new values of its head fit (at most 448 times it), within 2^-64 .. 2^64; one that held tokens keeps its scale while that is
+ * enough, and if not gets such a power of two, by which the tokens that it held are divided and rounded anew.  Values are turned and
+ * scaled in fp32 and rounded once; those that are not finite become NaN and have no say in the scale.  No two
+ * tokens may be given the same block of slots by shared pages.
+ */
+int b2a_cache8_append(const b2a_append_args* args, const b2a_cache_scales* scales, void* cuda_stream);
+
+/*
+ * b2a_tree_fwd_with_scratch over a cache in 8 bits; workspace and scratch have the same sizes.  Q and the probabilities take part in the
+ * products as sums of two 8-bit numbers: Q is off by 2^-18 of a row's largest value at most, a probability by 2^-7 of itself or
+ * 2^-22 of the row's largest.  V's scales are taken within 2^-64 .. 2^64, and infinities of q as NaN.
+ */
+int b2a_tree8_fwd(const b2a_tree_args* args, const b2a_cache_scales* scales, void* scratch, size_t scratch_bytes, void* cuda_stream);
 
 /* Scratch of b2a_cache_weights. */
 size_t b2a_cache_weights_workspace_bytes(void);

@@ -169,6 +169,7 @@ class RotaryAxes(Structure):
         ("pairs", c_int32),
         ("axes", c_int32),
         ("adjacent", c_int32),
+        ("magnitude", c_float),
     ]
 
 
@@ -264,6 +265,18 @@ class TreeArgs(Structure):
     ]
 
 
+class CacheScales(Structure):
+    """Mirror of ``b2a_cache_scales``."""
+
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3),
+        ("block", c_int32),
+    ]
+
+
 class EvictArgs(Structure):
     """Mirror of ``b2a_evict_args``."""
 
@@ -289,6 +302,7 @@ _CACHE_FORMAT = "3Qq3q3q4i"
 ROTARY = struct.Struct("<6Q3q3q3q6i")
 APPEND = struct.Struct(f"<{_CACHE_FORMAT}8Q3q3q3q3q5i4x2Q")
 TREE = struct.Struct(f"<{_CACHE_FORMAT}6Q2q2q4if4xQ2qi4x2Q")
+SCALES = struct.Struct("<2Q3q3qi4x")
 EVICT = struct.Struct(f"<{_CACHE_FORMAT}2Q2q4i5Q")
 
 
@@ -321,6 +335,8 @@ SIGNATURES = {
     "b2a_tree_fwd": (c_int32, [c_void_p, c_void_p]),
     "b2a_tree_fwd_with_scratch": (c_int32, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "b2a_tree_fwd_kept_workspace_bytes": (c_size_t, []),
+    "b2a_cache8_append": (c_int32, [c_void_p, c_void_p, c_void_p]),
+    "b2a_tree8_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "b2a_cache_weights_workspace_bytes": (c_size_t, []),
     "b2a_cache_weights": (c_int32, [c_void_p, c_void_p]),
     "b2a_cache_evict_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),

@@ -183,10 +183,10 @@ def _rows_in_order(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, turn: Sequence[int], axis: Sequence[int],
-            adjacent: bool, inverse: bool) -> List[torch.Tensor]:
+            adjacent: bool, inverse: bool, magnitude: float = 1.0) -> List[torch.Tensor]:
     _require_cuda(q, "q")
     out = _op.rotary(_rows_in_order(q), None if k is None else _rows_in_order(k), positions,
-                     _op.RotaryAxes._from_plain(turn, axis, adjacent), inverse=inverse)
+                     _op.RotaryAxes._from_plain(turn, axis, adjacent, magnitude), inverse=inverse)
     return [t for t in out if t is not None]
 
 
@@ -194,7 +194,7 @@ _rotary_op = torch.library.custom_op("b200attn::rotary", _rotary, mutates_args=(
 
 
 @_rotary_op.register_fake
-def _(q, k, positions, turn, axis, adjacent, inverse):
+def _(q, k, positions, turn, axis, adjacent, inverse, magnitude=1.0):
     return [t.new_empty(t.shape) for t in (q, k) if t is not None]
 
 
@@ -204,7 +204,7 @@ def _turned(q, k, positions, axes, inverse: bool, plain: bool):
     if not isinstance(axes, _op.RotaryAxes):
         raise RuntimeError("axes must be a RotaryAxes")
     turn, axis, adjacent = axes._plain
-    out = torch.ops.b200attn.rotary(q, k, positions, turn, axis, adjacent, inverse)
+    out = torch.ops.b200attn.rotary(q, k, positions, turn, axis, adjacent, inverse, axes.magnitude)
     return out[0], None if k is None else out[1]
 
 
@@ -224,7 +224,7 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        # A rotation's gradient is the rotation back, whatever q and k were; with create_graph through the same function, so
+        # A rotation's gradient is the rotation back (times the same magnitude), whatever q and k were; with create_graph through the same function, so
         # that it can be differentiated again.
         positions, = ctx.saved_tensors
         need_q, need_k = ctx.needs_input_grad[:2]

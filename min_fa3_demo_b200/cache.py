@@ -5,6 +5,11 @@ which pages hold a sequence, or, without a block table, ``[B, slots, KVH, 128]``
 values of a head are adjacent: pages with k and v side by side, heads before slots, one layer of many.  ``cache_lens``
 ``[B]`` (int32, on the device) is the number of slots that are in use; no call changes it, so that the host never waits.
 
+A cache may also be in 8 bits: k and v in ``torch.float8_e4m3fn`` and, for each block of 16, 32, 64 or 128 slots and head, a scale:
+``k_scales`` and ``v_scales`` ``[pages, page_size / block, KVH]`` (fp32; of any strides, the number of blocks rounded up where there are
+no pages, whose size is a multiple of the block).  :func:`append_cache` finds the scales, :func:`forward_tree` takes
+any positive ones; the other two want bf16.
+
 A decoding step: :func:`append_cache` writes the drafted tokens behind ``cache_lens``, :func:`forward_tree` lets them attend,
 and once some are accepted the caller writes those again (their positions are the same) and adds them to ``cache_lens``.
 :func:`cache_weights` adds up the attention that slots receive, :func:`evict_cache` drops those that received least.
@@ -29,14 +34,18 @@ from .rotary import (_BF16, _INT32, _INT64, _NONE3, RotaryAxes, _are_positions, 
 __all__ = ["append_cache", "forward_tree", "cache_weights", "evict_cache"]
 
 
-def _check_cache(cache: torch.Tensor, name: str) -> None:
+_E4M3 = torch.float8_e4m3fn
+
+
+def _check_cache(cache: torch.Tensor, name: str, dtype: torch.dtype = _BF16) -> None:
     _check(cache.is_cuda, f"{name} must be a CUDA tensor")
-    _check(cache.dtype == torch.bfloat16, f"{name} must have dtype torch.bfloat16")
+    _check(cache.dtype == dtype, f"{name} must have dtype {dtype}" + (" or, with scales, torch.float8_e4m3fn" if dtype is _BF16 else ""))
+    few = 7 if dtype is _BF16 else 15
     _check(cache.dim() == 4, f"{name} must have shape [pages, page_size, KVH, D]")
     _check(cache.size(3) == 128, f"{name} must have head_dim D=128")
     _check(cache.size(0) > 0 and cache.size(1) > 0 and cache.size(2) > 0, f"{name} must not be empty")
-    _check(cache.stride(3) == 1 and not any(s & 7 for s in _rows(cache)) and cache.data_ptr() % 16 == 0,
-           f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of 8")
+    _check(cache.stride(3) == 1 and not any(n > 1 and s & few for n, s in zip(cache.shape, cache.stride()[:3])) and cache.data_ptr() % 16 == 0,
+           f"{name} must be 16-byte aligned, with adjacent values in a head and other strides multiples of {few + 1}")
     _check(all(n == 1 or s > 0 for n, s in zip(cache.shape, cache.stride())), f"{name} must not be expanded")
 
 
@@ -47,28 +56,28 @@ def _is_int32(t: torch.Tensor, index: int, n: int) -> bool:
     return t.dtype is _INT32 and t.get_device() == index and t.dim() == 1 and t.size(0) == n and t.is_contiguous()
 
 
-def _simple_cache(k, v, cache_lens, block_table, index: int, batch: int):
-    """``b2a_cache`` for struct.pack, or None where something is wrong or needs a closer look."""
+def _simple_cache(k, v, cache_lens, block_table, index: int, batch: int, dtype=_BF16, few: int = 7):
+    """``b2a_cache`` for struct.pack, or None where something is wrong or needs a closer look.  few: elements of 16 bytes less one."""
     ks, kst, kp = k.shape, k.stride(), k.data_ptr()
-    if len(ks) != 4 or k.dtype is not _BF16 or index not in _SM100 or not _is_int32(cache_lens, index, batch):
+    if len(ks) != 4 or k.dtype is not dtype or index not in _SM100 or not _is_int32(cache_lens, index, batch):
         return None
     pages, size, heads, dim = ks
     k0, k1, k2, k3 = kst
     if v is None:
         vp = v0 = v1 = v2 = 0
     else:
-        if v.dtype is not _BF16 or v.get_device() != index or v.shape != ks:
+        if v.dtype is not dtype or v.get_device() != index or v.shape != ks:
             return None
         vp, vst = v.data_ptr(), v.stride()
         v0, v1, v2, v3 = vst
         if v3 != 1 or v0 * v1 * v2 == 0:
             return None
-    if (dim != 128 or k3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & 7 or (kp | vp) & 15 or k0 * k1 * k2 * pages * size * heads == 0
+    if (dim != 128 or k3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & few or (kp | vp) & 15 or k0 * k1 * k2 * pages * size * heads == 0
             or batch == 0):
         return None
     if block_table is None:
         return (kp, vp, 0, 0, k0, k1, k2, v0, v1, v2, pages, size, heads, 1) if pages >= batch else None
-    if block_table.dtype is not _INT32 or block_table.get_device() != index or block_table.dim() != 2 or size & 7:
+    if block_table.dtype is not _INT32 or block_table.get_device() != index or block_table.dim() != 2 or size & few:
         return None
     rows, width = block_table.shape
     t0, t1 = block_table.stride()
@@ -98,9 +107,9 @@ def _check_table(block_table: Optional[torch.Tensor], k_cache: torch.Tensor, bat
     _check(k_cache.size(1) % 8 == 0, f"page_size must be a multiple of 8. Got {k_cache.size(1)}")
 
 
-def _check_pair(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    _check_cache(k_cache, "k_cache")
-    _check_cache(v_cache, "v_cache")
+def _check_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype = _BF16) -> None:
+    _check_cache(k_cache, "k_cache", dtype)
+    _check_cache(v_cache, "v_cache", dtype)
     _check(k_cache.device == v_cache.device, "k_cache and v_cache must be on the same CUDA device")
     _check(k_cache.shape == v_cache.shape, "k_cache and v_cache must have the same shape")
 
@@ -124,16 +133,54 @@ def _check_lens(cache_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], na
     return batch
 
 
+def _cache_rows(cache: torch.Tensor) -> Tuple[int, int, int]:
+    """Elements from page to page, slot to slot, head to head; 0 where there is only one."""
+    return tuple(0 if n == 1 else s for n, s in zip(cache.shape[:3], cache.stride()))
+
+
 def _cache_fields(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: Optional[torch.Tensor]):
     """``b2a_cache`` for struct.pack, of a cache that has been checked."""
     pages, size, heads, _ = k_cache.shape
     at, width, step = (0, 1, 0) if block_table is None else (block_table.data_ptr(), block_table.size(1), block_table.stride(0))
-    v = (0, _NONE3) if v_cache is None else (v_cache.data_ptr(), _rows(v_cache))
-    return (k_cache.data_ptr(), v[0], at, step, *_rows(k_cache), *v[1], pages, size, heads, width)
+    v = (0, _NONE3) if v_cache is None else (v_cache.data_ptr(), _cache_rows(v_cache))
+    return (k_cache.data_ptr(), v[0], at, step, *_cache_rows(k_cache), *v[1], pages, size, heads, width)
 
 
-def _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes) -> None:
-    _check_pair(k_cache, v_cache)
+@functools.lru_cache(maxsize=4096)
+def _scale_block(size: int, blocks: int, paged: bool) -> int:
+    """Slots of a scale; 0: none fits."""
+    for block in (16, 32, 64, 128):
+        if -(-size // block) == blocks and not (paged and size % block):
+            return block
+    return 0
+
+
+def _scale_fields(k_scales, v_scales, k_cache, paged: bool, index: int, written: bool) -> tuple:
+    """``b2a_cache_scales`` for struct.pack; k_cache has four dimensions."""
+    if type(k_scales) is torch.Tensor and type(v_scales) is torch.Tensor:
+        ks, vs, (pages, size, heads, _) = k_scales.shape, v_scales.shape, k_cache.shape
+        if (ks == vs and len(ks) == 3 and ks[0] == pages and ks[2] == heads and k_scales.dtype is torch.float32 is v_scales.dtype
+                and k_scales.get_device() == index == v_scales.get_device()):
+            block = _scale_block(size, ks[1], paged)
+            k_step, v_step = k_scales.stride(), v_scales.stride()
+            if block and not (written and 0 in k_step + v_step and any(n > 1 and 0 in (a, b) for n, a, b in zip(ks, k_step, v_step))):
+                return k_scales.data_ptr(), v_scales.data_ptr(), *k_step, *v_step, block
+    _check(k_scales is not None and v_scales is not None, "a cache of dtype torch.float8_e4m3fn and k_scales and v_scales go together")
+    pages, size, heads, _ = k_cache.shape
+    for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        _check(t.is_cuda and t.device == k_cache.device, f"{name} must be on the same CUDA device as the cache")
+        _check(t.dtype == torch.float32, f"{name} must have dtype torch.float32")
+        _check(t.dim() == 3 and t.size(0) == pages and t.size(2) == heads and _scale_block(size, t.size(1), paged) > 0,
+               f"{name} must have shape [{pages}, blocks, {heads}] with blocks of 16, 32, 64 or 128 of {size} slots"
+               + (", which they divide" if paged else "") + f". Got {list(t.shape)}")
+        _check(not written or all(n == 1 or s > 0 for n, s in zip(t.shape, t.stride())), f"{name} must not be expanded")
+    _check(k_scales.shape == v_scales.shape, "k_scales and v_scales must have the same shape")
+    block = _scale_block(size, k_scales.size(1), paged)
+    return k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(), *v_scales.stride(), block
+
+
+def _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes, dtype) -> None:
+    _check_pair(k_cache, v_cache, dtype)
     device = k_cache.device
     batch = _check_lens(cache_lens, cu_seqlens, "cu_seqlens", device)
     _check_table(block_table, k_cache, batch)
@@ -157,7 +204,8 @@ _NO_POSITIONS = (0, 0)
 def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
                  block_table: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
                  q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
-                 axes: Optional[RotaryAxes] = None) -> Optional[torch.Tensor]:
+                 axes: Optional[RotaryAxes] = None, k_scales: Optional[torch.Tensor] = None,
+                 v_scales: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Writes new tokens behind those that the cache holds, in place, and turns k (and q) by their positions on the way.
 
     k, v ``[B, n, KVH, 128]``, or ``[total, KVH, 128]`` with ``cu_seqlens`` ``[B + 1]`` (int32, on the device): token ``i`` of
@@ -165,16 +213,27 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     k is turned as :func:`rotary` turns it; q, if given, likewise, and is returned.  Packed tokens behind
     ``cu_seqlens[B]`` go nowhere, and their rows of the returned q are not written.  A token without a slot is left out
     and reported by ``check_last_status("append_cache")``.  No two tokens may be given the same slot by shared pages.
+
+    Into a cache in 8 bits, with ``k_scales`` and ``v_scales``: a block that its first new token begins gets, for each head, the smallest
+    power of two as its scale with which the new values fit (at most 448 times it; within 2^-64 .. 2^64).  One that held tokens
+    keeps its scale while that is enough; if not, they are divided by the new one and rounded again.  New values are turned and
+    divided in fp32 and rounded once, to e4m3; what is not finite becomes NaN and has no say.  Nothing but the block that a
+    sequence ends in may be shared by pages with another one that goes on in it.
     """
     index, batch, ks = k_cache.get_device(), cache_lens.numel(), k.shape
     dim, tokens = 4 if cu_seqlens is None else 3, ks[:-2]
-    fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
+    in8 = k_cache.dtype is _E4M3 or k_scales is not None or v_scales is not None
+    if in8:
+        fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch, _E4M3, 15)
+    else:
+        fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
     if not (fields is not None and _is_rows(k, dim, index) and _is_rows(v, dim, index) and v.shape == ks
             and ks[-2] == fields[12] and (ks[0] == batch if dim == 4 else _is_int32(cu_seqlens, index, batch + 1))
             and (positions is None if axes is None else positions is not None and _are_positions(positions, axes, tokens, index))
             and (q is None or (axes is not None and _is_rows(q, dim, index) and q.shape[:-2] == tokens))):
-        _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes)
+        _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes, _E4M3 if in8 else _BF16)
         fields = _cache_fields(k_cache, v_cache, block_table)
+    scales = _scale_fields(k_scales, v_scales, k_cache, block_table is not None, index, True) if in8 else None
     q_out = None if q is None else _like(q)
     if k.numel() == 0:
         return q_out
@@ -188,7 +247,10 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         axes is not None and positions.dtype is _INT64, batch, ks[1] if dim == 4 else 0, ks[0] * ks[1] if dim == 4 else ks[0],
         0 if q is None else q.size(-2), ws.data_ptr(), 16)
     with _on_device(device):
-        _cabi.check(_cabi.load().b2a_cache_append(args, _stream_ptr(device)))
+        if in8:
+            _cabi.check(_cabi.load().b2a_cache8_append(args, _cabi.SCALES.pack(*scales), _stream_ptr(device)))
+        else:
+            _cabi.check(_cabi.load().b2a_cache_append(args, _stream_ptr(device)))
     _remember_workspace("append_cache", ws)
     return q_out
 
@@ -270,8 +332,8 @@ def _query_fields(q, max_seqlen_q, tree_mask):
     return at, qs[0], int(max_seqlen_q), qs[1], st[0], st[1], 0, 0 if tree_mask is None else tree_mask.stride(0)
 
 
-def _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask) -> None:
-    _check_pair(k_cache, v_cache)
+def _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask, dtype) -> None:
+    _check_pair(k_cache, v_cache, dtype)
     batch = _check_lens(cache_lens, cu_seqlens_q, "cu_seqlens_q", k_cache.device)
     _check_table(block_table, k_cache, batch)
     _check_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, k_cache)
@@ -300,7 +362,8 @@ def _evict_bytes(lib, batch: int, kvh: int, budget: int, slots: int) -> Tuple[in
 def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor, *,
                  block_table: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[torch.Tensor] = None,
                  max_seqlen_q: Optional[int] = None, tree_mask: Optional[torch.Tensor] = None, return_lse: bool = False,
-                 out: Optional[torch.Tensor] = None):
+                 out: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                 v_scales: Optional[torch.Tensor] = None):
     """Attention of drafted tokens, or of the next token, over the cache.
 
     q ``[B, n, QH, 128]``, or ``[total_q, QH, 128]`` with ``cu_seqlens_q`` ``[B + 1]`` (int32, on the device) and
@@ -314,14 +377,23 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     ``check_last_status("forward_tree")``.  Repeated calls give the same bits; the last bits can depend on the other sequences of
     the call.  As in ``forward``, probabilities are rounded to bf16 for their product with v (sums and LSE are of the unrounded ones):
     out is off by 0.0023 of its 2-norm on random inputs, of which its own rounding is 0.0017.
+
+    Over a cache in 8 bits, with its ``k_scales`` and ``v_scales`` (positive and finite; they may be expanded, one for all blocks or
+    heads): a slot's values are its e4m3 times its block's scale.  q and the probabilities go into the products as sums of two 8-bit numbers:
+    out is no further off than over a bf16 cache with the same values.  Infinities in q count as NaN.
     """
     index, batch = k_cache.get_device(), cache_lens.numel()
-    fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
+    in8 = k_cache.dtype is _E4M3 or k_scales is not None or v_scales is not None
+    if in8:
+        fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch, _E4M3, 15)
+    else:
+        fields = _simple_cache(k_cache, v_cache, cache_lens, block_table, index, batch)
     query = fields and _simple_queries(q, batch, cu_seqlens_q, max_seqlen_q, tree_mask, fields[12], index)
     if query is None:
-        _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask)
+        _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask, _E4M3 if in8 else _BF16)
         fields, query = _cache_fields(k_cache, v_cache, block_table), _query_fields(q, max_seqlen_q, tree_mask)
     mask, total, most, heads, s_tok, s_head, m_seq, m_row = query
+    scales = _scale_fields(k_scales, v_scales, k_cache, block_table is not None, index, False) if in8 else None
     device = k_cache.device
     if out is None:
         out = _like(q)
@@ -340,7 +412,11 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         ws = _workspace(nbytes, device)
         args = _cabi.TREE.pack(*fields, cache_lens.data_ptr(), cu, q.data_ptr(), mask, out.data_ptr(), lse.data_ptr(), s_tok, s_head,
                                m_seq, m_row, batch, most, total, heads, 0.0, 0, 0, 0, 0, ws.data_ptr(), nbytes)
-        if more:
+        if in8:
+            scratch = ws.new_empty(more) if more else None
+            at, size = (scratch.data_ptr(), more) if more else (ws.data_ptr() + _TREE_KEPT, nbytes - _TREE_KEPT)
+            _cabi.check(lib.b2a_tree8_fwd(args, _cabi.SCALES.pack(*scales), at, size, _stream_ptr(device)))
+        elif more:
             scratch = ws.new_empty(more)
             _cabi.check(lib.b2a_tree_fwd_with_scratch(args, scratch.data_ptr(), more, _stream_ptr(device)))
         else:

@@ -53,6 +53,9 @@ int make_token_map(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t
 // outermost first, a (64 columns, box_heads, box_rows[, 1 page]) box and 128-byte swizzle.
 int make_strided_map(CUtensorMap* map, const void* base, int dims, const uint64_t* sizes, const int64_t* strides,
                      uint32_t box_heads, uint32_t box_rows);
+// The same over 8-bit values, 128 columns a box.
+int make_strided_map8(CUtensorMap* map, const void* base, int dims, const uint64_t* sizes, const int64_t* strides,
+                      uint32_t box_heads, uint32_t box_rows);
 
 // Header words at the start of every workspace.
 struct WorkspaceHeader {

@@ -721,30 +721,14 @@ int set_tree_smem() {
     return B2A_OK;
 }
 
-struct TreeLayout {
-    int ctas, tile_tokens, tiles, rows;   // rows of a tile; few rows: of an item, which is one tile
-    bool few;
-    size_t o, scratch;                    // of the pieces' results behind their sums, and of both
-};
-
-// What is kept after a call: header, status words and cuts.
-constexpr size_t kTreeCutsAt = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
-constexpr size_t kTreeKept = align_up(kTreeCutsAt + kTreeMaxCtas * sizeof(TreeCut), 256);
-
-TreeLayout tree_layout(int seqlen_q, int group, int sms) {
-    TreeLayout t{};
-    t.ctas = sms < kTreeMaxCtas ? sms : kTreeMaxCtas;
-    t.few = static_cast<long long>(seqlen_q) * group <= kFewRows;
-    t.tile_tokens = t.few ? seqlen_q : kTileM / group;
-    t.tiles = seqlen_q > t.tile_tokens ? 2 : 1;
-    t.rows = (t.tiles == 2 ? t.tile_tokens : seqlen_q) * group;
-    const size_t parts = 2ull * t.ctas * t.tiles * t.rows;
-    t.o = align_up(parts * sizeof(float2), 256);
-    t.scratch = t.o + parts * kHeadDim * sizeof(float);
-    return t;
-}
-
 }  // namespace
+
+int launch_tree_combine(const TreeParams& p, int ctas, cudaStream_t stream) {
+    const int strips = p.part_tiles * ((p.part_rows + kTreeStrip - 1) / kTreeStrip);
+    auto combine = tree_combine;
+    B2A_CUDA_OK(launch_early(combine, dim3(ctas - 1, strips), 256, 0, stream, p));
+    return B2A_OK;
+}
 
 }  // namespace b2a
 
@@ -825,11 +809,8 @@ int b2a_tree_fwd_with_scratch(const b2a_tree_args* a, void* scratch, size_t scra
     if (t.few) return launch_tree_few(map_q, map_k, map_v, p, t.ctas, dev, stream);
     auto attention = t.tiles == 2 ? tree_attention<true> : tree_attention<false>;
     const size_t smem = t.tiles == 2 ? tree_smem_bytes<true>() : tree_smem_bytes<false>();
-    auto combine = tree_combine;
     B2A_CUDA_OK(launch_early(attention, t.ctas, kTreeThreads, smem, stream, map_q, map_k, map_v, p));
-    const int strips = t.tiles * ((t.rows + kTreeStrip - 1) / kTreeStrip);
-    if (t.ctas > 1) B2A_CUDA_OK(launch_early(combine, dim3(t.ctas - 1, strips), 256, 0, stream, p));
-    return B2A_OK;
+    return t.ctas > 1 ? launch_tree_combine(p, t.ctas, stream) : B2A_OK;
 }
 
 }  // extern "C"

@@ -168,4 +168,64 @@ constexpr int kFewRows = 32;
 int launch_tree_few(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, int ctas,
                     const DeviceInfo& dev, cudaStream_t stream);
 
+// Adds up the pieces of items that ends of runs cut: of calls of few rows, and of the others.
+int launch_tree_combine_few(const TreeParams& p, int ctas, cudaStream_t stream);
+int launch_tree_combine(const TreeParams& p, int ctas, cudaStream_t stream);
+
+struct TreeLayout {
+    int ctas, tile_tokens, tiles, rows;   // rows of a tile; few rows: of an item, which is one tile
+    bool few;
+    size_t o, scratch;                    // of the pieces' results behind their sums, and of both
+};
+
+// What is kept after a call: header, status words and cuts.
+constexpr size_t kTreeCutsAt = align_up(sizeof(WorkspaceHeader) + kFwdStatusWords * sizeof(unsigned int), 256);
+constexpr size_t kTreeKept = align_up(kTreeCutsAt + kTreeMaxCtas * sizeof(TreeCut), 256);
+
+inline TreeLayout tree_layout(int seqlen_q, int group, int sms) {
+    TreeLayout t{};
+    t.ctas = sms < kTreeMaxCtas ? sms : kTreeMaxCtas;
+    t.few = static_cast<long long>(seqlen_q) * group <= kFewRows;
+    t.tile_tokens = t.few ? seqlen_q : kTileM / group;
+    t.tiles = seqlen_q > t.tile_tokens ? 2 : 1;
+    t.rows = (t.tiles == 2 ? t.tile_tokens : seqlen_q) * group;
+    const size_t parts = 2ull * t.ctas * t.tiles * t.rows;
+    t.o = align_up(parts * sizeof(float2), 256);
+    t.scratch = t.o + parts * kHeadDim * sizeof(float);
+    return t;
+}
+
+// N columns of tensor memory.
+template <int N>
+__device__ __forceinline__ void few_ld(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(taddr)
+                     : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 16) tmem_ld_x16(taddr + i, r + i);
+    }
+}
+
+// Sums of N columns over the lanes of a warp, halving the columns as it halves the lanes: lane j ends with the sum of column
+// j % N.
+template <int N>
+__device__ __forceinline__ void few_column_sums(float (&v)[N], int lane) {
+    if constexpr (N == 16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], 16);
+    }
+#pragma unroll
+    for (int d = N / 2; d > 0; d >>= 1) {
+        const bool upper = (lane & d) != 0;
+#pragma unroll
+        for (int i = 0; i < d; ++i) {
+            const float low = v[i], high = v[i + d];
+            v[i] = (upper ? high : low) + __shfl_xor_sync(0xFFFFFFFFu, upper ? low : high, d);
+        }
+    }
+}
+
 }  // namespace b2a

@@ -65,39 +65,6 @@ template <int N>
 constexpr size_t few_smem_bytes() { return sizeof(FewShared<N>) + 1024; }
 static_assert(few_smem_bytes<16>() <= 227 * 1024 && few_smem_bytes<32>() <= 227 * 1024, "");
 
-// N columns of tensor memory.
-template <int N>
-__device__ __forceinline__ void few_ld(uint32_t taddr, uint32_t (&r)[N]) {
-    if constexpr (N == 8) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                     : "r"(taddr)
-                     : "memory");
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 16) tmem_ld_x16(taddr + i, r + i);
-    }
-}
-
-// Sums of N columns over the lanes of a warp, halving the columns as it halves the lanes: lane j ends with the sum of column
-// j % N.
-template <int N>
-__device__ __forceinline__ void few_column_sums(float (&v)[N], int lane) {
-    if constexpr (N == 16) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], 16);
-    }
-#pragma unroll
-    for (int d = N / 2; d > 0; d >>= 1) {
-        const bool upper = (lane & d) != 0;
-#pragma unroll
-        for (int i = 0; i < d; ++i) {
-            const float low = v[i], high = v[i + d];
-            v[i] = (upper ? high : low) + __shfl_xor_sync(0xFFFFFFFFu, upper ? low : high, d);
-        }
-    }
-}
-
 // The eight k-steps of a 128 x N x 128 product, B with two halves of N rows of 128 bytes.
 template <int N, bool kAMnMajor>
 __device__ __forceinline__ void few_product(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t accumulate) {
@@ -670,7 +637,10 @@ int launch_tree_few(const CUtensorMap& map_q, const CUtensorMap& map_k, const CU
         rc = once_per_device(dev.device, 9, set_few_smem<32>);
         if (rc == B2A_OK) rc = launch_few<32>(map_q, map_k, map_v, p, ctas, stream);
     }
-    if (rc != B2A_OK || ctas == 1) return rc;
+    return rc != B2A_OK || ctas == 1 ? rc : launch_tree_combine_few(p, ctas, stream);
+}
+
+int launch_tree_combine_few(const TreeParams& p, int ctas, cudaStream_t stream) {
     auto combine = tree_combine_few;
     B2A_CUDA_OK(launch_early(combine, dim3(ctas - 1, (p.part_rows + 7) / 8), 256, 0, stream, p));
     return B2A_OK;

@@ -6,8 +6,9 @@ No counterpart in the reference, which takes q and k as they are (``bindings.cpp
 from __future__ import annotations
 
 import ctypes
+from ctypes import c_float
 from fractions import Fraction
-from math import isfinite
+from math import isfinite, log, pi
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -34,11 +35,12 @@ class RotaryAxes:
 
     Pair ``i`` turns by ``positions[axis[i]] * inv_freq[i]``; there are 8, 16, ... or 64 pairs, and the dimensions behind the
     first ``2 * pairs`` stay as they are.  ``adjacent``: pair ``i`` is dimensions ``(2 i, 2 i + 1)``, otherwise
-    ``(i, i + pairs)``.  Frequencies are taken as the 64-bit floats they are.  An angle is within 1.1e-7 for
+    ``(i, i + pairs)``.  ``magnitude``: what turned pairs are multiplied by (:meth:`stretched`).  Frequencies are taken as the 64-bit floats they are.  An angle is within 1.1e-7 for
     positions up to 2^36, and 1.7e-19 times the position more beyond (2^45: 6e-6).
     """
 
-    def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False):
+    def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False,
+                 magnitude: float = 1.0):
         inv_freq = [float(f) for f in inv_freq]
         axis = [0] * len(inv_freq) if axis is None else [int(a) for a in axis]
         pairs = len(inv_freq)
@@ -47,26 +49,33 @@ class RotaryAxes:
         _check(len(axis) == pairs, f"inv_freq and axis must have the same length. Got {pairs} vs {len(axis)}")
         _check(all(0 <= a < _MAX_PAIRS for a in axis), f"an axis must be between 0 and {_MAX_PAIRS - 1}")
         _check(all(isfinite(f) for f in inv_freq), "inv_freq must be finite")
+        magnitude = c_float(magnitude).value
+        _check(isfinite(magnitude) and magnitude > 0, f"magnitude must be positive and finite, got {magnitude}")
         self.axes = max(axis) + 1
         self.pairs = pairs
         c = _cabi.RotaryAxes()
         c.turn[:pairs] = [_turn(f) for f in inv_freq]
         c.axis[:pairs] = axis
-        c.pairs, c.axes, c.adjacent = pairs, self.axes, int(bool(adjacent))
+        c.pairs, c.axes, c.adjacent, c.magnitude = pairs, self.axes, int(bool(adjacent)), magnitude
         self._c = c
+        self._inv_freq = inv_freq
         # The same as plain values, which an operator's schema can hold: turns as signed numbers of 64 bits.
         self._plain = ([t - 2**64 if t >= 2**63 else t for t in c.turn[:pairs]], axis, bool(adjacent))
 
     @classmethod
-    def _from_plain(cls, turn: Sequence[int], axis: Sequence[int], adjacent: bool) -> "RotaryAxes":
+    def _from_plain(cls, turn: Sequence[int], axis: Sequence[int], adjacent: bool, magnitude: float = 1.0) -> "RotaryAxes":
         self = cls.__new__(cls)
         self.axes, self.pairs = max(axis) + 1, len(axis)
         self._c = c = _cabi.RotaryAxes()
         c.turn[:self.pairs] = [t % 2**64 for t in turn]
         c.axis[:self.pairs] = axis
-        c.pairs, c.axes, c.adjacent = self.pairs, self.axes, int(adjacent)
+        c.pairs, c.axes, c.adjacent, c.magnitude = self.pairs, self.axes, int(adjacent), magnitude
         self._plain = (list(turn), list(axis), bool(adjacent))
         return self
+
+    @property
+    def magnitude(self) -> float:
+        return self._c.magnitude or 1.0
 
     @property
     def _at(self) -> int:
@@ -86,6 +95,31 @@ class RotaryAxes:
                 freq.append(float(base) ** (-(j / n if restart else len(freq) / total)))
                 axis.append(a)
         return cls(freq, axis, adjacent=adjacent)
+
+
+    def stretched(self, factor: float, original_length: float, *, slow: float = 1.0, fast: float = 32.0,
+                  magnitude: Optional[float] = None) -> "RotaryAxes":
+        """The same axes for contexts ``factor`` times as long as the ``original_length`` positions that a model was trained on.
+
+        A pair that turns fewer than ``slow`` times within that length gets its frequency divided by ``factor`` (its angles stay within
+        those of the training), one that turns more than ``fast`` times keeps it (it tells neighbours apart), and between the two the
+        frequency goes over from one to the other linearly in the number of turns.  ``magnitude`` multiplies turned pairs of q and of
+        k, a score by its square; by default ``0.1 ln(factor) + 1``.  (Peng et al., "Efficient Context Window
+        Extension of Large Language Models", 2023, "NTK-by-parts" and its temperature; with ``magnitude=1`` and a small ``fast`` the
+        smooth ramp that is in use without one.)  ``slow = fast = inf``: all frequencies divided.
+        """
+        _check(hasattr(self, "_inv_freq"), "these axes do not know their frequencies")
+        _check(isfinite(factor) and factor >= 1, f"factor must be 1 or more, got {factor}")
+        _check(isfinite(original_length) and original_length > 0, f"original_length must be positive, got {original_length}")
+        _check(0 <= slow <= fast, f"slow must be between 0 and fast. Got {slow} vs {fast}")
+        frequencies = []
+        for f in self._inv_freq:
+            turns = original_length * abs(f) / (2 * pi)
+            keep = 0.0 if turns <= slow else 1.0 if turns >= fast else (turns - slow) / (fast - slow)
+            frequencies.append((1 - keep) * (f / factor) + keep * f)
+        if magnitude is None:
+            magnitude = self.magnitude * (0.1 * log(factor) + 1)
+        return RotaryAxes(frequencies, self._plain[1], adjacent=self._plain[2], magnitude=magnitude)
 
 
 _BF16, _INT32, _INT64 = torch.bfloat16, torch.int32, torch.int64
