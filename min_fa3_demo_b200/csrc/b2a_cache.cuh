@@ -268,9 +268,10 @@ struct SlotLoader {
     int page, row;
     int bad;                 // this lane met a page that does not exist
 
-    __device__ __forceinline__ explicit SlotLoader(int box_rows) {
+    // blocks: that are looked up and loaded together; their boxes are at most 32.
+    __device__ __forceinline__ explicit SlotLoader(int box_rows, int blocks = 1) {
         shift = __ffs(box_rows) - 1;
-        boxes = kSlotBlock >> shift;
+        boxes = blocks * kSlotBlock >> shift;
         page = row = bad = 0;
     }
 

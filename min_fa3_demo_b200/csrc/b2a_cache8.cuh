@@ -1,15 +1,18 @@
 // A cache of e4m3 values with a scale for each block of slots and K/V head, as the kernels see it, and products with it.
 //
-// The tensor cores multiply 8-bit operands as they lie in memory, so K and V are never converted: a tile goes from global memory
-// to shared memory by TMA and from there into the product.  What is multiplied by them has to have 8 bits too, and e4m3 has only
-// four significant bits.  So Q and P are sums of two such numbers, of which each takes part in the product with the same
-// accumulator: the value rounded to e4m3, and what is left over.
-//   Q: bf16 has eight significant bits; the first four, rounded, leave a signed rest of four, which e4m3 holds exactly.  A row is
-//      scaled so that its largest value lies in [2^7, 2^8); rests below 2^-9 lose bits, which is 2^-18 of that value.
-//   P: the rest is rounded to e5m2, whose exponents reach to 2^-16: P is off by 2^-7 of itself at most, 0.0013 in the mean
-//      square (bf16: 2^-8 and 0.0016), and by 2^-17 where it is small, 2^-22 of a row's largest or less.
-// Twice the products at twice the rate of bf16.  Scales never meet the values: K's multiplies a score, V's is an addend of the
-// exponent, by which P takes it into the product, and the row's sum is divided by it again.
+// K Q^T is a product of 8-bit operands: K's tiles go from global memory to shared memory by TMA and from there into the product, and are
+// never converted.  Q has to have 8 bits too, and e4m3 has only four significant ones, so Q is the sum of two such
+// numbers, which take part one after the other in the same accumulator: a bf16 rounded to e4m3 leaves a signed rest of four
+// bits, which e4m3 holds exactly.  A row is scaled so that its largest value lies in [2^7, 2^8); rests below 2^-9 lose bits, which
+// is 2^-18 of that value.  Twice the products at twice the rate of bf16.
+//
+// P V is a product of f16: e4m3 is exact in f16, and four warps convert V's tiles (16 KiB in, 32 KiB out, an instruction for two
+// values).  P in f16 is off by 2^-11 of itself, or by 2^-25 where it is small, 2^-27 of a row's largest or less.  P as
+// a sum of two 8-bit numbers, as Q is, needs no conversion of V but six instructions for two probabilities instead of one, which the
+// softmax has no time for (trees of 64 tokens, 64 heads over 8, 8 sequences of up to 16,000 slots: 344 us).
+//
+// Scales never meet the values: K's multiplies a score, V's is an addend of the exponent, by which P takes it into the
+// product, and what goes into the row's sum is divided by it again.
 #pragma once
 
 #include "b2a_tree.cuh"
@@ -65,6 +68,74 @@ __device__ __forceinline__ void load_slots8(const SlotLoader& at, const CUtensor
     __syncwarp();
 }
 
+// mbar_wait with little code at each wait: the roles of these kernels run different code at the same time, and with mbar_wait's loop
+// everywhere it is more than the instruction cache holds (one token, 16 sequences of up to 8,001 slots: a third of the
+// requests missed, and the kernel took twice the time).  The loop that looks at the clock is a function, which a caller
+// with many live registers should hardly ever need to call.
+static __device__ __noinline__ bool wait8_longer(uint32_t abort_smem, unsigned int* status, uint32_t timeout_ns, uint32_t bar, uint32_t parity,
+                                                 uint32_t tag) {
+    return mbar_wait(WaitCtx{abort_smem, status, timeout_ns, 1u}, bar, parity, tag);
+}
+
+constexpr int kWait8Polls = 1024;
+
+__device__ __forceinline__ bool wait8(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t tag) {
+#pragma unroll 1
+    for (int i = 0; i < kWait8Polls; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+    }
+    return wait8_longer(ctx.abort_smem, ctx.status, ctx.timeout_ns, bar, parity, tag);
+}
+
+// As warp_wait: one answer for all lanes.
+__device__ __forceinline__ bool warp_wait8(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t tag) {
+#pragma unroll 1
+    for (int i = 0; i < kWait8Polls; ++i) {
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+    }
+    return __all_sync(0xFFFFFFFFu, wait8_longer(ctx.abort_smem, ctx.status, ctx.timeout_ns, bar, parity, tag));
+}
+
+// The scales of the steps under way, kBlocks blocks each: one of K and one of V for 16 slots.  The warp that loads K asks for them, as it
+// has the pages at hand, and copies them without waiting; the softmax warps take them from shared memory, where they
+// cost no registers while they are on their way.
+constexpr int kScaleSlots = 8;
+
+template <int kBlocks>
+struct ScaleRing {
+    float scale[kScaleSlots][2][8 * kBlocks];
+    uint64_t full[kScaleSlots], empty[kScaleSlots];
+
+    // consumers: arrivals that give a slot back.
+    __device__ __forceinline__ void init(int consumers) {
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(smem_u32(&full[i]), 32);
+            mbar_init(smem_u32(&empty[i]), consumers);
+        }
+    }
+    // By a warp, of the blocks from `block` on, which `at` has looked up.  What does not exist is zero, and masked.
+    __device__ __forceinline__ bool load(const WaitCtx& wctx, uint32_t it, const CacheView& c, const CacheScales& s, const SlotLoader& at,
+                                         int block, int slots, int head, int lane) {
+        constexpr int kGroups = 8 * kBlocks;
+        const uint32_t slot = it % kScaleSlots;
+        const int group = lane % kGroups, box = (group * 16) >> at.shift;
+        const bool keys = lane < kGroups;
+        const int page = __shfl_sync(0xFFFFFFFFu, at.page, box);
+        const int row = __shfl_sync(0xFFFFFFFFu, at.row, box) + ((group * 16) & ((1 << at.shift) - 1));
+        if (!warp_wait8(wctx, smem_u32(&empty[slot]), ((it / kScaleSlots) & 1u) ^ 1u, 20)) return false;
+        if (lane < 2 * kGroups) {
+            const bool there = block * kSlotBlock + group * 16 < slots && static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
+            const float* from = keys ? s.k : s.v;
+            if (there) from += s.at(keys ? s.k_stride : s.v_stride, page, row, head);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&scale[slot][keys ? 0 : 1][group])), "l"(from), "r"(there ? 4 : 0)
+                         : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
+        __syncwarp();
+        return true;
+    }
+};
+
 // ---------------------------------------------------------------------------------------
 // Numbers as sums of two of 8 bits
 // ---------------------------------------------------------------------------------------
@@ -81,6 +152,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
     return r;
 }
 
+__device__ __forceinline__ void e4m3x4_to_half4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, u;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+}
+
 __device__ __forceinline__ float2 half2_to_float2(uint32_t h) {
     float2 f;
     asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, u;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
@@ -89,55 +164,64 @@ __device__ __forceinline__ float2 half2_to_float2(uint32_t h) {
 
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) { return half2_to_float2(e4m3x2_to_half2(two)); }
 
-// Two probabilities of at most 2^8: e4m3, and e5m2 of the rest.  f16 has 11 bits, so the difference is that of p rounded
-// to them, which is what is left of it after the two.
-__device__ __forceinline__ void split_p(float p0, float p1, uint32_t& first, uint32_t& rest) {
-    uint32_t p;
-    uint16_t r;
-    first = pack_e4m3x2(p0, p1);
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(p1), "f"(p0));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p) : "r"(p), "r"(e4m3x2_to_half2(first)));
-    asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(p));
-    rest = r;
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
-// Rows of Q by a warp into [rows][128 bytes] of both parts, 16-byte chunks exchanged by the row's number: a lane has four
-// dimensions.  What a row has been divided by goes to `scale`.
-__device__ __forceinline__ void split_q_row(uint2 q, int row, int lane, uint8_t* first, uint8_t* rest, float* scale) {
-    const uint32_t abs0 = q.x & 0x7FFF7FFFu, abs1 = q.y & 0x7FFF7FFFu;
-    auto finite = [](uint32_t bits) { return bits < 0x7F80u ? bits : 0u; };
-    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, max(max(finite(abs0 & 0xFFFFu), finite(abs0 >> 16)),
-                                                             max(finite(abs1 & 0xFFFFu), finite(abs1 >> 16))));
-    // Exponent field e of the largest value: times 2^(134 - e).  A row of zeros keeps its own.
-    const int up = most == 0u ? 0 : min(134 - static_cast<int>(most >> 7), 126);
-    const float mul = __int_as_float((127 + up) << 23);
-    float x[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xFFFF0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xFFFF0000u)};
+// Rows of Q by a warp into [rows][128 bytes] of both parts, 16-byte chunks exchanged by the row's number: half a warp a row, a lane has
+// the eight dimensions from (lane & 15) * 8 on.  What a row has been divided by goes to `scale`.  `there`: the lane's row exists (the
+// whole warp calls).  In f16, which holds the eight bits of a bf16 and the difference of the two.
+__device__ __forceinline__ void split_q_rows(const uint4& q, bool there, int row, int lane, uint8_t* first, uint8_t* rest, float* scale) {
+    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+    uint32_t most = 0;      // two magnitudes
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) < INFINITY ? x[i] * mul : NAN;      // an infinity has no part to leave over
-    const uint32_t a = pack_e4m3x2(x[0], x[1]), b = pack_e4m3x2(x[2], x[3]);
-    const float2 fa = e4m3x2_to_float2(a), fb = e4m3x2_to_float2(b);
-    const int at = row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4;
-    *reinterpret_cast<uint32_t*>(first + at) = a | b << 16;
-    *reinterpret_cast<uint32_t*>(rest + at) = pack_e4m3x2(x[0] - fa.x, x[1] - fa.y) | pack_e4m3x2(x[2] - fb.x, x[3] - fb.y) << 16;
-    if (lane == 0) *scale = __int_as_float((127 - up) << 23);
+    for (int i = 0; i < 4; ++i) most = __vmaxu2(most, words[i] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+    most = max(most & 0xFFFFu, most >> 16);
+    // Exponent field e of the largest value: times 2^(134 - e).  A row of zeros keeps its own.  A row with infinities or NaN, whose
+    // scores with anything are NaN as well, becomes NaN whole.
+    const int up = most == 0u ? 0 : min(134 - static_cast<int>(most >> 7), 126);
+    const float mul = most >= 0x7F80u ? NAN : __int_as_float((127 + up) << 23);
+    uint32_t a[2], b[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t part[2], left[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t w = words[2 * i + e];
+            const uint32_t x = pack_half2(__uint_as_float(w << 16) * mul, __uint_as_float(w & 0xFFFF0000u) * mul);
+            uint16_t u, v;
+            uint32_t d;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(u) : "r"(x));
+            asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(e4m3x2_to_half2(u)));
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(v) : "r"(d));
+            part[e] = u;
+            left[e] = v;
+        }
+        a[i] = part[0] | part[1] << 16;
+        b[i] = left[0] | left[1] << 16;
+    }
+    if (there) {
+        const int at = row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(first + at) = make_uint2(a[0], a[1]);
+        *reinterpret_cast<uint2*>(rest + at) = make_uint2(b[0], b[1]);
+        if ((lane & 15) == 0) *scale = __int_as_float((127 - up) << 23);
+    }
 }
 
 // ---------------------------------------------------------------------------------------
 // Products of 8-bit operands
 // ---------------------------------------------------------------------------------------
-// Instruction descriptor: D in f32, A and B in e4m3 (0) or e5m2 (1).
-__host__ __device__ constexpr uint32_t make_idesc_8(int m, int n, int a_mn_major, int b_mn_major, int a_e5m2, int b_e5m2) {
-    return (1u << 4) | (static_cast<uint32_t>(a_e5m2) << 7) | (static_cast<uint32_t>(b_e5m2) << 10) |
-           (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
-           (static_cast<uint32_t>(m >> 4) << 24);
+// Instruction descriptor with D in f32 and both operands in the kind's first format: e4m3 (kind::f8f6f4) or f16 (kind::f16).
+__host__ __device__ constexpr uint32_t make_idesc_first(int m, int n, int a_mn_major, int b_mn_major) {
+    return (1u << 4) | (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(b_mn_major) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Steps of 32 elements of the contraction: 32 bytes of a row where it runs along the rows, 32 rows where it runs across them.
-// A tile of 128 columns is one swizzle atom wide, so an operand across has no second one for a leading offset to lead to.
-constexpr int kStep8Along = 32 >> 4, kStep8Across = 32 * 128 >> 4;
-
-// The four k-steps of a product over 128, as umma_ss_kk_x8_w.
-template <int kAStep, int kBStep>
+// The four k-steps of a product over 128, 32 bytes each along the rows of A and B, as umma_ss_kk_x8_w.
 __device__ __forceinline__ void umma8_ss_x4_w(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t"
@@ -150,53 +234,77 @@ __device__ __forceinline__ void umma8_ss_x4_w(uint32_t d_tmem, uint32_t a_lo, ui
         "mov.b64 da, {%1, %5};\n\t"
         "mov.b64 db, {%2, %5};\n\t"
         "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t"
-        "add.u32 ra, %1, %6;\n\t"
-        "add.u32 rb, %2, %7;\n\t"
+        "add.u32 ra, %1, 2;\n\t"
+        "add.u32 rb, %2, 2;\n\t"
         "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
         "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, pt;\n\t"
-        "add.u32 ra, ra, %6;\n\t"
-        "add.u32 rb, rb, %7;\n\t"
+        "add.u32 ra, ra, 2;\n\t"
+        "add.u32 rb, rb, 2;\n\t"
         "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
         "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, pt;\n\t"
-        "add.u32 ra, ra, %6;\n\t"
-        "add.u32 rb, rb, %7;\n\t"
+        "add.u32 ra, ra, 2;\n\t"
+        "add.u32 rb, rb, 2;\n\t"
         "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
         "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, pt;\n\t"
         "}\n"
-        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128), "n"(kAStep), "n"(kBStep)
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128)
         : "memory");
 }
 
-// A from tensor memory, four elements a column.
-template <int kBStep>
-__device__ __forceinline__ void umma8_ts_x4_w(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+// The eight k-steps of a product of f16 over 128, A across two halves of 64 columns, B with two halves of N rows of 128 bytes.
+template <int N>
+__device__ __forceinline__ void umma_ss_nk_x8_w(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t"
         ".reg .pred p, pe, pt;\n\t"
-        ".reg .b64 db;\n\t"
+        ".reg .b64 da, db;\n\t"
         ".reg .b32 ra, rb;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
         "elect.sync _|pe, 0xFFFFFFFF;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
         "mov.b64 db, {%2, %5};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %3, p;\n\t"
-        "add.u32 ra, %1, 8;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+        "add.u32 ra, %1, 128;\n\t"
+        "add.u32 rb, %2, 2;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
+        "mov.b64 db, {rb, %5};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 256;\n\t"
+        "add.u32 rb, %2, 4;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
+        "mov.b64 db, {rb, %5};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 384;\n\t"
+        "add.u32 rb, %2, 6;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
+        "mov.b64 db, {rb, %5};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 512;\n\t"
         "add.u32 rb, %2, %6;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [ra], db, %3, pt;\n\t"
-        "add.u32 ra, ra, 8;\n\t"
-        "add.u32 rb, rb, %6;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 640;\n\t"
+        "add.u32 rb, rb, 2;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [ra], db, %3, pt;\n\t"
-        "add.u32 ra, ra, 8;\n\t"
-        "add.u32 rb, rb, %6;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 768;\n\t"
+        "add.u32 rb, rb, 2;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
         "mov.b64 db, {rb, %5};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [ra], db, %3, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
+        "add.u32 ra, %1, 896;\n\t"
+        "add.u32 rb, rb, 2;\n\t"
+        "mov.b64 da, {ra, %5};\n\t"
+        "mov.b64 db, {rb, %5};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, pt;\n\t"
         "}\n"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128), "n"(kBStep)
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128), "n"(N * 128 >> 4)
         : "memory");
 }
 
@@ -210,63 +318,96 @@ struct Tree8Params {
     long long q_stride[2];       // token, head
 };
 
-// Probabilities are at most 2^8 for the product; a new reference puts the largest one at 2^5, so that it moves only when the
-// maximum has grown by a factor of eight.
-constexpr float kP8Most = 8.f, kP8At = 5.f;
+// Probabilities, with V's scale, are at most 2^15; a new reference puts the score that it is taken from at 2^2, so that it moves only when
+// the maximum has grown by a factor of 2^13.
+constexpr float kP8Most = 15.f, kP8At = 2.f;
 
 __device__ __forceinline__ bool e4m3_not_finite(uint32_t byte) { return (byte & 0x7Fu) == 0x7Fu; }
 
-// As tree_clean_row, for a row of 128 bytes: e4m3 has no infinities.
-__device__ __forceinline__ bool tree8_clean_row(uint8_t* row, int r, bool behind) {
-    auto chunk = [&](int c) { return reinterpret_cast<uint4*>(row + ((c + r) & 7) * 16); };
-    if (behind) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) *chunk(c) = make_uint4(0u, 0u, 0u, 0u);
-        return false;
-    }
+// As tree_clean_row, for a row of 128 bytes, whose only values that are not finite are NaN.  Little code, as few rows need it.
+static __device__ __noinline__ bool tree8_clean_row(uint8_t* row, int r, bool behind) {
     // A magnitude of 0x7F plus one carries into its byte's sign bit, and no other does.
     auto ones = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };
     uint32_t any = 0;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const uint4 v = *chunk(c);
-        any |= ones(v.x) | ones(v.y) | ones(v.z) | ones(v.w);
-    }
-    if (any == 0u) return false;
 #pragma unroll 1
     for (int c = 0; c < 8; ++c) {
-        const uint4 v = *chunk(c);
-        auto without = [&](uint32_t w) { return w & ~((ones(w) >> 7) * 0xFFu); };
-        *chunk(c) = make_uint4(without(v.x), without(v.y), without(v.z), without(v.w));
+        // Another chunk first in each row, so that rows of 128 bytes do not meet in the same banks.
+        uint4* chunk = reinterpret_cast<uint4*>(row + ((c + r) & 7) * 16);
+        uint4 v = behind ? make_uint4(0u, 0u, 0u, 0u) : *chunk;
+        const uint4 n = make_uint4(ones(v.x), ones(v.y), ones(v.z), ones(v.w));
+        any |= n.x | n.y | n.z | n.w;
+        v = make_uint4(v.x & ~((n.x >> 7) * 0xFFu), v.y & ~((n.y >> 7) * 0xFFu), v.z & ~((n.z >> 7) * 0xFFu), v.w & ~((n.w >> 7) * 0xFFu));
+        if (behind || (n.x | n.y | n.z | n.w) != 0u) *chunk = v;
     }
-    return true;
+    return any != 0u;
 }
 
-// Loads of V by one warp, as tree_load_v.
-template <int kSlots, int kStages, typename Shared>
-__device__ __forceinline__ void tree8_load_v(const TreeParams& p, Shared& sh, const CUtensorMap* map, const WaitCtx& wctx, int lane) {
-    SlotLoader loader(p.box_rows);
+// V's tiles from e4m3 to f16 by kWarps warps, r being the thread's number among them, a row at a time.  What a product must not see is left out on the way: rows behind the last
+// slot, and of drafted tokens NaN, since 0 * NaN is NaN (e4m3 has no infinities); that there was one is noted for the piece.
+// begin(piece, number): what there is to do before a piece's blocks.
+template <int kWarps, int kSlots, int kStages, int kTiles, typename Shared, typename Begin>
+__device__ __forceinline__ void tree8_convert_v(const TreeParams& p, Shared& sh, const WaitCtx& wctx, int r, Begin begin) {
     uint32_t v_it = 0;
     bool ok = true;
+    PH_DECL(4)   // 0 other, 1 wait for V, 2 wait for a tile, 3 convert
     for (uint32_t it = 0; ok; ++it) {
         const uint32_t at = it % kSlots;
-        ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kSlots) & 1u, 4);
+        ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kSlots) & 1u, 22);
         if (!ok) break;
-        const TreePiece w = sh.piece[at];
+        const TreePiece& piece = sh.piece[at];
+        const int valid = piece.valid, j0 = piece.j0, slots = piece.slots, blocks = piece.blocks;
+        const int len = piece.n > 1 || p.c.mask != nullptr ? piece.len : slots;      // from here on tokens that not all rows see
+        ok = !valid || begin(piece, it);
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
-        if (!w.valid) break;
-        loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-        for (int i = 0; i < w.blocks; ++i, ++v_it) {
-            SlotLoader now = loader;
-            if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-            const int boxes = now.count(w.j0 + i, w.slots);
-            const uint32_t stage = v_it % kStages;
-            ok = warp_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kStages) & 1u) ^ 1u, 18);
+        if ((r & 31) == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+        if (!valid || !ok) break;
+        for (int i = 0; i < blocks; ++i, ++v_it) {
+            const uint32_t stage = v_it % kStages, tile = v_it % kTiles;
+            PH_MARK(0);
+            ok = warp_wait8(wctx, smem_u32(&sh.v_full[stage]), (v_it / kStages) & 1u, 23);
             if (!ok) break;
-            load_slots8(now, map, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
+            PH_MARK(1);
+            ok = warp_wait8(wctx, smem_u32(&sh.v16_empty[tile]), ((v_it / kTiles) & 1u) ^ 1u, 24);
+            if (!ok) break;
+            PH_MARK(2);
+#pragma unroll 1
+            for (int row = r; row < kSlotBlock; row += 32 * kWarps) {
+                uint8_t* from = &sh.v[stage][row * 128];
+                uint8_t* to = &sh.v16[tile][row * 128];
+                const int slot = (j0 + i) * kSlotBlock + row;
+                if (slot >= len && tree8_clean_row(from, row, slot >= slots)) {
+                    *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) = it + 1;
+                }
+                // 16 values: chunks 2 c and 2 c + 1 of 8, which lie in a half of 64 columns.
+#pragma unroll 1
+                for (int c = 0; c < 8; c += 2) {
+                    uint4 v[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) v[e] = *reinterpret_cast<const uint4*>(from + (((c + e) ^ (row & 7)) << 4));
+                    uint8_t* half = to + (c >> 2) * kHalfTileBytes;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        uint4 x, y;
+                        e4m3x4_to_half4(v[e].x, x.x, x.y);
+                        e4m3x4_to_half4(v[e].y, x.z, x.w);
+                        e4m3x4_to_half4(v[e].z, y.x, y.y);
+                        e4m3x4_to_half4(v[e].w, y.z, y.w);
+                        const int first = ((c + e) & 3) * 2;
+                        *reinterpret_cast<uint4*>(half + ((first ^ (row & 7)) << 4)) = x;
+                        *reinterpret_cast<uint4*>(half + (((first + 1) ^ (row & 7)) << 4)) = y;
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if ((r & 31) == 0) {
+                mbar_arrive(smem_u32(&sh.v_empty[stage]));
+                mbar_arrive(smem_u32(&sh.v16_full[tile]));
+            }
+            PH_MARK(3);
         }
     }
+    PH_PRINT("tree8 convert", 4);
 }
 
 // b2a_tree8_few.cu: calls of at most kFewRows rows an item.

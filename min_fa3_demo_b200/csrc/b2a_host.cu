@@ -151,7 +151,9 @@ int strided_map(CUtensorMap* map, const void* base, int bytes, int dims, const u
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / bytes), box_heads, box_rows, 1}, elem_strides[4] = {1, 1, 1, 1};
     const CUresult res = encode(map, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, dims,
                                 const_cast<void*>(base), size, stride, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                CU_TENSOR_MAP_SWIZZLE_128B,
+                                bytes == 2 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (res != CUDA_SUCCESS) {
         return fail(B2A_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(res));
     }

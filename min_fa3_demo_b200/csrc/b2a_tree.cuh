@@ -198,7 +198,12 @@ inline TreeLayout tree_layout(int seqlen_q, int group, int sms) {
 // N columns of tensor memory.
 template <int N>
 __device__ __forceinline__ void few_ld(uint32_t taddr, uint32_t (&r)[N]) {
-    if constexpr (N == 8) {
+    if constexpr (N == 4) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(taddr)
+                     : "memory");
+    } else if constexpr (N == 8) {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                      : "r"(taddr)
@@ -213,9 +218,10 @@ __device__ __forceinline__ void few_ld(uint32_t taddr, uint32_t (&r)[N]) {
 // j % N.
 template <int N>
 __device__ __forceinline__ void few_column_sums(float (&v)[N], int lane) {
-    if constexpr (N == 16) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], 16);
+    for (int d = 16; d >= N; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], d);
     }
 #pragma unroll
     for (int d = N / 2; d > 0; d >>= 1) {

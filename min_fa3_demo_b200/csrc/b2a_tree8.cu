@@ -2,13 +2,13 @@
 // their order, masks and tensor memory are those of b2a_tree.cu, the numbers those of b2a_cache8.cuh.
 //
 // Q is turned into its two parts by the softmax warps, a warp a row, when a piece begins; a row's scale and the scales of K meet in
-// the factor of a score.  P lies in tensor memory as its two parts, 32 columns each, where bf16 has 64.  K and V take half the room,
-// so that twice as many blocks are on their way.
+// the factor of a score.
 //
 //   warp 0-3, 4-7   Q in two parts, then softmax, one thread a row
-//   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of K       warp 11   loads of V
+//   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of K, V and scales       warp 11   V to f16
 #include "b2a_cache8.cuh"
 
+#include <cfloat>
 #include <cmath>
 
 namespace b2a {
@@ -17,29 +17,30 @@ namespace {
 
 constexpr int kTree8Threads = 384;
 constexpr int kTree8Slots = 4;       // pieces in flight between the load warp and the others
-constexpr int kTree8QkWarp = 8, kTree8LoadWarp = 9, kTree8PvWarp = 10, kTree8VWarp = 11;
+constexpr int kTree8QkWarp = 8, kTree8LoadWarp = 9, kTree8PvWarp = 10, kTree8ConvertWarp = 11;
 
 // kTwo: items may have two tiles.
 template <bool kTwo>
 struct __align__(1024) Tree8Shared {
-    static constexpr int kTiles = kTwo ? 2 : 1, kK = kTwo ? 4 : 5, kV = kTwo ? 4 : 5;
+    static constexpr int kTiles = kTwo ? 2 : 1, kK = kTwo ? 3 : 4, kV = kTwo ? 2 : 3, kV16 = 2;
     uint8_t q[kTiles][2][kTile8Bytes];      // both parts
     uint8_t k[kK][kTile8Bytes];
     uint8_t v[kV][kTile8Bytes];
+    uint8_t v16[kV16][kTileBytes];          // V in f16, two halves of 64 columns
     float q_scale[kTiles][kTileM];          // what a row of Q is multiplied by
+    ScaleRing<1> scales;
     uint32_t seen[2][2][kTileM][4];   // warpgroup, turn, token: one bit for each slot of the block
     float2 stat[2][kTileM];           // row maximum and sum of the two warpgroups
     TreePiece piece[kTree8Slots];
     uint64_t q_full[2], q_empty[2];
     uint64_t k_full[kK], k_empty[kK];
     uint64_t v_full[kV], v_empty[kV];
+    uint64_t v16_full[kV16], v16_empty[kV16];
     uint64_t s_full[2], s_empty, p_full[2], pv_done[2];
     uint64_t seen_full[2];
     uint64_t both_done, both_read;
     uint64_t piece_full[kTree8Slots], piece_empty[kTree8Slots];
-    // Number of the last piece, of the even ones and of the odd ones, that met a drafted value that is not finite.  Of two tiles
-    // the first one's warpgroup may be a piece ahead of the other's, and no more: they take S from one place in turn.
-    uint32_t not_finite[2];
+    uint32_t not_finite[kTree8Slots]; // number, plus one, of the piece that met a drafted value that is NaN
     uint32_t missing;                 // the CTA has met a page that does not exist
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -95,6 +96,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             mbar_init(smem_u32(&sh.seen_full[i]), kTileM);
         }
         mbar_init(smem_u32(&sh.s_empty), kTileM);
+        sh.scales.init(8);                                  // warps, as for Q
         mbar_init(smem_u32(&sh.both_done), 2 * kTileM);
         mbar_init(smem_u32(&sh.both_read), 2 * kTileM);
         for (int i = 0; i < Shared::kK; ++i) {
@@ -105,12 +107,16 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             mbar_init(smem_u32(&sh.v_full[i]), 1);
             mbar_init(smem_u32(&sh.v_empty[i]), 1);
         }
+        for (int i = 0; i < Shared::kV16; ++i) {
+            mbar_init(smem_u32(&sh.v16_full[i]), 1);
+            mbar_init(smem_u32(&sh.v16_empty[i]), 1);
+        }
         for (int i = 0; i < kTree8Slots; ++i) {
             mbar_init(smem_u32(&sh.piece_full[i]), 1);
-            mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 8);   // MMA warps, V's load warp and softmax warps
+            mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 8);   // MMA warps, converting and softmax warps
+            sh.not_finite[i] = 0;
         }
         sh.abort_flag = 0;
-        sh.not_finite[0] = sh.not_finite[1] = 0;
         sh.missing = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
@@ -135,7 +141,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (warp >= 8) {
         reg_dealloc<72>();
         if (warp == kTree8LoadWarp) {
-            // ------------------------------------------------------------ plan, loads of K
+            // ------------------------------------------------------------ plan, loads
             if (lane == 0) {
                 tma_prefetch_desc(&map_k);
                 tma_prefetch_desc(&map_v);
@@ -150,7 +156,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             PH_DECL(3)   // 0 other, 1 wait for K's stage, 2 issue K
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTree8Slots;
-                ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTree8Slots) & 1u) ^ 1u, 1);
+                ok = warp_wait8(wctx, smem_u32(&sh.piece_empty[at]), ((it / kTree8Slots) & 1u) ^ 1u, 1);
                 if (!ok) break;
                 const TreePiece w = tree_piece(p, walk);
                 if (lane == 0) {
@@ -165,12 +171,18 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     const int boxes = now.count(w.j0 + i, w.slots);
                     const uint32_t stage = k_it % Shared::kK;
                     PH_MARK(0);
-                    ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
+                    ok = warp_wait8(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
                     if (!ok) break;
                     PH_MARK(1);
                     now.check(p.c.cache, boxes, lane, &sh.missing);
                     loader.bad |= now.bad;
+                    ok = sh.scales.load(wctx, k_it, p.c.cache, p8.scales, now, w.j0 + i, w.slots, w.head, lane);
+                    if (!ok) break;
                     load_slots8(now, &map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
+                    const uint32_t v_stage = k_it % Shared::kV;
+                    ok = warp_wait8(wctx, smem_u32(&sh.v_empty[v_stage]), ((k_it / Shared::kV) & 1u) ^ 1u, 18);
+                    if (!ok) break;
+                    load_slots8(now, &map_v, smem_u32(&sh.v[v_stage][0]), smem_u32(&sh.v_full[v_stage]), w.head, boxes, lane);
                     PH_MARK(2);
                 }
                 if (!ok) break;
@@ -178,24 +190,22 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             }
             if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
             PH_PRINT("tree8 load", 3);
-        } else if (warp == kTree8VWarp) {
-            // ------------------------------------------------------------ loads of V
-            tree8_load_v<kTree8Slots, Shared::kV>(p, sh, &map_v, wctx, lane);
+        } else if (warp == kTree8ConvertWarp) {
+            tree8_convert_v<1, kTree8Slots, Shared::kV, Shared::kV16>(p, sh, wctx, lane, [](const TreePiece&, uint32_t) { return true; });
         } else if (warp == kTree8QkWarp || warp == kTree8PvWarp) {
             // ------------------------------------------------------------ MMA warps
             const bool qk = warp == kTree8QkWarp;
-            constexpr uint32_t idesc_qk = make_idesc_8(kTileM, kTileN, 0, 0, 0, 0);
-            constexpr uint32_t idesc_pv = make_idesc_8(kTileM, kHeadDim, 0, 1, 0, 0), idesc_rest = make_idesc_8(kTileM, kHeadDim, 0, 1, 1, 0);
+            constexpr uint32_t idesc_qk = make_idesc_first(kTileM, kTileN, 0, 0), idesc_pv = make_idesc_first(kTileM, kHeadDim, 0, 1);
             constexpr uint32_t kStageStep = kTile8Bytes >> 4;
             const uint32_t q_lo0 = desc_lo_kmajor(smem_u32(&sh.q[0][0][0]));
             const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0]));
-            const uint32_t v_lo0 = desc_lo_kmajor(smem_u32(&sh.v[0][0]));
+            const uint32_t v_lo0 = desc_lo_mnmajor(smem_u32(&sh.v16[0][0]));
             uint32_t kv_it = 0, s_it = 0, par = 0;
             bool ok = true;
             PH_DECL(4)   // 0 other, 1 wait K (V), 2 wait S (P), 3 issue
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t at = it % kTree8Slots;
-                ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kTree8Slots) & 1u, 5);
+                ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kTree8Slots) & 1u, 5);
                 if (!ok) break;
                 const volatile TreePiece& w = sh.piece[at];
                 const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
@@ -205,10 +215,10 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 __syncwarp();
                 if (!valid) break;
                 for (int i = 0; i < blocks && ok; ++i, ++kv_it) {
-                    const uint32_t stages = qk ? Shared::kK : Shared::kV, stage = kv_it % stages, phase = (kv_it / stages) & 1u;
+                    const uint32_t stages = qk ? Shared::kK : Shared::kV16, stage = kv_it % stages, phase = (kv_it / stages) & 1u;
                     PH_MARK(0);
                     if (qk) {
-                        ok = mbar_wait(wctx, smem_u32(&sh.k_full[stage]), phase, 6);
+                        ok = wait8(wctx, smem_u32(&sh.k_full[stage]), phase, 6);
                         if (!ok) break;
                         PH_MARK(1);
 #pragma unroll
@@ -216,19 +226,19 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                             if (!tree8_takes(two, i, x)) continue;
                             const int tile = two ? x : 0;
                             if (i == 0) {
-                                ok = warp_wait(wctx, smem_u32(&sh.q_full[tile]), (par >> tile) & 1u, 7);
+                                ok = warp_wait8(wctx, smem_u32(&sh.q_full[tile]), (par >> tile) & 1u, 7);
                                 if (!ok) break;
                                 par ^= 1u << tile;
                             }
                             // The softmax warps have taken the S before this one out of tensor memory.
-                            ok = mbar_wait(wctx, smem_u32(&sh.s_empty), (s_it & 1u) ^ 1u, 8);
+                            ok = wait8(wctx, smem_u32(&sh.s_empty), (s_it & 1u) ^ 1u, 8);
                             if (!ok) break;
                             PH_MARK(2);
                             ++s_it;
                             tc_fence_after_sync();
                             const uint32_t q_lo = q_lo0 + tile * 2 * kStageStep, k_lo = k_lo0 + stage * kStageStep;
-                            umma8_ss_x4_w<kStep8Along, kStep8Along>(tmem_base + kFwdColS, q_lo, k_lo, idesc_qk, 0u);
-                            umma8_ss_x4_w<kStep8Along, kStep8Along>(tmem_base + kFwdColS, q_lo + kStageStep, k_lo, idesc_qk, 1u);
+                            umma8_ss_x4_w(tmem_base + kFwdColS, q_lo, k_lo, idesc_qk, 0u);
+                            umma8_ss_x4_w(tmem_base + kFwdColS, q_lo + kStageStep, k_lo, idesc_qk, 1u);
                             tc_commit_w(smem_u32(&sh.s_full[x]));
                             if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[tile]));
                             __syncwarp();
@@ -236,26 +246,24 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         }
                         tc_commit_w(smem_u32(&sh.k_empty[stage]));
                     } else {
-                        ok = mbar_wait(wctx, smem_u32(&sh.v_full[stage]), phase, 9);
+                        ok = wait8(wctx, smem_u32(&sh.v16_full[stage]), phase, 9);
                         if (!ok) break;
                         PH_MARK(1);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             if (!tree8_takes(two, i, x)) continue;
-                            ok = mbar_wait(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
+                            ok = wait8(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
                             if (!ok) break;
                             PH_MARK(2);
                             par ^= 1u << x;
                             tc_fence_after_sync();
-                            const uint32_t o = tmem_base + kFwdColO + x * 128u, first = tmem_base + kFwdColP + x * kFwdColPStep;
-                            const uint32_t v_lo = v_lo0 + stage * kStageStep;
-                            umma8_ts_x4_w<kStep8Across>(o, first, v_lo, idesc_pv, i > (two ? 0 : x) ? 1u : 0u);
-                            umma8_ts_x4_w<kStep8Across>(o, first + 32, v_lo, idesc_rest, 1u);
+                            umma_ts_x8_w(tmem_base + kFwdColO + x * 128u, tmem_base + kFwdColP + x * kFwdColPStep,
+                                         v_lo0 + stage * (kTileBytes >> 4), idesc_pv, i > (two ? 0 : x) ? 1u : 0u);
                             tc_commit_w(smem_u32(&sh.pv_done[x]));
                             __syncwarp();
                             PH_MARK(3);
                         }
-                        tc_commit_w(smem_u32(&sh.v_empty[stage]));
+                        tc_commit_w(smem_u32(&sh.v16_empty[stage]));
                     }
                 }
             }
@@ -301,25 +309,28 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             {
                 const int t0 = w.tok0 + tile * p.tile_tokens;
                 const __nv_bfloat16* q = p8.q + (static_cast<long long>(w.q_begin) + t0) * p8.q_stride[0] +
-                                         static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] + lane * 4;
-                const int r0 = two ? quarter * 32 : warp * 16, r1 = min(rows, r0 + (two ? 32 : 16));
-                uint2 v[8];
-                auto ask = [&](int from) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int row = min(from + e, rows - 1), t = row / p.c.group;
-                        v[e] = *reinterpret_cast<const uint2*>(q + t * p8.q_stride[0] + (row - t * p.c.group) * p8.q_stride[1]);
-                    }
+                                         static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] + (lane & 15) * 8;
+                const int r0 = two ? quarter * 32 : warp * 16, r1 = min(rows, r0 + (two ? 32 : 16)), second = lane >> 4;
+                auto ask = [&](int row) -> uint4 {
+                    row = min(row, rows - 1);
+                    const int t = row / p.c.group;
+                    return *reinterpret_cast<const uint4*>(q + t * p8.q_stride[0] + (row - t * p.c.group) * p8.q_stride[1]);
                 };
-                if (r0 < r1) ask(r0);
+                uint4 next[2] = {ask(r0 + second), ask(r0 + 2 + second)};
                 ok = warp_wait(wctx, smem_u32(&sh.q_empty[tile]), ((q_par >> tile) & 1u) ^ 1u, 2);
                 if (!ok) break;
-                for (int from = r0; from < r1; from += 8) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (from + e < r1) split_q_row(v[e], from + e, lane, &sh.q[tile][0][0], &sh.q[tile][1][0], &sh.q_scale[tile][from + e]);
+#pragma unroll 1
+                for (int from = r0; from < r1; from += 4) {
+                    const uint4 v[2] = {next[0], next[1]};
+                    if (from + 4 < r1) {
+                        next[0] = ask(from + 4 + second);
+                        next[1] = ask(from + 6 + second);
                     }
-                    if (from + 8 < r1) ask(from + 8);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = from + 2 * e + second;
+                        split_q_rows(v[e], row < r1, row, lane, &sh.q[tile][0][0], &sh.q[tile][1][0], &sh.q_scale[tile][row & (kTileM - 1)]);
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -336,30 +347,9 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             float m_used = -INFINITY;   // running reference maximum (log2 units, with V's scale)
             float l = 0.f;              // running row sum relative to m_used
             const int first = two ? 0 : x, step = two ? 1 : 2;
-            // Scales: lane g < 8 has K's of slots [16 g, 16 g + 16) of a block, lane 8 + g V's.  The page is asked for two blocks
-            // before the scale's use, the scale one.
-            int page, page_row;
-            float scale_next;
-            auto ask_page = [&](int i) {
-                const int slot = (w.j0 + min(i, w.blocks)) * kSlotBlock + (lane & 7) * 16;
-                page = lane < 16 && slot < w.slots ? p.c.cache.page_of(w.seq, slot, &page_row) : -1;
-            };
-            auto ask_scale = [&]() {
-                scale_next = 1.f;
-                if (page < 0) return;
-                scale_next = lane < 8 ? p8.scales.k[p8.scales.at(p8.scales.k_stride, page, page_row, w.head)]
-                                      : p8.scales.v[p8.scales.at(p8.scales.v_stride, page, page_row, w.head)];
-            };
-            ask_page(first);
-            ask_scale();
-            ask_page(first + step);
             for (int i = first; i < w.blocks; i += step) {
                 const int base = (w.j0 + i) * kSlotBlock;
                 const bool tail = base + kSlotBlock > w.len;   // drafted tokens, or no slots any more
-                const float scale = lane < 8 ? scale_next : fminf(fmaxf(scale_next, kScaleLeast), kScaleMost);
-                ask_scale();
-                ask_page(i + 2 * step);
-                const float scale_log2 = fast_log2(scale), scale_part = 1.f / scale;
                 uint32_t* seen = nullptr;
                 PH_MARK(0);
                 if (tail && masked) {
@@ -403,19 +393,22 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&sh.s_empty));
-                if (active) {
-                    // Scores in log2 units, with V's scale.
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const float mul = q_scale * __shfl_sync(0xFFFFFFFFu, scale, g), add = __shfl_sync(0xFFFFFFFFu, scale_log2, 8 + g);
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const float2 y = fma2(make_float2(s[g * 16 + e], s[g * 16 + e + 1]), make_float2(mul, mul), make_float2(add, add));
-                            s[g * 16 + e] = y.x;
-                            s[g * 16 + e + 1] = y.y;
-                        }
-                    }
+                // Lane g < 8 has K's scale of slots [16 g, 16 g + 16) of the block, lane 8 + g V's.
+                const uint32_t scale_slot = (kv_base + i) % kScaleSlots;
+                ok = warp_wait(wctx, smem_u32(&sh.scales.full[scale_slot]), ((kv_base + i) / kScaleSlots) & 1u, 21);
+                if (!ok) break;
+                float scale = sh.scales.scale[scale_slot][(lane >> 3) & 1][lane & 7];
+                if (lane >= 8) scale = fminf(fmaxf(scale, kScaleLeast), kScaleMost);
+                const float scale_log2 = fast_log2(scale), scale_part = 1.f / scale;
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&sh.scales.empty[scale_slot]));
+                    if (!two) mbar_arrive(smem_u32(&sh.scales.empty[scale_slot]));
                 }
+                // What a score of 16 slots is multiplied by, and what is added: scores in log2 units, with V's scale.  Masked ones are -inf, so
+                // the factor must not be 0.
+                auto factor_of = [&](int g) { return fmaxf(q_scale * __shfl_sync(0xFFFFFFFFu, scale, g), FLT_MIN); };
+                auto addend_of = [&](int g) { return __shfl_sync(0xFFFFFFFFu, scale_log2, 8 + g); };
                 PH_MARK(3);
 
                 const bool begins = i == first;
@@ -433,27 +426,6 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         ok = warp_wait(wctx, smem_u32(&sh.seen_full[x]), seen_cnt & 1u, 13);
                         if (!ok) break;
                         ++seen_cnt;
-                    }
-                    // V row r of the block (whichever warpgroup's product with it comes first): behind the last slot
-                    // zeros, and of drafted tokens no value that is not finite.
-                    const int slot = base + r;
-                    const bool look = slot >= w.len && slot < w.slots && (w.n > 1 || masked);
-                    if (!two || x == 0) {
-                        // A barrier tells the last phase from the one before it, no more: the V that lay in this stage two
-                        // blocks ago has to have come, which the product with it proves.
-                        if (pv_pending) {
-                            ok = wait_pv();
-                            if (!ok) break;
-                        }
-                        const uint32_t stage = (kv_base + i) % Shared::kV;
-                        ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), ((kv_base + i) / Shared::kV) & 1u, 14);
-                        if (!ok) break;
-                        if (slot >= w.slots || look) {
-                            if (tree8_clean_row(&sh.v[stage][r * 128], r, slot >= w.slots)) {
-                                *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[it & 1u]) = it + 1;
-                            }
-                        }
-                        fence_proxy_async_smem();
                     }
                 }
                 if (active && tail) {
@@ -496,20 +468,19 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     mbar_arrive(smem_u32(&sh.p_full[x]));
                     continue;
                 }
-                float bm;
-                {
-                    float m[8];
+                float bm = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) m[e] = s[e];
+                for (int g = 0; g < 8; ++g) {
+                    float m = fmaxf(s[g * 16], s[g * 16 + 1]);
 #pragma unroll
-                    for (int e = 8; e < kTileN; ++e) m[e & 7] = fmaxf(m[e & 7], s[e]);
-                    bm = fmaxf(max3(max3(m[0], m[1], m[2]), m[3], m[4]), max3(m[5], m[6], m[7]));
+                    for (int e = 2; e < 16; e += 2) m = max3(m, s[g * 16 + e], s[g * 16 + e + 1]);
+                    bm = fmaxf(bm, fmaf(m, factor_of(g), addend_of(g)));
                 }
                 const float m_new = fmaxf(m_used, bm);
                 if (begins) {
                     m_used = m_new;
                 } else if (__any_sync(0xFFFFFFFFu, row_valid && m_new - m_used > kP8Most - kP8At)) {
-                    // O is scaled only when the maximum has moved by a factor of 2^3: the division at the end uses the same
+                    // O is scaled only when the maximum has moved by a factor of 2^13: the division at the end uses the same
                     // one.  Rows of the tile that do not exist have no say: what lies there differs from call to call.
                     const float factor = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
                     l *= factor;
@@ -529,25 +500,20 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     }
                 }
                 const float neg_m = m_used == -INFINITY ? 0.f : kP8At - m_used;
-                const float2 negv = make_float2(neg_m, neg_m);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t first_part[16], rest[16];
+                    uint32_t t[32];
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
+                        const float mul = factor_of(c * 4 + g), add = addend_of(c * 4 + g) + neg_m;
                         float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int at = c * 64 + g * 16 + e * 4;
-                            const float2 x0 = add2(make_float2(s[at], s[at + 1]), negv), x1 = add2(make_float2(s[at + 2], s[at + 3]), negv);
-                            const float2 p0 = make_float2(fast_exp2(x0.x), fast_exp2(x0.y));
-                            const float2 p1 = make_float2(fast_exp2(x1.x), fast_exp2(x1.y));
-                            acc = add2(acc, add2(p0, p1));
-                            uint32_t a, b, a_rest, b_rest;
-                            split_p(p0.x, p0.y, a, a_rest);
-                            split_p(p1.x, p1.y, b, b_rest);
-                            first_part[g * 4 + e] = a | b << 16;
-                            rest[g * 4 + e] = a_rest | b_rest << 16;
+                        for (int e = 0; e < 8; ++e) {
+                            const int at = c * 64 + g * 16 + e * 2;
+                            const float2 x2 = fma2(make_float2(s[at], s[at + 1]), make_float2(mul, mul), make_float2(add, add));
+                            const float2 p2 = make_float2(fast_exp2(x2.x), fast_exp2(x2.y));
+                            acc = e == 0 ? p2 : add2(acc, p2);
+                            t[g * 8 + e] = pack_half2(p2.x, p2.y);
                         }
                         l = fmaf(acc.x + acc.y, __shfl_sync(0xFFFFFFFFu, scale_part, 8 + c * 4 + g), l);
                     }
@@ -555,8 +521,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         ok = wait_pv();
                         if (!ok) break;
                     }
-                    tmem_st_x16(p_tmem + c * 16, first_part);
-                    tmem_st_x16(p_tmem + 32 + c * 16, rest);
+                    tmem_st_x32(p_tmem + c * 32, t);
                 }
                 if (!ok) break;
                 tmem_wait_st();
@@ -590,7 +555,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 if (w.blocks == 1) a1 = 0.f;
             }
             if (active) {
-                const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[it & 1u]) == it + 1;
+                const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) == it + 1;
                 // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const bool whole = w.part < 0;

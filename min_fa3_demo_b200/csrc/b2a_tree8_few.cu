@@ -2,34 +2,47 @@
 // decoding, and small trees.  The work's order and the masks are those of b2a_tree_few.cu, the numbers those of b2a_cache8.cuh.
 //
 // S^T = K Q^T has a lane of tensor memory for each slot and a column for each row, O^T += V^T P^T a lane for each dimension: K
-// and V are the A operands, as they lie in shared memory, and the two 8-bit parts of Q and of P the B operands, N rows of 128
-// bytes each.  A thread has a slot, and so one scale of K and one of V, which it asks for a block ahead.
+// and V (in f16) are the A operands, the two 8-bit parts of Q and P in f16 the B operands.
 //
-// Softmax across threads: P has to lie within the few exponents of e4m3, so a row's reference is a maximum that was looked for, in
-// a piece's first block and again where a score lies more than 2^3 above it (with V's scale, which P takes into the
-// product); whether one does costs a barrier of the warpgroup a block.
+// A step is two blocks, 256 slots: K of 32 KiB, as much as a block of a bf16 cache, so that the warps that load and multiply do as
+// little for a byte as there.  A thread has two slots, and so two scales of K and two of V.  The products have at least 16
+// columns, but only as many as there are rows go through the softmax: 4, 8, 16, or, in steps of one block, 32.
+//
+// Softmax across threads, as in b2a_tree_few.cu: a row's reference is a score, the first slot's of a piece, and moves to a maximum
+// that is looked for when a score lies more than 2^13 above it (f16 has fewer exponents than bf16, so not 2^32 below); whether
+// one does costs a barrier of the warpgroup a step.  The two warpgroups take turns at the steps, each with a reference, a sum and an O^T
+// of its own.
 //
 //   warp 0-3, 4-7   softmax
-//   warp 8          K Q^T       warp 10   V^T P^T       warp 9   plan, loads of K       warp 11   Q in two parts, loads of V
+//   warp 8          K Q^T       warp 10   V^T P^T       warp 9   plan, loads of K and scales       warp 11   loads of V
+//   warp 12-15      Q in two parts, V to f16
 #include "b2a_cache8.cuh"
+
+#include <cuda_fp16.h>
 
 namespace b2a {
 
 namespace {
 
-constexpr int kFew8Threads = 384;
-constexpr int kFew8Slots = 4;
-constexpr int kFew8QkWarp = 8, kFew8LoadWarp = 9, kFew8PvWarp = 10, kFew8VWarp = 11;
+constexpr int kFew8Threads = 512;
+constexpr int kFew8Slots = 4;       // pieces in flight
+constexpr int kFew8QkWarp = 8, kFew8LoadWarp = 9, kFew8PvWarp = 10, kFew8VWarp = 11, kFew8ConvertWarp = 12;
 
-template <int N>
+// R: rows, of which there may be fewer.
+template <int R>
 struct __align__(1024) Few8Shared {
-    // More rows leave room for fewer blocks.
-    static constexpr int kQ = 2, kK = N == 16 ? 6 : 5, kV = kK;
+    static constexpr int N = R < 16 ? 16 : R;      // columns of the products
+    static constexpr int B = R == 32 ? 1 : 2;      // blocks of a step
+    static constexpr int kQ = 2, kK = 4 / B, kV = R == 32 ? 3 : 4, kV16 = 2;
+    static constexpr uint32_t kTmem = 128;         // S^T of the warpgroups, N columns a block, then O^T
+    static_assert(2 * B * N + 2 * N <= kTmem, "tensor memory");
     uint8_t q[kQ][2][N * 128];        // both parts
-    uint8_t p[2][2][N * 128];         // P^T of the warpgroups, likewise
-    uint8_t k[kK][kTile8Bytes];
+    uint8_t p[2][B][N * 256];         // P^T of the warpgroups in f16, a block as two halves of [N rows][128 bytes]
+    uint8_t k[kK][B * kTile8Bytes];
     uint8_t v[kV][kTile8Bytes];
+    uint8_t v16[kV16][kTileBytes];    // V in f16, two halves of 64 columns
     float q_scale[kQ][N];             // what a row of Q is multiplied by
+    ScaleRing<B> scales;
     float minus_ref[2][N];            // -reference of each row (log2 units); 0: none yet; -inf: there is no such row
     uint32_t none[2][N];              // the row has no reference yet
     long long lse_at[N];              // of each row of an item, from its first: where its lse lies,
@@ -42,50 +55,65 @@ struct __align__(1024) Few8Shared {
     uint64_t q_full[kQ], q_empty[kQ];
     uint64_t k_full[kK], k_empty[kK];
     uint64_t v_full[kV], v_empty[kV];
+    uint64_t v16_full[kV16], v16_empty[kV16];
     uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2], meet[2];
     uint64_t both_done, both_read;
     uint64_t piece_full[kFew8Slots], piece_empty[kFew8Slots];
-    uint32_t moves[2][2];             // of each warpgroup, in turn: number of the last block that had to move a reference
-    uint32_t not_finite;
+    uint32_t moves[2][2];             // of each warpgroup, in turn: number of the last step that had to move a reference
+    uint32_t not_finite[kFew8Slots];  // number, plus one, of the piece that met a drafted value that is NaN
     uint32_t missing;                 // the CTA has met a page that does not exist
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
 
-template <int N>
-constexpr size_t few8_smem_bytes() { return sizeof(Few8Shared<N>) + 1024; }
-static_assert(few8_smem_bytes<16>() <= 227 * 1024 && few8_smem_bytes<32>() <= 227 * 1024, "shared memory of a CTA");
+template <int R>
+constexpr size_t few8_smem_bytes() {
+    static_assert(sizeof(Few8Shared<R>) + 1024 <= 227 * 1024, "shared memory of a CTA");
+    return sizeof(Few8Shared<R>) + 1024;
+}
 
-// The scales of a thread's slot: the page is asked for a block before the scales, and they a block before their use.
-struct Few8Scales {
-    int page, row;               // of the slot two blocks on
-    float k, v;                  // of the next one
+__device__ __forceinline__ float v_scale_of(float scale) { return fminf(fmaxf(scale, kScaleLeast), kScaleMost); }
 
-    __device__ __forceinline__ void look_up(const CacheView& c, int seq, int slot, int slots) {
-        page = slot < slots ? c.page_of(seq, slot, &row) : -1;
+// Rows that see a slot, a bit each.  Little of it is needed often.
+static __device__ __noinline__ uint32_t few8_seen(const TreeParams& p, const TreePiece& w, const uint32_t* token_rows, int slot) {
+    if (slot >= w.slots || !p.c.cache.has(w.seq, slot)) return 0u;
+    const int u = slot - w.len;
+    if (u < 0) return ~0u;
+    if (p.c.mask == nullptr) return u * p.c.group >= 32 ? 0u : ~0u << (u * p.c.group);
+    uint32_t see = 0;
+    const unsigned char* byte = tree_mask_row(p, w, 0) + u;
+#pragma unroll 4
+    for (int t = 0; t < w.n; ++t) {
+        if (byte[t * p.c.mask_stride[1]] != 0) see |= token_rows[t];
     }
-    __device__ __forceinline__ void load(const CacheScales& s, int head) {
-        k = v = 1.f;
-        if (page < 0) return;
-        k = s.k[s.at(s.k_stride, page, row, head)];
-        v = s.v[s.at(s.v_stride, page, row, head)];
-    }
-};
+    return see;
+}
 
-template <int N>
+// Of four rows' values those of pair e: of a step of two blocks a row's value for both slots, of one block two rows'.
+template <int B>
+__device__ __forceinline__ float2 few8_rows(const float4& v, int e) {
+    if constexpr (B == 2) {
+        const float x = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+        return make_float2(x, x);
+    } else {
+        return e == 0 ? make_float2(v.x, v.y) : make_float2(v.z, v.w);
+    }
+}
+
+template <int R>
 __global__ void __launch_bounds__(kFew8Threads, 1)
 tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ Tree8Params p8) {
-    using Shared = Few8Shared<N>;
+    using Shared = Few8Shared<R>;
+    constexpr int N = Shared::N, B = Shared::B;
     const TreeParams& p = p8.t;
     extern __shared__ uint8_t smem_raw[];
     Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr uint32_t kTmem = N * 4;                 // S^T of the warpgroups [0, 2 N), O^T [2 N, 4 N)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Shared::kQ; ++i) {
-            mbar_init(smem_u32(&sh.q_full[i]), 1);
+            mbar_init(smem_u32(&sh.q_full[i]), 4);
             mbar_init(smem_u32(&sh.q_empty[i]), 1 + 8);      // the products, and the warps that read q_scale
         }
         for (int i = 0; i < Shared::kK; ++i) {
@@ -94,7 +122,11 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         for (int i = 0; i < Shared::kV; ++i) {
             mbar_init(smem_u32(&sh.v_full[i]), 1);
-            mbar_init(smem_u32(&sh.v_empty[i]), 1);
+            mbar_init(smem_u32(&sh.v_empty[i]), 4);
+        }
+        for (int i = 0; i < Shared::kV16; ++i) {
+            mbar_init(smem_u32(&sh.v16_full[i]), 4);
+            mbar_init(smem_u32(&sh.v16_empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.s_full[i]), 1);
@@ -104,18 +136,19 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             mbar_init(smem_u32(&sh.meet[i]), 4);
             sh.moves[i][0] = sh.moves[i][1] = 0;
         }
+        sh.scales.init(4);
         mbar_init(smem_u32(&sh.both_done), 8);
         mbar_init(smem_u32(&sh.both_read), 8);
         for (int i = 0; i < kFew8Slots; ++i) {
             mbar_init(smem_u32(&sh.piece_full[i]), 1);
-            mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 8);
+            mbar_init(smem_u32(&sh.piece_empty[i]), 3 + 4 + 8);     // MMA warps, V's load warp, converting and softmax warps
+            sh.not_finite[i] = 0;
         }
         sh.abort_flag = 0;
-        sh.not_finite = 0;
         sh.missing = 0;
         fence_mbar_init();
     }
-    // Rows of Q and P that are never written, and scales of the former.
+    // Rows of Q that are never written, and their scales.
     for (int i = threadIdx.x; i < Shared::kQ * 2 * N * 8; i += kFew8Threads) reinterpret_cast<uint4*>(&sh.q[0][0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
     if (threadIdx.x < N) {
         const int first = threadIdx.x * p.c.group, last = first + p.c.group;
@@ -129,7 +162,7 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     fence_proxy_async_smem();
     if (warp == kFew8QkWarp) {
-        tmem_alloc(smem_u32(&sh.tmem_base), kTmem);
+        tmem_alloc(smem_u32(&sh.tmem_base), Shared::kTmem);
         tmem_relinquish();
         tc_fence_before_sync();
     }
@@ -153,14 +186,14 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         CacheWalk walk;
         walk.start(p.c, blockIdx.x, gridDim.x, lane);
         if (lane == 0) p.cuts[blockIdx.x] = tree_cut(p, walk);
-        SlotLoader loader(p.box_rows);
+        SlotLoader loader(p.box_rows, B);
         loader.bad = walk.bad;
         uint32_t k_it = 0;
         bool ok = true;
         PH_DECL(3)   // 0 other, 1 wait for K's stage, 2 issue K
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kFew8Slots;
-            ok = warp_wait(wctx, smem_u32(&sh.piece_empty[at]), ((it / kFew8Slots) & 1u) ^ 1u, 1);
+            ok = warp_wait8(wctx, smem_u32(&sh.piece_empty[at]), ((it / kFew8Slots) & 1u) ^ 1u, 1);
             if (!ok) break;
             const TreePiece w = tree_piece(p, walk);
             if (lane == 0) {
@@ -168,19 +201,22 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 mbar_arrive(smem_u32(&sh.piece_full[at]));
             }
             if (!w.valid) break;
-            loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-            for (int i = 0; i < w.blocks; ++i, ++k_it) {
+            const int slots = min(w.slots, (w.j0 + w.blocks) * kSlotBlock);
+            loader.look_up(p.c.cache, w.seq, w.j0, slots, lane);
+            for (int i = 0; i < w.blocks; i += B, ++k_it) {
                 SlotLoader now = loader;
-                if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-                const int boxes = now.count(w.j0 + i, w.slots);
+                if (i + B < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + B, slots, lane);
+                const int boxes = now.count(w.j0 + i, slots);
                 const uint32_t stage = k_it % Shared::kK;
                 PH_MARK(0);
-                ok = warp_wait(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
+                ok = warp_wait8(wctx, smem_u32(&sh.k_empty[stage]), ((k_it / Shared::kK) & 1u) ^ 1u, 3);
                 if (!ok) break;
                 PH_MARK(1);
                 now.check(p.c.cache, boxes, lane, &sh.missing);
                 loader.bad |= now.bad;
                 load_slots8(now, &map_k, smem_u32(&sh.k[stage][0]), smem_u32(&sh.k_full[stage]), w.head, boxes, lane);
+                ok = sh.scales.load(wctx, k_it, p.c.cache, p8.scales, now, w.j0 + i, slots, w.head, lane);
+                if (!ok) break;
                 PH_MARK(2);
             }
             if (!ok) break;
@@ -189,61 +225,63 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
         PH_PRINT("few8 load", 3);
     } else if (warp == kFew8VWarp) {
-        // ---------------------------------------------------------------- Q, loads of V
+        // ---------------------------------------------------------------- loads of V
         SlotLoader loader(p.box_rows);
         uint32_t v_it = 0;
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kFew8Slots;
-            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 4);
+            ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 4);
             if (!ok) break;
             const TreePiece w = sh.piece[at];
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
             if (!w.valid) break;
             loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-            const int rows = w.n * p.c.group;
-            const uint32_t buf = it % Shared::kQ;
-            const __nv_bfloat16* q = p8.q + w.q_begin * p8.q_stride[0] + static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] + lane * 4;
-            ok = warp_wait(wctx, smem_u32(&sh.q_empty[buf]), ((it / Shared::kQ) & 1u) ^ 1u, 2);
-            if (!ok) break;
-            for (int r0 = 0; r0 < rows; r0 += 8) {
-                uint2 x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const uint2*>(q + sh.q_at[min(r0 + e, rows - 1)]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (r0 + e < rows) split_q_row(x[e], r0 + e, lane, &sh.q[buf][0][0], &sh.q[buf][1][0], &sh.q_scale[buf][r0 + e]);
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[buf]));
             for (int i = 0; i < w.blocks; ++i, ++v_it) {
                 SlotLoader now = loader;
                 if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
                 const int boxes = now.count(w.j0 + i, w.slots);
                 const uint32_t stage = v_it % Shared::kV;
-                ok = warp_wait(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / Shared::kV) & 1u) ^ 1u, 18);
+                ok = warp_wait8(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / Shared::kV) & 1u) ^ 1u, 18);
                 if (!ok) break;
                 load_slots8(now, &map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
             }
         }
+    } else if (warp >= kFew8ConvertWarp) {
+        // ---------------------------------------------------------------- Q in two parts, and then V to f16
+        const int mine = warp - kFew8ConvertWarp;
+        tree8_convert_v<4, kFew8Slots, Shared::kV, Shared::kV16>(p, sh, wctx, mine * 32 + lane, [&](const TreePiece& w, uint32_t it) {
+            const int rows = w.n * p.c.group;
+            const uint32_t buf = it % Shared::kQ;
+            const __nv_bfloat16* q = p8.q + w.q_begin * p8.q_stride[0] + static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] + (lane & 15) * 8;
+            bool waited = false;
+#pragma unroll 1
+            for (int row = 2 * mine + (lane >> 4); row - (lane >> 4) < rows; row += 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(q + sh.q_at[min(row, rows - 1)]);
+                if (!waited && !warp_wait8(wctx, smem_u32(&sh.q_empty[buf]), ((it / Shared::kQ) & 1u) ^ 1u, 2)) return false;
+                waited = true;
+                split_q_rows(x, row < rows, row, lane, &sh.q[buf][0][0], &sh.q[buf][1][0], &sh.q_scale[buf][row]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[buf]));
+            return true;
+        });
     } else if (warp == kFew8QkWarp || warp == kFew8PvWarp) {
         // ---------------------------------------------------------------- products
         const bool qk = warp == kFew8QkWarp;
-        constexpr uint32_t idesc_qk = make_idesc_8(kTileM, N, 0, 0, 0, 0);
-        constexpr uint32_t idesc_pv = make_idesc_8(kTileM, N, 1, 0, 0, 0), idesc_rest = make_idesc_8(kTileM, N, 1, 0, 0, 1);
+        constexpr uint32_t idesc_qk = make_idesc_first(kTileM, N, 0, 0), idesc_pv = make_idesc_first(kTileM, N, 1, 0);
         constexpr uint32_t kPart = N * 128 >> 4, kStage = kTile8Bytes >> 4;
         const uint32_t q_lo0 = desc_lo_kmajor(smem_u32(&sh.q[0][0][0])), p_lo0 = desc_lo_kmajor(smem_u32(&sh.p[0][0][0]));
-        const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0])), v_lo0 = desc_lo_kmajor(smem_u32(&sh.v[0][0]));
-        uint32_t kv_it = 0;
+        const uint32_t k_lo0 = desc_lo_kmajor(smem_u32(&sh.k[0][0])), v_lo0 = desc_lo_mnmajor(smem_u32(&sh.v16[0][0]));
+        uint32_t step = 0, v_it = 0;
         uint32_t par = 0;       // bit x: phase of warpgroup x's S^T (P^T)
         bool ok = true;
         PH_DECL(4)   // 0 other, 1 wait K (V), 2 wait S (P), 3 issue
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kFew8Slots;
-            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 5);
+            ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 5);
             if (!ok) break;
             const volatile TreePiece& w = sh.piece[at];
             const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
@@ -253,43 +291,49 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (!valid) break;
             const uint32_t buf = it % Shared::kQ;
             if (qk) {
-                ok = warp_wait(wctx, smem_u32(&sh.q_full[buf]), (it / Shared::kQ) & 1u, 7);
+                ok = warp_wait8(wctx, smem_u32(&sh.q_full[buf]), (it / Shared::kQ) & 1u, 7);
                 if (!ok) break;
             }
-            for (int i = 0; i < blocks; ++i, ++kv_it) {
-                const uint32_t x = i & 1;
+            for (int i = 0; i < blocks; i += B, ++step) {
+                const uint32_t x = (i / B) & 1;
+                const int here = min(B, blocks - i);
                 PH_MARK(0);
                 if (qk) {
-                    const uint32_t stage = kv_it % Shared::kK;
-                    ok = warp_wait(wctx, smem_u32(&sh.k_full[stage]), (kv_it / Shared::kK) & 1u, 6);
+                    const uint32_t stage = step % Shared::kK;
+                    ok = warp_wait8(wctx, smem_u32(&sh.k_full[stage]), (step / Shared::kK) & 1u, 6);
                     if (!ok) break;
                     PH_MARK(1);
-                    ok = warp_wait(wctx, smem_u32(&sh.s_empty[x]), ((par >> x) & 1u) ^ 1u, 8);
+                    ok = warp_wait8(wctx, smem_u32(&sh.s_empty[x]), ((par >> x) & 1u) ^ 1u, 8);
                     if (!ok) break;
                     par ^= 1u << x;
                     PH_MARK(2);
                     tc_fence_after_sync();
-                    const uint32_t k_lo = k_lo0 + stage * kStage, q_lo = q_lo0 + buf * 2 * kPart;
-                    umma8_ss_x4_w<kStep8Along, kStep8Along>(tmem_base + x * N, k_lo, q_lo, idesc_qk, 0u);
-                    umma8_ss_x4_w<kStep8Along, kStep8Along>(tmem_base + x * N, k_lo, q_lo + kPart, idesc_qk, 1u);
+                    const uint32_t q_lo = q_lo0 + buf * 2 * kPart;
+                    for (int h = 0; h < here; ++h) {
+                        const uint32_t k_lo = k_lo0 + (stage * B + h) * kStage, to = tmem_base + (x * B + h) * N;
+                        umma8_ss_x4_w(to, k_lo, q_lo, idesc_qk, 0u);
+                        umma8_ss_x4_w(to, k_lo, q_lo + kPart, idesc_qk, 1u);
+                    }
                     tc_commit_w(smem_u32(&sh.s_full[x]));
                     tc_commit_w(smem_u32(&sh.k_empty[stage]));
-                    if (i == blocks - 1) tc_commit_w(smem_u32(&sh.q_empty[buf]));
+                    if (i + B >= blocks) tc_commit_w(smem_u32(&sh.q_empty[buf]));
                 } else {
-                    const uint32_t stage = kv_it % Shared::kV;
-                    ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), (kv_it / Shared::kV) & 1u, 9);
-                    if (!ok) break;
-                    PH_MARK(1);
-                    ok = warp_wait(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
+                    ok = warp_wait8(wctx, smem_u32(&sh.p_full[x]), (par >> x) & 1u, 10);
                     if (!ok) break;
                     par ^= 1u << x;
                     PH_MARK(2);
-                    tc_fence_after_sync();
-                    const uint32_t v_lo = v_lo0 + stage * kStage, p_lo = p_lo0 + x * 2 * kPart;
-                    umma8_ss_x4_w<kStep8Across, kStep8Along>(tmem_base + (2 + x) * N, v_lo, p_lo, idesc_pv, i > static_cast<int>(x) ? 1u : 0u);
-                    umma8_ss_x4_w<kStep8Across, kStep8Along>(tmem_base + (2 + x) * N, v_lo, p_lo + kPart, idesc_rest, 1u);
+                    for (int h = 0; h < here; ++h, ++v_it) {
+                        const uint32_t tile = v_it % Shared::kV16;
+                        ok = warp_wait8(wctx, smem_u32(&sh.v16_full[tile]), (v_it / Shared::kV16) & 1u, 9);
+                        if (!ok) break;
+                        PH_MARK(1);
+                        tc_fence_after_sync();
+                        umma_ss_nk_x8_w<N>(tmem_base + (2 * B + x) * N, v_lo0 + tile * (kTileBytes >> 4),
+                                           p_lo0 + (x * B + h) * (N * 256 >> 4), idesc_pv, i + h >= 2 * B || h > 0 ? 1u : 0u);
+                        tc_commit_w(smem_u32(&sh.v16_empty[tile]));
+                    }
+                    if (!ok) break;
                     tc_commit_w(smem_u32(&sh.pv_done[x]));
-                    tc_commit_w(smem_u32(&sh.v_empty[stage]));
                 }
                 __syncwarp();
                 PH_MARK(3);
@@ -300,147 +344,146 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // ---------------------------------------------------------------- softmax
         const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;      // r: slot of the block, dimension of O^T
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_tmem = tmem_base + lane_base + x * N, o_tmem = tmem_base + lane_base + 2 * N;
+        const uint32_t s_tmem = tmem_base + lane_base + x * B * N, o_tmem = tmem_base + lane_base + 2 * B * N;
         const float sl2 = p.scale_log2;
-        // Where this slot's probabilities lie in P^T: 128-byte rows, 16-byte chunks exchanged by the row's number.
+        // Where a slot's probabilities lie in P^T: 128-byte rows, 16-byte chunks exchanged by the row's number.
         uint32_t p_at[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) p_at[c] = smem_u32(&sh.p[x][0][c * 128 + (((r >> 4) ^ c) << 4) + (r & 15)]);
-        uint32_t s_cnt = 0, pv_cnt = 0, meet_cnt = 0, both_cnt = 0, v_base = 0, block_cnt = 0;
+        for (int c = 0; c < 8; ++c) {
+            p_at[c] = smem_u32(&sh.p[x][0][(r >> 6) * (N * 128) + c * 128 + ((((r & 63) >> 3) ^ c) << 4) + (r & 7) * 2]);
+        }
+        uint32_t s_cnt = 0, pv_cnt = 0, meet_cnt = 0, both_cnt = 0, k_base = 0, step_cnt = 0;
         bool ok = true;
         auto meet = [&]() -> bool {      // of the warpgroup
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.meet[x]));
-            return warp_wait(wctx, smem_u32(&sh.meet[x]), meet_cnt++ & 1u, 13);
+            return warp_wait8(wctx, smem_u32(&sh.meet[x]), meet_cnt++ & 1u, 13);
         };
-        PH_DECL(6)   // 0 other, 1 wait S, 2 take S, 3 V rows and mask, 4 reference, 5 P
+        PH_DECL(10)   // 0 other, 1 wait S, 2 take S, 3 mask, 4 reference, 5 P, 6 wait for Q, 7 move references, 8 results, 9 wait for P V
 
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t at = it % kFew8Slots;
-            ok = warp_wait(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 11);
+            ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 11);
             if (!ok) break;
             const TreePiece& w = sh.piece[at];
             if (!w.valid) break;
             const int rows = w.n * p.c.group;
-            const int slot0 = w.j0 * kSlotBlock + r;
-            Few8Scales next;
-            next.look_up(p.c.cache, w.seq, slot0 + x * kSlotBlock, w.slots);
-            next.load(p8.scales, w.head);
-            next.look_up(p.c.cache, w.seq, slot0 + min(x + 2, w.blocks) * kSlotBlock, w.slots);
             const uint32_t buf = it % Shared::kQ;
-            ok = warp_wait(wctx, smem_u32(&sh.q_full[buf]), (it / Shared::kQ) & 1u, 19);
+            PH_MARK(0);
+            ok = warp_wait8(wctx, smem_u32(&sh.q_full[buf]), (it / Shared::kQ) & 1u, 19);
             if (!ok) break;
+            PH_MARK(6);
             const float4* q_scale = reinterpret_cast<const float4*>(&sh.q_scale[buf][0]);
-            float sum[N];
+            float sum[R];
 #pragma unroll
-            for (int c = 0; c < N; ++c) sum[c] = 0.f;
-            bool open = true;            // a row has no reference yet
-            if (r < N) {
-                sh.minus_ref[x][r] = r < rows ? 0.f : -INFINITY;
-                sh.none[x][r] = 1u;
-            }
+            for (int c = 0; c < R; ++c) sum[c] = 0.f;
+            bool open = false;           // a row has no reference yet
 
-            for (int i = x; i < w.blocks; i += 2) {
-                const int slot = slot0 + i * kSlotBlock;
-                const bool tail = (w.j0 + i + 1) * kSlotBlock > w.len;     // drafted tokens, or no slots any more
-                const float k_scale = next.k * sl2, v_scale = fminf(fmaxf(next.v, kScaleLeast), kScaleMost);
-                next.load(p8.scales, w.head);
-                next.look_up(p.c.cache, w.seq, slot0 + min(i + 4, w.blocks) * kSlotBlock, w.slots);
-                const float v_log2 = fast_log2(v_scale), v_part = 1.f / v_scale;
-                bool pv_pending = i > x;
+            for (int i = x * B; i < w.blocks; i += 2 * B) {
+                const bool first = i < 2 * B;
+                bool pv_pending = !first;
                 auto wait_pv = [&]() -> bool {
                     if (!pv_pending) return true;
-                    if (!warp_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15)) return false;
+                    if (!warp_wait8(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15)) return false;
                     ++pv_cnt;
                     tc_fence_after_sync();
                     pv_pending = false;
                     return true;
                 };
-                // Rows that see this slot: all of them if it lies before the drafted tokens.
-                uint32_t see = ~0u;
-                if (tail && slot >= w.len) {
-                    const int u = slot - w.len;
-                    see = 0;
-                    if (slot < w.slots && p.c.mask == nullptr) {
-                        see = u * p.c.group >= 32 ? 0u : ~0u << (u * p.c.group);
-                    } else if (slot < w.slots && u < w.n) {
-                        const unsigned char* byte = tree_mask_row(p, w, 0) + u;
-#pragma unroll 8
-                        for (int t = 0; t < w.n; ++t) {
-                            if (byte[t * p.c.mask_stride[1]] != 0) see |= sh.token_rows[t];
-                        }
-                    }
-                }
+                const uint32_t step = k_base + i / B, scale_slot = step % kScaleSlots;
                 PH_MARK(0);
-                ok = warp_wait(wctx, smem_u32(&sh.s_full[x]), s_cnt & 1u, 12);
+                ok = warp_wait8(wctx, smem_u32(&sh.s_full[x]), s_cnt & 1u, 12);
                 if (!ok) break;
                 ++s_cnt;
-                ++block_cnt;
+                ++step_cnt;
                 PH_MARK(1);
                 tc_fence_after_sync();
-                // One answer for the warp: the flag may go up, for a block still to come, between two lanes' looks.
-                const bool missing = __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u);
-                float y[N];              // scores in log2 units, with V's scale
+                // Scores in log2 units, with V's scale, in pairs: of rows c, c + 1, ... for slots r and 128 + r, or of rows c, c + 1
+                // and c + 2, c + 3 for slot r.
+                constexpr int kFour = 2 * B;       // pairs of four rows
+                float2 y[R / 4 * kFour];
                 {
-                    uint32_t s[N];
-                    few_ld<N>(s_tmem, s);
+                    uint32_t raw[B][R];
+#pragma unroll
+                    for (int h = 0; h < B; ++h) few_ld<R>(s_tmem + h * N, raw[h]);
+                    ok = warp_wait8(wctx, smem_u32(&sh.scales.full[scale_slot]), (step / kScaleSlots) & 1u, 21);
+                    if (!ok) break;
                     tmem_wait_ld();
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sh.s_empty[x]));
+                    const float* k_scale = &sh.scales.scale[scale_slot][0][r >> 4];
+                    const float* v_scale = &sh.scales.scale[scale_slot][1][r >> 4];
+                    const float2 k2 = make_float2(k_scale[0] * sl2, k_scale[(B - 1) * 8] * sl2);
+                    const float2 v2 = make_float2(fast_log2(v_scale_of(v_scale[0])), fast_log2(v_scale_of(v_scale[(B - 1) * 8])));
 #pragma unroll
-                    for (int c = 0; c < N; c += 4) {
+                    for (int c = 0; c < R; c += 4) {
                         const float4 q4 = q_scale[c / 4];
-                        y[c] = fmaf(__uint_as_float(s[c]) * k_scale, q4.x, v_log2);
-                        y[c + 1] = fmaf(__uint_as_float(s[c + 1]) * k_scale, q4.y, v_log2);
-                        y[c + 2] = fmaf(__uint_as_float(s[c + 2]) * k_scale, q4.z, v_log2);
-                        y[c + 3] = fmaf(__uint_as_float(s[c + 3]) * k_scale, q4.w, v_log2);
+#pragma unroll
+                        for (int e = 0; e < kFour; ++e) {
+                            const float2 s = B == 2 ? make_float2(__uint_as_float(raw[0][c + e]), __uint_as_float(raw[B - 1][c + e]))
+                                                    : make_float2(__uint_as_float(raw[0][c + 2 * (e & 1)]), __uint_as_float(raw[0][c + 2 * (e & 1) + 1]));
+                            y[c / 4 * kFour + e] = fma2(mul2(s, k2), few8_rows<B>(q4, e), v2);
+                        }
                     }
                 }
                 PH_MARK(2);
-                if (tail) {
-                    // As in b2a_tree.cu: a barrier tells the last phase from the one before it, so the V that lay in this
-                    // stage before has to have come, which the warpgroup's last product proves.
-                    ok = wait_pv();
-                    if (!ok) break;
-                    const uint32_t stage = (v_base + i) % Shared::kV;
-                    ok = warp_wait(wctx, smem_u32(&sh.v_full[stage]), ((v_base + i) / Shared::kV) & 1u, 14);
-                    if (!ok) break;
-                    if (slot >= w.slots || (slot >= w.len && (w.n > 1 || p.c.mask != nullptr))) {
-                        if (tree8_clean_row(&sh.v[stage][r * 128], r, slot >= w.slots)) {
-                            *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) = it + 1;
-                        }
-                    }
-                    fence_proxy_async_smem();
-                }
-                if (missing && !p.c.cache.has(w.seq, slot)) see = 0;
-                if ((tail || missing) && __any_sync(0xFFFFFFFFu, see != ~0u)) {
+                // Drafted tokens, or no slots any more; pages that do not exist (one answer for the warp: the flag may go up, for
+                // a step still to come, between two lanes' looks).
+                const bool tail = (w.j0 + i + B) * kSlotBlock > w.len;
+                if (__builtin_expect(tail || i + B > w.blocks || __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u), 0)) {
+                    uint32_t see[B];
 #pragma unroll
-                    for (int c = 0; c < N; ++c) {
-                        if (!((see >> c) & 1u)) y[c] = -INFINITY;
+                    for (int h = 0; h < B; ++h) {
+                        see[h] = i + h < w.blocks ? few8_seen(p, w, sh.token_rows, (w.j0 + i + h) * kSlotBlock + r) : 0u;
+                    }
+#pragma unroll
+                    for (int t = 0; t < R / 4 * kFour; ++t) {
+                        if (!((see[0] >> (B == 2 ? t : 2 * t)) & 1u)) y[t].x = -INFINITY;
+                        if (!((see[B - 1] >> (B == 2 ? t : 2 * t + 1)) & 1u)) y[t].y = -INFINITY;
                     }
                 }
                 PH_MARK(3);
 
                 const float4* minus_ref = reinterpret_cast<const float4*>(&sh.minus_ref[x][0]);
-                float top = -INFINITY;
-                if (i > x) {
+                if (first) {
+                    // A piece's first references are the scores of the block's first slot, if all rows see it.
+                    if (r == 0) {
 #pragma unroll
-                    for (int c = 0; c < N; c += 4) {
-                        const float4 m = minus_ref[c / 4];
-                        top = fmaxf(top, fmaxf(fmaxf(y[c] + m.x, y[c + 1] + m.y), fmaxf(y[c + 2] + m.z, y[c + 3] + m.w)));
+                        for (int c = 0; c < R; ++c) {
+                            const float score = B == 2 ? y[c].x : c & 1 ? y[c / 2].y : y[c / 2].x;
+                            const bool none = !(fabsf(score) < INFINITY);
+                            sh.minus_ref[x][c] = c >= rows ? -INFINITY : none ? 0.f : kP8At - score;
+                            sh.none[x][c] = none;
+                            open |= none && c < rows;
+                        }
+                        if (open) *reinterpret_cast<volatile uint32_t*>(&sh.moves[x][step_cnt & 1u]) = step_cnt;
+                    }
+                    ok = meet();
+                    if (!ok) break;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < R; c += 4) {
+                    const float4 m4 = minus_ref[c / 4];
+#pragma unroll
+                    for (int e = 0; e < kFour; ++e) {
+                        const float2 up = add2(y[c / 4 * kFour + e], few8_rows<B>(m4, e));
+                        top = max3(top, up.x, up.y);
                     }
                 }
                 if (__any_sync(0xFFFFFFFFu, open || top > kP8Most) && lane == 0) {
-                    *reinterpret_cast<volatile uint32_t*>(&sh.moves[x][block_cnt & 1u]) = block_cnt;
+                    *reinterpret_cast<volatile uint32_t*>(&sh.moves[x][step_cnt & 1u]) = step_cnt;
                 }
                 ok = meet();
                 if (!ok) break;
-                if (*reinterpret_cast<volatile uint32_t*>(&sh.moves[x][block_cnt & 1u]) == block_cnt) {
+                PH_MARK(4);
+                if (__builtin_expect(*reinterpret_cast<volatile uint32_t*>(&sh.moves[x][step_cnt & 1u]) == step_cnt, 0)) {
                     // The rows' maxima over the block: ordered as integers, for which a warp has a reduction.
 #pragma unroll
-                    for (int c = 0; c < N; ++c) {
-                        const int bits = y[c] == y[c] ? __float_as_int(y[c]) : static_cast<int>(0xFF800000u);
+                    for (int c = 0; c < R; ++c) {
+                        const float score = B == 2 ? fmaxf(y[c].x, y[c].y) : c & 1 ? y[c / 2].y : y[c / 2].x;
+                        const int bits = __float_as_int(fmaxf(score, -INFINITY));      // NaN has no say
                         const int key = __reduce_max_sync(0xFFFFFFFFu, bits ^ ((bits >> 31) & 0x7FFFFFFF));
                         if (lane == 0) sh.top[x][quarter][c] = __int_as_float(key ^ ((key >> 31) & 0x7FFFFFFF));
                     }
@@ -451,23 +494,25 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     open = false;
                     // In turn, so that no thread has more than a few factors at a time.
 #pragma unroll
-                    for (int c0 = 0; c0 < N; c0 += 8) {
+                    for (int c0 = 0; c0 < R; c0 += 8) {
                         float factor[8];
                         uint32_t o[8];
-                        if (i > x) {
+                        if (!first) {
                             few_ld<8>(o_tmem + x * N + c0, o);
                             tmem_wait_ld();
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int c = c0 + e;
+                            factor[e] = 1.f;
+                            if (c >= R) continue;
                             const float m = fmaxf(fmaxf(sh.top[x][0][c], sh.top[x][1][c]), fmaxf(sh.top[x][2][c], sh.top[x][3][c]));
                             const bool none = sh.none[x][c] != 0u;           // then sum and O are 0
-                            factor[e] = !none && m + sh.minus_ref[x][c] > kP8Most ? fast_exp2(kP8At - m - sh.minus_ref[x][c]) : 1.f;
+                            if (!none && m + sh.minus_ref[x][c] > kP8Most) factor[e] = fast_exp2(kP8At - m - sh.minus_ref[x][c]);
                             open |= c < rows && none && m == -INFINITY;
                             sum[c] *= factor[e];
                         }
-                        if (i > x) {
+                        if (!first) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor[e]);
                             asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
@@ -476,7 +521,7 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                          : "memory");
                         }
                     }
-                    if (i > x) tmem_wait_st();
+                    if (!first) tmem_wait_st();
                     ok = meet();                 // all have read the old references
                     if (!ok) break;
                     if (r < rows) {
@@ -489,51 +534,58 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     ok = meet();
                     if (!ok) break;
                 }
-                PH_MARK(4);
-                ok = wait_pv();                  // P^T of the block before has been read
+                PH_MARK(7);
+                ok = wait_pv();                  // P^T of the step before has been read
                 if (!ok) break;
+                PH_MARK(9);
+                const float* v_scale = &sh.scales.scale[scale_slot][1][r >> 4];
+                const float2 part = make_float2(1.f / v_scale_of(v_scale[0]), 1.f / v_scale_of(v_scale[(B - 1) * 8]));
 #pragma unroll
-                for (int c = 0; c < N; c += 4) {
+                for (int c = 0; c < R; c += 4) {
                     const float4 m4 = minus_ref[c / 4];
-                    const float m[4] = {m4.x, m4.y, m4.z, m4.w};
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float p0 = fast_exp2(y[c + e] + m[e]), p1 = fast_exp2(y[c + e + 1] + m[e + 1]);
-                        sum[c + e] = fmaf(p0, v_part, sum[c + e]);
-                        sum[c + e + 1] = fmaf(p1, v_part, sum[c + e + 1]);
-                        uint32_t first, rest;
-                        split_p(p0, p1, first, rest);
-                        const uint32_t to0 = p_at[(c + e) & 7] + (c >> 3) * 1024, to1 = p_at[(c + e + 1) & 7] + (c >> 3) * 1024;
-                        asm volatile("st.shared.b8 [%0], %1;" ::"r"(to0), "r"(first) : "memory");
-                        asm volatile("st.shared.b8 [%0], %1;" ::"r"(to1), "r"(first >> 8) : "memory");
-                        asm volatile("st.shared.b8 [%0], %1;" ::"r"(to0 + N * 128), "r"(rest) : "memory");
-                        asm volatile("st.shared.b8 [%0], %1;" ::"r"(to1 + N * 128), "r"(rest >> 8) : "memory");
+                    for (int e = 0; e < kFour; ++e) {
+                        const float2 up = add2(y[c / 4 * kFour + e], few8_rows<B>(m4, e));
+                        const float2 prob = make_float2(fast_exp2(up.x), fast_exp2(up.y));
+                        const int row = B == 2 ? c + e : c + 2 * (e & 1), other = B == 2 ? row : row + 1;
+                        if constexpr (B == 2) {
+                            sum[row] = fmaf(prob.x, part.x, fmaf(prob.y, part.y, sum[row]));
+                        } else {
+                            sum[row] = fmaf(prob.x, part.x, sum[row]);
+                            sum[other] = fmaf(prob.y, part.y, sum[other]);
+                        }
+                        const uint32_t to = p_at[row & 7] + (row >> 3) * 1024, to_other = p_at[other & 7] + (other >> 3) * 1024 + (B - 1) * N * 256;
+                        asm volatile("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tst.shared.b16 [%0], l;\n\tst.shared.b16 [%1], u;\n\t}"
+                                     ::"r"(to), "r"(to_other), "r"(pack_half2(prob.x, prob.y)) : "memory");
                     }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[x]));
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&sh.p_full[x]));
+                    mbar_arrive(smem_u32(&sh.scales.empty[scale_slot]));
+                }
                 PH_MARK(5);
             }
             if (!ok) break;
-            v_base += w.blocks;
-            if (w.blocks > x) {
-                ok = warp_wait(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15);
+            k_base += (w.blocks + B - 1) / B;
+            if (w.blocks > x * B) {
+                ok = warp_wait8(wctx, smem_u32(&sh.pv_done[x]), pv_cnt & 1u, 15);
                 if (!ok) break;
                 ++pv_cnt;
                 tc_fence_after_sync();
             }
 
-            // The warpgroup's sums, and then both warpgroups' parts: O = a0 O0 + a1 O1, half of the rows each.
-            few_column_sums<N>(sum, lane);
+            // The warpgroup's sums, and then both warpgroups' parts: O = a0 O0 + a1 O1, eight rows at a time.
+            few_column_sums<R>(sum, lane);
             ok = meet();                         // nobody still reads maxima
             if (!ok) break;
-            if (lane < N) sh.top[x][quarter][lane] = sum[0];
+            if (lane < R) sh.top[x][quarter][lane] = sum[0];
             ok = meet();
             if (!ok) break;
-            if (r < N) {
-                const float ref = w.blocks <= x || sh.none[x][r] != 0u ? -INFINITY : -sh.minus_ref[x][r];
+            if (r < R) {
+                const float ref = w.blocks <= x * B || sh.none[x][r] != 0u ? -INFINITY : -sh.minus_ref[x][r];
                 sh.stat[x][r] = make_float2(ref, (sh.top[x][0][r] + sh.top[x][1][r]) + (sh.top[x][2][r] + sh.top[x][3][r]));
             }
             tc_fence_before_sync();
@@ -542,15 +594,17 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 mbar_arrive(smem_u32(&sh.q_empty[buf]));
                 mbar_arrive(smem_u32(&sh.both_done));
             }
-            ok = warp_wait(wctx, smem_u32(&sh.both_done), both_cnt & 1u, 16);
+            ok = warp_wait8(wctx, smem_u32(&sh.both_done), both_cnt & 1u, 16);
             if (!ok) break;
             tc_fence_after_sync();
-            const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite) == it + 1;
+            const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) == it + 1;
             const bool whole = w.part < 0;
-            for (int c0 = x * (N / 2); c0 < min((x + 1) * (N / 2), rows); c0 += 8) {
+#pragma unroll 1
+            for (int c0 = 8 * x; c0 < rows; c0 += 16) {
+                const bool second = w.blocks > B;
                 uint32_t o0[8], o1[8];
                 few_ld<8>(o_tmem + c0, o0);
-                if (w.blocks > 1) few_ld<8>(o_tmem + N + c0, o1);
+                if (second) few_ld<8>(o_tmem + N + c0, o1);
                 tmem_wait_ld();
                 float o[8], ref[8], l[8];
 #pragma unroll
@@ -561,7 +615,7 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const float a1 = s1.x == ref[e] ? 1.f : fast_exp2(s1.x - ref[e]);
                     l[e] = s0.y * a0 + s1.y * a1;
                     o[e] = __uint_as_float(o0[e]) * a0;
-                    if (w.blocks > 1) o[e] = fmaf(__uint_as_float(o1[e]), a1, o[e]);
+                    if (second) o[e] = fmaf(__uint_as_float(o1[e]), a1, o[e]);
                 }
                 if (not_finite) {
                     // Values of drafted tokens that are NaN, given to the rows that see them.
@@ -603,34 +657,38 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.both_read));
-            ok = warp_wait(wctx, smem_u32(&sh.both_read), both_cnt & 1u, 17);
+            ok = warp_wait8(wctx, smem_u32(&sh.both_read), both_cnt & 1u, 17);
             ++both_cnt;
             if (!ok) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+            PH_MARK(8);
         }
-        PH_PRINT("few8 softmax", 6);
+        PH_PRINT("few8 softmax", 10);
     }
 
     tc_fence_before_sync();
     __syncthreads();
     if (warp == kFew8QkWarp) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem_base, kTmem);
+        tmem_dealloc(tmem_base, Shared::kTmem);
     }
 }
 
-template <int N>
+template <int R>
 int set_few8_smem() {
-    B2A_CUDA_OK(cudaFuncSetAttribute(tree8_attention_few<N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(few8_smem_bytes<N>())));
+    B2A_CUDA_OK(cudaFuncSetAttribute(tree8_attention_few<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(few8_smem_bytes<R>())));
     return B2A_OK;
 }
 
-template <int N>
-int launch_few8(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, cudaStream_t stream) {
-    auto attention = tree8_attention_few<N>;
-    B2A_CUDA_OK(launch_early(attention, ctas, kFew8Threads, few8_smem_bytes<N>(), stream, map_k, map_v, p));
+template <int R>
+int launch_few8(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev, int slot,
+                cudaStream_t stream) {
+    const int rc = once_per_device(dev.device, slot, set_few8_smem<R>);
+    if (rc != B2A_OK) return rc;
+    auto attention = tree8_attention_few<R>;
+    B2A_CUDA_OK(launch_early(attention, ctas, kFew8Threads, few8_smem_bytes<R>(), stream, map_k, map_v, p));
     return B2A_OK;
 }
 
@@ -638,14 +696,11 @@ int launch_few8(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8P
 
 int launch_tree8_few(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
                      cudaStream_t stream) {
-    int rc;
-    if (p.t.part_rows <= 16) {
-        rc = once_per_device(dev.device, 13, set_few8_smem<16>);
-        if (rc == B2A_OK) rc = launch_few8<16>(map_k, map_v, p, ctas, stream);
-    } else {
-        rc = once_per_device(dev.device, 14, set_few8_smem<32>);
-        if (rc == B2A_OK) rc = launch_few8<32>(map_k, map_v, p, ctas, stream);
-    }
+    const int rows = p.t.part_rows;
+    const int rc = rows <= 4    ? launch_few8<4>(map_k, map_v, p, ctas, dev, 13, stream)
+                   : rows <= 8  ? launch_few8<8>(map_k, map_v, p, ctas, dev, 14, stream)
+                   : rows <= 16 ? launch_few8<16>(map_k, map_v, p, ctas, dev, 21, stream)
+                                : launch_few8<32>(map_k, map_v, p, ctas, dev, 22, stream);
     return rc != B2A_OK || ctas == 1 ? rc : launch_tree_combine_few(p.t, ctas, stream);
 }
 
