@@ -324,6 +324,16 @@ constexpr float kP8Most = 15.f, kP8At = 2.f;
 
 __device__ __forceinline__ bool e4m3_not_finite(uint32_t byte) { return (byte & 0x7Fu) == 0x7Fu; }
 
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // As tree_clean_row, for a row of 128 bytes, whose only values that are not finite are NaN.  Little code, as few rows need it.
 static __device__ __noinline__ bool tree8_clean_row(uint8_t* row, int r, bool behind) {
     // A magnitude of 0x7F plus one carries into its byte's sign bit, and no other does.
@@ -372,29 +382,31 @@ __device__ __forceinline__ void tree8_convert_v(const TreeParams& p, Shared& sh,
             PH_MARK(2);
 #pragma unroll 1
             for (int row = r; row < kSlotBlock; row += 32 * kWarps) {
-                uint8_t* from = &sh.v[stage][row * 128];
-                uint8_t* to = &sh.v16[tile][row * 128];
                 const int slot = (j0 + i) * kSlotBlock + row;
-                if (slot >= len && tree8_clean_row(from, row, slot >= slots)) {
+                if (slot >= len && tree8_clean_row(&sh.v[stage][row * 128], row, slot >= slots)) {
                     *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) = it + 1;
                 }
-                // 16 values: chunks 2 c and 2 c + 1 of 8, which lie in a half of 64 columns.
+                // 16 values: chunks 2 c and 2 c + 1 of 8, which lie in a half of 64 columns.  Rows begin at multiples of 128 bytes, so chunks
+                // are exchanged by an exclusive or of the address.
+                const uint32_t from = smem_u32(&sh.v[stage][row * 128]) + (row & 7) * 16, to = smem_u32(&sh.v16[tile][row * 128]) + (row & 7) * 16;
 #pragma unroll 1
-                for (int c = 0; c < 8; c += 2) {
-                    uint4 v[2];
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) v[e] = *reinterpret_cast<const uint4*>(from + (((c + e) ^ (row & 7)) << 4));
-                    uint8_t* half = to + (c >> 2) * kHalfTileBytes;
+                    for (int c = 0; c < 4; c += 2) {
+                        uint4 v[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uint4 x, y;
-                        e4m3x4_to_half4(v[e].x, x.x, x.y);
-                        e4m3x4_to_half4(v[e].y, x.z, x.w);
-                        e4m3x4_to_half4(v[e].z, y.x, y.y);
-                        e4m3x4_to_half4(v[e].w, y.z, y.w);
-                        const int first = ((c + e) & 3) * 2;
-                        *reinterpret_cast<uint4*>(half + ((first ^ (row & 7)) << 4)) = x;
-                        *reinterpret_cast<uint4*>(half + (((first + 1) ^ (row & 7)) << 4)) = y;
+                        for (int e = 0; e < 2; ++e) v[e] = ld_shared_v4((from ^ (half * 64)) ^ ((c + e) * 16));
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint4 x, y;
+                            e4m3x4_to_half4(v[e].x, x.x, x.y);
+                            e4m3x4_to_half4(v[e].y, x.z, x.w);
+                            e4m3x4_to_half4(v[e].z, y.x, y.y);
+                            e4m3x4_to_half4(v[e].w, y.z, y.w);
+                            const uint32_t there = to + half * kHalfTileBytes;
+                            st_shared_v4(there ^ ((c + e) * 32), x);
+                            st_shared_v4(there ^ ((c + e) * 32 + 16), y);
+                        }
                     }
                 }
             }
@@ -410,7 +422,59 @@ __device__ __forceinline__ void tree8_convert_v(const TreeParams& p, Shared& sh,
     PH_PRINT("tree8 convert", 4);
 }
 
-// b2a_tree8_few.cu: calls of at most kFewRows rows an item.
+// Loads of V by one warp, as tree_load_v.
+template <int kSlots, int kStages, typename Shared>
+__device__ __forceinline__ void tree8_load_v(const TreeParams& p, Shared& sh, const CUtensorMap* map, const WaitCtx& wctx, int lane) {
+    SlotLoader loader(p.box_rows);
+    uint32_t v_it = 0;
+    bool ok = true;
+    for (uint32_t it = 0; ok; ++it) {
+        const uint32_t at = it % kSlots;
+        ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kSlots) & 1u, 4);
+        if (!ok) break;
+        const TreePiece w = sh.piece[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
+        if (!w.valid) break;
+        loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
+        for (int i = 0; i < w.blocks; ++i, ++v_it) {
+            SlotLoader now = loader;
+            if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
+            const int boxes = now.count(w.j0 + i, w.slots);
+            const uint32_t stage = v_it % kStages;
+            ok = warp_wait8(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / kStages) & 1u) ^ 1u, 18);
+            if (!ok) break;
+            load_slots8(now, map, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
+        }
+    }
+}
+
+// Values of drafted tokens that are NaN, given to a row that sees them: columns [column, column + 32) of O.
+__device__ __forceinline__ void tree8_add_not_finite(const TreeParams& p, const TreePiece& w, int token, int column, uint32_t (&t)[32]) {
+    const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
+#pragma unroll 1
+    for (int u = from; u < to; ++u) {
+        const long long slot = static_cast<long long>(w.len) + u;
+        if (slot >= w.slots || !tree_sees(p, w, token, u)) continue;
+        int row;
+        const int page = p.c.cache.page_of(w.seq, slot, &row);
+        if (page < 0) continue;
+        const uint8_t* v = reinterpret_cast<const uint8_t*>(p.c.cache.v) + p.c.cache.at(p.c.cache.v_stride, page, row, w.head) + column;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 chunk = reinterpret_cast<const uint4*>(v)[i];
+            const uint32_t words[4] = {chunk.x, chunk.y, chunk.z, chunk.w};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (e4m3_not_finite(words[e >> 2] >> (e & 3) * 8)) t[i * 16 + e] = 0x7FFFFFFFu;
+            }
+        }
+    }
+}
+
+// b2a_tree8_one.cu: calls of more rows an item, but no more than a tile's 128; b2a_tree8_few.cu: of at most kFewRows.
+int launch_tree8_one(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
+                     cudaStream_t stream);
 int launch_tree8_few(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
                      cudaStream_t stream);
 

@@ -1,8 +1,10 @@
 // Attention of drafted tokens, or of a prompt's next chunk, over a cache in 8 bits: O = softmax(scale Q K^T + mask) V.  Rows, items,
 // their order, masks and tensor memory are those of b2a_tree.cu, the numbers those of b2a_cache8.cuh.
 //
-// Q is turned into its two parts by the softmax warps, a warp a row, when a piece begins; a row's scale and the scales of K meet in
-// the factor of a score.
+// Two tiles of 128 rows use each block in turn, as there: a thread takes its row's 128 scores at once, so that the S which both use is
+// free again, and one warp turns V to f16 in the time that the two tiles' softmax needs.  (b2a_tree8_one.cu is for calls whose
+// items have one tile.)  Q is turned into its two parts by the softmax warps, two rows a warp at a time, when a piece begins; a row's scale
+// and K's meet in the factor of a score.
 //
 //   warp 0-3, 4-7   Q in two parts, then softmax, one thread a row
 //   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of K, V and scales       warp 11   V to f16
@@ -19,10 +21,8 @@ constexpr int kTree8Threads = 384;
 constexpr int kTree8Slots = 4;       // pieces in flight between the load warp and the others
 constexpr int kTree8QkWarp = 8, kTree8LoadWarp = 9, kTree8PvWarp = 10, kTree8ConvertWarp = 11;
 
-// kTwo: items may have two tiles.
-template <bool kTwo>
 struct __align__(1024) Tree8Shared {
-    static constexpr int kTiles = kTwo ? 2 : 1, kK = kTwo ? 3 : 4, kV = kTwo ? 2 : 3, kV16 = 2;
+    static constexpr int kTiles = 2, kK = 3, kV = 2, kV16 = 2;
     uint8_t q[kTiles][2][kTile8Bytes];      // both parts
     uint8_t k[kK][kTile8Bytes];
     uint8_t v[kV][kTile8Bytes];
@@ -46,43 +46,18 @@ struct __align__(1024) Tree8Shared {
     uint32_t abort_flag;
 };
 
-template <bool kTwo>
-constexpr size_t tree8_smem_bytes() { return sizeof(Tree8Shared<kTwo>) + 1024; }
-static_assert(tree8_smem_bytes<true>() <= 227 * 1024 && tree8_smem_bytes<false>() <= 227 * 1024, "shared memory of a CTA");
+constexpr size_t kTree8SmemBytes = sizeof(Tree8Shared) + 1024;
+static_assert(kTree8SmemBytes <= 227 * 1024, "shared memory of a CTA");
 
 // Whether a block goes to warpgroup x: both tiles take every block, one tile's warpgroups take turns.
 __device__ __forceinline__ bool tree8_takes(bool two, int i, int x) { return two || (i & 1) == x; }
 
-// Values of drafted tokens that are NaN, given to a row that sees them: columns [column, column + 32) of O.
-__device__ __forceinline__ void tree8_add_not_finite(const TreeParams& p, const TreePiece& w, int token, int column, uint32_t (&t)[32]) {
-    const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
-#pragma unroll 1
-    for (int u = from; u < to; ++u) {
-        const long long slot = static_cast<long long>(w.len) + u;
-        if (slot >= w.slots || !tree_sees(p, w, token, u)) continue;
-        int row;
-        const int page = p.c.cache.page_of(w.seq, slot, &row);
-        if (page < 0) continue;
-        const uint8_t* v = reinterpret_cast<const uint8_t*>(p.c.cache.v) + p.c.cache.at(p.c.cache.v_stride, page, row, w.head) + column;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 chunk = reinterpret_cast<const uint4*>(v)[i];
-            const uint32_t words[4] = {chunk.x, chunk.y, chunk.z, chunk.w};
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (e4m3_not_finite(words[e >> 2] >> (e & 3) * 8)) t[i * 16 + e] = 0x7FFFFFFFu;
-            }
-        }
-    }
-}
-
-template <bool kTwo>
 __global__ void __launch_bounds__(kTree8Threads, 1)
 tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ Tree8Params p8) {
     const TreeParams& p = p8.t;
     extern __shared__ uint8_t smem_raw[];
-    using Shared = Tree8Shared<kTwo>;
+    using Shared = Tree8Shared;
     Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -210,7 +185,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 const volatile TreePiece& w = sh.piece[at];
                 const int valid = __shfl_sync(0xFFFFFFFFu, w.valid, 0);
                 const int blocks = __shfl_sync(0xFFFFFFFFu, w.blocks, 0);
-                const bool two = kTwo && __shfl_sync(0xFFFFFFFFu, w.tokens[1], 0) > 0;
+                const bool two = __shfl_sync(0xFFFFFFFFu, w.tokens[1], 0) > 0;
                 if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
                 __syncwarp();
                 if (!valid) break;
@@ -296,7 +271,7 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
             };
             if (!w.valid) break;
-            const bool two = kTwo && w.tokens[1] > 0;
+            const bool two = w.tokens[1] > 0;
             const int tile = two ? x : 0;
             const int tokens = w.tokens[tile];
             const int rows = tokens * p.c.group;
@@ -638,10 +613,8 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
 }
 
-template <bool kTwo>
 int set_tree8_smem() {
-    B2A_CUDA_OK(cudaFuncSetAttribute(tree8_attention<kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(tree8_smem_bytes<kTwo>())));
+    B2A_CUDA_OK(cudaFuncSetAttribute(tree8_attention, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTree8SmemBytes)));
     return B2A_OK;
 }
 
@@ -684,8 +657,7 @@ int b2a_tree8_fwd(const b2a_tree_args* a, const b2a_cache_scales* scales, void* 
     CUtensorMap map_k, map_v;
     rc = make_slot_map8(&map_k, p.c.cache, true, p.box_rows);
     if (rc == B2A_OK) rc = make_slot_map8(&map_v, p.c.cache, false, p.box_rows);
-    if (rc == B2A_OK && t.tiles == 2) rc = once_per_device(dev.device, 15, set_tree8_smem<true>);
-    if (rc == B2A_OK && t.tiles == 1 && !t.few) rc = once_per_device(dev.device, 16, set_tree8_smem<false>);
+    if (rc == B2A_OK && t.tiles == 2) rc = once_per_device(dev.device, 15, set_tree8_smem);
     if (rc != B2A_OK) return rc;
 
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -705,9 +677,13 @@ int b2a_tree8_fwd(const b2a_tree_args* a, const b2a_cache_scales* scales, void* 
 
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     if (t.few) return launch_tree8_few(map_k, map_v, p8, t.ctas, dev, stream);
-    auto attention = t.tiles == 2 ? tree8_attention<true> : tree8_attention<false>;
-    const size_t smem = t.tiles == 2 ? tree8_smem_bytes<true>() : tree8_smem_bytes<false>();
-    B2A_CUDA_OK(launch_early(attention, t.ctas, kTree8Threads, smem, stream, map_k, map_v, p8));
+    if (t.tiles == 1) {
+        rc = launch_tree8_one(map_k, map_v, p8, t.ctas, dev, stream);
+        if (rc != B2A_OK) return rc;
+    } else {
+        auto attention = tree8_attention;
+        B2A_CUDA_OK(launch_early(attention, t.ctas, kTree8Threads, kTree8SmemBytes, stream, map_k, map_v, p8));
+    }
     if (t.ctas == 1) return B2A_OK;
     TreeParams parts = p;
     parts.scale_log2 = 1.f;      // the pieces' references are in log2 units already

@@ -225,29 +225,7 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (__any_sync(0xFFFFFFFFu, loader.bad) && lane == 0) set_status(wctx.status_word(), kStatusBadArg, 0x3Fu << 12);
         PH_PRINT("few8 load", 3);
     } else if (warp == kFew8VWarp) {
-        // ---------------------------------------------------------------- loads of V
-        SlotLoader loader(p.box_rows);
-        uint32_t v_it = 0;
-        bool ok = true;
-        for (uint32_t it = 0; ok; ++it) {
-            const uint32_t at = it % kFew8Slots;
-            ok = warp_wait8(wctx, smem_u32(&sh.piece_full[at]), (it / kFew8Slots) & 1u, 4);
-            if (!ok) break;
-            const TreePiece w = sh.piece[at];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.piece_empty[at]));
-            if (!w.valid) break;
-            loader.look_up(p.c.cache, w.seq, w.j0, w.slots, lane);
-            for (int i = 0; i < w.blocks; ++i, ++v_it) {
-                SlotLoader now = loader;
-                if (i + 1 < w.blocks) loader.look_up(p.c.cache, w.seq, w.j0 + i + 1, w.slots, lane);
-                const int boxes = now.count(w.j0 + i, w.slots);
-                const uint32_t stage = v_it % Shared::kV;
-                ok = warp_wait8(wctx, smem_u32(&sh.v_empty[stage]), ((v_it / Shared::kV) & 1u) ^ 1u, 18);
-                if (!ok) break;
-                load_slots8(now, &map_v, smem_u32(&sh.v[stage][0]), smem_u32(&sh.v_full[stage]), w.head, boxes, lane);
-            }
-        }
+        tree8_load_v<kFew8Slots, Shared::kV>(p, sh, &map_v, wctx, lane);
     } else if (warp >= kFew8ConvertWarp) {
         // ---------------------------------------------------------------- Q in two parts, and then V to f16
         const int mine = warp - kFew8ConvertWarp;
