@@ -1,14 +1,20 @@
 // New keys and values into a cache in 8 bits, turned by their positions on the way.
 //
-// All slots of a block share a head's scale, so a block's new tokens belong to one group of threads: 128 of a CTA for K, 128 for V, eight
-// threads a token with 16 dimensions each, as in b2a_rotary.cu.  They turn the values in fp32, look for the largest, find the
-// scale, and round.  e4m3 is a floating-point format, so a scale that is a power of two costs no accuracy (values keep
-// their four bits down to 2^-15 of the largest), divides exactly, and can grow with hardly a trace: x / 2 is a number of the
-// format as well, unless it is one of the smallest.  So a block whose tokens come one by one keeps its scale until a
-// token does not fit, and then the tokens that it holds are read, divided and written again, at most 127 of 128 bytes.
+// All slots of a block share a head's scale, so a block's new keys (or values) of a head belong to one warp: eight lanes a token with 16
+// dimensions each, as in b2a_rotary.cuh, and 16 tokens on their way at once, by asynchronous copies.  It turns them in fp32, looks for
+// the largest, finds the scale, turns them once more and rounds; nothing waits for another warp.  Blocks of more new tokens than 16
+// are read twice, the second time from L2.  e4m3 is a floating-point format, so a scale that is a power of two costs no accuracy
+// (values keep their four bits down to 2^-15 of the largest), divides exactly, and can grow with hardly a trace: x / 2 is a number
+// of the format as well, unless it is one of the smallest.  So a block whose tokens come one by one keeps its scale until a token does
+// not fit, and then the tokens that it holds are read, divided and written again, at most 127 of 128 bytes.
 //
-// Bound by memory: 256 bytes in and 128 out a token and head.  The CTAs of K and V come first, a block of slots and some of the heads
-// each; those behind them turn q.
+// Should be bound by memory: 256 bytes in and 128 out a token and head, and q's 256 and 256.  A CTA has a block of slots and some of the
+// heads, for which it computes the angles once; CTAs behind those turn q, and the first one looks for places that do not exist.
+// One new token of 16 sequences, 32 + 8 heads, is 4.8 us, what a launch with four reads one after another takes.  715 of 32
+// sequences: 11.8 us.  5,647 of 4: 139 MB in 34 us, of which q alone is 20 and k and v alone 21: each keeps the SMs' issue slots
+// half busy (9.3 and 9.6 million instructions, most of them of the turning, which k needs twice).  That was 58 us with a piece of
+// code for each of the two passes and four tokens, and a division where a product does: an instruction fetched for one use costs
+// more than its work.  64 registers and four CTAs an SM: with three 39 us for 35.6, with five 37.6.
 #include "b2a_cache8.cuh"
 #include "b2a_rotary.cuh"
 
@@ -24,6 +30,7 @@ struct Append8Params {
     int parts;                   // of them
     int part_heads;
     int seq_blocks;              // most blocks of a sequence
+    int stages;                  // of shared memory a warp: 1 where it has one unit of one tile
 };
 
 // A block of slots that new tokens fall into.
@@ -99,195 +106,261 @@ __device__ __forceinline__ float scale_for(float most) {
     return __int_as_float(min(max(e, 127 - 64), 127 + 64) << 23);
 }
 
-// Values divided by a scale: a power of two has an exact reciprocal.
+// Values divided by a scale: a power of two has an exact reciprocal, others are divided.
 struct Divider {
     float scale, inverse;
     __device__ __forceinline__ explicit Divider(float s) {
         scale = s;
         inverse = (__float_as_int(s) & 0x7FFFFF) == 0 ? 1.f / s : 0.f;
     }
-    __device__ __forceinline__ float operator()(float x) const { return inverse != 0.f ? x * inverse : x / scale; }
+    template <int N>
+    __device__ __forceinline__ void operator()(float (&x)[N]) const {
+        if (inverse != 0.f) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] *= inverse;
+        } else {
+            slowly<N>(x);
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void slowly(float (&x)[N]) const {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = divided(x[e], scale);
+    }
+    static __device__ __noinline__ float divided(float x, float by) { return x / by; }
 };
 
-// Eight values in e4m3; those that are not finite as NaN.
-__device__ __forceinline__ uint2 pack8(const float* x, const Divider& by) {
-    uint32_t two[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = by(x[2 * i]), b = by(x[2 * i + 1]);
-        two[i] = pack_e4m3x2(fabsf(x[2 * i]) < INFINITY ? a : NAN, fabsf(x[2 * i + 1]) < INFINITY ? b : NAN);
-    }
-    return make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+__device__ __forceinline__ __nv_bfloat162 as_bf16x2(uint32_t two) { return *reinterpret_cast<const __nv_bfloat162*>(&two); }
+
+__device__ __forceinline__ void turn_pair(float& a, float& b, float cos, float sin) {
+    const float x = a;
+    a = x * cos - b * sin;
+    b = b * cos + x * sin;
 }
 
-// kTiles: of 16 tokens, as many as a block may get.
-template <int kTiles>
-__global__ void __launch_bounds__(kRotaryThreads, kTiles <= 2 ? 4 : 2)
+constexpr int kQTokens = 4;     // a CTA that turns q: 1, 2, 4, 8 take 43.4, 43.9, 35.7, 36.6 us for 5,647, all the same 6.2 for 16
+constexpr int kTile8 = 16;      // tokens on their way to a warp at once
+constexpr int kStage8Bytes = kTile8 * kHeadDim * static_cast<int>(sizeof(__nv_bfloat16));
+
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Dynamic shared memory: one or two stages of kTile8 tokens for each warp, then the angles of the block's new tokens, 64 each.
+__global__ void __launch_bounds__(kRotaryThreads, 4)
 append8_tokens(const __grid_constant__ Append8Params p8) {
-    extern __shared__ __align__(16) float2 cos_sin[];      // [kTiles * 16][64]
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Append8Block block;
-    __shared__ float most_of[2][2][4];                     // turn, K or V, warp
     const RotaryParams& p = p8.r;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kWarps = kRotaryThreads / 32;
+    float2* cos_sin = reinterpret_cast<float2*>(smem + kWarps * p8.stages * kStage8Bytes);
     let_next_kernel_start();
     wait_for_previous_kernel();
 
-    if (blockIdx.x >= p8.kv_ctas) {
-        turn_tokens<false, 1>(p, blockIdx.x - p8.kv_ctas);
+    if (blockIdx.x == 0) {
+        check_append(p);
+    } else if (blockIdx.x > p8.kv_ctas) {
+        turn_tokens<false, kQTokens>(p, blockIdx.x - 1 - p8.kv_ctas);
     } else {
+        const int item = blockIdx.x - 1;
         if (warp == 0) {
-            const Append8Block at = append8_block(p, p8.scales, blockIdx.x / p8.parts, p8.seq_blocks, lane);
+            const Append8Block at = append8_block(p, p8.scales, item / p8.parts, p8.seq_blocks, lane);
             if (lane == 0) block = at;
         }
         __syncthreads();
         const Append8Block at = block;
+        const int h0 = (item % p8.parts) * p8.part_heads, units = at.count > 0 ? 2 * min(p8.part_heads, p8.heads - h0) : 0;
+        const int c = lane & 7, mine = lane >> 3;
+
+        // A unit: K (even) or V of a head.  A thread's 16 dimensions, as in turn_tokens: of V, and behind the pairs, 16 in a row.
+        const bool turned = !p.adjacent && c * 8 < p.pairs;
+        auto lo_of = [&](int which) { return which == 0 && p.pairs > 0 && (p.adjacent || turned) ? 8 * c : 16 * c; };
+        auto hi_of = [&](int which) {
+            return which == 0 && p.pairs > 0 && p.adjacent ? 64 + 8 * c : which == 0 && turned ? p.pairs + 8 * c : 16 * c + 8;
+        };
+        // A unit's tiles are loaded from the first to the last, for the largest value, and back, to be written: the last one, and so
+        // the only one of few tokens, once.  A thread reads back what it copied itself.
+        const int tiles = (at.count + kTile8 - 1) / kTile8, trips = 2 * tiles - 1;
+        const uint32_t stage0 = smem_u32(smem) + warp * p8.stages * kStage8Bytes + mine * 256 + c * 16;
+        auto load = [&](int unit, int trip, int stage) {
+            const int which = unit & 1, lo = lo_of(which), hi = hi_of(which);
+            const int token0 = (trip < tiles ? trip : 2 * tiles - 2 - trip) * kTile8;
+            const long long* stride = p.stride[1 + which];
+            const __nv_bfloat16* src = p.src[1 + which] + (h0 + (unit >> 1)) * stride[2] +
+                                       (p.cu_seqlens == nullptr ? at.seq * stride[0] + at.token * stride[1]
+                                                                : (static_cast<long long>(at.q_begin) + at.token) * stride[1]);
+#pragma unroll
+            for (int t = 0; t < kTile8 / 4; ++t) {
+                const int token = token0 + t * 4 + mine;
+                const __nv_bfloat16* from = src + (token < at.count ? token : 0) * stride[1];
+                const uint32_t to = stage0 + stage * kStage8Bytes + t * 1024;
+                copy16_or_zero(to, from + lo, token < at.count);
+                copy16_or_zero(to + 128, from + hi, token < at.count);
+            }
+        };
+        int unit = warp, trip = 0, stage = 0;
+        if (unit < units) load(unit, 0, 0);        // on their way while the angles are computed
+        asm volatile("cp.async.commit_group;" ::: "memory");
         if (p.pairs > 0) {
-            for (int i = threadIdx.x; i < at.count * 64; i += kRotaryThreads) {
-                const int pair = i & 63, number = at.token + (i >> 6);
+            // A thread's pair stays the same, for which it looks once: lanes that read different constants wait for one another.
+            const int pair = threadIdx.x & 63;
+            if (pair < p.pairs) {
+                const int axis = p.axis[pair];
+                const unsigned long long turn = p.turn[pair];
                 // Packed tokens are one sequence to the positions.
-                if (pair < p.pairs) {
-                    cos_sin[i] = p.cu_seqlens == nullptr ? pair_angle(p, pair, at.seq, number) : pair_angle(p, pair, 0, at.q_begin + number);
-                }
-            }
-        }
-        __syncthreads();
-
-        // A thread's 16 dimensions, as in turn_tokens: of V, and behind the pairs, 16 in a row.
-        const int which = warp >> 2, c = lane & 7, mine = (threadIdx.x & 127) >> 3;
-        const int pairs = which == 0 ? p.pairs : 0;
-        const bool adjacent = which == 0 && p.adjacent && pairs > 0, turned = !adjacent && c * 8 < pairs;
-        const int lo = adjacent || turned ? 8 * c : 16 * c;
-        const int hi = adjacent ? 64 + 8 * c : turned ? pairs + 8 * c : 16 * c + 8;
-        const int h0 = (blockIdx.x % p8.parts) * p8.part_heads, h1 = min(h0 + p8.part_heads, p8.heads);
-        const long long* stride = p.stride[1 + which];
-        const __nv_bfloat16* src = p.src[1 + which] + (p.cu_seqlens == nullptr ? at.seq * stride[0] + at.token * stride[1]
-                                                                               : (static_cast<long long>(at.q_begin) + at.token) * stride[1]);
-        const long long* to_stride = which == 0 ? p.cache.k_stride : p.cache.v_stride;
-        uint8_t* dst = reinterpret_cast<uint8_t*>(which == 0 ? p.cache.k : p.cache.v);
-        float* scales = which == 0 ? p8.scales.k : p8.scales.v;
-        if (at.count > 0) {
-            dst += at.page * to_stride[0] + at.row * to_stride[1];
-            scales += p8.scales.at(which == 0 ? p8.scales.k_stride : p8.scales.v_stride, at.page, at.row, 0);
-        }
-        const long long scale_step = which == 0 ? p8.scales.k_stride[2] : p8.scales.v_stride[2];
-
-        uint4 a[kTiles], b[kTiles];
-        auto load = [&](int h) {
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                a[t] = b[t] = make_uint4(0u, 0u, 0u, 0u);
-                if (t * 16 + mine < at.count) {
-                    const __nv_bfloat16* from = src + (t * 16 + mine) * stride[1] + h * stride[2];
-                    a[t] = *reinterpret_cast<const uint4*>(from + lo);
-                    b[t] = *reinterpret_cast<const uint4*>(from + hi);
-                }
-            }
-        };
-        // The values of a token, in the order of lo and hi.
-        auto values = [&](int t, float (&x)[16]) {
-            const uint32_t u[4] = {a[t].x, a[t].y, a[t].z, a[t].w}, w[4] = {b[t].x, b[t].y, b[t].z, b[t].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = bf16x2_to_float2(u[e]), g = bf16x2_to_float2(w[e]);
-                x[2 * e] = f.x;
-                x[2 * e + 1] = f.y;
-                x[8 + 2 * e] = g.x;
-                x[9 + 2 * e] = g.y;
-            }
-            const float2* cs = cos_sin + (t * 16 + mine) * 64;
-            if (t * 16 + mine >= at.count) return;
-            if (adjacent) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int pair = e < 4 ? 4 * c + e : 28 + 4 * c + e;
-                    if (pair >= pairs) continue;
-                    const float2 t2 = cs[pair];
-                    const float x0 = x[2 * e], x1 = x[2 * e + 1];
-                    x[2 * e] = x0 * t2.x - x1 * t2.y;
-                    x[2 * e + 1] = x1 * t2.x + x0 * t2.y;
-                }
-            } else if (turned) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 t2 = cs[8 * c + e];
-                    const float x0 = x[e], x1 = x[8 + e];
-                    x[e] = x0 * t2.x - x1 * t2.y;
-                    x[8 + e] = x1 * t2.x + x0 * t2.y;
-                }
-            }
-        };
-        if (h0 < h1) load(h0);
+                const int seq = p.cu_seqlens == nullptr ? at.seq : 0, first = p.cu_seqlens == nullptr ? at.token : at.q_begin + at.token;
+                // The eight pairs of a thread of a token as four pieces of 16 bytes, and those of eight threads in a row.
+                const int of = p.adjacent ? pair >> 2 & 7 : pair >> 3, e = p.adjacent ? (pair & 3) + (pair >> 5) * 4 : pair & 7;
+                float2* const to = cos_sin + (e >> 1) * 16 + of * 2 + (e & 1);
+                int token = threadIdx.x >> 6;
+                long long position = token < at.count ? position_of(p, axis, seq, first + token) : 0;
 #pragma unroll 1
-        for (int h = h0; h < h1 && at.count > 0; ++h) {
-            const float before = at.held > 0 ? scales[h * scale_step] : 0.f;
-            float most = 0.f;
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                float x[16];
-                values(t, x);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
-            }
-            most = __int_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_int(most)));      // not negative: ordered as integers
-            if (lane == 0) most_of[h & 1][which][warp & 3] = most;
-            named_barrier_sync(1 + which, 128);
-            const float* parts = most_of[h & 1][which];
-            most = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
-            const bool keep = at.held > 0 && most <= 448.f * before;
-            const float scale = keep ? before : scale_for(most);
-            const Divider by(scale);
-            uint8_t* rows = dst + h * to_stride[2];
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                const int token = t * 16 + mine;
-                if (token >= at.count) continue;
-                float x[16];
-                values(t, x);
-                uint8_t* row = rows + (at.held + token) * to_stride[1];
-                const uint2 first = pack8(x, by), second = pack8(x + 8, by);
-                if (hi == lo + 8) {
-                    *reinterpret_cast<uint4*>(row + lo) = make_uint4(first.x, first.y, second.x, second.y);
-                } else {
-                    *reinterpret_cast<uint2*>(row + lo) = first;
-                    *reinterpret_cast<uint2*>(row + hi) = second;
+                while (token < at.count) {
+                    const int next = token + kRotaryThreads / 64;
+                    const long long next_position = next < at.count ? position_of(p, axis, seq, first + next) : 0;
+                    to[token * 64] = angle_of(p, turn, position);
+                    token = next;
+                    position = next_position;
                 }
             }
-            if (h + 1 < h1) load(h + 1);
-            if (!keep) {
+            __syncthreads();
+        }
+        float most = 0.f, before = 0.f, scale = 0.f;
+        bool infinite = false;          // this thread has seen an infinity in the unit
+#pragma unroll 1
+        while (unit < units) {
+            const int next_unit = trip + 1 < trips ? unit : unit + kWarps, next_trip = trip + 1 < trips ? trip + 1 : 0;
+            if (next_unit < units) load(next_unit, next_trip, stage ^ 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+
+            const int which = unit & 1, head = h0 + (unit >> 1);
+            const int lo = lo_of(which), hi = hi_of(which), token0 = (trip < tiles ? trip : 2 * tiles - 2 - trip) * kTile8;
+            const int steps = (min(at.count - token0, kTile8) + 3) / 4;
+            const long long token_stride = (which == 0 ? p.cache.k_stride : p.cache.v_stride)[1];
+            uint8_t* rows = reinterpret_cast<uint8_t*>(which == 0 ? p.cache.k : p.cache.v) +
+                            p.cache.at(which == 0 ? p.cache.k_stride : p.cache.v_stride, at.page, at.row, head);
+            float* scale_at = (which == 0 ? p8.scales.k : p8.scales.v) +
+                              p8.scales.at(which == 0 ? p8.scales.k_stride : p8.scales.v_stride, at.page, at.row, head);
+            if (trip == 0) {
+                most = 0.f;
+                infinite = false;
+                before = at.held > 0 ? *scale_at : 0.f;
+            }
+            // The first half of the steps looks for the largest, the second one writes: one piece of code, which is what a short
+            // kernel's time goes to.
+#pragma unroll 1
+            for (int i = trip < tiles ? 0 : steps; i < (trip < tiles - 1 ? steps : 2 * steps); ++i) {
+                const bool writes = i >= steps;
+                const int t = writes ? i - steps : i, token = token0 + t * 4 + mine;
+                if (i == steps && trip == tiles - 1) {
+                    most = __int_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_int(most)));      // not negative: ordered as integers
+                    scale = at.held > 0 && most <= 448.f * before ? before : scale_for(most);
+                }
+                const uint32_t from = stage0 + stage * kStage8Bytes + t * 1024;
+                const uint4 a = ld_shared_v4(from), b = ld_shared_v4(from + 128);
+                const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                if (!writes && which == 1) {
+                    // The largest of V's as they come, two at a time.
+                    __nv_bfloat162 two = __habs2(as_bf16x2(u[0]));
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) two = __hmax2(two, __habs2(as_bf16x2(u[e])));
+                    const float top = fmaxf(__low2float(two), __high2float(two));
+                    if (top < INFINITY) {
+                        most = fmaxf(most, top);
+                        continue;
+                    }
+                }
+                float x[16];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = bf16x2_to_float2(u[e]);
+                    x[2 * e] = f.x;
+                    x[2 * e + 1] = f.y;
+                }
+                if (which == 0 && token < at.count) {
+                    const float4* cs = reinterpret_cast<const float4*>(cos_sin + token * 64) + c;
+                    if (p.adjacent) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            if ((e < 4 ? 4 * c + e : 28 + 4 * c + e) >= p.pairs) continue;
+                            const float4 two = cs[4 * e];
+                            turn_pair(x[2 * e], x[2 * e + 1], two.x, two.y);
+                            turn_pair(x[2 * e + 2], x[2 * e + 3], two.z, two.w);
+                        }
+                    } else if (turned) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float4 two = cs[4 * e];
+                            turn_pair(x[e], x[8 + e], two.x, two.y);
+                            turn_pair(x[e + 1], x[9 + e], two.z, two.w);
+                        }
+                    }
+                }
+                // Those that are not finite have no say, and are written as NaN.  fmaxf passes NaN over by itself.
+                if (!writes) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+                    if (top == INFINITY) {
+                        infinite = true;
+                        top = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+                    }
+                    most = fmaxf(most, top);
+                } else if (token < at.count) {
+                    uint32_t out[4];
+                    if (infinite) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = fabsf(x[e]) < INFINITY ? x[e] : NAN;
+                    }
+                    Divider by(scale);
+                    by(x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        out[e] = pack_e4m3x2(x[4 * e], x[4 * e + 1]) | pack_e4m3x2(x[4 * e + 2], x[4 * e + 3]) << 16;
+                    }
+                    uint8_t* row = rows + (at.held + token) * token_stride;
+                    if (hi == lo + 8) {
+                        *reinterpret_cast<uint4*>(row + lo) = make_uint4(out[0], out[1], out[2], out[3]);
+                    } else {
+                        *reinterpret_cast<uint2*>(row + lo) = make_uint2(out[0], out[1]);
+                        *reinterpret_cast<uint2*>(row + hi) = make_uint2(out[2], out[3]);
+                    }
+                }
+            }
+            if (next_trip == 0 && (at.held == 0 || scale != before)) {
                 // Tokens that the block held.
-                const Divider again(scale / before);
-                for (int token = mine; token < at.held; token += 16) {
-                    uint4* row = reinterpret_cast<uint4*>(rows + token * to_stride[1] + c * 16);
+                Divider again(scale / before);
+#pragma unroll 1
+                for (int token = mine; token < at.held; token += 4) {
+                    uint4* row = reinterpret_cast<uint4*>(rows + token * token_stride + c * 16);
                     const uint4 v = *row;
                     const uint32_t words[4] = {v.x, v.y, v.z, v.w};
                     uint32_t out[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 f = e4m3x2_to_float2(words[e] & 0xFFFFu), g = e4m3x2_to_float2(words[e] >> 16);
-                        out[e] = pack_e4m3x2(again(f.x), again(f.y)) | pack_e4m3x2(again(g.x), again(g.y)) << 16;
+                        float x[4] = {f.x, f.y, g.x, g.y};
+                        again(x);
+                        out[e] = pack_e4m3x2(x[0], x[1]) | pack_e4m3x2(x[2], x[3]) << 16;
                     }
                     *row = make_uint4(out[0], out[1], out[2], out[3]);
                 }
-                if ((threadIdx.x & 127) == 0) scales[h * scale_step] = scale;
+                if (lane == 0) *scale_at = scale;
             }
+            unit = next_unit;
+            trip = next_trip;
+            stage ^= 1;
         }
     }
-    if (blockIdx.x == 0) check_append(p);
 }
 
-template <int kTiles>
 int set_append8_smem() {
-    B2A_CUDA_OK(cudaFuncSetAttribute(append8_tokens<kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTiles * 16 * 64 * static_cast<int>(sizeof(float2))));
-    return B2A_OK;
-}
-
-template <int kTiles>
-int launch_append8(const Append8Params& p, int ctas, const DeviceInfo& dev, int slot, cudaStream_t stream) {
-    const int rc = once_per_device(dev.device, slot, set_append8_smem<kTiles>);
-    if (rc != B2A_OK) return rc;
-    auto kernel = append8_tokens<kTiles>;
-    const size_t smem = p.r.pairs > 0 ? kTiles * 16 * 64 * sizeof(float2) : 0;
-    B2A_CUDA_OK(launch_early(kernel, ctas, kRotaryThreads, smem, stream, p));
+    const int most = kRotaryThreads / 32 * 2 * kStage8Bytes + 128 * 64 * static_cast<int>(sizeof(float2));
+    B2A_CUDA_OK(cudaFuncSetAttribute(append8_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     return B2A_OK;
 }
 
@@ -310,25 +383,29 @@ int b2a_cache8_append(const b2a_append_args* a, const b2a_cache_scales* scales, 
     // n tokens that begin anywhere in a block touch this many.
     const int slots = scales->block;
     auto blocks = [&](long long n) { return (n + slots - 2) / slots + 1; };
-    const long long items = a->cu_seqlens == nullptr ? blocks(a->seqlen) * a->batch
-                                                     : std::min<long long>(a->total, static_cast<long long>(a->total) / slots + 2ll * a->batch);
-    // Heads go over to CTAs of their own until the GPU has enough.
+    const long long items = a->cu_seqlens == nullptr
+                                ? blocks(a->seqlen) * a->batch
+                                : std::min<long long>(a->total, static_cast<long long>(a->total) / slots + 2ll * a->batch);
+    // Heads go over to CTAs of their own, four at least, which is a unit a warp, until the GPU has enough: 357 blocks of 8 heads as
+    // 714 CTAs 35.6 us, as 357 36.7.
     const int heads = a->cache.heads_k;
-    p.parts = static_cast<int>(std::min<long long>(heads, std::max<long long>(1, 4ll * dev.sm_count / items)));
+    p.parts = static_cast<int>(std::min<long long>((heads + 3) / 4, std::max<long long>(1, 6ll * dev.sm_count / items)));
     p.part_heads = (heads + p.parts - 1) / p.parts;
     p.parts = (heads + p.part_heads - 1) / p.part_heads;
     p.seq_blocks = a->cu_seqlens == nullptr ? static_cast<int>(blocks(a->seqlen)) : 0;
-    const int q_ctas = a->q != nullptr ? a->total : 0;
-    B2A_REQUIRE(items * p.parts + q_ctas <= INT32_MAX, "too many tokens for a call");
+    const int q_ctas = a->q != nullptr ? (a->total - 1) / kQTokens + 1 : 0;
+    B2A_REQUIRE(items * p.parts + q_ctas < INT32_MAX, "too many tokens for a call");
     p.kv_ctas = static_cast<int>(items * p.parts);
     p.heads = heads;
     p.r.heads[1] = p.r.heads[2] = 0;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const int most = std::min<int>(slots, a->cu_seqlens == nullptr ? a->seqlen : a->total), ctas = p.kv_ctas + q_ctas;
-    if (most <= 16) return launch_append8<1>(p, ctas, dev, 17, stream);
-    if (most <= 32) return launch_append8<2>(p, ctas, dev, 18, stream);
-    if (most <= 64) return launch_append8<4>(p, ctas, dev, 19, stream);
-    return launch_append8<8>(p, ctas, dev, 20, stream);
+    rc = once_per_device(dev.device, 17, set_append8_smem);
+    if (rc != B2A_OK) return rc;
+    const int most = std::min<int>(slots, a->cu_seqlens == nullptr ? a->seqlen : a->total);
+    p.stages = most <= kTile8 && 2 * p.part_heads <= kRotaryThreads / 32 ? 1 : 2;
+    const size_t smem = kRotaryThreads / 32 * p.stages * kStage8Bytes + (p.r.pairs > 0 ? most * 64 * sizeof(float2) : 0);
+    B2A_CUDA_OK(launch_early(append8_tokens, 1 + p.kv_ctas + q_ctas, kRotaryThreads, smem, stream, p));
+    return B2A_OK;
 }
 
 }  // extern "C"

@@ -71,14 +71,21 @@ __device__ __forceinline__ float2 bf16x2_to_float2(uint32_t x) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
 }
 
+__device__ __forceinline__ long long position_of(const RotaryParams& p, int axis, int seq, int number) {
+    const long long at = axis * p.positions_stride[0] + seq * p.positions_stride[1] + number * p.positions_stride[2];
+    return p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+}
+
 // Cosine and sine of a pair's angle, times the magnitude.
-__device__ __forceinline__ float2 pair_angle(const RotaryParams& p, int pair, int seq, int number) {
-    const long long at = p.axis[pair] * p.positions_stride[0] + seq * p.positions_stride[1] + number * p.positions_stride[2];
-    const long long pos = p.positions_64 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
-    const unsigned long long turns = static_cast<unsigned long long>(pos) * p.turn[pair];
+__device__ __forceinline__ float2 angle_of(const RotaryParams& p, unsigned long long turn, long long position) {
+    const unsigned long long turns = static_cast<unsigned long long>(position) * turn;
     float s, c;
     sincospif(static_cast<float>(static_cast<int>(turns >> 32)) * 4.656612873077393e-10f, &s, &c);   // 2^-31
     return make_float2(c * p.magnitude, s * p.sign * p.magnitude);
+}
+
+__device__ __forceinline__ float2 pair_angle(const RotaryParams& p, int pair, int seq, int number) {
+    return angle_of(p, p.turn[pair], position_of(p, p.axis[pair], seq, number));
 }
 
 // Every sequence's new slots and pages exist?  CTA 0 of a cache write finds out and writes the whole header, so that no
