@@ -586,18 +586,27 @@ tree_combine_few(const __grid_constant__ TreeParams p) {
         const int second = i == 0 && cut.first > static_cast<long long>(cta - 1) * cut.run;
         return (2ll * (cta - 1 + i) + second) * p.part_rows + row;
     };
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) m = fmaxf(m, p.part_stat[part_of(i)].x);
+    // A lane a piece for the references and sums, 32 at a time, so that a long item's pieces cost one latency and not one each (one
+    // token of a sequence of 131,072 slots, 19 pieces an item: 13.3 us before, 9.9 after); added up one by one, in their order.
+    auto stat_of = [&](int i) { return i < pieces ? p.part_stat[part_of(i)] : make_float2(-INFINITY, 0.f); };
+    const float2 first = stat_of(lane);
+    float m = first.x;
+    for (int i = 32 + lane; i < pieces; i += 32) m = fmaxf(m, p.part_stat[part_of(i)].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-        const float2 st = p.part_stat[part_of(i)];
-        const float4 v = p.part_o[part_of(i) * 32 + lane];
-        const float f = st.x == m ? 1.f : fast_exp2(st.x - m);
-        l = fmaf(st.y, f, l);
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+        const float2 st = i0 == 0 ? first : stat_of(i0 + lane);
+        const float weight = st.x == m ? 1.f : fast_exp2(st.x - m);
+        const int here = min(32, pieces - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float4 v = p.part_o[part_of(i0 + i) * 32 + lane];
+            const float f = __shfl_sync(0xFFFFFFFFu, weight, i);
+            l = fmaf(__shfl_sync(0xFFFFFFFFu, st.y, i), f, l);
+            o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int token = row / p.c.group, head = cut.head * p.c.group + row - token * p.c.group;
