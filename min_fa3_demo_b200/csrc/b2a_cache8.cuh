@@ -61,7 +61,8 @@ inline int make_slot_map8(CUtensorMap* map, const CacheView& c, bool keys, int b
 }
 
 // As SlotLoader::load, rows of 128 bytes.
-__device__ __forceinline__ void load_slots8(const SlotLoader& at, const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int n, int lane) {
+__device__ __forceinline__ void load_slots8(const SlotLoader& at, const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int n,
+                                            int lane) {
     if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n << at.shift) * 128u);
     __syncwarp();
     if (lane < n) tma_load_4d(dst + static_cast<uint32_t>(lane << at.shift) * 128u, map, bar, 0, head, at.row, at.page);
@@ -127,8 +128,8 @@ struct ScaleRing {
             const bool there = block * kSlotBlock + group * 16 < slots && static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
             const float* from = keys ? s.k : s.v;
             if (there) from += s.at(keys ? s.k_stride : s.v_stride, page, row, head);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&scale[slot][keys ? 0 : 1][group])), "l"(from), "r"(there ? 4 : 0)
-                         : "memory");
+            const uint32_t to = smem_u32(&scale[slot][keys ? 0 : 1][group]);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
         __syncwarp();
@@ -153,7 +154,9 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
 }
 
 __device__ __forceinline__ void e4m3x4_to_half4(uint32_t four, uint32_t& lo, uint32_t& hi) {
-    asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, u;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+    asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, u;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
 }
 
 __device__ __forceinline__ float2 half2_to_float2(uint32_t h) {
@@ -352,8 +355,9 @@ static __device__ __noinline__ bool tree8_clean_row(uint8_t* row, int r, bool be
     return any != 0u;
 }
 
-// V's tiles from e4m3 to f16 by kWarps warps, r being the thread's number among them, a row at a time.  What a product must not see is left out on the way: rows behind the last
-// slot, and of drafted tokens NaN, since 0 * NaN is NaN (e4m3 has no infinities); that there was one is noted for the piece.
+// V's tiles from e4m3 to f16 by kWarps warps, r being the thread's number among them, a row at a time.  What a product must not see
+// is left out on the way: rows behind the last slot, and of drafted tokens NaN, since 0 * NaN is NaN (e4m3 has no infinities); that
+// there was one is noted for the piece.
 // begin(piece, number): what there is to do before a piece's blocks.
 template <int kWarps, int kSlots, int kStages, int kTiles, typename Shared, typename Begin>
 __device__ __forceinline__ void tree8_convert_v(const TreeParams& p, Shared& sh, const WaitCtx& wctx, int r, Begin begin) {
@@ -388,7 +392,8 @@ __device__ __forceinline__ void tree8_convert_v(const TreeParams& p, Shared& sh,
                 }
                 // 16 values: chunks 2 c and 2 c + 1 of 8, which lie in a half of 64 columns.  Rows begin at multiples of 128 bytes, so chunks
                 // are exchanged by an exclusive or of the address.
-                const uint32_t from = smem_u32(&sh.v[stage][row * 128]) + (row & 7) * 16, to = smem_u32(&sh.v16[tile][row * 128]) + (row & 7) * 16;
+                const uint32_t from = smem_u32(&sh.v[stage][row * 128]) + (row & 7) * 16;
+                const uint32_t to = smem_u32(&sh.v16[tile][row * 128]) + (row & 7) * 16;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
 #pragma unroll

@@ -6,6 +6,10 @@
 // items have one tile.)  Q is turned into its two parts by the softmax warps, two rows a warp at a time, when a piece begins; a row's scale
 // and K's meet in the factor of a score.
 //
+// Bound by what an SM does for a score rather than by memory: two products of K, one of V in f16, an exponential, and the sum with V's
+// scale.  8 sequences of 64 drafted tokens, 64 heads over 8, up to 16,000 slots: 222 us, 735 TFLOP/s; two chunks of 1,000 tokens, 32 heads
+// over 8, behind up to 8,000: 336 us, 721 TFLOP/s.
+//
 //   warp 0-3, 4-7   Q in two parts, then softmax, one thread a row
 //   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of K, V and scales       warp 11   V to f16
 #include "b2a_cache8.cuh"
@@ -304,7 +308,8 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int row = from + 2 * e + second;
-                        split_q_rows(v[e], row < r1, row, lane, &sh.q[tile][0][0], &sh.q[tile][1][0], &sh.q_scale[tile][row & (kTileM - 1)]);
+                        split_q_rows(v[e], row < r1, row, lane, &sh.q[tile][0][0], &sh.q[tile][1][0],
+                                     &sh.q_scale[tile][row & (kTileM - 1)]);
                     }
                 }
                 fence_proxy_async_smem();
@@ -652,7 +657,9 @@ int b2a_tree8_fwd(const b2a_tree_args* a, const b2a_cache_scales* scales, void* 
     }
     p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
     p.c.min_run = 2;
-    p.c.item_extra = t.few ? 4 : 6;
+    // What an item costs besides its blocks, in blocks, for the cuts between CTAs.  4 and 6, 16 sequences of a token over up to 8,001
+    // slots: 44.8, 44.5 us; 6 and 9, of up to 32 tokens with one tile: 80.3, 82.9, of 64 with two, 8 sequences of up to 16,000: 222.9, 220.2.
+    p.c.item_extra = t.tiles == 2 ? 9 : 6;
     p.box_rows = slot_box_rows(p.c.cache);
     CUtensorMap map_k, map_v;
     rc = make_slot_map8(&map_k, p.c.cache, true, p.box_rows);

@@ -6,12 +6,16 @@
 //
 // A step is two blocks, 256 slots: K of 32 KiB, as much as a block of a bf16 cache, so that the warps that load and multiply do as
 // little for a byte as there.  A thread has two slots, and so two scales of K and two of V.  The products have at least 16
-// columns, but only as many as there are rows go through the softmax: 4, 8, 16, or, in steps of one block, 32.
+// columns, but only as many as there may be rows go through the softmax: 8, 16, or, in steps of one block, 32.
 //
 // Softmax across threads, as in b2a_tree_few.cu: a row's reference is a score, the first slot's of a piece, and moves to a maximum
 // that is looked for when a score lies more than 2^13 above it (f16 has fewer exponents than bf16, so not 2^32 below); whether
 // one does costs a barrier of the warpgroup a step.  The two warpgroups take turns at the steps, each with a reference, a sum and an O^T
 // of its own.
+//
+// Bound by memory: 16 sequences of one token, 32 heads over 8, up to 8,001 slots, 173 MB in 44 us; one of 131,072 slots, 269 MB in 60.
+// Longer ones go at 6.3 TB/s behind 17 us that do not depend on the length: the first loads and products of a CTA, its pieces'
+// results, and the launch that joins them.
 //
 //   warp 0-3, 4-7   softmax
 //   warp 8          K Q^T       warp 10   V^T P^T       warp 9   plan, loads of K and scales       warp 11   loads of V
@@ -89,6 +93,20 @@ static __device__ __noinline__ uint32_t few8_seen(const TreeParams& p, const Tre
     return see;
 }
 
+// Whether a row's token sees a drafted token of the piece whose value of dimension `dim` is NaN.
+static __device__ __noinline__ bool few8_sees_nan(const TreeParams& p, const TreePiece& w, int token, int dim) {
+    const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
+    for (int u = from; u < to; ++u) {
+        const long long slot = static_cast<long long>(w.len) + u;
+        int row;
+        const int page = slot < w.slots ? p.c.cache.page_of(w.seq, slot, &row) : -1;
+        if (page < 0 || !tree_sees(p, w, token, u)) continue;
+        const uint8_t* v = reinterpret_cast<const uint8_t*>(p.c.cache.v) + p.c.cache.at(p.c.cache.v_stride, page, row, w.head);
+        if (e4m3_not_finite(v[dim])) return true;
+    }
+    return false;
+}
+
 // Of four rows' values those of pair e: of a step of two blocks a row's value for both slots, of one block two rows'.
 template <int B>
 __device__ __forceinline__ float2 few8_rows(const float4& v, int e) {
@@ -149,7 +167,9 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         fence_mbar_init();
     }
     // Rows of Q that are never written, and their scales.
-    for (int i = threadIdx.x; i < Shared::kQ * 2 * N * 8; i += kFew8Threads) reinterpret_cast<uint4*>(&sh.q[0][0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = threadIdx.x; i < Shared::kQ * 2 * N * 8; i += kFew8Threads) {
+        reinterpret_cast<uint4*>(&sh.q[0][0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
     if (threadIdx.x < N) {
         const int first = threadIdx.x * p.c.group, last = first + p.c.group;
         const uint32_t to = last >= 32 ? ~0u : (1u << last) - 1, from = first >= 32 ? ~0u : (1u << first) - 1;
@@ -232,7 +252,8 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         tree8_convert_v<4, kFew8Slots, Shared::kV, Shared::kV16>(p, sh, wctx, mine * 32 + lane, [&](const TreePiece& w, uint32_t it) {
             const int rows = w.n * p.c.group;
             const uint32_t buf = it % Shared::kQ;
-            const __nv_bfloat16* q = p8.q + w.q_begin * p8.q_stride[0] + static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] + (lane & 15) * 8;
+            const __nv_bfloat16* q = p8.q + w.q_begin * p8.q_stride[0] + static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] +
+                                     (lane & 15) * 8;
             bool waited = false;
 #pragma unroll 1
             for (int row = 2 * mine + (lane >> 4); row - (lane >> 4) < rows; row += 8) {
@@ -409,7 +430,8 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 // Drafted tokens, or no slots any more; pages that do not exist (one answer for the warp: the flag may go up, for
                 // a step still to come, between two lanes' looks).
                 const bool tail = (w.j0 + i + B) * kSlotBlock > w.len;
-                if (__builtin_expect(tail || i + B > w.blocks || __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u), 0)) {
+                const bool missing = __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&sh.missing) != 0u);
+                if (__builtin_expect(tail || i + B > w.blocks || missing, 0)) {
                     uint32_t see[B];
 #pragma unroll
                     for (int h = 0; h < B; ++h) {
@@ -532,7 +554,8 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             sum[row] = fmaf(prob.x, part.x, sum[row]);
                             sum[other] = fmaf(prob.y, part.y, sum[other]);
                         }
-                        const uint32_t to = p_at[row & 7] + (row >> 3) * 1024, to_other = p_at[other & 7] + (other >> 3) * 1024 + (B - 1) * N * 256;
+                        const uint32_t to = p_at[row & 7] + (row >> 3) * 1024;
+                        const uint32_t to_other = p_at[other & 7] + (other >> 3) * 1024 + (B - 1) * N * 256;
                         asm volatile("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tst.shared.b16 [%0], l;\n\tst.shared.b16 [%1], u;\n\t}"
                                      ::"r"(to), "r"(to_other), "r"(pack_half2(prob.x, prob.y)) : "memory");
                     }
@@ -577,58 +600,40 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             tc_fence_after_sync();
             const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) == it + 1;
             const bool whole = w.part < 0;
+            const bool second = w.blocks > B;
+            // Four rows at a time: this runs once a piece, and all its code comes from L2.
 #pragma unroll 1
-            for (int c0 = 8 * x; c0 < rows; c0 += 16) {
-                const bool second = w.blocks > B;
-                uint32_t o0[8], o1[8];
-                few_ld<8>(o_tmem + c0, o0);
-                if (second) few_ld<8>(o_tmem + N + c0, o1);
+            for (int c0 = 4 * x; c0 < rows; c0 += 8) {
+                uint32_t o0[4], o1[4];
+                few_ld<4>(o_tmem + c0, o0);
+                if (second) few_ld<4>(o_tmem + N + c0, o1);
                 tmem_wait_ld();
-                float o[8], ref[8], l[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 s0 = sh.stat[0][c0 + e], s1 = sh.stat[1][c0 + e];
-                    ref[e] = fmaxf(s0.x, s1.x);
-                    const float a0 = s0.x == ref[e] ? 1.f : fast_exp2(s0.x - ref[e]);
-                    const float a1 = s1.x == ref[e] ? 1.f : fast_exp2(s1.x - ref[e]);
-                    l[e] = s0.y * a0 + s1.y * a1;
-                    o[e] = __uint_as_float(o0[e]) * a0;
-                    if (second) o[e] = fmaf(__uint_as_float(o1[e]), a1, o[e]);
-                }
-                if (not_finite) {
-                    // Values of drafted tokens that are NaN, given to the rows that see them.
-                    const int from = max(0, w.j0 * kSlotBlock - w.len), to = min(w.n, (w.j0 + w.blocks) * kSlotBlock - w.len);
-                    for (int u = from; u < to; ++u) {
-                        const long long slot = static_cast<long long>(w.len) + u;
-                        int row;
-                        const int page = slot < w.slots ? p.c.cache.page_of(w.seq, slot, &row) : -1;
-                        if (page < 0) continue;
-                        const uint8_t* v = reinterpret_cast<const uint8_t*>(p.c.cache.v) + p.c.cache.at(p.c.cache.v_stride, page, row, w.head);
-                        if (!e4m3_not_finite(v[r])) continue;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (c0 + e < rows && tree_sees(p, w, (c0 + e) / p.c.group, u)) o[e] = NAN;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 4; ++e) {
                     const int row = c0 + e;
                     if (row >= rows) continue;
+                    const float2 s0 = sh.stat[0][row], s1 = sh.stat[1][row];
+                    const float ref = fmaxf(s0.x, s1.x);
+                    const float a0 = s0.x == ref ? 1.f : fast_exp2(s0.x - ref);
+                    const float a1 = s1.x == ref ? 1.f : fast_exp2(s1.x - ref);
+                    const float l = s0.y * a0 + s1.y * a1;
+                    float o = __uint_as_float(o0[e]) * a0;
+                    if (second) o = fmaf(__uint_as_float(o1[e]), a1, o);
+                    if (not_finite && few8_sees_nan(p, w, row / p.c.group, r)) o = NAN;
                     if (whole) {
                         const long long to = static_cast<long long>(w.q_begin) * p.c.heads_q + w.head * p.c.group + sh.out_at[row];
-                        // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.
-                        const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
-                        p.out[to * kHeadDim + r] = __float2bfloat16_rn(o[e] * inv);
+                        // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.  The sum of weights, each at
+                        // most 2^15 over a scale, is far below the 2^126 that the fast division wants.
+                        p.out[to * kHeadDim + r] = __float2bfloat16_rn(o * (l == 0.f ? 0.f : __fdividef(1.f, l)));
                         if (r == 0) {
                             p.lse[w.seq * p.lse_seq_stride + w.head * p.c.group * p.lse_head_stride +
                                   (p.c.cu_seqlens_q == nullptr ? 0 : w.q_begin) + sh.lse_at[row]] =
-                                l[e] == 0.f ? -INFINITY : (ref[e] + fast_log2(l[e])) * kLn2;
+                                l == 0.f ? -INFINITY : (ref + fast_log2(l)) * kLn2;
                         }
                     } else {
                         const long long to = static_cast<long long>(w.part) * p.part_rows + row;
-                        reinterpret_cast<float*>(p.part_o)[to * kHeadDim + r] = o[e];
-                        if (r == 0) p.part_stat[to] = make_float2(ref[e], l[e]);
+                        reinterpret_cast<float*>(p.part_o)[to * kHeadDim + r] = o;
+                        if (r == 0) p.part_stat[to] = make_float2(ref, l);
                     }
                 }
             }
@@ -675,8 +680,8 @@ int launch_few8(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8P
 int launch_tree8_few(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
                      cudaStream_t stream) {
     const int rows = p.t.part_rows;
-    const int rc = rows <= 4    ? launch_few8<4>(map_k, map_v, p, ctas, dev, 13, stream)
-                   : rows <= 8  ? launch_few8<8>(map_k, map_v, p, ctas, dev, 14, stream)
+    // 4 rows, 16 sequences of up to 8,001 slots, with 8, 16 and 32: 43.7, 51.0, 75.3 us; one of 131,072: 59.8, 65.1, 97.8.
+    const int rc = rows <= 8    ? launch_few8<8>(map_k, map_v, p, ctas, dev, 14, stream)
                    : rows <= 16 ? launch_few8<16>(map_k, map_v, p, ctas, dev, 21, stream)
                                 : launch_few8<32>(map_k, map_v, p, ctas, dev, 22, stream);
     return rc != B2A_OK || ctas == 1 ? rc : launch_tree_combine_few(p.t, ctas, stream);

@@ -239,8 +239,8 @@ tree8_attention_one(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int quarter = warp & 3;
         const int r = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_tmem = tmem_base + lane_base + static_cast<uint32_t>(x) * 128u, p_tmem = s_tmem;      // half h of P in the columns of
-                                                                                                               // S's first half, read by then
+        const uint32_t s_tmem = tmem_base + lane_base + static_cast<uint32_t>(x) * 128u;
+        const uint32_t p_tmem = s_tmem;      // both halves of P in the columns of S's first half, read by then
         const uint32_t o_tmem = tmem_base + lane_base + kFwdColO;
         const float sl2 = p.scale_log2;
         const int row_token = r / p.c.group;           // of the tile
