@@ -486,7 +486,7 @@ typedef struct b2a_cache_scales {
     float* v;
     int64_t k_stride[3];        /* elements from page to page, block to block, head to head */
     int64_t v_stride[3];
-    int32_t block;              /* slots of a scale: a power of two, 16 or more; with a block table it divides page_size */
+    int32_t block;              /* slots of a scale: 16, 32, 64 or 128; with a block table it divides page_size */
 } b2a_cache_scales;
 
 /*
@@ -499,9 +499,9 @@ typedef struct b2a_cache_scales {
 int b2a_cache8_append(const b2a_append_args* args, const b2a_cache_scales* scales, void* cuda_stream);
 
 /*
- * b2a_tree_fwd_with_scratch over a cache in 8 bits; workspace and scratch have the same sizes.  Q and the probabilities take part in the
- * products as sums of two 8-bit numbers: Q is off by 2^-18 of a row's largest value at most, a probability by 2^-7 of itself or
- * 2^-22 of the row's largest.  V's scales are taken within 2^-64 .. 2^64, and infinities of q as NaN.
+ * b2a_tree_fwd_with_scratch over a cache in 8 bits; workspace and scratch have the same sizes.  Q takes part in its product as the sum
+ * of two 8-bit numbers, off by 2^-18 of a row's largest value at most, a probability (times V's scale) in fp16, off by 2^-11 of itself
+ * or 2^-27 of the row's largest.  V's scales are taken within 2^-64 .. 2^64, and infinities of q as NaN.
  */
 int b2a_tree8_fwd(const b2a_tree_args* args, const b2a_cache_scales* scales, void* scratch, size_t scratch_bytes, void* cuda_stream);
 

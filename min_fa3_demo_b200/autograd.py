@@ -224,8 +224,8 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        # A rotation's gradient is the rotation back (times the same magnitude), whatever q and k were; with create_graph through the same function, so
-        # that it can be differentiated again.
+        # A rotation's gradient is the rotation back (times the same magnitude), whatever q and k were; with create_graph through
+        # the same function, so that it can be differentiated again.
         positions, = ctx.saved_tensors
         need_q, need_k = ctx.needs_input_grad[:2]
         dq, dk = dq if need_q else None, dk if need_k else None

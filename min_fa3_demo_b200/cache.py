@@ -214,11 +214,12 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ``cu_seqlens[B]`` go nowhere, and their rows of the returned q are not written.  A token without a slot is left out
     and reported by ``check_last_status("append_cache")``.  No two tokens may be given the same slot by shared pages.
 
-    Into a cache in 8 bits, with ``k_scales`` and ``v_scales``: a block that its first new token begins gets, for each head, the smallest
-    power of two as its scale with which the new values fit (at most 448 times it; within 2^-64 .. 2^64).  One that held tokens
-    keeps its scale while that is enough; if not, they are divided by the new one and rounded again.  New values are turned and
-    divided in fp32 and rounded once, to e4m3; what is not finite becomes NaN and has no say.  Nothing but the block that a
-    sequence ends in may be shared by pages with another one that goes on in it.
+    Into a cache in 8 bits, with ``k_scales`` and ``v_scales``: a block that its first new token begins gets, for each head, the
+    smallest power of two as its scale with which the new values fit (at most 448 times it; within 2^-64 .. 2^64).  One that held
+    tokens keeps its scale while that is enough; if not, they are divided by the new one and rounded again.  New values are turned
+    and divided in fp32 and rounded once, to e4m3; what is not finite becomes NaN and has no say.  So a block that a sequence
+    goes on in is written as a whole: no two sequences of a call may go on in the same one by shared pages, and who else shares it
+    sees its tokens rounded anew.
     """
     index, batch, ks = k_cache.get_device(), cache_lens.numel(), k.shape
     dim, tokens = 4 if cu_seqlens is None else 3, ks[:-2]
@@ -379,8 +380,9 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     out is off by 0.0023 of its 2-norm on random inputs, of which its own rounding is 0.0017.
 
     Over a cache in 8 bits, with its ``k_scales`` and ``v_scales`` (positive and finite; they may be expanded, one for all blocks or
-    heads): a slot's values are its e4m3 times its block's scale.  q and the probabilities go into the products as sums of two 8-bit numbers:
-    out is no further off than over a bf16 cache with the same values.  Infinities in q count as NaN.
+    heads): a slot's values are its e4m3 times its block's scale.  q goes into its product as the sum of two 8-bit numbers (off by
+    2^-18 of a row's largest value), the probabilities times V's scale in fp16 (off by 2^-11 of themselves, or by 2^-27 of a row's
+    largest): out is no further off than over a bf16 cache with the same values.  Infinities in q count as NaN.
     """
     index, batch = k_cache.get_device(), cache_lens.numel()
     in8 = k_cache.dtype is _E4M3 or k_scales is not None or v_scales is not None

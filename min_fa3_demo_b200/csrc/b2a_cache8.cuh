@@ -37,9 +37,10 @@ struct CacheScales {
 
 inline int make_cache_scales(const b2a_cache_scales& s, const b2a_cache& c, CacheScales* out) {
     B2A_REQUIRE(s.k != nullptr && s.v != nullptr, "the scales of the cache must not be NULL");
-    B2A_REQUIRE(s.block >= 16 && (s.block & (s.block - 1)) == 0, "slots of a scale must be a power of two, 16 or more, got %d", s.block);
-    B2A_REQUIRE(c.block_table == nullptr || c.page_size % s.block == 0, "page_size must be a multiple of a scale's slots, got %d and %d",
-                c.page_size, s.block);
+    B2A_REQUIRE(s.block == 16 || s.block == 32 || s.block == 64 || s.block == 128, "a scale must have 16, 32, 64 or 128 slots, got %d",
+                s.block);
+    B2A_REQUIRE(c.block_table == nullptr || c.page_size % s.block == 0,
+                "page_size must be a multiple of a scale's slots, got %d and %d", c.page_size, s.block);
     for (int i = 0; i < 3; ++i) {
         B2A_REQUIRE(s.k_stride[i] >= 0 && s.v_stride[i] >= 0, "strides of the scales must not be negative");
         B2A_REQUIRE(c.k_stride[i] % 16 == 0 && c.v_stride[i] % 16 == 0, "strides of a cache in 8 bits must be multiples of 16 elements");

@@ -35,8 +35,9 @@ class RotaryAxes:
 
     Pair ``i`` turns by ``positions[axis[i]] * inv_freq[i]``; there are 8, 16, ... or 64 pairs, and the dimensions behind the
     first ``2 * pairs`` stay as they are.  ``adjacent``: pair ``i`` is dimensions ``(2 i, 2 i + 1)``, otherwise
-    ``(i, i + pairs)``.  ``magnitude``: what turned pairs are multiplied by (:meth:`stretched`).  Frequencies are taken as the 64-bit floats they are.  An angle is within 1.1e-7 for
-    positions up to 2^36, and 1.7e-19 times the position more beyond (2^45: 6e-6).
+    ``(i, i + pairs)``.  ``magnitude``: what turned pairs are multiplied by (:meth:`stretched`).  Frequencies are taken as the
+    64-bit floats they are.  An angle is within 1.1e-7 for positions up to 2^36, and 1.7e-19 times the position more beyond
+    (2^45: 6e-6).
     """
 
     def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False,
@@ -96,17 +97,16 @@ class RotaryAxes:
                 axis.append(a)
         return cls(freq, axis, adjacent=adjacent)
 
-
     def stretched(self, factor: float, original_length: float, *, slow: float = 1.0, fast: float = 32.0,
                   magnitude: Optional[float] = None) -> "RotaryAxes":
         """The same axes for contexts ``factor`` times as long as the ``original_length`` positions that a model was trained on.
 
-        A pair that turns fewer than ``slow`` times within that length gets its frequency divided by ``factor`` (its angles stay within
-        those of the training), one that turns more than ``fast`` times keeps it (it tells neighbours apart), and between the two the
-        frequency goes over from one to the other linearly in the number of turns.  ``magnitude`` multiplies turned pairs of q and of
-        k, a score by its square; by default ``0.1 ln(factor) + 1``.  (Peng et al., "Efficient Context Window
-        Extension of Large Language Models", 2023, "NTK-by-parts" and its temperature; with ``magnitude=1`` and a small ``fast`` the
-        smooth ramp that is in use without one.)  ``slow = fast = inf``: all frequencies divided.
+        A pair that turns fewer than ``slow`` times within that length gets its frequency divided by ``factor`` (its angles stay
+        within those of the training), one that turns more than ``fast`` times keeps it (it tells neighbours apart), and between the
+        two the frequency goes over from one to the other linearly in the number of turns.  ``magnitude`` multiplies turned pairs of q
+        and of k, a score by its square; by default ``0.1 ln(factor) + 1`` times what it was.  (Peng et al., "Efficient Context Window
+        Extension of Large Language Models", 2023, "NTK-by-parts" and its temperature; with ``magnitude=1`` and a small ``fast``
+        the smooth ramp that is in use without one.)  ``slow = fast = inf``: all frequencies divided.
         """
         _check(hasattr(self, "_inv_freq"), "these axes do not know their frequencies")
         _check(isfinite(factor) and factor >= 1, f"factor must be 1 or more, got {factor}")
@@ -116,7 +116,7 @@ class RotaryAxes:
         for f in self._inv_freq:
             turns = original_length * abs(f) / (2 * pi)
             keep = 0.0 if turns <= slow else 1.0 if turns >= fast else (turns - slow) / (fast - slow)
-            frequencies.append((1 - keep) * (f / factor) + keep * f)
+            frequencies.append(f if keep == 1 else f / factor + keep * (f - f / factor))      # unchanged bit for bit, where it is
         if magnitude is None:
             magnitude = self.magnitude * (0.1 * log(factor) + 1)
         return RotaryAxes(frequencies, self._plain[1], adjacent=self._plain[2], magnitude=magnitude)
@@ -194,7 +194,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     q ``[B, S, QH, 128]``, k ``[B, S, KVH, 128]`` or None, positions ``[axes, B, S]`` (packed tokens: ``[T, H, 128]`` and
     ``[axes, T]``), int32 or int64, of any strides (``expand`` one row of positions over a batch).  q and k may be slices of
     one projection: only the 128 values of a head have to be adjacent.  Returns new contiguous tensors.  ``inverse``
-    turns the other way, which is what the gradients want; ``autograd.rotary`` does it by itself.
+    turns the other way, and multiplies by the axes' magnitude as well, which is what the gradients want; ``autograd.rotary`` does
+    it by itself.
     """
     index, qs, q_at = q.get_device(), q.shape, q.data_ptr()
     dim = len(qs)
