@@ -84,7 +84,8 @@ def arguments(call):
     return dict(q=t(11, 4, 128), **pages, tree_mask=t(11, 6, dtype=torch.bool), max_seqlen_q=6, cu_seqlens_q=i32(4), out=None)
 
 
-FUNCTIONS = {"append": cache.append_cache, "append packed": cache.append_cache, "tree": cache.forward_tree, "tree packed": cache.forward_tree}
+FUNCTIONS = {"append": cache.append_cache, "append packed": cache.append_cache, "tree": cache.forward_tree,
+             "tree packed": cache.forward_tree}
 
 
 def launch(call, **change):
@@ -110,7 +111,8 @@ def test_calls_in_order_reach_the_library(fake, call):
 @pytest.mark.parametrize("call", ["append", "tree"])
 @pytest.mark.parametrize("size,blocks,block", [(32, 1, 32), (64, 2, 32), (64, 1, 64), (128, 1, 128), (256, 2, 128), (48, 3, 16)])
 def test_slots_of_a_scale_with_pages(fake, call, size, blocks, block):
-    _, scales = launch(call, k_cache=f8(9, size, 2, 128), v_cache=f8(9, size, 2, 128), k_scales=f32(9, blocks, 2), v_scales=f32(9, blocks, 2))
+    _, scales = launch(call, k_cache=f8(9, size, 2, 128), v_cache=f8(9, size, 2, 128), k_scales=f32(9, blocks, 2),
+                       v_scales=f32(9, blocks, 2))
     assert scales.block == block
 
 
@@ -207,8 +209,8 @@ def test_layout(tmp_path):
     names = [field[0] for field in _cabi.CacheScales._fields_]
     src = tmp_path / "sizes.c"
     offsets = "".join(f'printf(" %zu", offsetof(b2a_cache_scales, {name}));' for name in names)
-    src.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{header}"\nint main(void) {{ printf("%zu %zu", sizeof(b2a_cache_scales),'
-                   f' offsetof(b2a_rotary_axes, magnitude)); {offsets} return 0; }}\n')
+    src.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{header}"\nint main(void) {{ printf("%zu %zu",'
+                   f' sizeof(b2a_cache_scales), offsetof(b2a_rotary_axes, magnitude)); {offsets} return 0; }}\n')
     subprocess.run([gcc, "-std=c99", "-Wall", "-Werror", str(src), "-o", str(tmp_path / "sizes")], check=True)
     size, magnitude, *at = map(int, subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split())
     assert size == ctypes.sizeof(_cabi.CacheScales) == _cabi.SCALES.size and magnitude == _cabi.RotaryAxes.magnitude.offset
@@ -228,11 +230,12 @@ def filled(struct, **fields):
 
 
 def c_call(lib, name, scales=None, cache_fields=None, **change):
-    view = dict(k=256, v=256, block_table=256, table_stride=4, k_stride=(8192, 256, 128), v_stride=(8192, 256, 128), pages=9, page_size=32,
-                heads_k=2, table_width=4)
+    view = dict(k=256, v=256, block_table=256, table_stride=4, k_stride=(8192, 256, 128), v_stride=(8192, 256, 128), pages=9,
+                page_size=32, heads_k=2, table_width=4)
     given = dict(k=256, v=256, k_stride=(4, 2, 1), v_stride=(4, 2, 1), block=16)
     given.update(scales or {})
-    common = dict(cache=filled(_cabi.Cache, **dict(view, **(cache_fields or {}))), cache_lens=256, batch=3, workspace=256, workspace_bytes=1 << 30)
+    common = dict(cache=filled(_cabi.Cache, **dict(view, **(cache_fields or {}))), cache_lens=256, batch=3, workspace=256,
+                  workspace_bytes=1 << 30)
     if name == "b2a_cache8_append":
         fields = dict(common, k=256, v=256, k_stride=(1280, 256, 128), v_stride=(1280, 256, 128), seqlen=5, total=15)
         fields.update(change)
@@ -246,7 +249,8 @@ def c_call(lib, name, scales=None, cache_fields=None, **change):
 
 
 C_REFUSALS = [(name, change, words) for name in ("b2a_cache8_append", "b2a_tree8_fwd") for change, words in [
-    (dict(scales=dict(k=0)), "the scales of the cache must not be NULL"), (dict(scales=dict(v=0)), "the scales of the cache must not be NULL"),
+    (dict(scales=dict(k=0)), "the scales of the cache must not be NULL"),
+    (dict(scales=dict(v=0)), "the scales of the cache must not be NULL"),
     *[(dict(scales=dict(block=n)), f"a scale must have 16, 32, 64 or 128 slots, got {n}") for n in (0, 8, 24, 256, -16)],
     (dict(scales=dict(block=64)), "page_size must be a multiple of a scale's slots, got 32 and 64"),
     (dict(scales=dict(k_stride=(4, -2, 1))), "strides of the scales must not be negative"),
@@ -259,7 +263,8 @@ C_REFUSALS = [(name, change, words) for name in ("b2a_cache8_append", "b2a_tree8
     ("b2a_cache8_append", dict(workspace=0), "workspace must be a 16-byte aligned"),
     ("b2a_tree8_fwd", dict(out=0), "out must be a 16-byte aligned"), ("b2a_tree8_fwd", dict(heads_q=3), "heads_q % heads_k must be 0"),
     ("b2a_tree8_fwd", dict(q_stride=(512, 100)), "strides of q must be multiples of 8 elements"),
-    ("b2a_tree8_fwd", dict(scratch=8), "scratch must be a 16-byte aligned"), ("b2a_tree8_fwd", dict(scratch=None), "scratch must be a 16-byte aligned"),
+    ("b2a_tree8_fwd", dict(scratch=8), "scratch must be a 16-byte aligned"),
+    ("b2a_tree8_fwd", dict(scratch=None), "scratch must be a 16-byte aligned"),
     ("b2a_tree8_fwd", dict(workspace=0), "workspace must be a 16-byte aligned"),
 ]
 
@@ -282,8 +287,8 @@ def test_null_arguments(lib, args, scales):
 # ---------------------------------------------------------------------------------------
 # Stretched axes
 # ---------------------------------------------------------------------------------------
-@pytest.mark.parametrize("factor,length,slow,fast", [(1, 4096, 1, 32), (4, 4096, 1, 32), (8, 8192, 1, 4), (2.5, 300, 0, 7.5), (16, 100, 3, 3),
-                                                     (4, 4096, math.inf, math.inf), (4, 4096, 0, 0)])
+@pytest.mark.parametrize("factor,length,slow,fast", [(1, 4096, 1, 32), (4, 4096, 1, 32), (8, 8192, 1, 4), (2.5, 300, 0, 7.5),
+                                                     (16, 100, 3, 3), (4, 4096, math.inf, math.inf), (4, 4096, 0, 0)])
 @pytest.mark.parametrize("adjacent", [False, True])
 def test_stretched_frequencies(factor, length, slow, fast, adjacent):
     plain = rotary.RotaryAxes.from_sections((16, 24, 24), 1e6, adjacent=adjacent)
