@@ -40,6 +40,8 @@ class RotaryAxes:
     (2^45: 6e-6).
     """
 
+    magnitude = 1.0
+
     def __init__(self, inv_freq: Sequence[float], axis: Optional[Sequence[int]] = None, *, adjacent: bool = False,
                  magnitude: float = 1.0):
         inv_freq = [float(f) for f in inv_freq]
@@ -54,6 +56,7 @@ class RotaryAxes:
         _check(isfinite(magnitude) and magnitude > 0, f"magnitude must be positive and finite, got {magnitude}")
         self.axes = max(axis) + 1
         self.pairs = pairs
+        self.magnitude = magnitude              # a plain number: a traced step reads it, and cannot read the structure's
         c = _cabi.RotaryAxes()
         c.turn[:pairs] = [_turn(f) for f in inv_freq]
         c.axis[:pairs] = axis
@@ -66,17 +69,13 @@ class RotaryAxes:
     @classmethod
     def _from_plain(cls, turn: Sequence[int], axis: Sequence[int], adjacent: bool, magnitude: float = 1.0) -> "RotaryAxes":
         self = cls.__new__(cls)
-        self.axes, self.pairs = max(axis) + 1, len(axis)
+        self.axes, self.pairs, self.magnitude = max(axis) + 1, len(axis), magnitude
         self._c = c = _cabi.RotaryAxes()
         c.turn[:self.pairs] = [t % 2**64 for t in turn]
         c.axis[:self.pairs] = axis
         c.pairs, c.axes, c.adjacent, c.magnitude = self.pairs, self.axes, int(adjacent), magnitude
         self._plain = (list(turn), list(axis), bool(adjacent))
         return self
-
-    @property
-    def magnitude(self) -> float:
-        return self._c.magnitude or 1.0
 
     @property
     def _at(self) -> int:

@@ -130,6 +130,20 @@ def test_captured_backward_while_an_eager_graph_lives():
     assert eager.shape == leaf.shape
 
 
+def test_traced_step():
+    gen = torch.Generator().manual_seed(9)
+    axes = make("axes")[0]
+    q, k = randn(gen, 2, 33, 4, 128).cuda().requires_grad_(), randn(gen, 2, 33, 2, 128).cuda().requires_grad_()
+    positions = torch.randint(0, 9000, (3, 2, 33), generator=gen).cuda()
+
+    def step(a, b):
+        return autograd.rotary(a * 2, b, positions, axes)
+    want, ours = step(q, k), torch.compile(step, backend="aot_eager", fullgraph=True)(q, k)
+    assert all(torch.equal(a, b) for a, b in zip(ours, want))
+    grads = [torch.autograd.grad(out, (q, k), [torch.ones_like(t) for t in out]) for out in (ours, want)]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 @pytest.mark.parametrize("name", list(CASES))
 @pytest.mark.parametrize("count", [1, 50])
 def test_written_into_a_cache_in_16_bits(name, count):
