@@ -13,7 +13,7 @@
 // one does costs a barrier of the warpgroup a step.  The two warpgroups take turns at the steps, each with a reference, a sum and an O^T
 // of its own.
 //
-// Bound by memory: 16 sequences of one token, 32 heads over 8, up to 8,001 slots, 173 MB in 44 us; one of 131,072 slots, 269 MB in 60.
+// Bound by memory: 16 sequences of one token, 32 heads over 8, up to 8,001 slots, 173 MB in 43 us; one of 131,072 slots, 269 MB in 60.
 // Longer ones go at 6.3 TB/s behind 17 us that do not depend on the length: the first loads and products of a CTA, its pieces'
 // results, and the launch that joins them.
 //
@@ -601,39 +601,52 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const bool not_finite = *reinterpret_cast<volatile uint32_t*>(&sh.not_finite[at]) == it + 1;
             const bool whole = w.part < 0;
             const bool second = w.blocks > B;
+            // A thread a row for what it needs once; the sums' places take the two parts' factors.
+            if (r < rows) {
+                const float2 s0 = sh.stat[0][r], s1 = sh.stat[1][r];
+                const float ref = fmaxf(s0.x, s1.x);
+                float a0 = s0.x == ref ? 1.f : fast_exp2(s0.x - ref);
+                float a1 = s1.x == ref ? 1.f : fast_exp2(s1.x - ref);
+                const float l = s0.y * a0 + s1.y * a1;
+                if (whole) {
+                    // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.  The sum of weights, each at
+                    // most 2^15 over a scale, is far below the 2^126 that the fast division wants.
+                    const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
+                    a0 *= inv;
+                    a1 *= inv;
+                    if (x == 0) {
+                        p.lse[w.seq * p.lse_seq_stride + w.head * p.c.group * p.lse_head_stride +
+                              (p.c.cu_seqlens_q == nullptr ? 0 : w.q_begin) + sh.lse_at[r]] =
+                            l == 0.f ? -INFINITY : (ref + fast_log2(l)) * kLn2;
+                    }
+                } else if (x == 0) {
+                    p.part_stat[static_cast<long long>(w.part) * p.part_rows + r] = make_float2(ref, l);
+                }
+                sh.top[x][0][r] = a0;
+                sh.top[x][1][r] = a1;
+            }
+            ok = meet();
+            if (!ok) break;
             // Four rows at a time: this runs once a piece, and all its code comes from L2.
+            __nv_bfloat16* const out = p.out + (static_cast<long long>(w.q_begin) * p.c.heads_q + w.head * p.c.group) * kHeadDim + r;
+            float* const part = reinterpret_cast<float*>(p.part_o) + static_cast<long long>(w.part) * p.part_rows * kHeadDim + r;
 #pragma unroll 1
             for (int c0 = 4 * x; c0 < rows; c0 += 8) {
-                uint32_t o0[4], o1[4];
+                uint32_t o0[4], o1[4] = {0u, 0u, 0u, 0u};
                 few_ld<4>(o_tmem + c0, o0);
                 if (second) few_ld<4>(o_tmem + N + c0, o1);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = c0 + e;
-                    if (row >= rows) continue;
-                    const float2 s0 = sh.stat[0][row], s1 = sh.stat[1][row];
-                    const float ref = fmaxf(s0.x, s1.x);
-                    const float a0 = s0.x == ref ? 1.f : fast_exp2(s0.x - ref);
-                    const float a1 = s1.x == ref ? 1.f : fast_exp2(s1.x - ref);
-                    const float l = s0.y * a0 + s1.y * a1;
-                    float o = __uint_as_float(o0[e]) * a0;
-                    if (second) o = fmaf(__uint_as_float(o1[e]), a1, o);
+                    if (row >= rows) break;
+                    float o = __uint_as_float(o0[e]) * sh.top[x][0][row];
+                    if (second) o = fmaf(__uint_as_float(o1[e]), sh.top[x][1][row], o);
                     if (not_finite && few8_sees_nan(p, w, row / p.c.group, r)) o = NAN;
                     if (whole) {
-                        const long long to = static_cast<long long>(w.q_begin) * p.c.heads_q + w.head * p.c.group + sh.out_at[row];
-                        // A sum of 0: the row sees nothing (or only what is -inf).  NaN stays NaN.  The sum of weights, each at
-                        // most 2^15 over a scale, is far below the 2^126 that the fast division wants.
-                        p.out[to * kHeadDim + r] = __float2bfloat16_rn(o * (l == 0.f ? 0.f : __fdividef(1.f, l)));
-                        if (r == 0) {
-                            p.lse[w.seq * p.lse_seq_stride + w.head * p.c.group * p.lse_head_stride +
-                                  (p.c.cu_seqlens_q == nullptr ? 0 : w.q_begin) + sh.lse_at[row]] =
-                                l == 0.f ? -INFINITY : (ref + fast_log2(l)) * kLn2;
-                        }
+                        out[static_cast<long long>(sh.out_at[row]) * kHeadDim] = __float2bfloat16_rn(o);
                     } else {
-                        const long long to = static_cast<long long>(w.part) * p.part_rows + row;
-                        reinterpret_cast<float*>(p.part_o)[to * kHeadDim + r] = o;
-                        if (r == 0) p.part_stat[to] = make_float2(ref, l);
+                        part[row * kHeadDim] = o;
                     }
                 }
             }
