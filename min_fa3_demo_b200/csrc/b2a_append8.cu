@@ -11,7 +11,7 @@
 // Should be bound by memory: 256 bytes in and 128 out a token and head, and q's 256 and 256.  A CTA has a block of slots and some of the
 // heads, for which it computes the angles once; CTAs behind those turn q, and the first one looks for places that do not exist.
 // One new token of 16 sequences, 32 + 8 heads, is 4.8 us, what a launch with four reads one after another takes.  715 of 32
-// sequences: 11.8 us.  5,647 of 4: 139 MB in 34 us, of which q alone is 20 and k and v alone 21: each keeps the SMs' issue slots
+// sequences: 11.3 us.  5,647 of 4: 139 MB in 34 us, of which q alone is 20 and k and v alone 21: each keeps the SMs' issue slots
 // half busy (9.3 and 9.6 million instructions, most of them of the turning, which k needs twice).  That was 58 us with a piece of
 // code for each of the two passes and four tokens, and a division where a product does: an instruction fetched for one use costs
 // more than its work.  64 registers and four CTAs an SM: with three 39 us for 35.6, with five 37.6.
@@ -180,10 +180,12 @@ append8_tokens(const __grid_constant__ Append8Params p8) {
             return which == 0 && p.pairs > 0 && p.adjacent ? 64 + 8 * c : which == 0 && turned ? p.pairs + 8 * c : 16 * c + 8;
         };
         // A unit's tiles are loaded from the first to the last, for the largest value, and back, to be written: the last one, and so
-        // the only one of few tokens, once.  A thread reads back what it copied itself.
+        // the only one of few tokens, once, and of two the first one once as well, which is still there.  A thread reads back what it
+        // copied itself.
         const int tiles = (at.count + kTile8 - 1) / kTile8, trips = 2 * tiles - 1;
         const uint32_t stage0 = smem_u32(smem) + warp * p8.stages * kStage8Bytes + mine * 256 + c * 16;
         auto load = [&](int unit, int trip, int stage) {
+            if (tiles == 2 && trip == 2) return;
             const int which = unit & 1, lo = lo_of(which), hi = hi_of(which);
             const int token0 = (trip < tiles ? trip : 2 * tiles - 2 - trip) * kTile8;
             const long long* stride = p.stride[1 + which];
