@@ -149,24 +149,26 @@ def _cache_fields(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_
 @functools.lru_cache(maxsize=4096)
 def _scale_block(size: int, blocks: int, paged: bool) -> int:
     """Slots of a scale; 0: none fits."""
+    if paged:
+        block = size // blocks if blocks > 0 else 0
+        return block if block * blocks == size and block in (16, 32, 64, 128) else 0
     for block in (16, 32, 64, 128):
-        if -(-size // block) == blocks and not (paged and size % block):
+        if -(-size // block) == blocks:
             return block
     return 0
 
 
-def _scale_fields(k_scales, v_scales, k_cache, paged: bool, index: int, written: bool) -> tuple:
-    """``b2a_cache_scales`` for struct.pack; k_cache has four dimensions."""
+def _scale_fields(k_scales, v_scales, k_cache, fields: tuple, paged: bool, index: int, written: bool) -> tuple:
+    """``b2a_cache_scales`` for struct.pack; fields are the cache's."""
+    pages, size, heads = fields[10:13]
     if type(k_scales) is torch.Tensor and type(v_scales) is torch.Tensor:
-        ks, vs, (pages, size, heads, _) = k_scales.shape, v_scales.shape, k_cache.shape
-        if (ks == vs and len(ks) == 3 and ks[0] == pages and ks[2] == heads and k_scales.dtype is torch.float32 is v_scales.dtype
-                and k_scales.get_device() == index == v_scales.get_device()):
+        ks, k_step, v_step = k_scales.shape, k_scales.stride(), v_scales.stride()
+        if (len(ks) == 3 and v_scales.shape == ks and ks[0] == pages and ks[2] == heads
+                and k_scales.dtype is torch.float32 is v_scales.dtype and k_scales.get_device() == index == v_scales.get_device()):
             block = _scale_block(size, ks[1], paged)
-            k_step, v_step = k_scales.stride(), v_scales.stride()
             if block and not (written and 0 in k_step + v_step and any(n > 1 and 0 in (a, b) for n, a, b in zip(ks, k_step, v_step))):
                 return k_scales.data_ptr(), v_scales.data_ptr(), *k_step, *v_step, block
     _check(k_scales is not None and v_scales is not None, "a cache of dtype torch.float8_e4m3fn and k_scales and v_scales go together")
-    pages, size, heads, _ = k_cache.shape
     for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
         _check(t.is_cuda and t.device == k_cache.device, f"{name} must be on the same CUDA device as the cache")
         _check(t.dtype == torch.float32, f"{name} must have dtype torch.float32")
@@ -234,7 +236,7 @@ def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             and (q is None or (axes is not None and _is_rows(q, dim, index) and q.shape[:-2] == tokens))):
         _check_append(k, v, k_cache, v_cache, cache_lens, block_table, cu_seqlens, q, positions, axes, _E4M3 if in8 else _BF16)
         fields = _cache_fields(k_cache, v_cache, block_table)
-    scales = _scale_fields(k_scales, v_scales, k_cache, block_table is not None, index, True) if in8 else None
+    scales = _scale_fields(k_scales, v_scales, k_cache, fields, block_table is not None, index, True) if in8 else None
     q_out = None if q is None else _like(q)
     if k.numel() == 0:
         return q_out
@@ -395,7 +397,7 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         _check_forward_tree(q, k_cache, v_cache, cache_lens, block_table, cu_seqlens_q, max_seqlen_q, tree_mask, _E4M3 if in8 else _BF16)
         fields, query = _cache_fields(k_cache, v_cache, block_table), _query_fields(q, max_seqlen_q, tree_mask)
     mask, total, most, heads, s_tok, s_head, m_seq, m_row = query
-    scales = _scale_fields(k_scales, v_scales, k_cache, block_table is not None, index, False) if in8 else None
+    scales = _scale_fields(k_scales, v_scales, k_cache, fields, block_table is not None, index, False) if in8 else None
     device = k_cache.device
     if out is None:
         out = _like(q)
