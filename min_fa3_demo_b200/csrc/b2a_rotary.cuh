@@ -51,8 +51,13 @@ __device__ __forceinline__ TokenPlace find_token(const RotaryParams& p, int toke
         at.number = token - at.seq * p.seqlen;
         return at;
     }
+    // Of more than 64, first which 32nd of them it is in.
     int ended = 0;
-    for (int b = 0; b < p.batch; b += 32) {
+    if (p.batch > 64) {
+        const int part = (p.batch + 31) / 32, last = (lane + 1) * part;
+        ended = part * __popc(__ballot_sync(0xFFFFFFFFu, last <= p.batch && p.cu_seqlens[min(last, p.batch)] <= token));
+    }
+    for (int b = ended; b < p.batch; b += 32) {
         const bool before = b + lane < p.batch && p.cu_seqlens[b + lane + 1] <= token;
         const int n = __popc(__ballot_sync(0xFFFFFFFFu, before));
         ended += n;
@@ -94,7 +99,9 @@ __device__ __forceinline__ void check_append(const RotaryParams& p) {
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
-    for (int b = threadIdx.x >> 5; b < p.batch; b += kRotaryThreads / 32) {      // a warp a sequence, a lane a page
+    // A warp a sequence and a lane a page, or, of more sequences than 64, which have few new pages each, a thread a sequence.
+    const int lanes = p.batch > 64 ? 1 : 32;
+    for (int b = threadIdx.x / lanes; b < p.batch; b += kRotaryThreads / lanes) {
         const long long first = p.cache_lens[b];
         const int begin = p.cu_seqlens == nullptr ? 0 : p.cu_seqlens[b];
         const int end = p.cu_seqlens == nullptr ? p.seqlen : p.cu_seqlens[b + 1];
@@ -106,7 +113,8 @@ __device__ __forceinline__ void check_append(const RotaryParams& p) {
         if (p.cache.block_table == nullptr || last == first) continue;
         int row;
         const int entry = p.cache.entry_of(static_cast<int>(first), &row);
-        for (long long slot = (entry + (threadIdx.x & 31ll)) * p.cache.page_size; slot < last; slot += 32ll * p.cache.page_size) {
+        const long long step = static_cast<long long>(lanes) * p.cache.page_size;
+        for (long long slot = (entry + static_cast<long long>(threadIdx.x % lanes)) * p.cache.page_size; slot < last; slot += step) {
             if (p.cache.page_of(b, slot, &row) < 0) bad = 1;
         }
     }

@@ -1,0 +1,108 @@
+"""Writes of caches for many packed sequences, which the kernels look up in other ways than few: slots, scales, turned
+queries, what has no place, and padding, in 16 and in 8 bits."""
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+import min_fa3_op
+from cache8_util import Cache8
+from cache_util import BF16_HALF_STEP, Cache, randn, turn
+from test_append_cache8_gpu import check, held
+
+pytestmark = pytest.mark.gpu
+
+FREQ = [1e4 ** (-i / 64) for i in range(64)]
+
+
+def lengths(seqs, most, slots):
+    """Tokens before and behind; a third of the sequences has none or one, a few have many."""
+    rng = random.Random(seqs + most)
+    counts = [rng.choice([0, 1, rng.randint(1, most), most if b % 50 == 0 else 2]) for b in range(seqs)]
+    counts[-1] = 0
+    return [rng.randint(0, slots - c) for c in counts], counts
+
+
+def offsets(counts):
+    return torch.tensor([0, *torch.tensor(counts).cumsum(0)], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("seqs", [64, 65, 256, 257, 700, 1100])
+@pytest.mark.parametrize("most,block", [(1, 16), (9, 16), (70, 32), (40, 128)])
+def test_slots_and_scales_in_8_bits(seqs, most, block):
+    gen = torch.Generator().manual_seed(seqs)
+    slots = 128
+    lens, counts = lengths(seqs, most, slots)
+    cache = Cache8(seqs, seqs, slots, 1, 128 if block == 128 else 32, block)
+    before = {which: [held(cache, which, b, slots) for b in range(seqs)] for which in "kv"}
+    total = sum(counts)
+    new = {which: randn(gen, total + 3, 1, 128) for which in "kv"}
+    min_fa3_op.append_cache(new["k"].cuda(), new["v"].cuda(), cache.k, cache.v, torch.tensor(lens, dtype=torch.int32).cuda(),
+                            cu_seqlens=offsets(counts).cuda(), **cache.more())
+    min_fa3_op.check_last_status("append_cache")
+    # Of those that got nothing it is enough to look at some: their pages belong to nobody else.
+    for b, first in enumerate(offsets(counts)[:-1].tolist()):
+        if counts[b] or b % 20 == 0:
+            for which in "kv":
+                check(cache, before[which][b], which, b, lens[b], new[which][first:first + counts[b]].double(), slots)
+
+
+@pytest.mark.parametrize("in8", [False, True])
+@pytest.mark.parametrize("seqs", [65, 700])
+def test_turned_queries(seqs, in8):
+    gen = torch.Generator().manual_seed(seqs)
+    lens, counts = lengths(seqs, 9, 64)
+    cache = Cache8(seqs, seqs, 64, 1, 16) if in8 else Cache(seqs, seqs, 64, 1, 16)
+    more = cache.more() if in8 else dict(block_table=cache.table)
+    total = sum(counts)
+    q, k, v = (randn(gen, total, h, 128) for h in (3, 1, 1))
+    positions = torch.randint(0, 5000, (1, total), generator=gen)
+    out = min_fa3_op.append_cache(k.cuda(), v.cuda(), cache.k, cache.v, torch.tensor(lens, dtype=torch.int32).cuda(), q=q.cuda(),
+                                  positions=positions.cuda(), axes=min_fa3_op.RotaryAxes(FREQ), cu_seqlens=offsets(counts).cuda(), **more)
+    min_fa3_op.check_last_status("append_cache")
+    # One rounding to bf16 and a few in 32 bits, as in the tests of ``rotary``.
+    ref = turn(q, positions, FREQ, [0] * 64, False)
+    assert ((out.double().cpu() - ref).abs() <= ref.abs() * BF16_HALF_STEP * (1 + 2**-10) + 2**-20 * q.double().abs().max()).all()
+    if not in8:
+        ref = turn(k, positions, FREQ, [0] * 64, False)
+        for b, first in enumerate(offsets(counts)[:-1].tolist()):
+            want = ref[first:first + counts[b]]
+            off = (cache.rows("k", b, lens[b] + counts[b])[lens[b]:] - want).abs()
+            assert (off <= want.abs() * BF16_HALF_STEP * (1 + 2**-10) + 2**-20 * k.double().abs().max()).all(), f"sequence {b}"
+            assert torch.equal(cache.rows("v", b, lens[b] + counts[b])[lens[b]:], v[first:first + counts[b]].double())
+
+
+@pytest.mark.parametrize("in8", [False, True])
+@pytest.mark.parametrize("what", ["negative length", "beyond the slots", "page", "order"])
+def test_what_does_not_fit_is_left_out_and_reported(in8, what):
+    seqs, slots = 400, 48
+    gen = torch.Generator().manual_seed(5)
+    lens, counts = [b % 40 for b in range(seqs)], [b % 5 + 1 for b in range(seqs)]
+    cache = Cache8(1, seqs, slots, 1, 16) if in8 else Cache(1, seqs, slots, 1, 16)
+    cu = offsets(counts)
+    bad = 333
+    if what == "negative length":
+        lens[bad] = -3
+    elif what == "beyond the slots":
+        lens[bad] = slots
+    elif what == "page":
+        cache.table[bad, lens[bad] // 16] = 10**6
+    else:
+        cu[bad + 1] = cu[bad] - 2
+    k, v = (randn(gen, sum(counts), 1, 128) for _ in range(2))
+    more = cache.more() if in8 else dict(block_table=cache.table)
+    if in8:
+        before = [held(cache, "v", b, slots) for b in range(seqs) if abs(b - bad) > 1]
+    min_fa3_op.append_cache(k.cuda(), v.cuda(), cache.k, cache.v, torch.tensor(lens, dtype=torch.int32).cuda(), cu_seqlens=cu.cuda(), **more)
+    with pytest.raises(RuntimeError):
+        min_fa3_op.check_last_status("append_cache")
+    # Its neighbours apart, whose numbers of tokens an entry out of order changes, everybody else has theirs.
+    others = [b for b in range(seqs) if abs(b - bad) > 1]
+    for n, b in enumerate(others):
+        new = v[cu[b]:cu[b + 1]].double()
+        if in8:
+            check(cache, before[n], "v", b, lens[b], new, slots)
+        else:
+            assert torch.equal(cache.rows("v", b, lens[b] + counts[b])[lens[b]:], new)
