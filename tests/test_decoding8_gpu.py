@@ -184,3 +184,43 @@ def test_calls_at_once_on_streams_of_their_own():
         for _ in range(3):
             min_fa3_op.append_cache(k, v, alone.k, alone.v, lens, **alone.more())
         assert all(torch.equal(a, b) for a, b in zip(cache.snapshot(), alone.snapshot()))
+
+
+def test_pages_beyond_32_bits():
+    """The same step in a cache of 3 pages and in one of 66,000 (4.3 GB each of K and V), on its last ones: the same bits."""
+    gen = torch.Generator().manual_seed(10)
+    q, k, v = (randn(gen, 1, 150, h, 128).cuda() for h in (8, 8, 8))
+    lens = torch.zeros(1, dtype=torch.int32, device="cuda")
+    results = []
+    for pages in (3, 66000):
+        k_cache, v_cache = (torch.empty(pages, 64, 8, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+        k_scales, v_scales = (torch.empty(pages, 4, 8, device="cuda") for _ in range(2))
+        more = dict(block_table=torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32, device="cuda"), k_scales=k_scales,
+                    v_scales=v_scales)
+        min_fa3_op.append_cache(k, v, k_cache, v_cache, lens, **more)
+        min_fa3_op.check_last_status("append_cache")
+        results.append(min_fa3_op.forward_tree(q, k_cache, v_cache, lens, return_lse=True, **more))
+        results[-1] += (min_fa3_op.forward_tree(q[:, :1], k_cache, v_cache, lens + 149, **more),)
+        min_fa3_op.check_last_status("forward_tree")
+        del k_cache, v_cache
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_a_prefix_shared_by_pages():
+    """Sequences that read the same full pages and go on in pages of their own, against each of them alone."""
+    gen = torch.Generator().manual_seed(11)
+    cache = Cache8(11, 1, 64 * 8, 2, 64, 16)
+    pages = cache.table[0].tolist()
+    table = torch.tensor([pages[:2] + [pages[2 + b]] for b in range(4)], dtype=torch.int32).cuda()
+    q, k, v = (randn(gen, 4, 5, h, 128).cuda() for h in (8, 2, 2))
+    lens = torch.full((4,), 128, dtype=torch.int32, device="cuda")
+    scales = dict(k_scales=cache.k_scales, v_scales=cache.v_scales)
+    before = cache.snapshot()
+    min_fa3_op.append_cache(k, v, cache.k, cache.v, lens, block_table=table, **scales)
+    out = min_fa3_op.forward_tree(q, cache.k, cache.v, lens, block_table=table, **scales)
+    for b in range(4):
+        one = dict(scales, block_table=table[b:b + 1])
+        alone = min_fa3_op.forward_tree(q[b:b + 1], cache.k, cache.v, lens[:1], **one)
+        assert (out[b:b + 1].float() - alone.float()).abs().max().item() <= 2**-7 * alone.float().abs().max().item()
+    for old, new in zip(before, cache.snapshot()):
+        assert torch.equal(old[pages[:2]], new[pages[:2]])
