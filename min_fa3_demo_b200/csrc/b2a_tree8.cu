@@ -385,8 +385,8 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     mbar_arrive(smem_u32(&sh.scales.empty[scale_slot]));
                     if (!two) mbar_arrive(smem_u32(&sh.scales.empty[scale_slot]));
                 }
-                // What a score of 16 slots is multiplied by, and what is added: scores in log2 units, with V's scale.  Masked ones are -inf, so
-                // the factor must not be 0.
+                // What a score of 16 slots is multiplied by, and what is added: scores in log2 units, with V's scale.  Masked ones
+                // are -inf, so the factor must not be 0.
                 auto factor_of = [&](int g) { return fmaxf(q_scale * __shfl_sync(0xFFFFFFFFu, scale, g), FLT_MIN); };
                 auto addend_of = [&](int g) { return __shfl_sync(0xFFFFFFFFu, scale_log2, 8 + g); };
                 PH_MARK(3);
@@ -656,7 +656,7 @@ int b2a_tree8_fwd(const b2a_tree_args* a, const b2a_cache_scales* scales, void* 
                     scratch_bytes, kTreeKept, t.scratch);
     }
     p.c.item_tokens = t.few ? t.tile_tokens : 2 * t.tile_tokens;
-    p.c.min_run = 2;
+    p.c.min_run = 2;      // blocks of a CTA, at least: 1, 2, 4, 8 take 20.5, 20.3, 22.5, 26.6 us for a tree of 8 over 700 slots
     // What an item costs besides its blocks, in blocks, for the cuts between CTAs.  4 and 6, 16 sequences of a token over up to 8,001
     // slots: 44.8, 44.5 us; 6 and 9, of up to 32 tokens with one tile: 80.3, 82.9, of 64 with two, 8 sequences of up to 16,000: 222.9, 220.2.
     p.c.item_extra = t.tiles == 2 ? 9 : 6;
