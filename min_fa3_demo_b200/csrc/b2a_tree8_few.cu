@@ -254,13 +254,17 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const uint32_t buf = it % Shared::kQ;
             const __nv_bfloat16* q = p8.q + w.q_begin * p8.q_stride[0] + static_cast<long long>(w.head) * p.c.group * p8.q_stride[1] +
                                      (lane & 15) * 8;
-            bool waited = false;
+            auto ask = [&](int row) { return *reinterpret_cast<const uint4*>(q + sh.q_at[min(row, rows - 1)]); };
+            int row = 2 * mine + (lane >> 4);
+            uint4 x{};
+            if (2 * mine < rows) x = ask(row);
+            // A warp without rows waits as well: it could be as far as the next piece that uses this buffer, and what it then adds to
+            // q_full would stand for a warp that is still waiting for its rows of this one.
+            if (!warp_wait8(wctx, smem_u32(&sh.q_empty[buf]), ((it / Shared::kQ) & 1u) ^ 1u, 2)) return false;
 #pragma unroll 1
-            for (int row = 2 * mine + (lane >> 4); row - (lane >> 4) < rows; row += 8) {
-                const uint4 x = *reinterpret_cast<const uint4*>(q + sh.q_at[min(row, rows - 1)]);
-                if (!waited && !warp_wait8(wctx, smem_u32(&sh.q_empty[buf]), ((it / Shared::kQ) & 1u) ^ 1u, 2)) return false;
-                waited = true;
+            for (; row - (lane >> 4) < rows; row += 8) {
                 split_q_rows(x, row < rows, row, lane, &sh.q[buf][0][0], &sh.q[buf][1][0], &sh.q_scale[buf][row]);
+                if (row - (lane >> 4) + 8 < rows) x = ask(row + 8);
             }
             fence_proxy_async_smem();
             __syncwarp();

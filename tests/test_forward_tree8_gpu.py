@@ -410,3 +410,24 @@ def test_near_the_same_over_a_cache_in_16_bits():
                                              return_lse=True)
     assert (out.float() - wide.float()).norm().item() <= 2**-7 * wide.float().norm().item()
     assert (lse - wide_lse).abs().max().item() <= 3e-5
+
+
+@pytest.mark.parametrize("count,qh,kvh", [(1, 2, 2), (1, 4, 2), (2, 2, 2), (3, 2, 2), (1, 8, 2), (5, 2, 2), (3, 4, 2), (7, 2, 2), (8, 4, 2)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_pieces_of_one_block_each_with_its_own_queries(count, qh, kvh, shared):
+    """Some hundred sequences of a block or less, so that a CTA's pieces have one block each: 1 to 16 rows, of which some leave a warp
+    without any.  ``shared``: all sequences have the same pages, which are at hand, while their queries come from memory."""
+    rng = random.Random(count)
+    batch = Batch(count, [rng.randint(1, 128 - count) for _ in range(400)], [count] * 400, qh, kvh, 32)
+    if shared:
+        batch.cache.table.copy_(batch.cache.table[:1].expand_as(batch.cache.table))
+        batch.cache.place = [batch.cache.place[0]] * 400
+    out, lse = run(batch)
+    junk = torch.empty(64 << 20, device="cuda")
+    for fill in range(10):
+        junk.fill_(float(fill))                     # nothing is in L2 any more; then K, V and their scales, but no queries
+        for t in batch.cache.snapshot():
+            t.view(torch.uint8).sum()
+        again = batch.call()
+        min_fa3_op.check_last_status("forward_tree")
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
