@@ -500,7 +500,7 @@ int b2a_cache8_append(const b2a_append_args* args, const b2a_cache_scales* scale
 
 /*
  * b2a_tree_fwd_with_scratch over a cache in 8 bits; workspace and scratch have the same sizes.  Q takes part in its product as the sum
- * of two 8-bit numbers, off by 2^-18 of a row's largest value at most, a probability (times V's scale) in fp16, off by 2^-11 of itself
+ * of two 8-bit numbers, off by 2^-17 of a row's largest value at most, a probability (times V's scale) in fp16, off by 2^-11 of itself
  * or 2^-27 of the row's largest.  V's scales are taken within 2^-64 .. 2^64, and infinities of q as NaN.
  */
 int b2a_tree8_fwd(const b2a_tree_args* args, const b2a_cache_scales* scales, void* scratch, size_t scratch_bytes, void* cuda_stream);

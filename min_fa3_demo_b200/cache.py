@@ -383,7 +383,7 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
     Over a cache in 8 bits, with its ``k_scales`` and ``v_scales`` (positive and finite; they may be expanded, one for all blocks or
     heads): a slot's values are its e4m3 times its block's scale.  q goes into its product as the sum of two 8-bit numbers (off by
-    2^-18 of a row's largest value), the probabilities times V's scale in fp16 (off by 2^-11 of themselves, or by 2^-27 of a row's
+    2^-17 of a row's largest value), the probabilities times V's scale in fp16 (off by 2^-11 of themselves, or by 2^-27 of a row's
     largest): out is no further off than over a bf16 cache with the same values.  Infinities in q count as NaN.
     """
     index, batch = k_cache.get_device(), cache_lens.numel()

@@ -3,8 +3,8 @@
 // K Q^T is a product of 8-bit operands: K's tiles go from global memory to shared memory by TMA and from there into the product, and are
 // never converted.  Q has to have 8 bits too, and e4m3 has only four significant ones, so Q is the sum of two such
 // numbers, which take part one after the other in the same accumulator: a bf16 rounded to e4m3 leaves a signed rest of four
-// bits, which e4m3 holds exactly.  A row is scaled so that its largest value lies in [2^7, 2^8); rests below 2^-9 lose bits, which
-// is 2^-18 of that value.  Twice the products at twice the rate of bf16.
+// bits, which e4m3 holds exactly.  A row is scaled so that its largest value lies in [2^7, 2^8); rests of values below 2^-2 are rounded
+// to a multiple of 2^-9, so they are off by 2^-10 at most, 2^-17 of that value.  Twice the products at twice the rate of bf16.
 //
 // P V is a product of f16: e4m3 is exact in f16, and four warps convert V's tiles (16 KiB in, 32 KiB out, an instruction for two
 // values).  P in f16 is off by 2^-11 of itself, or by 2^-25 where it is small, 2^-27 of a row's largest or less.  P as

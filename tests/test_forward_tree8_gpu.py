@@ -431,3 +431,26 @@ def test_pieces_of_one_block_each_with_its_own_queries(count, qh, kvh, shared):
         again = batch.call()
         min_fa3_op.check_last_status("forward_tree")
         assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("count", [1, 5, 9, 20, 60, 200])
+def test_queries_that_the_two_parts_hold_worst(count):
+    """A largest value of 128 and others of 2^-3 + 2^-10, whose rest of 2^-10 lies halfway between two numbers of 8 bits and is lost: 2^-17
+    of the largest value in each of 127 terms, all with the same sign.  A row sees its own slot only, so that its lse is the score."""
+    batch = Batch(7, [0], [count], 1, 1, 16)
+    batch.tree_mask.copy_(torch.eye(count, dtype=torch.bool).view(1, count, count))
+    sign = torch.randint(0, 2, (count, 128), generator=torch.Generator().manual_seed(count)) * 2.0 - 1
+    q = sign * (2.0**-3 + 2.0**-10)
+    q[torch.arange(count), torch.arange(count) % 128] *= 128 / (2.0**-3 + 2.0**-10)
+    batch.q.copy_(q.view(1, count, 1, 128))
+    assert torch.equal(batch.q.double().cpu().view(count, 128), q.double())
+    for s in range(count):
+        batch.cache.set("k", 0, s, sign[s] * 448)
+    batch.cache.k_scales.fill_(2.0**-9)
+    out, lse = batch.call()
+    min_fa3_op.check_last_status("forward_tree")
+    assert torch.equal(out[0, :, 0].double().cpu(), batch.cache.rows("v", 0, count)[:, 0].to(torch.bfloat16).double())
+    score = (q.double() * batch.cache.rows("k", 0, count)[:, 0]).sum(1) / math.sqrt(128)
+    off = (lse[0, 0].double().cpu() - score).abs()
+    # The 128 terms' roundings, and those of some operations in 32 bits on values of up to the score.
+    assert (off <= 2.0**-17 * 128 * 128 * 448 * 2.0**-9 / math.sqrt(128) + 2.0**-20 * score.abs()).all()
