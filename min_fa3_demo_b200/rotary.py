@@ -77,6 +77,12 @@ class RotaryAxes:
         self._plain = (list(turn), list(axis), bool(adjacent))
         return self
 
+    def __setattr__(self, name, value) -> None:
+        # Kernels read the structure, a traced step the attribute: one that went its own way would change half of the calls.
+        if name == "magnitude" and name in self.__dict__:
+            raise AttributeError("magnitude cannot be changed: make new axes, RotaryAxes(..., magnitude=) or stretched(..., magnitude=)")
+        super().__setattr__(name, value)
+
     @property
     def _at(self) -> int:
         # Asked for at each call: a copy or an unpickled object has a structure of its own, elsewhere.

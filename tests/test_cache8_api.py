@@ -351,3 +351,13 @@ def test_magnitude_of_the_c_interface(lib):
     args = filled(_cabi.RotaryArgs, axes=axes._at, q=256, q_out=256, positions=256, q_stride=(2560, 512, 128), positions_stride=(15, 5, 1),
                   batch=3, seqlen=5, heads_q=4)
     assert lib.b2a_rotary(ctypes.byref(args), None) == _cabi.B2A_ERR_INVALID_ARGUMENT and "magnitude must be finite" in _cabi.last_error()
+
+
+@pytest.mark.parametrize("how", [lambda a: a, copy.copy, copy.deepcopy, lambda a: pickle.loads(pickle.dumps(a)),
+                                 lambda a: rotary.RotaryAxes._from_plain(*a._plain, a.magnitude)])
+def test_the_magnitude_is_the_same_for_all_calls(how):
+    """The attribute is what traced steps read, the structure what kernels read."""
+    axes = how(rotary.RotaryAxes([0.5] * 8, magnitude=1.25))
+    with pytest.raises(AttributeError, match="magnitude cannot be changed"):
+        axes.magnitude = 2.0
+    assert axes.magnitude == axes._c.magnitude == 1.25
