@@ -37,10 +37,12 @@ __all__ = ["append_cache", "forward_tree", "cache_weights", "evict_cache"]
 _E4M3 = torch.float8_e4m3fn
 
 
-def _check_cache(cache: torch.Tensor, name: str, dtype: torch.dtype = _BF16) -> None:
+def _check_cache(cache: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> None:
+    """dtype: what a call that takes scales wants of it, with those that it got; None: of one that takes none."""
     _check(cache.is_cuda, f"{name} must be a CUDA tensor")
-    _check(cache.dtype == dtype, f"{name} must have dtype {dtype}" + (" or, with scales, torch.float8_e4m3fn" if dtype is _BF16 else ""))
-    few = 7 if dtype is _BF16 else 15
+    _check(cache.dtype == (dtype or _BF16),
+           f"{name} must have dtype {dtype or _BF16}" + (" or, with scales, torch.float8_e4m3fn" if dtype is _BF16 else ""))
+    few = 15 if dtype is _E4M3 else 7
     _check(cache.dim() == 4, f"{name} must have shape [pages, page_size, KVH, D]")
     _check(cache.size(3) == 128, f"{name} must have head_dim D=128")
     _check(cache.size(0) > 0 and cache.size(1) > 0 and cache.size(2) > 0, f"{name} must not be empty")
@@ -107,7 +109,7 @@ def _check_table(block_table: Optional[torch.Tensor], k_cache: torch.Tensor, bat
     _check(k_cache.size(1) % 8 == 0, f"page_size must be a multiple of 8. Got {k_cache.size(1)}")
 
 
-def _check_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype = _BF16) -> None:
+def _check_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: Optional[torch.dtype] = None) -> None:
     _check_cache(k_cache, "k_cache", dtype)
     _check_cache(v_cache, "v_cache", dtype)
     _check(k_cache.device == v_cache.device, "k_cache and v_cache must be on the same CUDA device")

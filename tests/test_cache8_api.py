@@ -361,3 +361,20 @@ def test_the_magnitude_is_the_same_for_all_calls(how):
     with pytest.raises(AttributeError, match="magnitude cannot be changed"):
         axes.magnitude = 2.0
     assert axes.magnitude == axes._c.magnitude == 1.25
+
+
+def test_which_types_a_call_says_it_takes(fake):
+    """Calls without scales do not speak of them."""
+    k8, v8, weights = f8(9, 32, 2, 128), f8(9, 32, 2, 128), f32(3, 2, 128)
+    where = dict(cache_lens=i32(3), block_table=i32(3, 4))
+    wide = dict(k_cache=t(9, 32, 2, 128), v_cache=t(9, 32, 2, 128), k_scales=None, v_scales=None)
+    only = r"k_cache must have dtype torch\.bfloat16$"
+    with pytest.raises(RuntimeError, match=only):
+        cache.cache_weights(t(3, 5, 4, 128), f32(3, 4, 5), k8, weights=weights, **where)
+    with pytest.raises(RuntimeError, match=only):
+        cache.evict_cache(k8, v8, weights, budget=64, **where)
+    for call, function in FUNCTIONS.items():
+        with pytest.raises(RuntimeError, match=r"k_cache must have dtype torch\.bfloat16 or, with scales, torch\.float8_e4m3fn$"):
+            function(**dict(arguments(call), **dict(wide, k_cache=t(9, 32, 2, 128, dtype=torch.float16))))
+        with pytest.raises(RuntimeError, match=r"k_cache must have dtype torch\.float8_e4m3fn$"):
+            function(**dict(arguments(call), k_cache=t(9, 32, 2, 128)))
