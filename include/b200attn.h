@@ -31,7 +31,7 @@ extern "C" {
 #define B2A_ERR_UNSUPPORTED_DEVICE (-4)
 #define B2A_ERR_DEVICE_STATUS (-5)
 
-/* Version of this ABI (bumped when a struct layout changes). */
+/* Version of this ABI (bumped when a struct layout changes).  3: b2a_rotary_axes has a magnitude, where 2 had padding. */
 int b2a_abi_version(void);
 
 /* Thread-local text of the last error returned on this thread ("" if none). */

@@ -225,7 +225,7 @@ int b2a_profile_read(int kernel, float* ms, int capacity) {
     return n;
 }
 
-int b2a_abi_version(void) { return 2; }
+int b2a_abi_version(void) { return 3; }
 
 const char* b2a_last_error(void) { return b2a::error_buffer(); }
 

@@ -104,3 +104,19 @@ def test_kernels_that_start_early_use_ordinary_loads():
         signature = re.search(rf"__global__[^;{{]*?\b{name}\(([^{{]*?)\)\s*{{", source).group(1)
         assert "__restrict__" not in signature, name
     assert not re.search(r"__ldg\b|ld\.global\.nc", source)
+
+
+# What the structures looked like under each version: a hash of every field's name, offset and size.
+LAYOUTS = {3: "f10e2b66225f8689991580633d9bf0494f240eb3615c6b802b1ba0c31d0cd492"}
+
+
+def test_a_layout_of_its_own_for_each_version(lib):
+    """A caller that was built for other structures finds out by the version, so whoever changes one gives it a new number, and a line
+    here.  (Version 2 stood for axes with and without a magnitude.)"""
+    import hashlib
+    text = ""
+    for name, struct in sorted(vars(_cabi).items()):
+        if isinstance(struct, type) and issubclass(struct, ctypes.Structure) and struct is not ctypes.Structure:
+            fields = [(f, getattr(struct, f).offset, getattr(struct, f).size) for f, _ in struct._fields_]
+            text += f"{name} {ctypes.sizeof(struct)} {fields}\n"
+    assert LAYOUTS.get(lib.b2a_abi_version()) == hashlib.sha256(text.encode()).hexdigest()
