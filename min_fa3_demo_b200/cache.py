@@ -8,7 +8,7 @@ values of a head are adjacent: pages with k and v side by side, heads before slo
 A cache may also be in 8 bits: k and v in ``torch.float8_e4m3fn`` and, for each block of 16, 32, 64 or 128 slots and head, a scale:
 ``k_scales`` and ``v_scales`` ``[pages, page_size / block, KVH]`` (fp32; of any strides, the number of blocks rounded up where there are
 no pages, whose size is a multiple of the block).  :func:`append_cache` finds the scales, :func:`forward_tree` takes
-any positive ones; the other two want bf16.
+any positive ones (V's from 2^-64 to 2^64, as those that are found); the other two want bf16.
 
 A decoding step: :func:`append_cache` writes the drafted tokens behind ``cache_lens``, :func:`forward_tree` lets them attend,
 and once some are accepted the caller writes those again (their positions are the same) and adds them to ``cache_lens``.
@@ -383,8 +383,8 @@ def forward_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     the call.  As in ``forward``, probabilities are rounded to bf16 for their product with v (sums and LSE are of the unrounded ones):
     out is off by 0.0023 of its 2-norm on random inputs, of which its own rounding is 0.0017.
 
-    Over a cache in 8 bits, with its ``k_scales`` and ``v_scales`` (positive and finite; they may be expanded, one for all blocks or
-    heads): a slot's values are its e4m3 times its block's scale.  q goes into its product as the sum of two 8-bit numbers (off by
+    Over a cache in 8 bits, with its ``k_scales`` and ``v_scales`` (positive and finite, V's taken within 2^-64 .. 2^64; they may be
+    expanded, one for all blocks or heads): a slot's values are its e4m3 times its block's scale.  q goes into its product as the sum of two 8-bit numbers (off by
     2^-17 of a row's largest value), the probabilities times V's scale in fp16 (off by 2^-11 of themselves, or by 2^-27 of a row's
     largest): out is no further off than over a bf16 cache with the same values.  Infinities in q count as NaN.
     """

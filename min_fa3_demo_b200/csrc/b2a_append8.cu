@@ -4,9 +4,10 @@
 // dimensions each, as in b2a_rotary.cuh, and 16 tokens on their way at once, by asynchronous copies.  It turns them in fp32, looks for
 // the largest, finds the scale, turns them once more and rounds; nothing waits for another warp.  Blocks of more new tokens than 16
 // are read twice, the second time from L2.  e4m3 is a floating-point format, so a scale that is a power of two costs no accuracy
-// (values keep their four bits down to 2^-15 of the largest), divides exactly, and can grow with hardly a trace: x / 2 is a number
-// of the format as well, unless it is one of the smallest.  So a block whose tokens come one by one keeps its scale until a token does
-// not fit, and then the tokens that it holds are read, divided and written again, at most 127 of 128 bytes.
+// (it puts the largest value above 224, and values keep their four bits down to 2^-6, 2^-13.8 of it; down to 2^-6 times the scale where
+// a block keeps an older, larger one), divides exactly, and can grow with hardly a trace: x / 2 is a number of the format as well,
+// unless it is one of the smallest.  So a block whose tokens come one by one keeps its scale until a token does not fit, and then the
+// tokens that it holds are read, divided and written again, at most 127 of 128 bytes.
 //
 // Should be bound by memory: 256 bytes in and 128 out a token and head, and q's 256 and 256.  A CTA has a block of slots and some of the
 // heads, for which it computes the angles once; CTAs behind those turn q, and the first one looks for places that do not exist.
