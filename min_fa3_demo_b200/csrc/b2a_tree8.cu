@@ -465,10 +465,8 @@ tree8_attention(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     const float factor = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
                     l *= factor;
                     m_used = m_new;
-                    if (pv_pending) {         // a block that ends a sequence has waited already
-                        ok = wait_pv();
-                        if (!ok) break;
-                    }
+                    ok = wait_pv();
+                    if (!ok) break;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t t[32];
