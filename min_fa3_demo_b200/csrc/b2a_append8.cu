@@ -216,7 +216,7 @@ append8_tokens(const __grid_constant__ Append8Params p8) {
                 if (p.cu_seqlens == nullptr) {
                     at.seq = item / p8.parts / p8.seq_blocks;
                     const int j = item / p8.parts - at.seq * p8.seq_blocks, len = p.cache_lens[at.seq];
-                        const long long token = j == 0 ? 0 : (static_cast<long long>(j) << p8.scales.shift) - (len & mask);
+                    const long long token = j == 0 ? 0 : (static_cast<long long>(j) << p8.scales.shift) - (len & mask);
                     if (len >= 0 && token < p.seqlen) fill_block(p, mask, len, p.seqlen, static_cast<int>(token), at);
                     at.last = 1;
                 } else if (p8.run == 0) {

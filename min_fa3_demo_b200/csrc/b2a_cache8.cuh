@@ -6,10 +6,11 @@
 // bits, which e4m3 holds exactly.  A row is scaled so that its largest value lies in [2^7, 2^8); rests of values below 2^-2 are rounded
 // to a multiple of 2^-9, so they are off by 2^-10 at most, 2^-17 of that value.  Twice the products at twice the rate of bf16.
 //
-// P V is a product of f16: e4m3 is exact in f16, and four warps convert V's tiles (16 KiB in, 32 KiB out, an instruction for two
-// values).  P in f16 is off by 2^-11 of itself, or by 2^-25 where it is small, 2^-27 of a row's largest or less.  P as
-// a sum of two 8-bit numbers, as Q is, needs no conversion of V but six instructions for two probabilities instead of one, which the
-// softmax has no time for (trees of 64 tokens, 64 heads over 8, 8 sequences of up to 16,000 slots: 344 us).
+// P V is a product of f16: e4m3 is exact in f16, and warps of their own convert V's tiles (16 KiB in, 32 KiB out, an instruction for
+// two values): four, or one where two tiles of rows give it the time.  P in f16 is off by 2^-11 of itself, or by 2^-25 where it is
+// small, 2^-27 of a row's largest or less.  P as a sum of two 8-bit numbers, as Q is, needs no conversion of V but six instructions for
+// two probabilities instead of one, which the softmax has no time for (trees of 64 tokens, 64 heads over 8, 8 sequences of up to
+// 16,000 slots: 344 us).
 //
 // Scales never meet the values: K's multiplies a score, V's is an addend of the exponent, by which P takes it into the
 // product, and what goes into the row's sum is divided by it again.

@@ -519,10 +519,7 @@ tree8_attention_few(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         if (!first) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor[e]);
-                            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                                         ::"r"(o_tmem + x * N + c0), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]),
-                                           "r"(o[6]), "r"(o[7])
-                                         : "memory");
+                            tmem_st_x8(o_tmem + x * N + c0, o);
                         }
                     }
                     if (!first) tmem_wait_st();
