@@ -112,6 +112,10 @@ class RotaryAxes:
         and of k, a score by its square; by default ``0.1 ln(factor) + 1`` times what it was.  (Peng et al., "Efficient Context Window
         Extension of Large Language Models", 2023, "NTK-by-parts" and its temperature; with ``magnitude=1`` and a small ``fast``
         the smooth ramp that is in use without one.)  ``slow = fast = inf``: all frequencies divided.
+
+        Where a model was trained or tuned with another ramp, its pairs between the two have other frequencies: loaders commonly
+        go over linearly in the number of the pair, not of its turns.  Give such frequencies as they are, with their magnitude:
+        ``RotaryAxes(inv_freq, magnitude=...)``.
         """
         _check(hasattr(self, "_inv_freq"), "these axes do not know their frequencies")
         _check(isfinite(factor) and factor >= 1, f"factor must be 1 or more, got {factor}")
