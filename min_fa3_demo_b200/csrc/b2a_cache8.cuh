@@ -479,7 +479,15 @@ __device__ __forceinline__ void tree8_add_not_finite(const TreeParams& p, const 
     }
 }
 
-// b2a_tree8_one.cu: calls of more rows an item, but no more than a tile's 128; b2a_tree8_few.cu: of at most kFewRows.
+// b2a_tree8_one.cu: calls of more rows an item, but no more than a tile's 128; b2a_tree8_few.cu: of at most kFewRows, which is as
+// many as it takes.  Us of the latter and the former, 8 K/V heads, sequences x slots:
+//              1 x 16,384     64 x 2,048      16 x 16,384     4 x 400        32 x 1,000
+//    4 rows    19.5  30.4     66.4  128.1     104.8  198.8    13.0  16.8     29.1  42.9
+//    9         21.2  32.0     78.0  132.0     107.6  199.8    14.4  17.7     33.3  44.3
+//   16         21.6  33.0     78.6  135.1     108.3  201.3    14.7  18.3     33.7  46.8
+//   17         24.7  33.8    111.9  136.7     160.1  201.6    16.5  18.4     40.4  47.3
+//   24         25.0  33.4    113.4  136.1     160.9  201.5    16.8  18.6     41.1  47.3
+//   32         26.0  34.0    115.6  136.4     162.0  202.1    17.0  19.0     42.9  47.9
 int launch_tree8_one(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
                      cudaStream_t stream);
 int launch_tree8_few(const CUtensorMap& map_k, const CUtensorMap& map_v, const Tree8Params& p, int ctas, const DeviceInfo& dev,
