@@ -7,8 +7,10 @@
 // and K's meet in the factor of a score.
 //
 // Bound by what an SM does for a score rather than by memory: two products of K, one of V in f16, an exponential, and the sum with V's
-// scale.  8 sequences of 64 drafted tokens, 64 heads over 8, up to 16,000 slots: 222 us, 735 TFLOP/s; two chunks of 1,000 tokens, 32 heads
-// over 8, behind up to 8,000: 336 us, 721 TFLOP/s.
+// scale.  8 sequences of 64 drafted tokens, 64 heads over 8, up to 16,000 slots: 222 to 242 us (bf16: 189 to 208), up to 735 TFLOP/s; two
+// chunks of 1,000 tokens, 32 heads over 8, behind up to 8,000: 338 us, 717 TFLOP/s.  No unit is near its limit (tensor pipe 38 %, special
+// functions 39 %, issue slots 34 %; over bf16 49, 49, 32), and what the difference waits for is not found: that kernel uses one S for
+// two tiles as well, and executes 57 million instructions for 81.
 //
 //   warp 0-3, 4-7   Q in two parts, then softmax, one thread a row
 //   warp 8          Q K^T       warp 10   P V       warp 9   plan, loads of K, V and scales       warp 11   V to f16
