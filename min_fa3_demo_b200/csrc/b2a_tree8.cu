@@ -638,8 +638,9 @@ int b2a_tree8_fwd(const b2a_tree_args* a, const b2a_cache_scales* scales, void* 
     if (rc == B2A_OK) rc = make_cache_scales(*scales, a->cache, &p8.scales);
     if (rc != B2A_OK) return rc;
     for (int i = 0; i < 2; ++i) {
-        B2A_REQUIRE(a->q_stride[i] >= 0 && a->q_stride[i] % 8 == 0, "strides of q must be multiples of 8 elements");
-        p8.q_stride[i] = a->q_stride[i];
+        // Of one token or head it is never stepped, and a caller may say anything.
+        p8.q_stride[i] = (i == 0 ? a->total_q : a->heads_q) == 1 ? 0 : a->q_stride[i];
+        B2A_REQUIRE(p8.q_stride[i] >= 0 && p8.q_stride[i] % 8 == 0, "strides of q must be multiples of 8 elements");
     }
     p8.q = static_cast<const __nv_bfloat16*>(a->q);
     B2A_REQUIRE(a->out != nullptr && (reinterpret_cast<uintptr_t>(a->out) & 0xF) == 0, "out must be a 16-byte aligned device pointer");

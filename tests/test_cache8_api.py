@@ -378,3 +378,12 @@ def test_which_types_a_call_says_it_takes(fake):
             function(**dict(arguments(call), **dict(wide, k_cache=t(9, 32, 2, 128, dtype=torch.float16))))
         with pytest.raises(RuntimeError, match=r"k_cache must have dtype torch\.float8_e4m3fn$"):
             function(**dict(arguments(call), k_cache=t(9, 32, 2, 128)))
+
+
+@pytest.mark.parametrize("total,heads,stride", [(1, 4, (1001, 128)), (1, 2, (0, 256)), (15, 2, (512, 77)), (1, 1, (3, 5))])
+def test_strides_that_nobody_looks_at_over_the_c_interface(lib, total, heads, stride):
+    """One token, or one query head: as over a bf16 cache, the stride may be anything.  (Two heads of 15 tokens: it may not.)"""
+    kvh = dict(cache_fields=dict(heads_k=1)) if heads == 1 else {}
+    rc = c_call(lib, "b2a_tree8_fwd", batch=total // min(total, 5), seqlen_q=min(total, 5), total_q=total, heads_q=heads, q_stride=stride, **kvh)
+    refused = rc == _cabi.B2A_ERR_INVALID_ARGUMENT and "strides of q" in _cabi.last_error()
+    assert rc != _cabi.B2A_OK and refused == (total > 1)

@@ -454,3 +454,12 @@ def test_queries_that_the_two_parts_hold_worst(count):
     off = (lse[0, 0].double().cpu() - score).abs()
     # The 128 terms' roundings, and those of some operations in 32 bits on values of up to the score.
     assert (off <= 2.0**-17 * 128 * 128 * 448 * 2.0**-9 / math.sqrt(128) + 2.0**-20 * score.abs()).all()
+
+
+@pytest.mark.parametrize("qh,kvh", [(4, 1), (1, 1), (64, 1)])
+def test_one_token_with_strides_that_nobody_looks_at(qh, kvh):
+    batch = Batch(3, [77], [1], qh, kvh, 16)
+    want, want_lse = run(batch)
+    batch.q = torch.as_strided(batch.q.clone(), batch.q.shape, (1003, 1001, 5 if qh == 1 else 128, 1))
+    out, lse = run(batch)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
